@@ -480,6 +480,99 @@ typedef struct ss_decode_linear_args {
 int64_t ss_decode_linear_workspace_bytes(const ss_decode_linear_args* a);
 int ss_decode_linear(const ss_decode_linear_args* a, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Linear attention with a decay for each head.  No counterpart in the
+ * reference.  Per (batch b, head h), with group j = h / (heads / groups):
+ *   S_t = exp(g[b, t, h]) S_{t-1} + k[b, t, j] v[b, t, h]^T        (d_key x d_value, fp32)
+ *   out[b, t, h] = scale * q[b, t, j]^T S_t
+ * from S_{-1} = initial_state (zero when NULL); last_state is S after the
+ * last token.  q, k: (batch, seqlen, groups, d_key); v, out: (batch, seqlen,
+ * heads, d_value); element type dtype, unit stride along the last dim, other
+ * strides free and not negative.  g: fp32 log decays (batch, seqlen, heads), any strides (0
+ * too); minus infinity empties the state.  initial_state, last_state: fp32
+ * (batch, heads, d_key, d_value) contiguous.  lengths: int32 (batch),
+ * row b holds lengths[b] tokens (clamped to [0, seqlen]): tokens past them
+ * are not read, their outputs are zero, and last_state is the state after
+ * the row's own last token.  d_key and d_value: 1 to 256.
+ * ends: fp32 (batch, heads, segments, d_key, d_value), the state after each
+ * segment of ss_linear_attn_segment() tokens, kept for the backward.
+ * ------------------------------------------------------------------------ */
+typedef struct ss_linear_attn_args {
+    int64_t batch, seqlen, heads, groups, d_key, d_value;
+    int32_t dtype;                       /* enum ss_dtype */
+    float scale;
+    int64_t q_batch_stride, q_len_stride, q_head_stride;
+    int64_t k_batch_stride, k_len_stride, k_head_stride;
+    int64_t v_batch_stride, v_len_stride, v_head_stride;
+    int64_t out_batch_stride, out_len_stride, out_head_stride;
+    int64_t g_batch_stride, g_len_stride, g_head_stride;
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* g;
+    const float* initial_state;          /* may be NULL */
+    const int32_t* lengths;              /* may be NULL: every row holds seqlen tokens */
+    void* out;                           /* ignored by ss_linear_attn_bwd */
+    float* last_state;                   /* may be NULL (not written); ignored by ss_linear_attn_bwd */
+    float* ends;                         /* written by the forward unless NULL, read by the backward */
+    void* workspace;                     /* the entry point's workspace_bytes, 16-byte aligned; NULL iff 0 */
+    int64_t workspace_bytes;
+} ss_linear_attn_args;
+
+/* dq, dk: (batch, seqlen, groups, d_key), dv: (batch, seqlen, heads,
+ * d_value), contiguous, dtype (the sums over the heads of a group in fp32,
+ * rounded once).  dg: fp32 (batch, seqlen, heads) contiguous, or (heads)
+ * when g_per_head (the sum over batch and tokens).  Every sum has a fixed
+ * order: the same bits on every run. */
+typedef struct ss_linear_attn_bwd_args {
+    ss_linear_attn_args f;               /* as for the forward; f.ends from it */
+    int64_t dout_batch_stride, dout_len_stride, dout_head_stride;
+    const void* dout;
+    const float* dlast_state;            /* may be NULL: zero */
+    void* dq;
+    void* dk;
+    void* dv;
+    float* dg;
+    float* dinitial_state;               /* may be NULL (not written) */
+    int32_t g_per_head;
+    int32_t pad_;
+} ss_linear_attn_bwd_args;
+
+/* Tokens per segment for these sizes (a state per segment is kept for the
+   backward; a long row's segments run side by side), or -1 (with
+   ss_last_error set) when the arguments fail the checks.  The number of
+   segments is max(1, ceil(seqlen / that)). */
+int64_t ss_linear_attn_segment(const ss_linear_attn_args* a);
+/* Bytes of workspace the calls need (0: none), or -1 on failing checks.
+   No device work. */
+int64_t ss_linear_attn_fwd_workspace_bytes(const ss_linear_attn_args* a);
+int64_t ss_linear_attn_bwd_workspace_bytes(const ss_linear_attn_bwd_args* a);
+int ss_linear_attn_fwd(const ss_linear_attn_args* a, void* stream);
+int ss_linear_attn_bwd(const ss_linear_attn_bwd_args* a, void* stream);
+
+/* One token: state <- exp(g) state + k v^T in place, out = scale q^T state.
+ * q, k: (batch, groups, d_key); v, out: (batch, heads, d_value), unit stride
+ * along the last dim; g: fp32 (batch, heads); state: fp32 (batch, heads,
+ * d_key, d_value), the last two dims contiguous. */
+typedef struct ss_linear_attn_update_args {
+    int64_t batch, heads, groups, d_key, d_value;
+    int32_t dtype;                       /* enum ss_dtype */
+    float scale;
+    int64_t state_batch_stride, state_head_stride;
+    int64_t q_batch_stride, q_head_stride;
+    int64_t k_batch_stride, k_head_stride;
+    int64_t v_batch_stride, v_head_stride;
+    int64_t out_batch_stride, out_head_stride;
+    int64_t g_batch_stride, g_head_stride;
+    float* state;
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* g;
+    void* out;
+} ss_linear_attn_update_args;
+int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,8 @@ EXPORTED = (
     "ss_rmsnorm_fwd", "ss_rmsnorm_bwd", "ss_rmsnorm_bwd_workspace_bytes",
     "ss_state_update", "ss_conv1d_update", "ss_decode_linear", "ss_decode_linear_workspace_bytes",
     "ss_conv1d_bwd_workspace_bytes", "ss_conv1d_fwd_typed", "ss_conv1d_bwd_typed",
+    "ss_linear_attn_segment", "ss_linear_attn_fwd_workspace_bytes", "ss_linear_attn_bwd_workspace_bytes",
+    "ss_linear_attn_fwd", "ss_linear_attn_bwd", "ss_linear_attn_update",
 )
 
 _i64, _i32, _p = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
@@ -154,6 +156,34 @@ class DecodeLinearArgs(ctypes.Structure):
     ]
 
 
+class LinearAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("seqlen", _i64), ("heads", _i64), ("groups", _i64), ("d_key", _i64), ("d_value", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+    ] + [(f"{t}_{d}_stride", _i64) for t in ("q", "k", "v", "out", "g") for d in ("batch", "len", "head")] + [
+        ("q", _p), ("k", _p), ("v", _p), ("g", _p), ("initial_state", _p), ("lengths", _p),
+        ("out", _p), ("last_state", _p), ("ends", _p), ("workspace", _p), ("workspace_bytes", _i64),
+    ]
+
+
+class LinearAttnBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", LinearAttnArgs),
+        ("dout_batch_stride", _i64), ("dout_len_stride", _i64), ("dout_head_stride", _i64),
+        ("dout", _p), ("dlast_state", _p), ("dq", _p), ("dk", _p), ("dv", _p), ("dg", _p), ("dinitial_state", _p),
+        ("g_per_head", _i32), ("pad_", _i32),
+    ]
+
+
+class LinearAttnUpdateArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("groups", _i64), ("d_key", _i64), ("d_value", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+    ] + [(f"{t}_{d}_stride", _i64) for t in ("state", "q", "k", "v", "out", "g") for d in ("batch", "head")] + [
+        ("state", _p), ("q", _p), ("k", _p), ("v", _p), ("g", _p), ("out", _p),
+    ]
+
+
 _lib = None
 _host = None
 _lock = threading.Lock()
@@ -216,6 +246,16 @@ def load():
         lib.ss_bwd.restype = ctypes.c_int
         lib.ss_bwd_noalloc.argtypes = [ctypes.POINTER(BwdArgs), _p]
         lib.ss_bwd_noalloc.restype = ctypes.c_int
+        for name, T in (("ss_linear_attn_segment", LinearAttnArgs), ("ss_linear_attn_fwd_workspace_bytes", LinearAttnArgs),
+                        ("ss_linear_attn_bwd_workspace_bytes", LinearAttnBwdArgs)):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(T)]
+            fn.restype = _i64
+        for name, T in (("ss_linear_attn_fwd", LinearAttnArgs), ("ss_linear_attn_bwd", LinearAttnBwdArgs),
+                        ("ss_linear_attn_update", LinearAttnUpdateArgs)):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(T), _p]
+            fn.restype = ctypes.c_int
         if lib.ss_abi_version() != ABI_VERSION:
             raise RuntimeError(f"mamba_amd: library ABI {lib.ss_abi_version()} != binding ABI {ABI_VERSION}")
         fs, bs = _i64(), _i64()

@@ -624,6 +624,183 @@ Tensor state_update(const Tensor& state, const Tensor& x, const OptT& dt, const 
     return *out;
 }
 
+// ------------------------------------------------------ linear attention --
+constexpr const char* kLin = "linear_attn";
+
+void on_device(const char* what, const char* name, const Tensor& t, const at::Device& dev) {
+    REQUIRE(what, t.device() == dev, std::string(name) + " is on " + t.device().str() + ", expected " + dev.str());
+}
+void of_type(const char* what, const char* name, const Tensor& t, at::ScalarType ty) {
+    REQUIRE(what, t.scalar_type() == ty,
+            std::string(name) + " has dtype " + dtype_str(t.scalar_type()) + ", expected " + dtype_str(ty));
+}
+// The log decays as the library reads them: fp32, (batch, seqlen, heads) with
+// strides (0 along batch and seqlen where every head has one decay).
+Tensor decays(const char* what, const Tensor& g_, int64_t batch, int64_t seqlen, int64_t heads, const Tensor& v) {
+    on_device(what, "g", g_, v.device());
+    REQUIRE(what, g_.scalar_type() == at::kFloat || g_.scalar_type() == v.scalar_type(),
+            "g has dtype " + dtype_str(g_.scalar_type()) + ", expected float32 or v's");
+    const bool per_head = g_.dim() == 1;
+    const bool ok = per_head ? same_shape(g_, {heads}) : seqlen < 0 ? same_shape(g_, {batch, heads})
+                                                                    : same_shape(g_, {batch, seqlen, heads});
+    REQUIRE(what, ok, std::string("g must be ") + (seqlen < 0 ? "(batch, heads)" : "(batch, seqlen, heads)") +
+                          " or (heads,), got " + shape_str(g_.sizes()));
+    const Tensor g = g_.to(at::kFloat);
+    return !per_head ? g : seqlen < 0 ? g.expand({batch, heads}) : g.expand({batch, seqlen, heads});
+}
+Tensor state_arg(const char* name, const Tensor& t, at::IntArrayRef shape, const at::Device& dev) {
+    on_device(kLin, name, t, dev);
+    of_type(kLin, name, t, at::kFloat);
+    REQUIRE(kLin, t.sizes() == shape, std::string(name) + " has shape " + shape_str(t.sizes()) + ", expected " + shape_str(shape));
+    return t.contiguous();
+}
+
+struct LinIn { Tensor q, k, v, g; OptT initial, lengths; };
+
+LinIn fill_linear(ss_linear_attn_args& a, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_,
+                  const OptT& initial, const OptT& lengths, double scale) {
+    a = ss_linear_attn_args{};
+    REQUIRE(kLin, v_.dim() == 4, "v must be (batch, seqlen, heads, d_value), got shape " + shape_str(v_.sizes()));
+    const at::Device dev = v_.device();
+    REQUIRE(kLin, dev.is_cuda(), "tensors must be on a ROCm GPU device (no CPU path)");
+    REQUIRE(kLin, itype_of(v_.scalar_type(), &a.dtype), "unsupported dtype " + dtype_str(v_.scalar_type()));
+    const int64_t B = v_.size(0), L = v_.size(1), H = v_.size(2), V = v_.size(3);
+    REQUIRE(kLin, q_.dim() == 4 && q_.size(0) == B && q_.size(1) == L,
+            "q must be (batch, seqlen, groups, d_key), got shape " + shape_str(q_.sizes()));
+    REQUIRE(kLin, k_.sizes() == q_.sizes(), "k has shape " + shape_str(k_.sizes()) + ", expected " + shape_str(q_.sizes()));
+    const int64_t G = q_.size(2), K = q_.size(3);
+    REQUIRE(kLin, H == 0 || (G > 0 && H % G == 0),
+            "heads " + std::to_string(H) + " is not a multiple of groups " + std::to_string(G));
+    on_device(kLin, "q", q_, dev); on_device(kLin, "k", k_, dev);
+    of_type(kLin, "q", q_, v_.scalar_type()); of_type(kLin, "k", k_, v_.scalar_type());
+    LinIn in{seq_unit(q_), seq_unit(k_), seq_unit(v_), decays(kLin, g_, B, L, H, v_), {}, {}};
+    if (initial) in.initial = state_arg("initial_state", *initial, {B, H, K, V}, dev);
+    if (lengths) {
+        on_device(kLin, "lengths", *lengths, dev);
+        REQUIRE(kLin, same_shape(*lengths, {B}) && (lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong),
+                "lengths must be a (batch,) integer tensor, got " + shape_str(lengths->sizes()) + " " + dtype_str(lengths->scalar_type()));
+        in.lengths = lengths->to(at::kInt).contiguous();
+    }
+    a.batch = B; a.seqlen = L; a.heads = H; a.groups = G; a.d_key = K; a.d_value = V;
+    a.scale = float(scale);
+    a.q_batch_stride = in.q.stride(0); a.q_len_stride = in.q.stride(1); a.q_head_stride = in.q.stride(2);
+    a.k_batch_stride = in.k.stride(0); a.k_len_stride = in.k.stride(1); a.k_head_stride = in.k.stride(2);
+    a.v_batch_stride = in.v.stride(0); a.v_len_stride = in.v.stride(1); a.v_head_stride = in.v.stride(2);
+    a.g_batch_stride = in.g.stride(0); a.g_len_stride = in.g.stride(1); a.g_head_stride = in.g.stride(2);
+    a.q = ptr(in.q); a.k = ptr(in.k); a.v = ptr(in.v); a.g = static_cast<float*>(ptr(in.g));
+    a.initial_state = fptr<float>(in.initial); a.lengths = fptr<int32_t>(in.lengths);
+    return in;
+}
+
+int64_t lin_segs(const ss_linear_attn_args& a) {
+    const int64_t n = ss_linear_attn_segment(&a);
+    if (n < 0) check(SS_ERR_INVALID, kLin);
+    return std::max<int64_t>(1, (a.seqlen + n - 1) / n);
+}
+
+// (out, last_state or None, ends or None, the tensors as read: q, k, v, g, initial_state, lengths)
+py::tuple lin_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
+                  const OptT& lengths, double scale, bool want_last, bool want_ends, int64_t stream) {
+    ss_linear_attn_args a;
+    const LinIn in = fill_linear(a, q, k, v, g, initial, lengths, scale);
+    const Tensor out = at::empty({a.batch, a.seqlen, a.heads, a.d_value}, in.v.options());
+    OptT last, ends, ws;
+    if (want_last) last = f32_like({a.batch, a.heads, a.d_key, a.d_value}, in.v);
+    const int64_t segs = lin_segs(a);
+    if (want_ends) ends = f32_like({a.batch, a.heads, segs, a.d_key, a.d_value}, in.v);
+    a.out_batch_stride = out.stride(0); a.out_len_stride = out.stride(1); a.out_head_stride = out.stride(2);
+    a.out = ptr(out); a.last_state = fptr<float>(last); a.ends = fptr<float>(ends);
+    const int64_t n = ss_linear_attn_fwd_workspace_bytes(&a);
+    if (n < 0) check(SS_ERR_INVALID, kLin);
+    if (n > 0) {
+        ws = bytes_on(n, in.v);
+        a.workspace = ptr(*ws); a.workspace_bytes = n;
+    }
+    launch(in.v.device(), "linear_attn forward", [&] { return ss_linear_attn_fwd(&a, reinterpret_cast<void*>(stream)); });
+    return py::make_tuple(out, last, ends, py::make_tuple(in.q, in.k, in.v, in.g, in.initial, in.lengths));
+}
+
+// (dq, dk, dv, dg fp32, dinitial_state or None)
+py::tuple lin_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
+                  const OptT& lengths, const Tensor& ends, double scale, bool g_per_head, const Tensor& dout_,
+                  const OptT& dlast_, bool want_dinitial, int64_t stream) {
+    ss_linear_attn_bwd_args b{};
+    const LinIn in = fill_linear(b.f, q, k, v, g, initial, lengths, scale);
+    const ss_linear_attn_args& a = b.f;
+    const at::Device dev = in.v.device();
+    REQUIRE(kLin, dout_.sizes() == in.v.sizes() && dout_.scalar_type() == in.v.scalar_type() && dout_.device() == dev,
+            "dout must match v, got " + shape_str(dout_.sizes()) + " " + dtype_str(dout_.scalar_type()));
+    const Tensor dout = seq_unit(dout_);
+    REQUIRE(kLin, same_shape(ends, {a.batch, a.heads, lin_segs(a), a.d_key, a.d_value}) && ends.is_contiguous() &&
+                      ends.scalar_type() == at::kFloat && ends.device() == dev,
+            "ends does not come from the forward");
+    OptT dlast, dinitial, ws;
+    if (dlast_) dlast = state_arg("dlast_state", *dlast_, {a.batch, a.heads, a.d_key, a.d_value}, dev);
+    if (want_dinitial) dinitial = f32_like({a.batch, a.heads, a.d_key, a.d_value}, in.v);
+    const Tensor dq = at::empty(in.q.sizes(), in.q.options()), dk = at::empty(in.q.sizes(), in.q.options()),
+                 dv = at::empty(in.v.sizes(), in.v.options());
+    const Tensor dg = g_per_head ? f32_like({a.heads}, in.v) : f32_like({a.batch, a.seqlen, a.heads}, in.v);
+    if (a.batch == 0) dg.zero_();
+    b.f.ends = static_cast<float*>(ptr(ends));
+    b.dout_batch_stride = dout.stride(0); b.dout_len_stride = dout.stride(1); b.dout_head_stride = dout.stride(2);
+    b.dout = ptr(dout); b.dlast_state = fptr<float>(dlast);
+    b.dq = ptr(dq); b.dk = ptr(dk); b.dv = ptr(dv); b.dg = static_cast<float*>(ptr(dg));
+    b.dinitial_state = fptr<float>(dinitial);
+    b.g_per_head = g_per_head;
+    if (a.batch > 0 && a.heads > 0) {
+        // (an empty tensor has no address; the library asks for one)
+        if (!b.dg) b.dg = b.f.ends;
+        const int64_t n = ss_linear_attn_bwd_workspace_bytes(&b);
+        if (n < 0) check(SS_ERR_INVALID, kLin);
+        if (n > 0) {
+            ws = bytes_on(n, in.v);
+            b.f.workspace = ptr(*ws); b.f.workspace_bytes = n;
+        }
+        launch(dev, "linear_attn backward", [&] { return ss_linear_attn_bwd(&b, reinterpret_cast<void*>(stream)); });
+    }
+    return py::make_tuple(dq, dk, dv, dg, dinitial);
+}
+
+constexpr const char* kLinUp = "linear_attn_update";
+
+Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, double scale,
+                  OptT out, int64_t stream) {
+    REQUIRE(kLinUp, v_.dim() == 3 && v_.is_cuda(), "v must be (batch, heads, d_value) on a ROCm GPU device (no CPU path)");
+    ss_linear_attn_update_args a{};
+    REQUIRE(kLinUp, itype_of(v_.scalar_type(), &a.dtype), "unsupported dtype " + dtype_str(v_.scalar_type()));
+    const at::Device dev = v_.device();
+    const int64_t B = v_.size(0), H = v_.size(1), V = v_.size(2);
+    REQUIRE(kLinUp, q_.dim() == 3 && q_.size(0) == B, "q must be (batch, groups, d_key), got shape " + shape_str(q_.sizes()));
+    REQUIRE(kLinUp, k_.sizes() == q_.sizes(), "k has shape " + shape_str(k_.sizes()) + ", expected " + shape_str(q_.sizes()));
+    const int64_t G = q_.size(1), K = q_.size(2);
+    REQUIRE(kLinUp, H == 0 || (G > 0 && H % G == 0),
+            "heads " + std::to_string(H) + " is not a multiple of groups " + std::to_string(G));
+    on_device(kLinUp, "q", q_, dev); on_device(kLinUp, "k", k_, dev); on_device(kLinUp, "state", state, dev);
+    of_type(kLinUp, "q", q_, v_.scalar_type()); of_type(kLinUp, "k", k_, v_.scalar_type());
+    of_type(kLinUp, "state", state, at::kFloat);
+    REQUIRE(kLinUp, same_shape(state, {B, H, K, V}),
+            "state has shape " + shape_str(state.sizes()) + ", expected " + shape_str({B, H, K, V}));
+    REQUIRE(kLinUp, state.numel() == 0 || ((V <= 1 || state.stride(3) == 1) && (K <= 1 || state.stride(2) == V)),
+            "state must be contiguous along its last two dims (it is updated in place)");
+    const Tensor q = seq_unit(q_), k = seq_unit(k_), v = seq_unit(v_), g = decays(kLinUp, g_, B, -1, H, v_);
+    if (out)
+        REQUIRE(kLinUp, out->sizes() == v.sizes() && out->scalar_type() == v.scalar_type() && out->device() == dev && unit(*out),
+                "out must match v, with unit stride along the last dim");
+    else out = at::empty({B, H, V}, v.options());
+    a.batch = B; a.heads = H; a.groups = G; a.d_key = K; a.d_value = V;
+    a.scale = float(scale);
+    a.state_batch_stride = state.stride(0); a.state_head_stride = state.stride(1);
+    a.q_batch_stride = q.stride(0); a.q_head_stride = q.stride(1);
+    a.k_batch_stride = k.stride(0); a.k_head_stride = k.stride(1);
+    a.v_batch_stride = v.stride(0); a.v_head_stride = v.stride(1);
+    a.out_batch_stride = out->stride(0); a.out_head_stride = out->stride(1);
+    a.g_batch_stride = g.stride(0); a.g_head_stride = g.stride(1);
+    a.state = static_cast<float*>(ptr(state)); a.q = ptr(q); a.k = ptr(k); a.v = ptr(v);
+    a.g = static_cast<float*>(ptr(g)); a.out = ptr(*out);
+    launch(dev, kLinUp, [&] { return ss_linear_attn_update(&a, reinterpret_cast<void*>(stream)); });
+    return *out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(mamba_host, m) {
@@ -654,5 +831,8 @@ PYBIND11_MODULE(mamba_host, m) {
     m.def("linear_ws_bytes", &linear_ws_bytes);
     m.def("linear", &linear);
     m.def("state_update", &state_update);
+    m.def("lin_fwd", &lin_fwd);
+    m.def("lin_bwd", &lin_bwd);
+    m.def("lin_update", &lin_update);
     m.def("abi", [] { return py::make_tuple(SS_ABI_VERSION, sizeof(ss_fwd_args), sizeof(ss_bwd_args)); });
 }

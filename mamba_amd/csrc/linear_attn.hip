@@ -1,0 +1,450 @@
+// Linear attention with a decay for each head, on gfx950: the token-by-token
+// form, and the kernels that finish the backward.
+//
+// A pass (LaJob) walks the recurrence of linear_attn.hpp.  The backward is
+// three passes, then the decay's gradient.  With D_s = q_s . dq_s - k_s . dk_s
+// and M_ij the share of token j in the output at i (times its gradient),
+// D_s is row s of M less column s, and
+//   dg_t = sum of M_ij over i >= t > j
+//        = <S_e, dS_e> + sum of D_s over t <= s < e
+// for any e >= t: S_e the state before token e, dS_e the gradient arriving at
+// it from token e on.  e is the end of t's segment, so the sum, which cancels,
+// runs over one segment and not the whole row.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "linear_attn.hpp"
+#include "ss_device.hpp"
+#include "ss_kernels.hpp"
+
+namespace ss {
+
+namespace {
+
+constexpr int kVTile = 64;           // value columns per workgroup
+constexpr int kBatchTok = 16;        // tokens staged at a time
+
+__device__ __forceinline__ int64_t row_len(const int32_t* lens, int64_t b, int64_t L) {
+    if (!lens) return L;
+    const int64_t n = lens[b];
+    return n < 0 ? 0 : n < L ? n : L;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const LaRows& r, int64_t b, int64_t t, int64_t h) {
+    return static_cast<const T*>(r.p) + b * r.b + t * r.l + (h / r.rep) * r.h;
+}
+
+// One workgroup per (batch, head) and 64 value columns; thread (i, n) holds
+// rows i * KD / 4 .. of column n of the state.
+template <typename T, int KD>
+__global__ __launch_bounds__(256) void la_recurrent(const LaParams p) {
+    const LaJob& J = p.job[blockIdx.z];
+    const int64_t bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
+    const int n0 = int(blockIdx.y) * kVTile;
+    if (n0 >= J.V) return;
+    constexpr int R = KD / 4;
+    __shared__ float qs[kBatchTok][KD], ks[kBatchTok][KD], red[4][kVTile];
+    const int col = threadIdx.x & 63, part = threadIdx.x >> 6, n = n0 + col;
+    const int64_t len = row_len(p.lens, b, p.L);
+    const int64_t KV = int64_t(J.K) * J.V;
+
+    float S[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int d = part * R + i;
+        S[i] = J.in && d < J.K && n < J.V ? J.in[bh * KV + int64_t(d) * J.st_k + int64_t(n) * J.st_v] : 0.f;
+    }
+    auto write_state = [&](float* to) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int d = part * R + i;
+            if (d < J.K && n < J.V) to[int64_t(d) * J.st_k + int64_t(n) * J.st_v] = S[i];
+        }
+    };
+    for (int si = 0; si < p.segs; ++si) {
+        const int seg = J.rev ? p.segs - 1 - si : si;
+        const int64_t s0 = seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
+        for (int64_t done = 0; done < s1 - s0; done += kBatchTok) {
+            const int cnt = int(s1 - s0 - done < kBatchTok ? s1 - s0 - done : kBatchTok);
+            __syncthreads();
+            for (int i = threadIdx.x; i < kBatchTok * KD; i += 256) {
+                const int u = i / KD, d = i % KD;
+                const int64_t t = J.rev ? s1 - 1 - done - u : s0 + done + u;
+                const bool in = u < cnt && d < J.K && t < len;
+                qs[u][d] = in ? io<T>::load(row_ptr<T>(J.q, b, t, h) + d) : 0.f;
+                ks[u][d] = in ? io<T>::load(row_ptr<T>(J.k, b, t, h) + d) : 0.f;
+            }
+            __syncthreads();
+            for (int u = 0; u < cnt; ++u) {
+                const int64_t t = J.rev ? s1 - 1 - done - u : s0 + done + u;
+                const bool live = t < len;
+                const float a = live ? expf(p.g[b * p.g_b + t * p.g_l + h * p.g_h]) : 1.f;
+                const float v = live && n < J.V ? J.vscale * io<T>::load(row_ptr<T>(J.v, b, t, h) + n) : 0.f;
+                float acc = 0.f;
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    if (!J.rev) S[i] *= a;
+                    S[i] = __builtin_fmaf(ks[u][part * R + i], v, S[i]);
+                    acc = __builtin_fmaf(qs[u][part * R + i], S[i], acc);
+                    if (J.rev) S[i] *= a;
+                }
+                red[part][col] = acc;
+                __syncthreads();
+                if (part == 0) {
+                    const float o = live ? J.oscale * ((red[0][col] + red[1][col]) + (red[2][col] + red[3][col])) : 0.f;
+                    if (n < J.V) {
+                        const int64_t at = b * J.o.b + t * J.o.l + h * J.o.h + n;
+                        if (J.o_f32) static_cast<float*>(const_cast<void*>(J.o.p))[at] = o;
+                        else io<T>::store(static_cast<T*>(const_cast<void*>(J.o.p)) + at, o);
+                    }
+                    if (J.dot) {
+                        const float x = live && n < J.V ? io<T>::load(row_ptr<T>(J.x, b, t, h) + n) : 0.f;
+                        const float s = wave_allsum(o * x);
+                        if (col == 0) J.dot[(int64_t(blockIdx.y) * p.B * p.H + bh) * p.L + t] = s;
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        if (J.ends) write_state(J.ends + (bh * p.segs + seg) * KV);
+    }
+    if (J.out_state) write_state(J.out_state + bh * KV);
+}
+
+// dg of one segment: the inner product of the two states at its end, and the
+// sums of D from its last token down.  256 threads, up to 4 tokens each.
+constexpr int kDgTok = 4;
+
+__global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
+    const int64_t bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
+    const int seg = int(blockIdx.y), tid = int(threadIdx.x);
+    const int64_t s0 = seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
+    const int64_t len = row_len(p.lens, b, p.L);
+    __shared__ double red[256];
+
+    double f = 0.0;
+    const float* dS = seg + 1 < p.segs ? p.rends + (bh * p.segs + seg + 1) * int64_t(p.KV)
+                                       : p.dlast ? p.dlast + bh * int64_t(p.KV) : nullptr;
+    if (dS) {
+        const float* S = p.ends + (bh * p.segs + seg) * int64_t(p.KV);
+        for (int i = tid; i < p.KV; i += 256) f += double(S[i]) * double(dS[i]);
+    }
+    red[tid] = f;
+    __syncthreads();
+    for (int m = 128; m >= 1; m >>= 1) {
+        if (tid < m) red[tid] += red[tid + m];
+        __syncthreads();
+    }
+    const double F = red[0];
+    __syncthreads();
+
+    // this thread's tokens, from the segment's end down
+    double d[kDgTok], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kDgTok; ++i) {
+        const int64_t t = s1 - 1 - (int64_t(tid) * kDgTok + i);
+        double v = 0.0;
+        if (t >= s0 && t < len) {
+            for (int q = 0; q < p.qtiles; ++q) v += p.dotq[(int64_t(q) * p.B * p.H + bh) * p.L + t];
+            for (int k = 0; k < p.ktiles; ++k) v -= p.dotk[(int64_t(k) * p.B * p.H + bh) * p.L + t];
+        }
+        sum += v;
+        d[i] = sum;
+    }
+    red[tid] = sum;
+    __syncthreads();
+    for (int m = 1; m < 256; m <<= 1) {                 // sums over the threads up to this one
+        const double o = tid >= m ? red[tid - m] : 0.0;
+        __syncthreads();
+        red[tid] += o;
+        __syncthreads();
+    }
+    const double base = F + (tid ? red[tid - 1] : 0.0);
+    __syncthreads();
+    double mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < kDgTok; ++i) {
+        const int64_t t = s1 - 1 - (int64_t(tid) * kDgTok + i);
+        if (t >= s0) {
+            const double v = t < len ? base + d[i] : 0.0;
+            if (p.dg) p.dg[(b * p.L + t) * p.H + h] = float(v);
+            mine += v;
+        }
+    }
+    if (!p.part) return;
+    red[tid] = mine;
+    __syncthreads();
+    for (int m = 128; m >= 1; m >>= 1) {
+        if (tid < m) red[tid] += red[tid + m];
+        __syncthreads();
+    }
+    if (tid == 0) p.part[bh * p.segs + seg] = red[0];
+}
+
+// dg of a head with one decay: the sum over batch rows and segments
+__global__ __launch_bounds__(256) void la_decay_grad_heads(const double* part, float* dg, int64_t B, int64_t H, int segs) {
+    const int64_t h = blockIdx.x;
+    __shared__ double red[256];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < B * segs; i += 256) s += part[((i / segs) * H + h) * segs + i % segs];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int m = 128; m >= 1; m >>= 1) {
+        if (int(threadIdx.x) < m) red[threadIdx.x] += red[threadIdx.x + m];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) dg[h] = float(red[0]);
+}
+
+// The heads of a group share q and k: out[r, j, :] = sum over i of part[r, j * rep + i, :]
+template <typename T>
+__global__ __launch_bounds__(256) void la_group_sum(const float* part0, T* out0, const float* part1, T* out1, int64_t n,
+                                                    int rep, int dim) {
+    const float* part = blockIdx.y ? part1 : part0;
+    T* out = blockIdx.y ? out1 : out0;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        const int64_t g = i / dim, c = i % dim;
+        float s = 0.f;
+        for (int r = 0; r < rep; ++r) s += part[(g * rep + r) * dim + c];
+        io<T>::store(out + i, s);
+    }
+}
+
+template <typename T>
+hipError_t launch_walk(const LaParams& p, hipStream_t stream) {
+    int kmax = 0, vmax = 0;
+    for (int j = 0; j < p.njobs; ++j) {
+        kmax = p.job[j].K > kmax ? p.job[j].K : kmax;
+        vmax = p.job[j].V > vmax ? p.job[j].V : vmax;
+    }
+    const dim3 grid(unsigned(p.B * p.H), unsigned((vmax + kVTile - 1) / kVTile), unsigned(p.njobs));
+    if (kmax <= 64) hipLaunchKernelGGL((la_recurrent<T, 64>), grid, dim3(256), 0, stream, p);
+    else if (kmax <= 128) hipLaunchKernelGGL((la_recurrent<T, 128>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((la_recurrent<T, 256>), grid, dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t vtiles(int64_t v) { return (v + kVTile - 1) / kVTile; }
+
+struct BwdSpace { int64_t dotq, dotk, rends, part, dq, dk, bytes; };
+BwdSpace bwd_space(const ss_linear_attn_bwd_args* g) {
+    const ss_linear_attn_args& a = g->f;
+    const int64_t bh = a.batch * a.heads, segs = linear_attn_segs(&a);
+    BwdSpace s{};
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) { const int64_t r = at; at += round16(bytes); return r; };
+    s.dotq = take(vtiles(a.d_key) * bh * a.seqlen * 4);
+    s.dotk = take(vtiles(a.d_key) * bh * a.seqlen * 4);
+    s.rends = take(bh * segs * a.d_key * a.d_value * 4);
+    s.part = take(g->g_per_head ? bh * segs * 8 : 0);
+    const int64_t shared = a.heads > a.groups ? a.batch * a.seqlen * a.heads * a.d_key * 4 : 0;
+    s.dq = take(shared);
+    s.dk = take(shared);
+    s.bytes = at;
+    return s;
+}
+
+LaParams common(const ss_linear_attn_args& a) {
+    LaParams p{};
+    p.B = a.batch; p.L = a.seqlen; p.H = a.heads;
+    p.g = a.g; p.g_b = a.g_batch_stride; p.g_l = a.g_len_stride; p.g_h = a.g_head_stride;
+    p.lens = a.lengths;
+    p.seg_tokens = linear_attn_segment(&a);
+    p.segs = int(linear_attn_segs(&a));
+    return p;
+}
+
+hipError_t walk(int dtype, const LaParams& p, hipStream_t stream) {
+    switch (dtype) {
+        case SS_F32: return launch_walk<float>(p, stream);
+        case SS_BF16: return launch_walk<bf16_t>(p, stream);
+        default: return launch_walk<_Float16>(p, stream);
+    }
+}
+
+}  // namespace
+
+int64_t linear_attn_segment(const ss_linear_attn_args*) { return 256; }
+int64_t linear_attn_segs(const ss_linear_attn_args* a) {
+    const int64_t n = linear_attn_segment(a);
+    return a->seqlen <= n ? 1 : (a->seqlen + n - 1) / n;
+}
+int64_t linear_attn_fwd_space(const ss_linear_attn_args*) { return 0; }
+int64_t linear_attn_bwd_space(const ss_linear_attn_bwd_args* g) { return bwd_space(g).bytes; }
+
+hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stream) {
+    LaParams p = common(*a);
+    const int rep = int(a->heads / a->groups);
+    p.njobs = 1;
+    LaJob& j = p.job[0];
+    j.q = {a->q, a->q_batch_stride, a->q_len_stride, a->q_head_stride, rep};
+    j.k = {a->k, a->k_batch_stride, a->k_len_stride, a->k_head_stride, rep};
+    j.v = {a->v, a->v_batch_stride, a->v_len_stride, a->v_head_stride, 1};
+    j.o = {a->out, a->out_batch_stride, a->out_len_stride, a->out_head_stride, 1};
+    j.K = int(a->d_key); j.V = int(a->d_value);
+    j.oscale = a->scale; j.vscale = 1.f;
+    j.st_k = j.V; j.st_v = 1;
+    j.in = a->initial_state; j.ends = a->ends; j.out_state = a->last_state;
+    return walk(a->dtype, p, stream);
+}
+
+hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t stream) {
+    const ss_linear_attn_args& a = g->f;
+    const BwdSpace sp = bwd_space(g);
+    char* ws = static_cast<char*>(a.workspace);
+    const int rep = int(a.heads / a.groups), K = int(a.d_key), V = int(a.d_value);
+    LaParams p = common(a);
+    const LaRows q{a.q, a.q_batch_stride, a.q_len_stride, a.q_head_stride, rep};
+    const LaRows k{a.k, a.k_batch_stride, a.k_len_stride, a.k_head_stride, rep};
+    const LaRows v{a.v, a.v_batch_stride, a.v_len_stride, a.v_head_stride, 1};
+    const LaRows dout{g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1};
+    const auto grad = [&](void* p, int dim) {           // contiguous (batch, seqlen, heads, dim)
+        return LaRows{p, a.seqlen * a.heads * dim, a.heads * dim, dim, 1};
+    };
+    const bool part = rep > 1;
+    float* rends = reinterpret_cast<float*>(ws + sp.rends);
+    p.njobs = 3;
+    LaJob& jq = p.job[0];
+    jq.q = dout; jq.k = v; jq.v = k; jq.x = q;
+    jq.o = grad(part ? ws + sp.dq : g->dq, K);
+    jq.o_f32 = part;
+    jq.K = V; jq.V = K;
+    jq.oscale = a.scale; jq.vscale = 1.f;
+    jq.st_k = 1; jq.st_v = V;
+    jq.in = a.initial_state;
+    jq.dot = reinterpret_cast<float*>(ws + sp.dotq);
+    LaJob& jk = p.job[1];
+    jk.q = v; jk.k = dout; jk.v = q; jk.x = k;
+    jk.o = grad(part ? ws + sp.dk : g->dk, K);
+    jk.o_f32 = part;
+    jk.K = V; jk.V = K; jk.rev = 1;
+    jk.oscale = 1.f; jk.vscale = a.scale;
+    jk.st_k = 1; jk.st_v = V;
+    jk.in = g->dlast_state;
+    jk.dot = reinterpret_cast<float*>(ws + sp.dotk);
+    LaJob& jv = p.job[2];
+    jv.q = k; jv.k = q; jv.v = dout;
+    jv.o = grad(g->dv, V);
+    jv.K = K; jv.V = V; jv.rev = 1;
+    jv.oscale = 1.f; jv.vscale = a.scale;
+    jv.st_k = V; jv.st_v = 1;
+    jv.in = g->dlast_state; jv.ends = rends; jv.out_state = g->dinitial_state;
+    hipError_t e = walk(a.dtype, p, stream);
+    if (e != hipSuccess) return e;
+
+    LaDgParams d{};
+    d.B = a.batch; d.L = a.seqlen; d.H = a.heads;
+    d.lens = a.lengths; d.seg_tokens = p.seg_tokens; d.segs = p.segs;
+    d.qtiles = d.ktiles = int(vtiles(K));
+    d.KV = K * V;
+    d.dotq = jq.dot; d.dotk = jk.dot; d.ends = a.ends; d.rends = rends; d.dlast = g->dlast_state;
+    d.dg = g->g_per_head ? nullptr : g->dg;
+    d.part = g->g_per_head ? reinterpret_cast<double*>(ws + sp.part) : nullptr;
+    hipLaunchKernelGGL(la_decay_grad, dim3(unsigned(a.batch * a.heads), unsigned(p.segs)), dim3(256), 0, stream, d);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (g->g_per_head) {
+        hipLaunchKernelGGL(la_decay_grad_heads, dim3(unsigned(a.heads)), dim3(256), 0, stream, d.part, g->dg, a.batch,
+                           a.heads, p.segs);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (part && a.seqlen > 0) {
+        const int64_t n = a.batch * a.seqlen * a.groups * K;
+        const int64_t want = (n + 255) / 256;
+        const dim3 grid(unsigned(want < 65536 ? want : 65536), 2);
+        const float* pq = reinterpret_cast<const float*>(ws + sp.dq);
+        const float* pk = reinterpret_cast<const float*>(ws + sp.dk);
+        const auto sum = [&](auto* dq, auto* dk) {
+            using T = std::remove_pointer_t<decltype(dq)>;
+            hipLaunchKernelGGL((la_group_sum<T>), grid, dim3(256), 0, stream, pq, dq, pk, dk, n, rep, K);
+        };
+        if (a.dtype == SS_F32) sum(static_cast<float*>(g->dq), static_cast<float*>(g->dk));
+        else if (a.dtype == SS_BF16) sum(static_cast<bf16_t*>(g->dq), static_cast<bf16_t*>(g->dk));
+        else sum(static_cast<_Float16*>(g->dq), static_cast<_Float16*>(g->dk));
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+namespace {
+
+// One token.  A workgroup owns kUpCols value columns of one (batch, head):
+// thread (i, c) holds 4 neighbouring columns of rows i, i + rows ... and reads
+// and writes them as 16-byte vectors (element by element where the rows are
+// not 16-byte aligned); the outputs' sums over the rows meet in LDS.
+template <typename T, int COLS, bool VEC>
+__global__ __launch_bounds__(256) void la_update(const ss_linear_attn_update_args a) {
+    constexpr int C = VEC ? COLS / 4 : COLS, RG = 256 / C, W = VEC ? 4 : 1;
+    const int64_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads, j = h / (a.heads / a.groups);
+    const int c = int(threadIdx.x) % C, rg = int(threadIdx.x) / C;
+    const int n = int(blockIdx.y) * COLS + c * W;
+    const int K = int(a.d_key), V = int(a.d_value);
+    __shared__ float qs[256], ks[256], red[RG][COLS];
+    if (int(threadIdx.x) < K) {
+        qs[threadIdx.x] = a.scale * io<T>::load(static_cast<const T*>(a.q) + b * a.q_batch_stride + j * a.q_head_stride + threadIdx.x);
+        ks[threadIdx.x] = io<T>::load(static_cast<const T*>(a.k) + b * a.k_batch_stride + j * a.k_head_stride + threadIdx.x);
+    }
+    const float dec = expf(a.g[b * a.g_batch_stride + h * a.g_head_stride]);
+    float v[W], o[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        v[w] = n + w < V ? io<T>::load(static_cast<const T*>(a.v) + b * a.v_batch_stride + h * a.v_head_stride + n + w) : 0.f;
+        o[w] = 0.f;
+    }
+    __syncthreads();
+    float* S = a.state + b * a.state_batch_stride + h * a.state_head_stride;
+    if (n < V) {
+        for (int d = rg; d < K; d += RG) {
+            float* at = S + int64_t(d) * V + n;
+            float s[W];
+            if constexpr (VEC) {
+                const float4 t = *reinterpret_cast<const float4*>(at);
+                s[0] = t.x; s[1] = t.y; s[2] = t.z; s[3] = t.w;
+            } else {
+                s[0] = *at;
+            }
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                s[w] = __builtin_fmaf(ks[d], v[w], dec * s[w]);
+                o[w] = __builtin_fmaf(qs[d], s[w], o[w]);
+            }
+            if constexpr (VEC) *reinterpret_cast<float4*>(at) = make_float4(s[0], s[1], s[2], s[3]);
+            else *at = s[0];
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) red[rg][c * W + w] = o[w];
+    __syncthreads();
+    if (int(threadIdx.x) < COLS) {
+        const int m = int(blockIdx.y) * COLS + int(threadIdx.x);
+        float t = 0.f;
+        for (int i = 0; i < RG; ++i) t += red[i][threadIdx.x];
+        if (m < V) io<T>::store(static_cast<T*>(a.out) + b * a.out_batch_stride + h * a.out_head_stride + m, t);
+    }
+}
+
+template <typename T>
+hipError_t update_t(const ss_linear_attn_update_args* a, hipStream_t stream) {
+    const bool vec = a->d_value % 4 == 0 && a->state_batch_stride % 4 == 0 && a->state_head_stride % 4 == 0 &&
+                     (reinterpret_cast<uintptr_t>(a->state) & 15) == 0;
+    const unsigned bh = unsigned(a->batch * a->heads), V = unsigned(a->d_value);
+    if (vec) hipLaunchKernelGGL((la_update<T, 64, true>), dim3(bh, (V + 63) / 64), dim3(256), 0, stream, *a);
+    else hipLaunchKernelGGL((la_update<T, 64, false>), dim3(bh, (V + 63) / 64), dim3(256), 0, stream, *a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t linear_attn_update_launch(const ss_linear_attn_update_args* a, hipStream_t stream) {
+    switch (a->dtype) {
+        case SS_F32: return update_t<float>(a, stream);
+        case SS_BF16: return update_t<bf16_t>(a, stream);
+        default: return update_t<_Float16>(a, stream);
+    }
+}
+
+}  // namespace ss

@@ -1,0 +1,67 @@
+// Linear attention with a decay for each head: what its host and device
+// sides share.
+#pragma once
+#include <cstdint>
+
+#include "../../include/mamba_ss.h"
+
+namespace ss {
+
+// rows of a (batch, len, head, dim) tensor: strides in elements, unit along dim
+struct LaRows {
+    const void* p;
+    int64_t b, l, h;
+    int rep;              // heads per row head: head index is h / rep
+};
+
+// One pass of the recurrence
+//   S_t = exp(g_t) S_{t-1} + k_t (vscale v_t)^T,   o_t = oscale q_t^T S_t
+// in time order, or (rev) from the last token to the first with the decay
+// after the token instead of before it:
+//   R_t = C_t + k_t (vscale v_t)^T,  o_t = oscale q_t^T R_t,  C_{t-1} = exp(g_t) R_t.
+// The forward is one pass; the backward is three, each a linear attention of
+// its own:
+//   dq = pass(q: dout, k: v, v: k), oscale scale, its state S^T
+//   dk = rev (q: v, k: dout, v: q), vscale scale, its state dS^T
+//   dv = rev (q: k, k: q, v: dout), vscale scale, its state dS
+struct LaJob {
+    LaRows q, k, v, o, x;             // x.p: rows for dot, or null
+    int K, V;                         // dims of q, k and of v, o
+    int rev, o_f32;                   // o in fp32 (partials of shared heads) instead of the rows' type
+    float oscale, vscale;
+    // states: fp32, element (i, j) of head (b, h) at ((b * H + h) * segs + s) * K * V + i * st_k + j * st_v
+    int st_k, st_v;
+    const float* in;                  // state before the first token of the walk (segs 1), or null: zero
+    const float* carry;               // with it: state after each segment (in time order); the walk of segment s
+                                      // starts from the one before it in walk order
+    float* ends;                      // written: state after each segment in walk order, or null
+    float* out_state;                 // written: state after the whole walk (segs 1), or null
+    float* dot;                       // written: (V tiles, B, H, L) sums over the tile's columns of o * x, or null
+};
+
+struct LaParams {
+    LaJob job[3];
+    int njobs;
+    int64_t B, L, H;
+    const float* g;
+    int64_t g_b, g_l, g_h;
+    const int32_t* lens;
+    int64_t seg_tokens;
+    int segs;
+};
+
+// dg of the tokens of one segment (see linear_attn.hip)
+struct LaDgParams {
+    int64_t B, L, H;
+    const int32_t* lens;
+    int64_t seg_tokens;
+    int segs, qtiles, ktiles, KV;
+    const float* dotq; const float* dotk;   // (tiles, B, H, L)
+    const float* ends;                      // S after each segment (B, H, segs, K, V)
+    const float* rends;                     // dS after each segment's walk (before it in time), same layout
+    const float* dlast;                     // (B, H, K, V) or null
+    float* dg;                              // (B, L, H), or null with part
+    double* part;                           // (B, H, segs) sums over the segment's tokens, or null
+};
+
+}  // namespace ss

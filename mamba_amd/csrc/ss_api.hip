@@ -1036,4 +1036,131 @@ int ss_rmsnorm_bwd(const ss_rmsnorm_bwd_args* g, void* stream) {
     return ok();
 }
 
+// Checks shared by the linear attention's calls.
+static int check_linear_attn(const ss_linear_attn_args* a, bool bwd) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    const int64_t sizes[] = {a->batch, a->seqlen, a->heads, a->groups};
+    for (int64_t n : sizes)
+        if (n < 0)
+            return fail(SS_ERR_INVALID, "negative size (batch=%lld seqlen=%lld heads=%lld groups=%lld)", (long long)a->batch,
+                        (long long)a->seqlen, (long long)a->heads, (long long)a->groups);
+    if (a->dtype != SS_F32 && a->dtype != SS_BF16 && a->dtype != SS_F16)
+        return fail(SS_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->d_key < 1 || a->d_key > ss::kLinearAttnMaxDim || a->d_value < 1 || a->d_value > ss::kLinearAttnMaxDim)
+        return fail(SS_ERR_UNSUPPORTED, "d_key=%lld, d_value=%lld outside [1, %lld]", (long long)a->d_key,
+                    (long long)a->d_value, (long long)ss::kLinearAttnMaxDim);
+    if (a->heads > 0 && (a->groups < 1 || a->heads % a->groups != 0))
+        return fail(SS_ERR_INVALID, "heads=%lld is not a multiple of groups=%lld", (long long)a->heads, (long long)a->groups);
+    // (token, head and column offsets of one workgroup's loop stay far below 2^63; the grid is batch x heads)
+    if (a->batch > 0 && a->heads > INT32_MAX / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
+    if (a->seqlen > (int64_t(1) << 24)) return fail(SS_ERR_UNSUPPORTED, "seqlen=%lld above 2^24", (long long)a->seqlen);
+    const int64_t st[] = {a->q_batch_stride, a->q_len_stride, a->q_head_stride, a->k_batch_stride, a->k_len_stride,
+                          a->k_head_stride, a->v_batch_stride, a->v_len_stride, a->v_head_stride, a->g_batch_stride,
+                          a->g_len_stride, a->g_head_stride};
+    for (int64_t v : st)
+        if (v < 0) return fail(SS_ERR_INVALID, "negative stride");
+    if (a->batch == 0 || a->heads == 0) return ok();
+    const size_t es = elem_size(a->dtype);
+    if (a->seqlen > 0) {
+        if (!a->q || !a->k || !a->v || !a->g) return fail(SS_ERR_INVALID, "q / k / v / g is NULL");
+        if (!aligned(a->q, es) || !aligned(a->k, es) || !aligned(a->v, es) || !aligned(a->g, 4))
+            return fail(SS_ERR_INVALID, "q / k / v / g is misaligned");
+    }
+    if (!aligned(a->initial_state, 4) || !aligned(a->lengths, 4) || !aligned(a->ends, 4))
+        return fail(SS_ERR_INVALID, "initial_state / lengths / ends is misaligned");
+    if (!bwd) {
+        if (a->out_batch_stride < 0 || a->out_len_stride < 0 || a->out_head_stride < 0)
+            return fail(SS_ERR_INVALID, "negative stride");
+        if (a->seqlen > 0 && !a->out) return fail(SS_ERR_INVALID, "out is NULL");
+        if (!aligned(a->out, es) || !aligned(a->last_state, 4))
+            return fail(SS_ERR_INVALID, "out / last_state is misaligned");
+    }
+    return ok();
+}
+
+static int check_linear_attn_bwd(const ss_linear_attn_bwd_args* g) {
+    const int rc = check_linear_attn(g ? &g->f : nullptr, true);
+    if (rc != SS_OK || g->f.batch == 0 || g->f.heads == 0) return rc;
+    if (g->dout_batch_stride < 0 || g->dout_len_stride < 0 || g->dout_head_stride < 0)
+        return fail(SS_ERR_INVALID, "negative stride");
+    if (!g->dg || (g->f.seqlen > 0 && (!g->dout || !g->dq || !g->dk || !g->dv)))
+        return fail(SS_ERR_INVALID, "dout / dq / dk / dv / dg is NULL");
+    if (!g->f.ends) return fail(SS_ERR_INVALID, "ends (the forward's states) is NULL");
+    const size_t es = elem_size(g->f.dtype);
+    if (!aligned(g->dout, es) || !aligned(g->dq, es) || !aligned(g->dk, es) || !aligned(g->dv, es) ||
+        !aligned(g->dg, 4) || !aligned(g->dlast_state, 4) || !aligned(g->dinitial_state, 4))
+        return fail(SS_ERR_INVALID, "a gradient is misaligned");
+    return ok();
+}
+
+static int check_space(const void* workspace, int64_t bytes, int64_t need) {
+    if (need > 0 && (!workspace || bytes < need))
+        return fail(SS_ERR_INVALID, "workspace of %lld bytes needed (got %lld)", (long long)need,
+                    (long long)(workspace ? bytes : 0));
+    if (workspace && !aligned(workspace, 16)) return fail(SS_ERR_INVALID, "workspace must be 16-byte aligned");
+    return SS_OK;
+}
+
+int64_t ss_linear_attn_segment(const ss_linear_attn_args* a) {
+    return check_linear_attn(a, true) == SS_OK ? ss::linear_attn_segment(a) : -1;
+}
+
+int64_t ss_linear_attn_fwd_workspace_bytes(const ss_linear_attn_args* a) {
+    return check_linear_attn(a, false) == SS_OK ? ss::linear_attn_fwd_space(a) : -1;
+}
+
+int64_t ss_linear_attn_bwd_workspace_bytes(const ss_linear_attn_bwd_args* g) {
+    return check_linear_attn_bwd(g) == SS_OK ? ss::linear_attn_bwd_space(g) : -1;
+}
+
+int ss_linear_attn_fwd(const ss_linear_attn_args* a, void* stream) {
+    int rc = check_linear_attn(a, false);
+    if (rc != SS_OK || a->batch == 0 || a->heads == 0) return rc;
+    rc = check_space(a->workspace, a->workspace_bytes, ss::linear_attn_fwd_space(a));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::linear_attn_fwd_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "linear attention forward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_linear_attn_bwd(const ss_linear_attn_bwd_args* g, void* stream) {
+    int rc = check_linear_attn_bwd(g);
+    if (rc != SS_OK || g->f.batch == 0 || g->f.heads == 0) return rc;
+    rc = check_space(g->f.workspace, g->f.workspace_bytes, ss::linear_attn_bwd_space(g));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::linear_attn_bwd_launch(g, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "linear attention backward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    if (a->batch < 0 || a->heads < 0 || a->groups < 0)
+        return fail(SS_ERR_INVALID, "negative size (batch=%lld heads=%lld groups=%lld)", (long long)a->batch,
+                    (long long)a->heads, (long long)a->groups);
+    if (a->dtype != SS_F32 && a->dtype != SS_BF16 && a->dtype != SS_F16)
+        return fail(SS_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->d_key < 1 || a->d_key > ss::kLinearAttnMaxDim || a->d_value < 1 || a->d_value > ss::kLinearAttnMaxDim)
+        return fail(SS_ERR_UNSUPPORTED, "d_key=%lld, d_value=%lld outside [1, %lld]", (long long)a->d_key,
+                    (long long)a->d_value, (long long)ss::kLinearAttnMaxDim);
+    if (a->heads > 0 && (a->groups < 1 || a->heads % a->groups != 0))
+        return fail(SS_ERR_INVALID, "heads=%lld is not a multiple of groups=%lld", (long long)a->heads, (long long)a->groups);
+    if (a->batch > 0 && a->heads > INT32_MAX / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
+    const int64_t st[] = {a->state_batch_stride, a->state_head_stride, a->q_batch_stride, a->q_head_stride, a->k_batch_stride,
+                          a->k_head_stride, a->v_batch_stride, a->v_head_stride, a->out_batch_stride, a->out_head_stride,
+                          a->g_batch_stride, a->g_head_stride};
+    for (int64_t v : st)
+        if (v < 0) return fail(SS_ERR_INVALID, "negative stride");
+    if (a->batch == 0 || a->heads == 0) return ok();
+    if (!a->state || !a->q || !a->k || !a->v || !a->g || !a->out)
+        return fail(SS_ERR_INVALID, "state / q / k / v / g / out is NULL");
+    const size_t es = elem_size(a->dtype);
+    if (!aligned(a->state, 4) || !aligned(a->g, 4) || !aligned(a->q, es) || !aligned(a->k, es) || !aligned(a->v, es) ||
+        !aligned(a->out, es))
+        return fail(SS_ERR_INVALID, "state / q / k / v / g / out is misaligned");
+    const hipError_t e = ss::linear_attn_update_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "linear attention update launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
 }  // extern "C"

@@ -225,6 +225,16 @@ int64_t rmsnorm_bwd_parts(int64_t rows);
 constexpr int64_t kRmsNormMaxParts = 512;
 // the backward keeps one fp32 column sum per element of a row in LDS
 constexpr int64_t kRmsNormMaxBwdDim = 16384;
+// linear attention with a decay for each head (linear_attn.hip): tokens per
+// segment, segments (at least 1), workspace bytes, launches
+int64_t linear_attn_segment(const ss_linear_attn_args* a);
+int64_t linear_attn_segs(const ss_linear_attn_args* a);
+int64_t linear_attn_fwd_space(const ss_linear_attn_args* a);
+int64_t linear_attn_bwd_space(const ss_linear_attn_bwd_args* g);
+hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stream);
+hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t stream);
+hipError_t linear_attn_update_launch(const ss_linear_attn_update_args* a, hipStream_t stream);
+constexpr int64_t kLinearAttnMaxDim = 256;
 // base name of the kernel template launch_fwd / launch_bwd picks for p
 const char* fwd_kernel_name(const FwdParams& p);
 const char* bwd_kernel_name(const BwdParams& p, int itype, bool sliced);
