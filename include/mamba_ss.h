@@ -573,6 +573,121 @@ typedef struct ss_linear_attn_update_args {
 } ss_linear_attn_update_args;
 int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The norms around a block.  No counterpart in the reference, whose block
+ * has the norm in front only (models/causal_lm.py:30-35).  With rms(v) =
+ * v * rsqrt(mean(v^2) + eps) over a row, in fp32:
+ *   t   = rms(x) * (1 + post) (* silu(gate))
+ *   s   = residual + scale * t              (residual_out, rounded to dtype)
+ *   out = rms(s) * (1 + pre)                (of the unrounded s, rounded to dtype)
+ * scale_vec: a factor per column, or NULL: the number `scale`.  Rows of
+ * `dim` (1 to 16384) elements with unit column stride and free row strides,
+ * element type dtype; post, pre, scale_vec: (dim) contiguous, w_dtype =
+ * dtype or SS_F32.  Outputs must not overlap inputs.
+ * ------------------------------------------------------------------------ */
+typedef struct ss_block_norm_args {
+    int64_t rows, dim;
+    int32_t dtype, w_dtype;              /* enum ss_dtype */
+    float eps, scale;
+    int64_t x_row_stride, residual_row_stride, gate_row_stride, out_row_stride, residual_out_row_stride;
+    const void* x;
+    const void* residual;
+    const void* gate;                    /* may be NULL: no gate */
+    const void* post;
+    const void* pre;
+    const void* scale_vec;               /* may be NULL */
+    void* out;
+    void* residual_out;
+    float* rstd;                         /* fp32 (rows, 2); may be NULL (not written); kept for the backward */
+} ss_block_norm_args;
+
+typedef struct ss_block_norm_bwd_args {
+    int64_t rows, dim;
+    int32_t dtype, w_dtype;
+    float scale;
+    int32_t pad_;
+    int64_t x_row_stride, residual_row_stride, gate_row_stride, dout_row_stride, dresidual_out_row_stride;
+    const void* x;                       /* the forward's inputs */
+    const void* residual;
+    const void* gate;
+    const void* post;
+    const void* pre;
+    const void* scale_vec;
+    const float* rstd;                   /* from the forward */
+    const void* dout;                    /* may be NULL: zero */
+    const void* dresidual_out;           /* may be NULL: zero */
+    void* dx;                            /* (rows, dim) contiguous, dtype */
+    void* dresidual;                     /* the same; may be NULL (not written) */
+    void* dgate;                         /* the same; ignored without gate */
+    void* dpost;                         /* (dim), w_dtype, written (not accumulated); sums of a fixed order */
+    void* dpre;
+    void* dscale;                        /* may be NULL (not written) */
+    void* workspace;                     /* ss_block_norm_bwd_workspace_bytes(rows, dim) bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} ss_block_norm_bwd_args;
+
+int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream);
+int ss_block_norm_bwd(const ss_block_norm_bwd_args* a, void* stream);
+int64_t ss_block_norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+
+/* The gated norm of each head: a row is `groups` groups of dim / groups
+ * elements, each normalised by itself:
+ *   out = rms(x's group) * (1 + weight) * silu(gate)
+ * weight, dweight: (dim), w_dtype = dtype or SS_F32. */
+typedef struct ss_gated_norm_args {
+    int64_t rows, dim, groups;           /* dim 1 to 16384, a multiple of groups */
+    int32_t dtype, w_dtype;
+    float eps;
+    int32_t pad_;
+    int64_t x_row_stride, gate_row_stride, out_row_stride;
+    const void* x;
+    const void* gate;
+    const void* weight;
+    void* out;
+} ss_gated_norm_args;
+
+typedef struct ss_gated_norm_bwd_args {
+    int64_t rows, dim, groups;
+    int32_t dtype, w_dtype;
+    float eps;
+    int32_t pad_;
+    int64_t x_row_stride, gate_row_stride, dout_row_stride;
+    const void* x;
+    const void* gate;
+    const void* weight;
+    const void* dout;
+    void* dx;                            /* (rows, dim) contiguous, dtype */
+    void* dgate;
+    void* dweight;                       /* written (not accumulated), a fixed order of sums */
+    void* workspace;                     /* ss_gated_norm_bwd_workspace_bytes(rows, dim, groups) bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} ss_gated_norm_bwd_args;
+
+int ss_gated_norm_fwd(const ss_gated_norm_args* a, void* stream);
+int ss_gated_norm_bwd(const ss_gated_norm_bwd_args* a, void* stream);
+int64_t ss_gated_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t groups);
+
+/* ------------------------------------------------------------------------
+ * The norm over many gradient tensors, and the gradients clipped to it:
+ *   norm = sqrt(sum g^2),  outs[i] = grads[i] * min(1, max_norm / (norm + eps))
+ * (squares summed in 64 bits, in a fixed order; the product in fp32, rounded
+ * to the tensor's type).  The arrays are host memory, read before the call
+ * returns.  outs[i] may be grads[i]; other overlaps are not allowed.
+ * ------------------------------------------------------------------------ */
+typedef struct ss_clip_grads_args {
+    int64_t count;                       /* tensors */
+    const void* const* grads;            /* count device pointers, elements contiguous */
+    void* const* outs;
+    const int64_t* numels;
+    const int32_t* dtypes;               /* enum ss_dtype of each */
+    float max_norm, eps;
+    float* norm;                         /* written: device, one fp32 */
+    void* workspace;                     /* ss_clip_grads_workspace_bytes() bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} ss_clip_grads_args;
+int ss_clip_grads(const ss_clip_grads_args* a, void* stream);
+int64_t ss_clip_grads_workspace_bytes(const ss_clip_grads_args* a);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,9 @@ EXPORTED = (
     "ss_conv1d_bwd_workspace_bytes", "ss_conv1d_fwd_typed", "ss_conv1d_bwd_typed",
     "ss_linear_attn_segment", "ss_linear_attn_fwd_workspace_bytes", "ss_linear_attn_bwd_workspace_bytes",
     "ss_linear_attn_fwd", "ss_linear_attn_bwd", "ss_linear_attn_update",
+    "ss_block_norm_fwd", "ss_block_norm_bwd", "ss_block_norm_bwd_workspace_bytes",
+    "ss_gated_norm_fwd", "ss_gated_norm_bwd", "ss_gated_norm_bwd_workspace_bytes",
+    "ss_clip_grads", "ss_clip_grads_workspace_bytes",
 )
 
 _i64, _i32, _p = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p
@@ -184,6 +187,41 @@ class LinearAttnUpdateArgs(ctypes.Structure):
     ]
 
 
+class BlockNormArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("dim", _i64), ("dtype", _i32), ("w_dtype", _i32), ("eps", ctypes.c_float),
+                ("scale", ctypes.c_float)] + [
+        (f"{t}_row_stride", _i64) for t in ("x", "residual", "gate", "out", "residual_out")] + [
+        (t, _p) for t in ("x", "residual", "gate", "post", "pre", "scale_vec", "out", "residual_out", "rstd")]
+
+
+class BlockNormBwdArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("dim", _i64), ("dtype", _i32), ("w_dtype", _i32), ("scale", ctypes.c_float),
+                ("pad_", _i32)] + [
+        (f"{t}_row_stride", _i64) for t in ("x", "residual", "gate", "dout", "dresidual_out")] + [
+        (t, _p) for t in ("x", "residual", "gate", "post", "pre", "scale_vec", "rstd", "dout", "dresidual_out", "dx",
+                          "dresidual", "dgate", "dpost", "dpre", "dscale", "workspace")] + [("workspace_bytes", _i64)]
+
+
+class GatedNormArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("dim", _i64), ("groups", _i64), ("dtype", _i32), ("w_dtype", _i32),
+                ("eps", ctypes.c_float), ("pad_", _i32)] + [
+        (f"{t}_row_stride", _i64) for t in ("x", "gate", "out")] + [(t, _p) for t in ("x", "gate", "weight", "out")]
+
+
+class GatedNormBwdArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("dim", _i64), ("groups", _i64), ("dtype", _i32), ("w_dtype", _i32),
+                ("eps", ctypes.c_float), ("pad_", _i32)] + [
+        (f"{t}_row_stride", _i64) for t in ("x", "gate", "dout")] + [
+        (t, _p) for t in ("x", "gate", "weight", "dout", "dx", "dgate", "dweight", "workspace")] + [
+        ("workspace_bytes", _i64)]
+
+
+class ClipGradsArgs(ctypes.Structure):
+    _fields_ = [("count", _i64), ("grads", _p), ("outs", _p), ("numels", _p), ("dtypes", _p),
+                ("max_norm", ctypes.c_float), ("eps", ctypes.c_float), ("norm", _p), ("workspace", _p),
+                ("workspace_bytes", _i64)]
+
+
 _lib = None
 _host = None
 _lock = threading.Lock()
@@ -256,6 +294,17 @@ def load():
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(T), _p]
             fn.restype = ctypes.c_int
+        for name, T in (("ss_block_norm_fwd", BlockNormArgs), ("ss_block_norm_bwd", BlockNormBwdArgs),
+                        ("ss_gated_norm_fwd", GatedNormArgs), ("ss_gated_norm_bwd", GatedNormBwdArgs),
+                        ("ss_clip_grads", ClipGradsArgs)):
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(T), _p]
+            fn.restype = ctypes.c_int
+        lib.ss_block_norm_bwd_workspace_bytes.argtypes = [_i64, _i64]
+        lib.ss_gated_norm_bwd_workspace_bytes.argtypes = [_i64, _i64, _i64]
+        lib.ss_clip_grads_workspace_bytes.argtypes = [ctypes.POINTER(ClipGradsArgs)]
+        for name in ("ss_block_norm_bwd_workspace_bytes", "ss_gated_norm_bwd_workspace_bytes", "ss_clip_grads_workspace_bytes"):
+            getattr(lib, name).restype = _i64
         if lib.ss_abi_version() != ABI_VERSION:
             raise RuntimeError(f"mamba_amd: library ABI {lib.ss_abi_version()} != binding ABI {ABI_VERSION}")
         fs, bs = _i64(), _i64()

@@ -679,7 +679,7 @@ LinIn fill_linear(ss_linear_attn_args& a, const Tensor& q_, const Tensor& k_, co
         on_device(kLin, "lengths", *lengths, dev);
         REQUIRE(kLin, same_shape(*lengths, {B}) && (lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong),
                 "lengths must be a (batch,) integer tensor, got " + shape_str(lengths->sizes()) + " " + dtype_str(lengths->scalar_type()));
-        in.lengths = lengths->to(at::kInt).contiguous();
+        in.lengths = (lengths->scalar_type() == at::kInt ? *lengths : lengths->clamp(0, L).to(at::kInt)).contiguous();
     }
     a.batch = B; a.seqlen = L; a.heads = H; a.groups = G; a.d_key = K; a.d_value = V;
     a.scale = float(scale);
@@ -801,6 +801,189 @@ Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const
     return *out;
 }
 
+// ------------------------------------------------------------ block norms --
+constexpr const char* kBlockNorm = "block_norm";
+constexpr const char* kGatedNorm = "gated_rms_norm";
+
+// as norm_rows, rows of no elements too
+Tensor any_rows(const Tensor& t) {
+    const int64_t dim = t.size(-1);
+    if (dim > 0) return norm_rows(t, dim);
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) rows *= t.size(i);
+    return t.reshape({rows, 0});
+}
+// rows of x's shape and type
+Tensor like_rows(const char* what, const char* name, const Tensor& t, const Tensor& x) {
+    REQUIRE(what, t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(),
+            std::string(name) + " must match x in shape, dtype and device, got " + shape_str(t.sizes()) + " " +
+                dtype_str(t.scalar_type()));
+    return any_rows(t);
+}
+// weights as the library reads them: all of x's type, or all fp32
+struct Weights { std::vector<OptT> w; int32_t dtype; };
+Weights weights_of(const char* what, const Tensor& x, std::initializer_list<std::pair<const char*, const OptT*>> ws) {
+    Weights r{{}, 0};
+    bool same = true;
+    for (const auto& [name, w] : ws) {
+        if (!*w) continue;
+        const Tensor& t = **w;
+        REQUIRE(what, t.dim() == 1 && t.size(0) == x.size(-1),
+                std::string(name) + " must be (" + std::to_string(x.size(-1)) + ",), got " + shape_str(t.sizes()));
+        REQUIRE(what, t.device() == x.device(), std::string(name) + " is on " + t.device().str() + ", x on " + x.device().str());
+        REQUIRE(what, at::isFloatingType(t.scalar_type()), std::string(name) + " must be a float tensor");
+        same = same && t.scalar_type() == x.scalar_type();
+    }
+    const at::ScalarType ty = same ? x.scalar_type() : at::kFloat;
+    for (const auto& [name, w] : ws) r.w.push_back(*w ? OptT((*w)->to(ty).contiguous()) : OptT());
+    itype_of(ty, &r.dtype);
+    return r;
+}
+void norm_x(const char* what, const Tensor& x, int32_t* dtype) {
+    REQUIRE(what, x.is_cuda(), "tensors must be on a ROCm GPU device (no CPU path)");
+    REQUIRE(what, itype_of(x.scalar_type(), dtype), "unsupported dtype " + dtype_str(x.scalar_type()));
+    REQUIRE(what, x.dim() >= 1, "x must have at least one dimension");
+}
+
+// (out, s, rstd or None, the tensors as read: x, residual, gate, post, pre, scale_vec), rows as (rows, dim)
+py::tuple block_norm_fwd(const Tensor& x_, const Tensor& residual_, const OptT& gate_, const Tensor& post, const Tensor& pre,
+                         const OptT& scale_vec, double scale, double eps, bool want_rstd, int64_t stream) {
+    ss_block_norm_args a{};
+    norm_x(kBlockNorm, x_, &a.dtype);
+    const Tensor x = any_rows(x_), residual = like_rows(kBlockNorm, "residual", residual_, x_);
+    const OptT gate = gate_ ? OptT(like_rows(kBlockNorm, "gate", *gate_, x_)) : OptT(), opost = post, opre = pre;
+    const Weights w = weights_of(kBlockNorm, x_, {{"post", &opost}, {"pre", &opre}, {"scale", &scale_vec}});
+    a.w_dtype = w.dtype;
+    a.rows = x.size(0); a.dim = x.size(1);
+    a.eps = float(eps); a.scale = float(scale);
+    const Tensor out = at::empty(x.sizes(), x.options()), s = at::empty(x.sizes(), x.options());
+    OptT rstd;
+    if (want_rstd) rstd = f32_like({a.rows, 2}, x);
+    a.x_row_stride = x.stride(0); a.residual_row_stride = residual.stride(0);
+    if (gate) a.gate_row_stride = gate->stride(0);
+    a.out_row_stride = out.stride(0); a.residual_out_row_stride = s.stride(0);
+    a.x = ptr(x); a.residual = ptr(residual); a.gate = ptr(gate);
+    a.post = ptr(w.w[0]); a.pre = ptr(w.w[1]); a.scale_vec = ptr(w.w[2]);
+    a.out = ptr(out); a.residual_out = ptr(s); a.rstd = fptr<float>(rstd);
+    launch(x.device(), "block_norm forward", [&] { return ss_block_norm_fwd(&a, reinterpret_cast<void*>(stream)); });
+    return py::make_tuple(out, s, rstd, py::make_tuple(x, residual, gate, w.w[0], w.w[1], w.w[2]));
+}
+
+// (dx, dresidual or None, dgate or None, dpost, dpre, dscale or None) from the forward's tensors as read
+py::tuple block_norm_bwd(const Tensor& x, const Tensor& residual, const OptT& gate, const Tensor& post, const Tensor& pre,
+                         const OptT& scale_vec, const Tensor& rstd, double scale, const OptT& dout_, const OptT& ds_,
+                         bool want_dresidual, int64_t stream) {
+    ss_block_norm_bwd_args g{};
+    norm_x(kBlockNorm, x, &g.dtype);
+    REQUIRE(kBlockNorm, x.dim() == 2, "x must be (rows, dim)");
+    const int64_t rows = x.size(0), dim = x.size(1);
+    REQUIRE(kBlockNorm, rstd.scalar_type() == at::kFloat && same_shape(rstd, {rows, 2}) && rstd.is_contiguous(),
+            "rstd must be fp32 (rows, 2) contiguous");
+    REQUIRE(kBlockNorm, itype_of(post.scalar_type(), &g.w_dtype), "unsupported dtype " + dtype_str(post.scalar_type()));
+    OptT dout, ds, dresidual, dgate, dscale;
+    if (dout_) dout = like_rows(kBlockNorm, "dout", *dout_, x);
+    if (ds_) ds = like_rows(kBlockNorm, "dresidual_out", *ds_, x);
+    const Tensor dx = at::empty(x.sizes(), x.options()), dpost = at::empty({dim}, post.options()),
+                 dpre = at::empty({dim}, post.options());
+    if (want_dresidual) dresidual = at::empty(x.sizes(), x.options());
+    if (gate) dgate = at::empty(x.sizes(), x.options());
+    if (scale_vec) dscale = at::empty({dim}, post.options());
+    const int64_t n = ss_block_norm_bwd_workspace_bytes(rows, dim);
+    if (n < 0) check(SS_ERR_INVALID, kBlockNorm);
+    const Tensor ws = bytes_on(std::max<int64_t>(n, 1), x);
+    g.rows = rows; g.dim = dim; g.scale = float(scale);
+    g.x_row_stride = x.stride(0); g.residual_row_stride = residual.stride(0);
+    if (gate) g.gate_row_stride = gate->stride(0);
+    if (dout) g.dout_row_stride = dout->stride(0);
+    if (ds) g.dresidual_out_row_stride = ds->stride(0);
+    g.x = ptr(x); g.residual = ptr(residual); g.gate = ptr(gate); g.post = ptr(post); g.pre = ptr(pre);
+    g.scale_vec = ptr(scale_vec); g.rstd = static_cast<float*>(ptr(rstd)); g.dout = ptr(dout); g.dresidual_out = ptr(ds);
+    g.dx = ptr(dx); g.dresidual = ptr(dresidual); g.dgate = ptr(dgate); g.dpost = ptr(dpost); g.dpre = ptr(dpre);
+    g.dscale = ptr(dscale); g.workspace = ptr(ws); g.workspace_bytes = n;
+    launch(x.device(), "block_norm backward", [&] { return ss_block_norm_bwd(&g, reinterpret_cast<void*>(stream)); });
+    return py::make_tuple(dx, dresidual, dgate, dpost, dpre, dscale);
+}
+
+// (out, x, gate, weight as read), rows as (rows, dim)
+py::tuple gated_norm_fwd(const Tensor& x_, const Tensor& gate_, const Tensor& weight, int64_t groups, double eps,
+                         int64_t stream) {
+    ss_gated_norm_args a{};
+    norm_x(kGatedNorm, x_, &a.dtype);
+    const Tensor x = any_rows(x_), gate = like_rows(kGatedNorm, "gate", gate_, x_);
+    const OptT ow = weight;
+    const Weights w = weights_of(kGatedNorm, x_, {{"weight", &ow}});
+    a.w_dtype = w.dtype;
+    a.rows = x.size(0); a.dim = x.size(1); a.groups = groups; a.eps = float(eps);
+    const Tensor out = at::empty(x.sizes(), x.options());
+    a.x_row_stride = x.stride(0); a.gate_row_stride = gate.stride(0); a.out_row_stride = out.stride(0);
+    a.x = ptr(x); a.gate = ptr(gate); a.weight = ptr(w.w[0]); a.out = ptr(out);
+    launch(x.device(), "gated_rms_norm forward", [&] { return ss_gated_norm_fwd(&a, reinterpret_cast<void*>(stream)); });
+    return py::make_tuple(out, x, gate, w.w[0]);
+}
+
+// (dx, dgate, dweight)
+py::tuple gated_norm_bwd(const Tensor& x, const Tensor& gate, const Tensor& weight, const Tensor& dout_, int64_t groups,
+                         double eps, int64_t stream) {
+    ss_gated_norm_bwd_args g{};
+    norm_x(kGatedNorm, x, &g.dtype);
+    REQUIRE(kGatedNorm, x.dim() == 2, "x must be (rows, dim)");
+    const Tensor dout = like_rows(kGatedNorm, "dout", dout_, x);
+    REQUIRE(kGatedNorm, itype_of(weight.scalar_type(), &g.w_dtype), "unsupported dtype " + dtype_str(weight.scalar_type()));
+    const int64_t rows = x.size(0), dim = x.size(1);
+    const Tensor dx = at::empty(x.sizes(), x.options()), dgate = at::empty(x.sizes(), x.options()),
+                 dw = at::empty({dim}, weight.options());
+    const int64_t n = ss_gated_norm_bwd_workspace_bytes(rows, dim, groups);
+    if (n < 0) check(SS_ERR_INVALID, kGatedNorm);
+    const Tensor ws = bytes_on(std::max<int64_t>(n, 1), x);
+    g.rows = rows; g.dim = dim; g.groups = groups; g.eps = float(eps);
+    g.x_row_stride = x.stride(0); g.gate_row_stride = gate.stride(0); g.dout_row_stride = dout.stride(0);
+    g.x = ptr(x); g.gate = ptr(gate); g.weight = ptr(weight); g.dout = ptr(dout);
+    g.dx = ptr(dx); g.dgate = ptr(dgate); g.dweight = ptr(dw); g.workspace = ptr(ws); g.workspace_bytes = n;
+    launch(x.device(), "gated_rms_norm backward", [&] { return ss_gated_norm_bwd(&g, reinterpret_cast<void*>(stream)); });
+    return py::make_tuple(dx, dgate, dw);
+}
+
+// -------------------------------------------------------------- clipping --
+constexpr const char* kClip = "clip_grads";
+
+// Clips grads into outs (the same list: in place); returns the norm, a 0-d fp32 tensor.
+Tensor clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs, double max_norm, double eps,
+                  int64_t device_index, int64_t stream) {
+    REQUIRE(kClip, outs.size() == grads.size(),
+            "out holds " + std::to_string(outs.size()) + " tensors, expected " + std::to_string(grads.size()));
+    const at::Device dev = grads.empty() ? at::Device(at::kCUDA, at::DeviceIndex(device_index)) : grads[0].device();
+    REQUIRE(kClip, dev.is_cuda(), "tensors must be on a ROCm GPU device (no CPU path)");
+    const size_t n = grads.size();
+    std::vector<const void*> in(n);
+    std::vector<void*> out(n);
+    std::vector<int64_t> numels(n);
+    std::vector<int32_t> dtypes(n);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor &g = grads[i], &o = outs[i];
+        const auto at_i = [&] { return " of tensor " + std::to_string(i); };
+        REQUIRE(kClip, g.device() == dev && o.device() == dev, "all tensors must be on one device");
+        REQUIRE(kClip, itype_of(g.scalar_type(), &dtypes[i]), "unsupported dtype " + dtype_str(g.scalar_type()) + at_i());
+        REQUIRE(kClip, g.is_non_overlapping_and_dense(), "gaps or overlaps in the elements" + at_i());
+        if (!o.is_same(g))
+            REQUIRE(kClip, o.scalar_type() == g.scalar_type() && o.sizes() == g.sizes() && o.strides() == g.strides(),
+                    "out must match the gradient in shape, strides and dtype" + at_i());
+        in[i] = g.data_ptr(); out[i] = o.data_ptr(); numels[i] = g.numel();
+    }
+    ss_clip_grads_args a{};
+    a.count = int64_t(n);
+    a.grads = in.data(); a.outs = out.data(); a.numels = numels.data(); a.dtypes = dtypes.data();
+    a.max_norm = float(max_norm); a.eps = float(eps);
+    const auto options = at::TensorOptions().device(dev);
+    const Tensor norm = at::empty({}, options.dtype(at::kFloat));
+    const int64_t bytes = ss_clip_grads_workspace_bytes(&a);
+    if (bytes < 0) check(SS_ERR_INVALID, kClip);
+    const Tensor ws = at::empty({bytes}, options.dtype(at::kByte));
+    a.norm = static_cast<float*>(ptr(norm)); a.workspace = ptr(ws); a.workspace_bytes = bytes;
+    launch(dev, kClip, [&] { return ss_clip_grads(&a, reinterpret_cast<void*>(stream)); });
+    for (const Tensor& o : outs) o.unsafeGetTensorImpl()->bump_version();
+    return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(mamba_host, m) {
@@ -834,5 +1017,10 @@ PYBIND11_MODULE(mamba_host, m) {
     m.def("lin_fwd", &lin_fwd);
     m.def("lin_bwd", &lin_bwd);
     m.def("lin_update", &lin_update);
+    m.def("block_norm_fwd", &block_norm_fwd);
+    m.def("block_norm_bwd", &block_norm_bwd);
+    m.def("gated_norm_fwd", &gated_norm_fwd);
+    m.def("gated_norm_bwd", &gated_norm_bwd);
+    m.def("clip_grads", &clip_grads);
     m.def("abi", [] { return py::make_tuple(SS_ABI_VERSION, sizeof(ss_fwd_args), sizeof(ss_bwd_args)); });
 }

@@ -1163,4 +1163,167 @@ int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream) {
     return ok();
 }
 
+static int check_block_norm(int64_t rows, int64_t dim, int dtype, int w_dtype) {
+    if (rows < 0 || dim < 0)
+        return fail(SS_ERR_INVALID, "negative size (rows=%lld dim=%lld)", (long long)rows, (long long)dim);
+    if (dtype != SS_F32 && dtype != SS_BF16 && dtype != SS_F16) return fail(SS_ERR_INVALID, "unknown dtype %d", dtype);
+    if (w_dtype != dtype && w_dtype != SS_F32)
+        return fail(SS_ERR_UNSUPPORTED, "weight dtype %d must be the row dtype or fp32", w_dtype);
+    if (dim > ss::kBlockNormMaxDim)
+        return fail(SS_ERR_UNSUPPORTED, "dim=%lld above %lld", (long long)dim, (long long)ss::kBlockNormMaxDim);
+    return SS_OK;
+}
+
+struct NormPtr { const void* p; int64_t stride; bool need; const char* name; };
+// rows: present where needed, aligned to the element, strides not negative
+static int check_norm_ptrs(std::initializer_list<NormPtr> rows, size_t es) {
+    for (const NormPtr& r : rows) {
+        if (!r.p) {
+            if (r.need) return fail(SS_ERR_INVALID, "%s is NULL", r.name);
+            continue;
+        }
+        if (!aligned(r.p, es)) return fail(SS_ERR_INVALID, "%s is misaligned", r.name);
+        if (r.stride < 0) return fail(SS_ERR_INVALID, "negative row stride of %s", r.name);
+    }
+    return SS_OK;
+}
+
+int64_t ss_block_norm_bwd_workspace_bytes(int64_t rows, int64_t dim) {
+    if (rows < 0 || dim < 0 || dim > ss::kBlockNormMaxDim) {
+        fail(SS_ERR_INVALID, "rows=%lld, dim=%lld out of range", (long long)rows, (long long)dim);
+        return -1;
+    }
+    return ss::block_norm_bwd_space(rows, dim);
+}
+
+int ss_block_norm_fwd(const ss_block_norm_args* a, void* stream) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    int rc = check_block_norm(a->rows, a->dim, a->dtype, a->w_dtype);
+    if (rc != SS_OK) return rc;
+    if (!(a->eps >= 0.f)) return fail(SS_ERR_INVALID, "eps must be >= 0");
+    if (a->rows == 0 || a->dim == 0) return ok();
+    rc = check_norm_ptrs({{a->x, a->x_row_stride, true, "x"}, {a->residual, a->residual_row_stride, true, "residual"},
+                          {a->gate, a->gate_row_stride, false, "gate"}, {a->out, a->out_row_stride, true, "out"},
+                          {a->residual_out, a->residual_out_row_stride, true, "residual_out"}}, elem_size(a->dtype));
+    if (rc == SS_OK)
+        rc = check_norm_ptrs({{a->post, 0, true, "post"}, {a->pre, 0, true, "pre"}, {a->scale_vec, 0, false, "scale_vec"}},
+                             elem_size(a->w_dtype));
+    if (rc == SS_OK) rc = check_norm_ptrs({{a->rstd, 0, false, "rstd"}}, 4);
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::block_norm_fwd_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "block norm forward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_block_norm_bwd(const ss_block_norm_bwd_args* g, void* stream) {
+    if (!g) return fail(SS_ERR_INVALID, "null argument block");
+    int rc = check_block_norm(g->rows, g->dim, g->dtype, g->w_dtype);
+    if (rc != SS_OK) return rc;
+    if (g->dim == 0) return ok();
+    rc = check_norm_ptrs({{g->post, 0, true, "post"}, {g->pre, 0, true, "pre"}, {g->scale_vec, 0, false, "scale_vec"},
+                          {g->dpost, 0, true, "dpost"}, {g->dpre, 0, true, "dpre"}, {g->dscale, 0, false, "dscale"}},
+                         elem_size(g->w_dtype));
+    if (rc == SS_OK && g->rows > 0) {
+        rc = check_norm_ptrs({{g->x, g->x_row_stride, true, "x"}, {g->residual, g->residual_row_stride, true, "residual"},
+                              {g->gate, g->gate_row_stride, false, "gate"}, {g->dout, g->dout_row_stride, false, "dout"},
+                              {g->dresidual_out, g->dresidual_out_row_stride, false, "dresidual_out"},
+                              {g->dx, 0, true, "dx"}, {g->dresidual, 0, false, "dresidual"},
+                              {g->gate ? g->dgate : nullptr, 0, g->gate != nullptr, "dgate"}}, elem_size(g->dtype));
+        if (rc == SS_OK) rc = check_norm_ptrs({{g->rstd, 0, true, "rstd"}}, 4);
+    }
+    if (rc == SS_OK) rc = check_space(g->workspace, g->workspace_bytes, ss::block_norm_bwd_space(g->rows, g->dim));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::block_norm_bwd_launch(g, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "block norm backward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+static int check_groups(int64_t dim, int64_t groups) {
+    if (groups < 1 || dim % groups != 0)
+        return fail(SS_ERR_INVALID, "dim=%lld is not a multiple of groups=%lld", (long long)dim, (long long)groups);
+    return SS_OK;
+}
+
+int64_t ss_gated_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t groups) {
+    if (rows < 0 || dim < 0 || dim > ss::kBlockNormMaxDim) {
+        fail(SS_ERR_INVALID, "rows=%lld, dim=%lld out of range", (long long)rows, (long long)dim);
+        return -1;
+    }
+    if (check_groups(dim, groups) != SS_OK) return -1;
+    return dim > 0 ? ss::gated_norm_bwd_space(rows, dim, groups) : 0;
+}
+
+int ss_gated_norm_fwd(const ss_gated_norm_args* a, void* stream) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    int rc = check_block_norm(a->rows, a->dim, a->dtype, a->w_dtype);
+    if (rc == SS_OK) rc = check_groups(a->dim, a->groups);
+    if (rc != SS_OK) return rc;
+    if (!(a->eps >= 0.f)) return fail(SS_ERR_INVALID, "eps must be >= 0");
+    if (a->rows == 0 || a->dim == 0) return ok();
+    rc = check_norm_ptrs({{a->x, a->x_row_stride, true, "x"}, {a->gate, a->gate_row_stride, true, "gate"},
+                          {a->out, a->out_row_stride, true, "out"}}, elem_size(a->dtype));
+    if (rc == SS_OK) rc = check_norm_ptrs({{a->weight, 0, true, "weight"}}, elem_size(a->w_dtype));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::gated_norm_fwd_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "gated norm forward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_gated_norm_bwd(const ss_gated_norm_bwd_args* g, void* stream) {
+    if (!g) return fail(SS_ERR_INVALID, "null argument block");
+    int rc = check_block_norm(g->rows, g->dim, g->dtype, g->w_dtype);
+    if (rc == SS_OK) rc = check_groups(g->dim, g->groups);
+    if (rc != SS_OK) return rc;
+    if (!(g->eps >= 0.f)) return fail(SS_ERR_INVALID, "eps must be >= 0");
+    if (g->dim == 0) return ok();
+    rc = check_norm_ptrs({{g->weight, 0, true, "weight"}, {g->dweight, 0, true, "dweight"}}, elem_size(g->w_dtype));
+    if (rc == SS_OK && g->rows > 0)
+        rc = check_norm_ptrs({{g->x, g->x_row_stride, true, "x"}, {g->gate, g->gate_row_stride, true, "gate"},
+                              {g->dout, g->dout_row_stride, true, "dout"}, {g->dx, 0, true, "dx"},
+                              {g->dgate, 0, true, "dgate"}}, elem_size(g->dtype));
+    if (rc == SS_OK)
+        rc = check_space(g->workspace, g->workspace_bytes, ss::gated_norm_bwd_space(g->rows, g->dim, g->groups));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::gated_norm_bwd_launch(g, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "gated norm backward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+static int check_clip_grads(const ss_clip_grads_args* a) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    if (a->count < 0) return fail(SS_ERR_INVALID, "negative count");
+    if (a->count > 0 && (!a->grads || !a->outs || !a->numels || !a->dtypes))
+        return fail(SS_ERR_INVALID, "grads / outs / numels / dtypes is NULL");
+    int64_t total = 0;
+    for (int64_t i = 0; i < a->count; ++i) {
+        if (a->dtypes[i] != SS_F32 && a->dtypes[i] != SS_BF16 && a->dtypes[i] != SS_F16)
+            return fail(SS_ERR_INVALID, "unknown dtype %d of tensor %lld", a->dtypes[i], (long long)i);
+        if (a->numels[i] < 0) return fail(SS_ERR_INVALID, "negative size of tensor %lld", (long long)i);
+        if (a->numels[i] > (int64_t(1) << 40) - total) return fail(SS_ERR_UNSUPPORTED, "more than 2^40 elements");
+        total += a->numels[i];
+        if (a->numels[i] == 0) continue;
+        if (!a->grads[i] || !a->outs[i]) return fail(SS_ERR_INVALID, "tensor %lld is NULL", (long long)i);
+        const size_t es = elem_size(a->dtypes[i]);
+        if (!aligned(a->grads[i], es) || !aligned(a->outs[i], es))
+            return fail(SS_ERR_INVALID, "tensor %lld is misaligned", (long long)i);
+    }
+    return ok();
+}
+
+int64_t ss_clip_grads_workspace_bytes(const ss_clip_grads_args* a) {
+    return check_clip_grads(a) == SS_OK ? 16 + 8 * ss::clip_grads_chunks(a) : -1;
+}
+
+int ss_clip_grads(const ss_clip_grads_args* a, void* stream) {
+    int rc = check_clip_grads(a);
+    if (rc != SS_OK) return rc;
+    if (!(a->max_norm >= 0.f) || !(a->eps >= 0.f)) return fail(SS_ERR_INVALID, "max_norm and eps must be >= 0");
+    if (!a->norm || !aligned(a->norm, 4)) return fail(SS_ERR_INVALID, "norm is NULL or misaligned");
+    rc = check_space(a->workspace, a->workspace_bytes, 16 + 8 * ss::clip_grads_chunks(a));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::clip_grads_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "gradient clipping launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
 }  // extern "C"
