@@ -1,8 +1,12 @@
-// Linear attention with a decay for each head, on gfx950: the token-by-token
-// form, and the kernels that finish the backward.
+// Linear attention with a decay for each head, on gfx950: the launches of a
+// prompt or a training step, the kernels that finish the backward, and the
+// recurrence for one token.
 //
-// A pass (LaJob) walks the recurrence of linear_attn.hpp.  The backward is
-// three passes, then the decay's gradient.  With D_s = q_s . dq_s - k_s . dk_s
+// A pass (LaJob) is the recurrence of linear_attn.hpp, run in chunks
+// (linear_attn_chunk.hpp).  With few rows a pass takes three launches: each
+// segment's state from a zero start, the states joined along the row, and the
+// segments walked side by side, each from its carry.  The backward is three
+// passes, then the decay's gradient.  With D_s = q_s . dq_s - k_s . dk_s
 // and M_ij the share of token j in the output at i (times its gradient),
 // D_s is row s of M less column s, and
 //   dg_t = sum of M_ij over i >= t > j
@@ -22,95 +26,39 @@ namespace ss {
 
 namespace {
 
-constexpr int kVTile = 64;           // value columns per workgroup
-constexpr int kBatchTok = 16;        // tokens staged at a time
-
 __device__ __forceinline__ int64_t row_len(const int32_t* lens, int64_t b, int64_t L) {
     if (!lens) return L;
     const int64_t n = lens[b];
     return n < 0 ? 0 : n < L ? n : L;
 }
 
-template <typename T>
-__device__ __forceinline__ const T* row_ptr(const LaRows& r, int64_t b, int64_t t, int64_t h) {
-    return static_cast<const T*>(r.p) + b * r.b + t * r.l + (h / r.rep) * r.h;
-}
-
-// One workgroup per (batch, head) and 64 value columns; thread (i, n) holds
-// rows i * KD / 4 .. of column n of the state.
-template <typename T, int KD>
-__global__ __launch_bounds__(256) void la_recurrent(const LaParams p) {
+// The segments' states in walk order, each from the one before it: ends[s] <-
+// ends[s] + decays[s] ends[before s].  A thread an element of the state.
+__global__ __launch_bounds__(256) void la_carry(const LaParams p) {
     const LaJob& J = p.job[blockIdx.z];
-    const int64_t bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-    const int n0 = int(blockIdx.y) * kVTile;
-    if (n0 >= J.V) return;
-    constexpr int R = KD / 4;
-    __shared__ float qs[kBatchTok][KD], ks[kBatchTok][KD], red[4][kVTile];
-    const int col = threadIdx.x & 63, part = threadIdx.x >> 6, n = n0 + col;
-    const int64_t len = row_len(p.lens, b, p.L);
-    const int64_t KV = int64_t(J.K) * J.V;
-
-    float S[R];
+    const int64_t bh = blockIdx.y, KV = int64_t(J.K) * J.V, i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= KV) return;
+    float s = J.in ? J.in[bh * KV + i] : 0.f;
+    float* ends = J.ends + bh * p.segs * KV + i;
+    const float* decays = J.decays + bh * p.segs;
+    const int step = J.rev ? -1 : 1;
+    int at = J.rev ? p.segs - 1 : 0;
+    constexpr int kAhead = 8;
+    for (int n = 0; n < p.segs; n += kAhead) {
+        const int cnt = p.segs - n < kAhead ? p.segs - n : kAhead;
+        float own[kAhead];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int d = part * R + i;
-        S[i] = J.in && d < J.K && n < J.V ? J.in[bh * KV + int64_t(d) * J.st_k + int64_t(n) * J.st_v] : 0.f;
-    }
-    auto write_state = [&](float* to) {
+        for (int k = 0; k < kAhead; ++k) own[k] = k < cnt ? ends[int64_t(at + step * k) * KV] : 0.f;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int d = part * R + i;
-            if (d < J.K && n < J.V) to[int64_t(d) * J.st_k + int64_t(n) * J.st_v] = S[i];
-        }
-    };
-    for (int si = 0; si < p.segs; ++si) {
-        const int seg = J.rev ? p.segs - 1 - si : si;
-        const int64_t s0 = seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
-        for (int64_t done = 0; done < s1 - s0; done += kBatchTok) {
-            const int cnt = int(s1 - s0 - done < kBatchTok ? s1 - s0 - done : kBatchTok);
-            __syncthreads();
-            for (int i = threadIdx.x; i < kBatchTok * KD; i += 256) {
-                const int u = i / KD, d = i % KD;
-                const int64_t t = J.rev ? s1 - 1 - done - u : s0 + done + u;
-                const bool in = u < cnt && d < J.K && t < len;
-                qs[u][d] = in ? io<T>::load(row_ptr<T>(J.q, b, t, h) + d) : 0.f;
-                ks[u][d] = in ? io<T>::load(row_ptr<T>(J.k, b, t, h) + d) : 0.f;
-            }
-            __syncthreads();
-            for (int u = 0; u < cnt; ++u) {
-                const int64_t t = J.rev ? s1 - 1 - done - u : s0 + done + u;
-                const bool live = t < len;
-                const float a = live ? expf(p.g[b * p.g_b + t * p.g_l + h * p.g_h]) : 1.f;
-                const float v = live && n < J.V ? J.vscale * io<T>::load(row_ptr<T>(J.v, b, t, h) + n) : 0.f;
-                float acc = 0.f;
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    if (!J.rev) S[i] *= a;
-                    S[i] = __builtin_fmaf(ks[u][part * R + i], v, S[i]);
-                    acc = __builtin_fmaf(qs[u][part * R + i], S[i], acc);
-                    if (J.rev) S[i] *= a;
-                }
-                red[part][col] = acc;
-                __syncthreads();
-                if (part == 0) {
-                    const float o = live ? J.oscale * ((red[0][col] + red[1][col]) + (red[2][col] + red[3][col])) : 0.f;
-                    if (n < J.V) {
-                        const int64_t at = b * J.o.b + t * J.o.l + h * J.o.h + n;
-                        if (J.o_f32) static_cast<float*>(const_cast<void*>(J.o.p))[at] = o;
-                        else io<T>::store(static_cast<T*>(const_cast<void*>(J.o.p)) + at, o);
-                    }
-                    if (J.dot) {
-                        const float x = live && n < J.V ? io<T>::load(row_ptr<T>(J.x, b, t, h) + n) : 0.f;
-                        const float s = wave_allsum(o * x);
-                        if (col == 0) J.dot[(int64_t(blockIdx.y) * p.B * p.H + bh) * p.L + t] = s;
-                    }
-                }
-                __syncthreads();
+        for (int k = 0; k < kAhead; ++k) {
+            if (k < cnt) {
+                s = __builtin_fmaf(decays[at + step * k], s, own[k]);
+                ends[int64_t(at + step * k) * KV] = s;
             }
         }
-        if (J.ends) write_state(J.ends + (bh * p.segs + seg) * KV);
+        at += step * cnt;
     }
-    if (J.out_state) write_state(J.out_state + bh * KV);
+    if (J.out_state) J.out_state[bh * KV + i] = s;
 }
 
 // dg of one segment: the inner product of the two states at its end, and the
@@ -212,38 +160,47 @@ __global__ __launch_bounds__(256) void la_group_sum(const float* part0, T* out0,
     }
 }
 
-template <typename T>
-hipError_t launch_walk(const LaParams& p, hipStream_t stream) {
-    int kmax = 0, vmax = 0;
-    for (int j = 0; j < p.njobs; ++j) {
-        kmax = p.job[j].K > kmax ? p.job[j].K : kmax;
-        vmax = p.job[j].V > vmax ? p.job[j].V : vmax;
-    }
-    const dim3 grid(unsigned(p.B * p.H), unsigned((vmax + kVTile - 1) / kVTile), unsigned(p.njobs));
-    if (kmax <= 64) hipLaunchKernelGGL((la_recurrent<T, 64>), grid, dim3(256), 0, stream, p);
-    else if (kmax <= 128) hipLaunchKernelGGL((la_recurrent<T, 128>), grid, dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((la_recurrent<T, 256>), grid, dim3(256), 0, stream, p);
-    return hipGetLastError();
-}
+// Workgroups that fill the GPU: with fewer rows (batch x heads x tiles) than
+// that a row's segments run side by side, about kSegsWanted of them in all.
+constexpr int64_t kFull = 1024, kSegsWanted = 1536, kSegTokMin = 128, kSegTokMax = 1024;
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
-int64_t vtiles(int64_t v) { return (v + kVTile - 1) / kVTile; }
 
-struct BwdSpace { int64_t dotq, dotk, rends, part, dq, dk, bytes; };
+int64_t tile_count(int64_t dim, int tile) { return (dim + tile - 1) / tile; }
+// the backward's passes share a launch: the tile of the widest
+int bwd_tile(const ss_linear_attn_args& a) { return la_tile(a.d_key > a.d_value ? a.d_key : a.d_value); }
+
+struct BwdSpace { int64_t dotq, dotk, rends, decays, part, dq, dk, bytes; };
 BwdSpace bwd_space(const ss_linear_attn_bwd_args* g) {
     const ss_linear_attn_args& a = g->f;
     const int64_t bh = a.batch * a.heads, segs = linear_attn_segs(&a);
     BwdSpace s{};
     int64_t at = 0;
     const auto take = [&](int64_t bytes) { const int64_t r = at; at += round16(bytes); return r; };
-    s.dotq = take(vtiles(a.d_key) * bh * a.seqlen * 4);
-    s.dotk = take(vtiles(a.d_key) * bh * a.seqlen * 4);
+    const int64_t tiles = tile_count(a.d_key, bwd_tile(a));
+    s.dotq = take(tiles * bh * a.seqlen * 4);
+    s.dotk = take(tiles * bh * a.seqlen * 4);
     s.rends = take(bh * segs * a.d_key * a.d_value * 4);
+    s.decays = take(bh * segs * 4);
     s.part = take(g->g_per_head ? bh * segs * 8 : 0);
     const int64_t shared = a.heads > a.groups ? a.batch * a.seqlen * a.heads * a.d_key * 4 : 0;
     s.dq = take(shared);
     s.dk = take(shared);
     s.bytes = at;
+    return s;
+}
+
+// The segments' states where the caller keeps none, and their decays.
+bool serial(const ss_linear_attn_args& a, int64_t tiles) {
+    return linear_attn_segs(&a) == 1 || a.batch * a.heads * tiles >= kFull;
+}
+struct FwdSpace { int64_t ends, decays, bytes; };
+FwdSpace fwd_space(const ss_linear_attn_args& a) {
+    FwdSpace s{};
+    if (serial(a, tile_count(a.d_value, la_tile(a.d_value)))) return s;
+    const int64_t n = a.batch * a.heads * linear_attn_segs(&a);
+    s.decays = a.ends ? 0 : round16(n * a.d_key * a.d_value * 4);
+    s.bytes = s.decays + round16(n * 4);
     return s;
 }
 
@@ -257,28 +214,52 @@ LaParams common(const ss_linear_attn_args& a) {
     return p;
 }
 
-hipError_t walk(int dtype, const LaParams& p, hipStream_t stream) {
+template <typename F>
+hipError_t for_type(int dtype, F&& f) {
     switch (dtype) {
-        case SS_F32: return launch_walk<float>(p, stream);
-        case SS_BF16: return launch_walk<bf16_t>(p, stream);
-        default: return launch_walk<_Float16>(p, stream);
+        case SS_F32: return f(float{});
+        case SS_BF16: return f(bf16_t{});
+        default: return f(_Float16{});
     }
+}
+
+// p's jobs over whole rows or, where segments run side by side, over the
+// segments: `local` (each job its own states) then gives their carries.
+hipError_t carries(int dtype, const LaParams& local, hipStream_t stream) {
+    const hipError_t e = for_type(dtype, [&](auto t) { return la_local_launch<decltype(t)>(local, stream); });
+    if (e != hipSuccess) return e;
+    const int64_t KV = int64_t(local.job[0].K) * local.job[0].V, bh = local.B * local.H;
+    hipLaunchKernelGGL(la_carry, dim3(unsigned((KV + 255) / 256), unsigned(bh), unsigned(local.njobs)), dim3(256), 0, stream, local);
+    return hipGetLastError();
+}
+hipError_t walk(int dtype, const LaParams& p, bool fine, hipStream_t stream) {
+    return for_type(dtype, [&](auto t) { return la_walk_launch<decltype(t)>(p, fine, stream); });
 }
 
 }  // namespace
 
-int64_t linear_attn_segment(const ss_linear_attn_args*) { return 256; }
+int64_t linear_attn_segment(const ss_linear_attn_args* a) {
+    const int64_t bh = a->batch * a->heads;
+    const int64_t segs = bh > 0 ? (kSegsWanted + bh - 1) / bh : 1, want = (a->seqlen + segs - 1) / segs;
+    int64_t n = kSegTokMin;
+    while (n < want && n < kSegTokMax) n *= 2;
+    return n;
+}
 int64_t linear_attn_segs(const ss_linear_attn_args* a) {
     const int64_t n = linear_attn_segment(a);
     return a->seqlen <= n ? 1 : (a->seqlen + n - 1) / n;
 }
-int64_t linear_attn_fwd_space(const ss_linear_attn_args*) { return 0; }
+
+int64_t linear_attn_fwd_space(const ss_linear_attn_args* a) { return fwd_space(*a).bytes; }
 int64_t linear_attn_bwd_space(const ss_linear_attn_bwd_args* g) { return bwd_space(g).bytes; }
 
 hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stream) {
     LaParams p = common(*a);
     const int rep = int(a->heads / a->groups);
     p.njobs = 1;
+    p.tile = la_tile(a->d_value);
+    p.tiles = int(tile_count(a->d_value, p.tile));
+    p.serial = serial(*a, p.tiles);
     LaJob& j = p.job[0];
     j.q = {a->q, a->q_batch_stride, a->q_len_stride, a->q_head_stride, rep};
     j.k = {a->k, a->k_batch_stride, a->k_len_stride, a->k_head_stride, rep};
@@ -288,7 +269,17 @@ hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stre
     j.oscale = a->scale; j.vscale = 1.f;
     j.st_k = j.V; j.st_v = 1;
     j.in = a->initial_state; j.ends = a->ends; j.out_state = a->last_state;
-    return walk(a->dtype, p, stream);
+    if (!p.serial) {
+        const FwdSpace sp = fwd_space(*a);
+        char* ws = static_cast<char*>(a->workspace);
+        if (!j.ends) j.ends = reinterpret_cast<float*>(ws + sp.ends);
+        j.decays = reinterpret_cast<float*>(ws + sp.decays);
+        const hipError_t e = carries(a->dtype, p, stream);
+        if (e != hipSuccess) return e;
+        j.carry = j.ends;
+        j.ends = j.out_state = nullptr;
+    }
+    return walk(a->dtype, p, false, stream);
 }
 
 hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t stream) {
@@ -307,6 +298,9 @@ hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t 
     const bool part = rep > 1;
     float* rends = reinterpret_cast<float*>(ws + sp.rends);
     p.njobs = 3;
+    p.tile = bwd_tile(a);
+    p.tiles = int(tile_count(K > V ? K : V, p.tile));
+    p.serial = serial(a, p.tiles);
     LaJob& jq = p.job[0];
     jq.q = dout; jq.k = v; jq.v = k; jq.x = q;
     jq.o = grad(part ? ws + sp.dq : g->dq, K);
@@ -332,13 +326,25 @@ hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t 
     jv.oscale = 1.f; jv.vscale = a.scale;
     jv.st_k = V; jv.st_v = 1;
     jv.in = g->dlast_state; jv.ends = rends; jv.out_state = g->dinitial_state;
-    hipError_t e = walk(a.dtype, p, stream);
+    hipError_t e = hipSuccess;
+    if (!p.serial) {
+        LaParams own = p;                               // dS of the segments: jv's states
+        own.njobs = 1;
+        own.job[0] = jv;
+        own.job[0].decays = reinterpret_cast<float*>(ws + sp.decays);
+        e = carries(a.dtype, own, stream);
+        if (e != hipSuccess) return e;
+        jq.carry = a.ends;
+        jk.carry = jv.carry = rends;
+        jv.ends = jv.out_state = nullptr;
+    }
+    e = walk(a.dtype, p, true, stream);
     if (e != hipSuccess) return e;
 
     LaDgParams d{};
     d.B = a.batch; d.L = a.seqlen; d.H = a.heads;
     d.lens = a.lengths; d.seg_tokens = p.seg_tokens; d.segs = p.segs;
-    d.qtiles = d.ktiles = int(vtiles(K));
+    d.qtiles = d.ktiles = int(tile_count(K, p.tile));
     d.KV = K * V;
     d.dotq = jq.dot; d.dotk = jk.dot; d.ends = a.ends; d.rends = rends; d.dlast = g->dlast_state;
     d.dg = g->g_per_head ? nullptr : g->dg;

@@ -1,6 +1,8 @@
 // Linear attention with a decay for each head: what its host and device
 // sides share.
 #pragma once
+#include <hip/hip_runtime.h>
+
 #include <cstdint>
 
 #include "../../include/mamba_ss.h"
@@ -35,6 +37,7 @@ struct LaJob {
     const float* carry;               // with it: state after each segment (in time order); the walk of segment s
                                       // starts from the one before it in walk order
     float* ends;                      // written: state after each segment in walk order, or null
+    float* decays;                    // la_local: (B, H, segs) product of a segment's decays
     float* out_state;                 // written: state after the whole walk (segs 1), or null
     float* dot;                       // written: (V tiles, B, H, L) sums over the tile's columns of o * x, or null
 };
@@ -48,7 +51,19 @@ struct LaParams {
     const int32_t* lens;
     int64_t seg_tokens;
     int segs;
+    int serial;                       // a workgroup walks a whole row (else a segment, from its carry)
+    int tile, tiles;                  // value columns per workgroup, and tiles of the widest job
 };
+
+// value columns per workgroup
+inline int la_tile(int64_t dim) { return dim <= 64 ? 64 : 128; }
+inline int la_tiles(int64_t dim) { return int((dim + la_tile(dim) - 1) / la_tile(dim)); }
+
+// The segments' states from a zero start and their decays (job.ends,
+// job.decays); and the walk itself.  fine: 16-bit rows, too, with what is
+// computed in 3 terms.
+template <typename T> hipError_t la_local_launch(const LaParams& p, hipStream_t stream);
+template <typename T> hipError_t la_walk_launch(const LaParams& p, bool fine, hipStream_t stream);
 
 // dg of the tokens of one segment (see linear_attn.hip)
 struct LaDgParams {

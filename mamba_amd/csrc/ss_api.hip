@@ -1051,8 +1051,8 @@ static int check_linear_attn(const ss_linear_attn_args* a, bool bwd) {
                     (long long)a->d_value, (long long)ss::kLinearAttnMaxDim);
     if (a->heads > 0 && (a->groups < 1 || a->heads % a->groups != 0))
         return fail(SS_ERR_INVALID, "heads=%lld is not a multiple of groups=%lld", (long long)a->heads, (long long)a->groups);
-    // (token, head and column offsets of one workgroup's loop stay far below 2^63; the grid is batch x heads)
-    if (a->batch > 0 && a->heads > INT32_MAX / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
+    // (a launch holds at most batch x heads x 6 workgroups of 256 threads, and 2^32 threads)
+    if (a->batch > 0 && a->heads > ss::kLinearAttnMaxRows / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
     if (a->seqlen > (int64_t(1) << 24)) return fail(SS_ERR_UNSUPPORTED, "seqlen=%lld above 2^24", (long long)a->seqlen);
     const int64_t st[] = {a->q_batch_stride, a->q_len_stride, a->q_head_stride, a->k_batch_stride, a->k_len_stride,
                           a->k_head_stride, a->v_batch_stride, a->v_len_stride, a->v_head_stride, a->g_batch_stride,
@@ -1145,7 +1145,7 @@ int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream) {
                     (long long)a->d_value, (long long)ss::kLinearAttnMaxDim);
     if (a->heads > 0 && (a->groups < 1 || a->heads % a->groups != 0))
         return fail(SS_ERR_INVALID, "heads=%lld is not a multiple of groups=%lld", (long long)a->heads, (long long)a->groups);
-    if (a->batch > 0 && a->heads > INT32_MAX / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
+    if (a->batch > 0 && a->heads > ss::kLinearAttnMaxRows / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
     const int64_t st[] = {a->state_batch_stride, a->state_head_stride, a->q_batch_stride, a->q_head_stride, a->k_batch_stride,
                           a->k_head_stride, a->v_batch_stride, a->v_head_stride, a->out_batch_stride, a->out_head_stride,
                           a->g_batch_stride, a->g_head_stride};

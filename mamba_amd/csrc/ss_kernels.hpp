@@ -234,7 +234,7 @@ int64_t linear_attn_bwd_space(const ss_linear_attn_bwd_args* g);
 hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stream);
 hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t stream);
 hipError_t linear_attn_update_launch(const ss_linear_attn_update_args* a, hipStream_t stream);
-constexpr int64_t kLinearAttnMaxDim = 256;
+constexpr int64_t kLinearAttnMaxDim = 256, kLinearAttnMaxRows = int64_t(1) << 21;   // rows: batch * heads
 // the norms around a block and the gated norm of each head (block_norm.hip)
 int64_t block_norm_bwd_space(int64_t rows, int64_t dim);
 int64_t gated_norm_bwd_space(int64_t rows, int64_t dim, int64_t groups);
