@@ -157,9 +157,25 @@ struct Stage {
     using R = rowvec<T>;
     static constexpr int PER_ROW = WIDTH / R::VE, N = (C * PER_ROW + 255) / 256, STRIDE = WIDTH + 8, TERMS = kTerms<T>;
     static constexpr int TERM = C * STRIDE;                  // elements of one term's tile
+    static constexpr int STEP = 256 / PER_ROW;               // rows between a thread's vectors
+    static constexpr bool PARTIAL = C * PER_ROW % 256 != 0;  // threads without a row
     uint4 v[N];
 
-    // rows t0 .. of p (a row every `step` elements), dim elements each; rows from `end` on are zero
+    // whether a tile of rows `step` elements apart is within 32-bit byte offsets of its first
+    static __device__ __forceinline__ bool near(int64_t step) { return step < (int64_t(1) << 24); }
+    // all rows of p (a row every `step` elements, a tile that is near), whole
+    __device__ __forceinline__ void load_all(const T* p, int64_t step) {
+        const int row = int(threadIdx.x) / PER_ROW, col = int(threadIdx.x) % PER_ROW * R::VE;
+        const uint32_t off = (uint32_t(row) * uint32_t(step) + uint32_t(col)) * uint32_t(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (PARTIAL && row >= C) continue;
+            const typename R::words w = *reinterpret_cast<const typename R::words*>(
+                reinterpret_cast<const char*>(p + int64_t(i * STEP) * step) + off);
+            v[i] = make_uint4(w.x, w.y, w.z, w.w);
+        }
+    }
+    // rows t0 .. of p, dim elements each; rows from `end` on are zero
     __device__ __forceinline__ void load(const T* p, int64_t step, int64_t t0, int64_t end, int dim) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -168,18 +184,21 @@ struct Stage {
             v[i] = R::load(p + t * step + col, row < C && t < end ? dim - col : 0);
         }
     }
-    // into the terms' tiles; whether an element is infinite or NaN
+    // into the terms' tiles; CHECK: whether an element is infinite or NaN
+    template <bool CHECK>
     __device__ __forceinline__ bool store(uint16_t* tile) const {
-        bool bad = false;
+        typedef uint16_t h2 __attribute__((ext_vector_type(2)));
+        h2 top = {0, 0};                                     // the largest exponents
+        const auto look = [&](uint32_t w) {
+            if constexpr (CHECK) top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, w & 0x7f807f80u));
+        };
+        const int row = int(threadIdx.x) / PER_ROW, col = int(threadIdx.x) % PER_ROW * R::VE;
+        if (PARTIAL && row >= C) return false;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int at = int(threadIdx.x) + 256 * i, row = at / PER_ROW, col = at % PER_ROW * R::VE;
-            if (C * PER_ROW % 256 != 0 && row >= C) continue;
-            uint16_t* to = tile + row * STRIDE + col;
+            uint16_t* to = tile + row * STRIDE + col + i * STEP * STRIDE;
             if constexpr (TERMS == 1) {
-                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) bad |= (((w[k] & 0x7fff7fffu) + 0x00800080u) & 0x80008000u) != 0;
+                look(v[i].x); look(v[i].y); look(v[i].z); look(v[i].w);
                 *reinterpret_cast<uint4*>(to) = v[i];
             } else {
                 float x[R::VE];
@@ -188,7 +207,7 @@ struct Stage {
 #pragma unroll
                 for (int k = 0; k < R::VE / 2; ++k) {
                     split<TERMS>(x[2 * k], x[2 * k + 1], t[k]);
-                    bad |= (((t[k][0] & 0x7fff7fffu) + 0x00800080u) & 0x80008000u) != 0;
+                    look(t[k][0]);
                 }
 #pragma unroll
                 for (int n = 0; n < TERMS; ++n) {
@@ -197,14 +216,14 @@ struct Stage {
                 }
             }
         }
-        return bad;
+        return top.x >= 0x7f80 || top.y >= 0x7f80;
     }
 };
 
 // The chunk's decays.  Lane t of one wave holds token t's log decay (0 past
 // the row's end).
 template <int C>
-struct Decays {
+struct __attribute__((aligned(16))) Decays {
     int I[C];              // integer part of H (G, or -G in reverse)
     float col[C];          // 2^-F, with the factor of v
     float row[C];          // 2^F, with the factor of o
@@ -256,7 +275,9 @@ __device__ __forceinline__ void update_state(f4 (&S)[KP / 16][NT], const uint16_
         for (int n = 0; n < NT; ++n) S[d][n] *= tot;
 #pragma unroll
     for (int ks = 0; ks < C / 32; ++ks) {
-        const float* u = dec.upd + 32 * ks + 8 * (lane >> 4);
+        const f4* up = reinterpret_cast<const f4*>(dec.upd + 32 * ks + 8 * (lane >> 4));
+        const f4 u0 = up[0], u1 = up[1];
+        const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
         u4 bv[NT][3];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -328,6 +349,7 @@ __global__ __launch_bounds__(256) void la_local(const LaParams) {
     const T* vp = static_cast<const T*>(J.v.p) + b * J.v.b + (h / J.v.rep) * J.v.h + n0;
     const float* gp = p.g + b * p.g_b + h * p.g_h;
     const int chunks = int((s1 - s0 + C - 1) / C), vdim = J.V - n0;
+    const bool whole = J.K == KP && vdim >= 64 * NT && SK::near(J.k.l) && SV::near(J.v.l);
 
     f4 S[KP / 16][NT];
 #pragma unroll
@@ -340,15 +362,20 @@ __global__ __launch_bounds__(256) void la_local(const LaParams) {
     float gv = 0.f;
     const auto fetch = [&](int i) __attribute__((always_inline)) {
         const int64_t t0 = s0 + int64_t(J.rev ? chunks - 1 - i : i) * C;
-        sk.load(kp, J.k.l, t0, end, J.K);
-        sv.load(vp, J.v.l, t0, end, vdim);
+        if (whole && t0 + C <= end) {
+            sk.load_all(kp + t0 * J.k.l, J.k.l);
+            sv.load_all(vp + t0 * J.v.l, J.v.l);
+        } else {
+            sk.load(kp, J.k.l, t0, end, J.K);
+            sv.load(vp, J.v.l, t0, end, vdim);
+        }
         gv = 0.f;
         if (wave == 0 && lane < C && t0 + lane < end) gv = gp[(t0 + lane) * p.g_l];
     };
     fetch(0);
     for (int i = 0; i < chunks; ++i) {
-        (void)sk.store(kt);
-        (void)sv.store(vt);
+        (void)sk.template store<false>(kt);
+        (void)sv.template store<false>(vt);
         if (wave == 0) dec.fill(lane, gv, J.rev, J.vscale, 1.f);
         __syncthreads();
         if (i + 1 < chunks) fetch(i + 1);
@@ -379,14 +406,36 @@ __global__ __launch_bounds__(256) void la_local(const LaParams) {
 }
 
 // ----------------------------------------------------------------- the walk --
+// P's 32 x 32 blocks that hold causal tiles: rows' half + tokens' half is
+// 0, 1 or 2, whichever way the walk goes.
+template <int C, int N>
+struct Causal {
+    static constexpr int STRIDE = 40, BLOCK = 32 * STRIDE, BLOCKS = C / 16 - 1, TERM = BLOCKS * BLOCK;
+    static __device__ __forceinline__ int at(int row, int token) {
+        return ((row >> 5) + (token >> 5)) * BLOCK + (row & 31) * STRIDE + (token & 31);
+    }
+};
+
+// Workgroups per CU that LDS has room for (160 KiB) set the registers a wave may
+// take: up to 3 waves a SIMD, which hide each other's barriers and loads.
 template <typename T, int KP, int NT, int N>
-__global__ __launch_bounds__(256) void la_walk(const LaParams) {
+constexpr int walk_lds() {
+    constexpr int C = kChunk<T>, R = kTerms<T>;
+    return 2 * (2 * R * Stage<T, C, KP>::TERM + R * Stage<T, C, 64 * NT>::TERM + N * Causal<C, N>::TERM) + 2 * int(sizeof(Decays<C>)) +
+           16 * C + 256 * NT + 16;
+}
+template <typename T, int KP, int NT, int N>
+constexpr int kWalkWaves = KP <= 64 && NT == 1 && 3 * walk_lds<T, KP, NT, N>() <= 163840 ? 3 : KP <= 128 && 2 * walk_lds<T, KP, NT, N>() <= 163840 ? 2 : 1;
+
+template <typename T, int KP, int NT, int N>
+__global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const LaParams) {
     Params& p = params();
-    constexpr int C = kChunk<T>, R = kTerms<T>, IT = C / 16, TRI = IT * (IT + 1) / 2, PS = C + 8, kMax = N == 2 ? 1 : 2;
+    constexpr int C = kChunk<T>, R = kTerms<T>, IT = C / 16, TRI = IT * (IT + 1) / 2, kMax = N == 2 ? 1 : 2;
     using SK = Stage<T, C, KP>;
     using SV = Stage<T, C, 64 * NT>;
-    __shared__ __attribute__((aligned(16))) uint16_t qt[R * SK::TERM], kt[R * SK::TERM], vt[R * SV::TERM], pt[N * C * PS];
-    __shared__ __attribute__((aligned(16))) Decays<C> dec;
+    using CP = Causal<C, N>;
+    __shared__ __attribute__((aligned(16))) uint16_t qt[R * SK::TERM], kt[R * SK::TERM], vt[R * SV::TERM], pt[N * CP::TERM];
+    __shared__ Decays<C> decs[2];
     __shared__ float dots[4][C];
     __shared__ int bad_any, bad_col[64 * NT];
     const int segs = p.serial ? 1 : p.segs;
@@ -403,9 +452,13 @@ __global__ __launch_bounds__(256) void la_walk(const LaParams) {
     const T* kp = static_cast<const T*>(J.k.p) + b * J.k.b + (h / J.k.rep) * J.k.h;
     const T* vp = static_cast<const T*>(J.v.p) + b * J.v.b + (h / J.v.rep) * J.v.h + n0;
     const T* xp = J.dot ? static_cast<const T*>(J.x.p) + b * J.x.b + (h / J.x.rep) * J.x.h + n0 : nullptr;
+    const int64_t op = b * J.o.b + h * J.o.h + n0;
     const float* gp = p.g + b * p.g_b + h * p.g_h;
-    const int64_t KV = int64_t(J.K) * J.V, chunks = (s1 - s0 + C - 1) / C;
-    const int vdim = J.V - n0, rev = J.rev;
+    const int64_t KV = int64_t(J.K) * J.V;
+    const int chunks = int((s1 - s0 + C - 1) / C), vdim = J.V - n0, rev = J.rev;
+    const bool whole_v = vdim >= 64 * NT;
+    const bool whole = J.K == KP && whole_v && SK::near(J.q.l) && SK::near(J.k.l) && SV::near(J.v.l);
+    const bool near_o = whole_v && SV::near(J.o.l) && SV::near(J.x.l);
 
     // the state before the walk's first token
     const float* from = J.in ? J.in + at.bh * KV : nullptr;
@@ -423,42 +476,61 @@ __global__ __launch_bounds__(256) void la_walk(const LaParams) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * d + 4 * g + r;
-                    S[d][n][r] = f(S[d][n][r], row < J.K && col < J.V, int64_t(row) * J.st_k + int64_t(col) * J.st_v);
+                    S[d][n][r] = f(S[d][n][r], row < J.K && col < J.V, uint32_t(row * J.st_k + col * J.st_v));
                 }
         }
     };
-    each_state([&](float, bool in, int64_t i) { return from && in ? from[i] : 0.f; });
+    if (from) each_state([&](float, bool in, uint32_t i) { return in ? from[i] : 0.f; });
+    else each_state([](float, bool, uint32_t) { return 0.f; });
     const auto write_state = [&](float* to) __attribute__((always_inline)) {
-        each_state([&](float s, bool in, int64_t i) {
+        each_state([&](float s, bool in, uint32_t i) {
             if (in) to[i] = s;
             return s;
         });
     };
 
-    // the halves of P's 32-token steps that no causal tile fills
-    for (int i = threadIdx.x; i < N * C * PS; i += 256) pt[i] = 0;
-    if (threadIdx.x == 0) bad_any = 0;
-
     SK sq, sk;
     SV sv;
-    float gv = 0.f;
-    const auto start = [&](int64_t i) { return s0 + (rev ? chunks - 1 - i : i) * C; };
-    const auto fetch = [&](int64_t i) __attribute__((always_inline)) {
+    float gv = 0.f;                                   // (wave 3) the decays of the chunk after the staged one
+    const auto start = [&](int i) { return s0 + int64_t(rev ? chunks - 1 - i : i) * C; };
+    const auto fetch = [&](int i) __attribute__((always_inline)) {
         const int64_t t0 = start(i);
-        sq.load(qp, J.q.l, t0, end, J.K);
-        sk.load(kp, J.k.l, t0, end, J.K);
-        sv.load(vp, J.v.l, t0, end, vdim);
-        gv = 0.f;
-        if (wave == 0 && lane < C && t0 + lane < end) gv = gp[(t0 + lane) * p.g_l];
+        if (whole && t0 + C <= end) {
+            sq.load_all(qp + t0 * J.q.l, J.q.l);
+            sk.load_all(kp + t0 * J.k.l, J.k.l);
+            sv.load_all(vp + t0 * J.v.l, J.v.l);
+        } else {
+            sq.load(qp, J.q.l, t0, end, J.K);
+            sk.load(kp, J.k.l, t0, end, J.K);
+            sv.load(vp, J.v.l, t0, end, vdim);
+        }
     };
+    const auto fetch_decay = [&](int i) __attribute__((always_inline)) {
+        gv = 0.f;
+        if (wave == 3 && i < chunks) {
+            const int64_t t = start(i) + lane;
+            if (lane < C && t < end) gv = gp[t * p.g_l];
+        }
+    };
+    // the tiles of P's blocks above (in reverse: below) the diagonal
+    for (int i = threadIdx.x; i < N * (C / 32) * 64; i += 256) {
+        const int e = i % 64, row = 32 * (i / 64 % (C / 32)) + (rev ? 16 : 0) + e / 4, token = 32 * (i / 64 % (C / 32)) + (rev ? 0 : 16) + 4 * (e % 4);
+        *reinterpret_cast<u2*>(pt + i / (64 * (C / 32)) * CP::TERM + CP::at(row, token)) = u2{0u, 0u};
+    }
+    if (threadIdx.x == 0) bad_any = 0;
+    if (chunks > 0) {
+        fetch_decay(0);
+        fetch(0);
+        if (wave == 3) decs[0].fill(lane, gv, rev, J.vscale, J.oscale);
+        fetch_decay(1);
+    }
     __syncthreads();
-    if (chunks > 0) fetch(0);
-    for (int64_t ci = 0; ci < chunks; ++ci) {
+    for (int ci = 0; ci < chunks; ++ci) {
         const int64_t t0 = start(ci);
-        (void)sq.store(qt);
-        (void)sk.store(kt);
-        if (sv.store(vt)) bad_any = 1;
-        if (wave == 0) dec.fill(lane, gv, rev, J.vscale, J.oscale);
+        const Decays<C>& dec = decs[ci & 1];
+        (void)sq.template store<false>(qt);
+        (void)sk.template store<false>(kt);
+        if (sv.template store<true>(vt)) bad_any = 1;
         __syncthreads();
         if (ci + 1 < chunks) fetch(ci + 1);
         // A sum over tokens multiplies every v, by P's zeros too: infinities and
@@ -504,22 +576,28 @@ __global__ __launch_bounds__(256) void la_walk(const LaParams) {
                     }
                     acc = mfma_terms<R, R, 2>(kf, qf, acc);
                 }
+                typedef int i4 __attribute__((ext_vector_type(4)));
+                const i4 Ij = *reinterpret_cast<const i4*>(dec.I + 16 * jt + 4 * g);
+                acc *= *reinterpret_cast<const f4*>(dec.col + 16 * jt + 4 * g);
                 const int Ii = dec.I[16 * it + c];
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 4 * g + r;
-                    v[r] = ldexpf(acc[r] * dec.col[16 * jt + j], Ii - dec.I[16 * jt + j]);
-                    if (it == jt && (rev ? j < c : j > c)) v[r] = 0.f;
+                for (int r = 0; r < 4; ++r) v[r] = __builtin_amdgcn_ldexpf(acc[r], Ii - Ij[r]);
+                if (it == jt) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = (rev ? 4 * g + r < c : 4 * g + r > c) ? 0.f : v[r];
                 }
                 uint32_t lo[N], hi[N];
                 split<N>(v[0], v[1], lo);
                 split<N>(v[2], v[3], hi);
 #pragma unroll
                 for (int t = 0; t < N; ++t)
-                    *reinterpret_cast<u2*>(pt + (t * C + 16 * it + c) * PS + 16 * jt + 4 * g) = u2{lo[t], hi[t]};
+                    *reinterpret_cast<u2*>(pt + t * CP::TERM + CP::at(16 * it + c, 16 * jt + 4 * g)) = u2{lo[t], hi[t]};
             }
         }
+        // the next chunk's decays, by the wave with the fewest tiles
+        if (wave == 3 && ci + 1 < chunks) decs[(ci + 1) & 1].fill(lane, gv, rev, J.vscale, J.oscale);
+        fetch_decay(ci + 2);
         __syncthreads();
 
         // o^T: q S with the carried state's factor, then P V
@@ -572,49 +650,75 @@ __global__ __launch_bounds__(256) void la_walk(const LaParams) {
                 if (rev ? 32 * ks + 31 < 16 * it : 32 * ks > 16 * it + 15) continue;
                 u4 pf[N];
 #pragma unroll
-                for (int t = 0; t < N; ++t) pf[t] = *reinterpret_cast<const u4*>(pt + (t * C + 16 * it + c) * PS + 32 * ks + 8 * g);
+                for (int t = 0; t < N; ++t) pf[t] = *reinterpret_cast<const u4*>(pt + t * CP::TERM + CP::at(16 * it + c, 32 * ks + 8 * g));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) o[it][n] = mfma_terms<R, N, kMax>(vf[ks][n], pf, o[it][n]);
             }
+            const float last = dec.row[16 * it + c];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[it][n] *= last;
         }
         const bool last = ci + 1 == chunks;
         if (!last || J.ends || J.out_state) update_state<T, KP, NT, C, SK>(S, kt, vf, dec, J.K, lane);
 
+        float dot[IT] = {};
+        if (near_o && t0 + C <= end && !bad) {
+            const int64_t first = op + t0 * J.o.l;
 #pragma unroll
-        for (int it = 0; it < IT; ++it) {
-            const int i = 16 * it + c;
-            const int64_t t = t0 + i;
-            const bool live = t < len;
-            const float f = dec.row[i];
-            float dot = 0.f;
+            for (int it = 0; it < IT; ++it) {
+                const uint32_t row = uint32_t(c) * uint32_t(J.o.l), xrow = uint32_t(c) * uint32_t(J.x.l);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int col = 16 * (4 * n + wave) + 4 * g, cnt = t < s1 ? vdim - col : 0;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v[r] = live ? o[it][n][r] * f : 0.f;
-                    if (bad && live && col + r < vdim && (rev ? i <= bad_col[col + r] : i >= bad_col[col + r])) v[r] = __builtin_nanf("");
-                }
-                if (cnt > 0) {
-                    const int64_t to = b * J.o.b + t * J.o.l + h * J.o.h + n0 + col;
-                    if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + to, v, cnt);
-                    else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + to, v, cnt);
-                    if (J.dot && live) {
+                for (int n = 0; n < NT; ++n) {
+                    const uint32_t col = uint32_t(16 * (4 * n + wave) + 4 * g);
+                    const float v[4] = {o[it][n][0], o[it][n][1], o[it][n][2], o[it][n][3]};
+                    if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + (first + 16 * it * J.o.l) + (row + col), v, 4);
+                    else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + (first + 16 * it * J.o.l) + (row + col), v, 4);
+                    if (J.dot) {
                         float x[4];
-                        load4<T>(xp + t * J.x.l + col, x, cnt);
+                        load4<T>(xp + (t0 + 16 * it) * J.x.l + (xrow + col), x, 4);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) dot = __builtin_fmaf(v[r], x[r], dot);
+                        for (int r = 0; r < 4; ++r) dot[it] = __builtin_fmaf(v[r], x[r], dot[it]);
                     }
                 }
             }
-            if (J.dot) {
+        } else {
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
+                const int i = 16 * it + c;
+                const int64_t t = t0 + i;
+                const bool live = t < len;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int col = 16 * (4 * n + wave) + 4 * g, cnt = t < s1 ? vdim - col : 0;
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        v[r] = live ? o[it][n][r] : 0.f;
+                        if (bad && live && (rev ? i <= bad_col[col + r] : i >= bad_col[col + r])) v[r] = __builtin_nanf("");
+                    }
+                    if (cnt > 0) {
+                        const int64_t to = op + t * J.o.l + col;
+                        if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + to, v, cnt);
+                        else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + to, v, cnt);
+                        if (J.dot && live) {
+                            float x[4];
+                            load4<T>(xp + t * J.x.l + col, x, cnt);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) dot[it] = __builtin_fmaf(r < cnt ? v[r] : 0.f, x[r], dot[it]);
+                        }
+                    }
+                }
+            }
+        }
+        if (J.dot) {
+#pragma unroll
+            for (int it = 0; it < IT; ++it) {
                 // over the lanes of the token's other columns: g = 0 .. 3
-                auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
-                dot = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-                s = __builtin_amdgcn_permlane16_swap(__float_as_uint(dot), __float_as_uint(dot), false, false);
-                dot = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-                if (g == 0) dots[wave][i] = dot;
+                auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot[it]), __float_as_uint(dot[it]), false, false);
+                float d = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+                s = __builtin_amdgcn_permlane16_swap(__float_as_uint(d), __float_as_uint(d), false, false);
+                d = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+                if (g == 0) dots[wave][16 * it + c] = d;
             }
         }
         if (bad) {
