@@ -77,6 +77,7 @@ __global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
                                        : p.dlast ? p.dlast + bh * int64_t(p.KV) : nullptr;
     if (dS) {
         const float* S = p.ends + (bh * p.segs + seg) * int64_t(p.KV);
+#pragma unroll 8
         for (int i = tid; i < p.KV; i += 256) f += double(S[i]) * double(dS[i]);
     }
     red[tid] = f;
@@ -210,7 +211,9 @@ LaParams common(const ss_linear_attn_args& a) {
     p.g = a.g; p.g_b = a.g_batch_stride; p.g_l = a.g_len_stride; p.g_h = a.g_head_stride;
     p.lens = a.lengths;
     p.seg_tokens = linear_attn_segment(&a);
+    while ((int64_t(1) << p.seg_shift) < p.seg_tokens) ++p.seg_shift;
     p.segs = int(linear_attn_segs(&a));
+    p.rep = int(a.heads / a.groups);
     return p;
 }
 

@@ -13,7 +13,7 @@ namespace ss {
 struct LaRows {
     const void* p;
     int64_t b, l, h;
-    int rep;              // heads per row head: head index is h / rep
+    int rep;              // heads per row head (1, or LaParams' rep): head index is h / rep
 };
 
 // One pass of the recurrence
@@ -49,8 +49,8 @@ struct LaParams {
     const float* g;
     int64_t g_b, g_l, g_h;
     const int32_t* lens;
-    int64_t seg_tokens;
-    int segs;
+    int64_t seg_tokens;               // a power of two, 2^seg_shift
+    int segs, seg_shift, rep;         // rep: heads per group
     int serial;                       // a workgroup walks a whole row (else a segment, from its carry)
     int tile, tiles;                  // value columns per workgroup, and tiles of the widest job
 };

@@ -316,15 +316,27 @@ __device__ __forceinline__ Params& params() { return *(Params*)__builtin_amdgcn_
 
 // Workgroup order: the jobs of a segment (they read the same rows), then its column
 // tiles, side by side on one XCD.
-struct Place { int job, tile, seg; int64_t bh; };      // (bh past the last one: nothing to do)
-__device__ __forceinline__ Place place(Params& p, int tiles, int segs) {
-    int64_t id = xcd_block_id();
+// (32-bit divisions: a launch holds fewer than 2^24 workgroups, and the 64-bit
+// ones cost a short walk a tenth of its time.)
+struct Place { int job, tile, seg; uint32_t bh, b, h, shared; };      // (bh past the last one: nothing to do)
+__device__ __forceinline__ Place place(Params& p, uint32_t segs) {
+    uint32_t id = uint32_t(xcd_block_id());
     Place r;
-    r.job = int(id % p.njobs); id /= p.njobs;
-    r.tile = int(id % tiles); id /= tiles;
+    const uint32_t jobs = p.njobs, tiles = p.tiles, H = uint32_t(p.H);
+    r.job = int(id % jobs);
+    id /= jobs;
+    r.tile = tiles > 1 ? int(id % tiles) : 0;
+    if (tiles > 1) id /= tiles;
     r.seg = int(id % segs);
     r.bh = id / segs;
+    r.b = r.bh / H;
+    r.h = r.bh - r.b * H;
+    r.shared = p.rep > 1 ? r.h / uint32_t(p.rep) : r.h;      // the group whose q and k head h reads
     return r;
+}
+template <typename T, typename Row>
+__device__ __forceinline__ const T* rows_of_head(Row& r, const Place& at) {
+    return static_cast<const T*>(r.p) + int64_t(at.b) * r.b + int64_t(r.rep > 1 ? at.shared : at.h) * r.h;
 }
 
 // ------------------------------------------------------- state of a segment --
@@ -337,16 +349,16 @@ __global__ __launch_bounds__(256) void la_local(const LaParams) {
     using SV = Stage<T, C, 64 * NT>;
     __shared__ __attribute__((aligned(16))) uint16_t kt[R * SK::TERM], vt[R * SV::TERM];
     __shared__ Decays<C> dec;
-    const Place at = place(p, p.tiles, p.segs);
+    const Place at = place(p, p.segs);
     Job& J = p.job[at.job];
     const int n0 = at.tile * 64 * NT;
-    if (n0 >= J.V || at.bh >= p.B * p.H) return;
-    const int64_t b = at.bh / p.H, h = at.bh % p.H;
+    if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
+    const int64_t b = at.b, h = at.h, bh = at.bh;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int64_t s0 = at.seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
     const int64_t len = tokens_of(p.lens, b, p.L), end = len < s1 ? len : s1;
-    const T* kp = static_cast<const T*>(J.k.p) + b * J.k.b + (h / J.k.rep) * J.k.h;
-    const T* vp = static_cast<const T*>(J.v.p) + b * J.v.b + (h / J.v.rep) * J.v.h + n0;
+    const T* kp = rows_of_head<T>(J.k, at);
+    const T* vp = rows_of_head<T>(J.v, at) + n0;
     const float* gp = p.g + b * p.g_b + h * p.g_h;
     const int chunks = int((s1 - s0 + C - 1) / C), vdim = J.V - n0;
     const bool whole = J.K == KP && vdim >= 64 * NT && SK::near(J.k.l) && SV::near(J.v.l);
@@ -390,7 +402,7 @@ __global__ __launch_bounds__(256) void la_local(const LaParams) {
         update_state<T, KP, NT, C, SK>(S, kt, vf, dec, J.K, lane);
         __syncthreads();
     }
-    float* to = J.ends + (at.bh * p.segs + at.seg) * int64_t(J.K) * J.V;
+    float* to = J.ends + (bh * p.segs + at.seg) * int64_t(J.K) * J.V;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int col = n0 + 16 * (4 * n + wave) + c;
@@ -402,7 +414,7 @@ __global__ __launch_bounds__(256) void la_local(const LaParams) {
                 if (row < J.K && col < J.V) to[int64_t(row) * J.st_k + int64_t(col) * J.st_v] = S[d][n][r];
             }
     }
-    if (threadIdx.x == 0 && at.tile == 0) J.decays[at.bh * p.segs + at.seg] = decay;
+    if (threadIdx.x == 0 && at.tile == 0) J.decays[bh * p.segs + at.seg] = decay;
 }
 
 // ----------------------------------------------------------------- the walk --
@@ -439,32 +451,33 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const
     __shared__ float dots[4][C];
     __shared__ int bad_any, bad_col[64 * NT];
     const int segs = p.serial ? 1 : p.segs;
-    const Place at = place(p, p.tiles, segs);
+    const Place at = place(p, segs);
     Job& J = p.job[at.job];
     const int n0 = at.tile * 64 * NT;
-    if (n0 >= J.V || at.bh >= p.B * p.H) return;
-    const int64_t b = at.bh / p.H, h = at.bh % p.H;
+    if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
+    const int64_t b = at.b, h = at.h, bh = at.bh;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int64_t span = p.serial ? p.L : p.seg_tokens;
     const int64_t s0 = at.seg * span, s1 = s0 + span < p.L ? s0 + span : p.L;
     const int64_t len = tokens_of(p.lens, b, p.L), end = len < s1 ? len : s1;
-    const T* qp = static_cast<const T*>(J.q.p) + b * J.q.b + (h / J.q.rep) * J.q.h;
-    const T* kp = static_cast<const T*>(J.k.p) + b * J.k.b + (h / J.k.rep) * J.k.h;
-    const T* vp = static_cast<const T*>(J.v.p) + b * J.v.b + (h / J.v.rep) * J.v.h + n0;
-    const T* xp = J.dot ? static_cast<const T*>(J.x.p) + b * J.x.b + (h / J.x.rep) * J.x.h + n0 : nullptr;
+    const T* qp = rows_of_head<T>(J.q, at);
+    const T* kp = rows_of_head<T>(J.k, at);
+    const T* vp = rows_of_head<T>(J.v, at) + n0;
+    const T* xp = J.dot ? rows_of_head<T>(J.x, at) + n0 : nullptr;
     const int64_t op = b * J.o.b + h * J.o.h + n0;
     const float* gp = p.g + b * p.g_b + h * p.g_h;
     const int64_t KV = int64_t(J.K) * J.V;
     const int chunks = int((s1 - s0 + C - 1) / C), vdim = J.V - n0, rev = J.rev;
+    const int64_t seg_mask = p.seg_tokens - 1;
     const bool whole_v = vdim >= 64 * NT;
     const bool whole = J.K == KP && whole_v && SK::near(J.q.l) && SK::near(J.k.l) && SV::near(J.v.l);
     const bool near_o = whole_v && SV::near(J.o.l) && SV::near(J.x.l);
 
     // the state before the walk's first token
-    const float* from = J.in ? J.in + at.bh * KV : nullptr;
+    const float* from = J.in ? J.in + bh * KV : nullptr;
     if (!p.serial) {
         const int before = rev ? at.seg + 1 : at.seg - 1;
-        if (before >= 0 && before < p.segs) from = J.carry + (at.bh * p.segs + before) * KV;
+        if (before >= 0 && before < p.segs) from = J.carry + (bh * p.segs + before) * KV;
     }
     f4 S[KP / 16][NT];
     const auto each_state = [&](auto&& f) __attribute__((always_inline)) {
@@ -733,15 +746,15 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const
                 }
             }
         }
-        if (J.ends && (rev ? t0 % p.seg_tokens == 0 : (t0 + C) % p.seg_tokens == 0 || last))
-            write_state(J.ends + (at.bh * p.segs + t0 / p.seg_tokens) * KV);
+        if (J.ends && ((rev ? t0 & seg_mask : (t0 + C) & seg_mask) == 0 || (!rev && last)))
+            write_state(J.ends + (bh * p.segs + (t0 >> p.seg_shift)) * KV);
         __syncthreads();
         if (J.dot && int(threadIdx.x) < C && t0 + threadIdx.x < s1)
-            J.dot[(int64_t(at.tile) * p.B * p.H + at.bh) * p.L + t0 + threadIdx.x] =
+            J.dot[(int64_t(at.tile) * p.B * p.H + bh) * p.L + t0 + threadIdx.x] =
                 (dots[0][threadIdx.x] + dots[1][threadIdx.x]) + (dots[2][threadIdx.x] + dots[3][threadIdx.x]);
     }
-    if (chunks == 0 && J.ends) write_state(J.ends + at.bh * p.segs * KV);
-    if (J.out_state) write_state(J.out_state + at.bh * KV);
+    if (chunks == 0 && J.ends) write_state(J.ends + bh * p.segs * KV);
+    if (J.out_state) write_state(J.out_state + bh * KV);
 }
 
 }  // namespace la
