@@ -163,13 +163,17 @@ __global__ __launch_bounds__(256) void la_group_sum(const float* part0, T* out0,
 
 // Workgroups that fill the GPU: with fewer rows (batch x heads x tiles) than
 // that a row's segments run side by side, about kSegsWanted of them in all.
-constexpr int64_t kFull = 1024, kSegsWanted = 1536, kSegTokMin = 128, kSegTokMax = 1024;
+constexpr int64_t kFull = 1024, kSegsWanted = 1536, kSegTokMin = 64, kSegTokMax = 1024;
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
+int64_t type_size(const ss_linear_attn_args& a) { return a.dtype == SS_F32 ? 4 : 2; }
 int64_t tile_count(int64_t dim, int tile) { return (dim + tile - 1) / tile; }
 // the backward's passes share a launch: the tile of the widest
-int bwd_tile(const ss_linear_attn_args& a) { return la_tile(a.d_key > a.d_value ? a.d_key : a.d_value); }
+int bwd_tile(const ss_linear_attn_args& a) {
+    const int64_t d = a.d_key > a.d_value ? a.d_key : a.d_value;
+    return la_tile(d, d, type_size(a));
+}
 
 struct BwdSpace { int64_t dotq, dotk, rends, decays, part, dq, dk, bytes; };
 BwdSpace bwd_space(const ss_linear_attn_bwd_args* g) {
@@ -198,7 +202,7 @@ bool serial(const ss_linear_attn_args& a, int64_t tiles) {
 struct FwdSpace { int64_t ends, decays, bytes; };
 FwdSpace fwd_space(const ss_linear_attn_args& a) {
     FwdSpace s{};
-    if (serial(a, tile_count(a.d_value, la_tile(a.d_value)))) return s;
+    if (serial(a, tile_count(a.d_value, la_tile(a.d_key, a.d_value, type_size(a))))) return s;
     const int64_t n = a.batch * a.heads * linear_attn_segs(&a);
     s.decays = a.ends ? 0 : round16(n * a.d_key * a.d_value * 4);
     s.bytes = s.decays + round16(n * 4);
@@ -260,7 +264,7 @@ hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stre
     LaParams p = common(*a);
     const int rep = int(a->heads / a->groups);
     p.njobs = 1;
-    p.tile = la_tile(a->d_value);
+    p.tile = la_tile(a->d_key, a->d_value, type_size(*a));
     p.tiles = int(tile_count(a->d_value, p.tile));
     p.serial = serial(*a, p.tiles);
     LaJob& j = p.job[0];

@@ -55,9 +55,15 @@ struct LaParams {
     int tile, tiles;                  // value columns per workgroup, and tiles of the widest job
 };
 
-// value columns per workgroup
-inline int la_tile(int64_t dim) { return dim <= 64 ? 64 : 128; }
-inline int la_tiles(int64_t dim) { return int((dim + la_tile(dim) - 1) / la_tile(dim)); }
+// Most value columns a workgroup takes for q and k of up to k columns, in rows of
+// this element size: the state's share and the rows on their way stay within the
+// 256 registers a lane that let two waves share a SIMD.
+constexpr int la_cols(int64_t k, int64_t size) { return k <= 64 ? (size == 2 ? 64 : 32) : k <= 128 ? 32 : 16; }
+// ... and those it takes of v columns: a multiple of 16, the shares even.
+inline int la_tile(int64_t k, int64_t v, int64_t size) {
+    const int64_t most = la_cols(k, size) / 16, cols = (v + 15) / 16, n = (cols + most - 1) / most;
+    return int((cols + n - 1) / n * 16);
+}
 
 // The segments' states from a zero start and their decays (job.ends,
 // job.decays); and the walk itself.  fine: 16-bit rows, too, with what is

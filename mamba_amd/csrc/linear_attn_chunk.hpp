@@ -1,9 +1,11 @@
 // Linear attention with a decay for each head: the chunked form of LaJob's
 // pass on the matrix cores (gfx950).
 //
-// A workgroup walks the chunks (C tokens) of one segment, or of a whole row,
-// for one (batch, head) and 64 NT value columns; its 4 waves share the
-// columns in tiles of 16 and hold the state of their tiles in registers.
+// A wave walks the chunks (32 tokens) of one segment, or of a whole row, for
+// one (batch, head) and up to 16 NT value columns, and holds the state of its
+// columns in registers.  Waves do not meet: a workgroup is one wave, and the 6 to
+// 12 of a CU hide each other's loads.  (Four waves that shared a 64-token chunk
+// and met at three barriers in it spent half their time waiting.)
 // With G the sum of the log2 decays from the chunk's start up to a token
 // (itself included), the forward chunk is
 //
@@ -25,12 +27,16 @@
 // to 16 bits; states, and gradients that the decay's gradient is summed from,
 // take 3.
 //
-// Layouts.  A 16x16x32 instruction takes 8 consecutive summands a lane (lane
-// l: row or column l % 16, summands 8 (l / 16) ..) and returns 4 consecutive
-// rows of a column.  q and k lie in LDS as rows, so q k^T reads both with
-// 16-byte loads; sums over tokens (P V, the state's update) read v and k through
-// the transposing LDS load; the state's registers are used as they are, with
-// q read in the same order of summands.  P crosses LDS between the waves.
+// Layouts.  A 16x16x32 instruction takes 8 summands a lane (lane l: row or
+// column l % 16, summands 8 (l / 16) ..) and returns 4 consecutive rows of a
+// column.  Which summand a slot holds is free as long as both operands agree,
+// and that keeps everything but k and v out of LDS:
+//  - q and k come from global memory as operands, 8 elements of a row a lane;
+//  - the state's rows are numbered so that the registers a lane holds are the 8
+//    elements of q that it multiplies (state_row);
+//  - P's registers are an operand as they are, in the token order of tok();
+//  - sums over tokens read k and v in that order through the transposing LDS
+//    load, where 16 lanes read 4 rows of 16 elements and get a column of 4 each.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -81,6 +87,13 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&t)[N]) {
 __device__ __forceinline__ float lo_half(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_half(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// LDS of a wave: its accesses run in order; this keeps the compiler's order.
+__device__ __forceinline__ void lds_in_order() { __asm__ volatile("" ::: "memory"); }
+
+// No instruction moves across: without it the scheduler raises the loads and
+// splits of all steps to the front and runs out of registers.
+__device__ __forceinline__ void stage_end() { __builtin_amdgcn_sched_barrier(0); }
+
 // c += sum of the products of a's NA and b's NB terms whose order is at most
 // kMax (2: down to 2^-24; 1: to 2^-16), small ones first
 template <int NA, int NB, int kMax>
@@ -96,18 +109,23 @@ __device__ __forceinline__ f4 mfma_terms(const u4 (&a)[NA], const u4 (&b)[NB], f
     return c;
 }
 
-// 8 summands of column col0 + lane % 16 of rows row0 + 8 (lane / 16) .. of a
-// row-major LDS tile, by two transposing loads (the 16 lanes of a group read
-// 4 rows of 16 elements and get a column of 4 each)
+constexpr int C = 32;                     // tokens per chunk
+
+// Slot i of lane group g holds token 4 g + i (i < 4) or 16 + 4 g + i - 4.
+// The 8 tokens of a column of a row-major LDS tile; block: first column of the 4
+// that this lane reads for its 16-lane group.
 template <int STRIDE>
-__device__ __forceinline__ u4 load_cols(const uint16_t* tile, int row0, int col0, int lane) {
+__device__ __forceinline__ u4 load_tokens(const uint16_t* tile, int block, int lane) {
     const int g = lane >> 4, c = lane & 15;
-    const uint16_t* p = tile + (row0 + 8 * g + (c >> 2)) * STRIDE + col0 + 4 * (c & 3);
+    const uint16_t* p = tile + (4 * g + (c >> 2)) * STRIDE + block;
     typedef __attribute__((address_space(3))) s4 lds_s4;
     const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
-    const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * STRIDE)));
+    const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 16 * STRIDE)));
     return u4{lo.x, lo.y, hi.x, hi.y};
 }
+
+// The state's tile t (16 rows), register r of lane group g: row of the state
+__device__ __forceinline__ int state_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
 
 // 4 consecutive elements, the first cnt of them
 typedef uint32_t half4_at2 __attribute__((ext_vector_type(2), aligned(2)));
@@ -149,54 +167,57 @@ __device__ __forceinline__ void load4(const T* p, float (&v)[4], int cnt) {
     for (int i = 0; i < 4; ++i) v[i] = i < cnt ? io<T>::load(p + i) : 0.f;
 }
 
-template <typename T> constexpr int kChunk = sizeof(T) == 2 && kTerms<T> == 1 ? 64 : 32;   // tokens per chunk
+// a vector of a row that may not exist, and (unless WHOLE) may end inside it
+template <typename T, bool WHOLE>
+__device__ __forceinline__ uint4 load_part(const T* p, bool in, int n) {
+    if constexpr (WHOLE) {
+        if (!in) return make_uint4(0u, 0u, 0u, 0u);
+        const typename rowvec<T>::words w = *reinterpret_cast<const typename rowvec<T>::words*>(p);
+        return make_uint4(w.x, w.y, w.z, w.w);
+    } else {
+        return rowvec<T>::load(p, in ? n : 0);
+    }
+}
 
-// Rows of a tile on their way from global memory to LDS.
-template <typename T, int C, int WIDTH>
+// A chunk's rows of v on their way from global memory to LDS.
+template <typename T, int WIDTH>
 struct Stage {
     using R = rowvec<T>;
-    static constexpr int PER_ROW = WIDTH / R::VE, N = (C * PER_ROW + 255) / 256, STRIDE = WIDTH + 8, TERMS = kTerms<T>;
+    static constexpr int PER_ROW = WIDTH / R::VE, N = C * PER_ROW / 64, STRIDE = WIDTH + 8, TERMS = kTerms<T>;
     static constexpr int TERM = C * STRIDE;                  // elements of one term's tile
-    static constexpr int STEP = 256 / PER_ROW;               // rows between a thread's vectors
-    static constexpr bool PARTIAL = C * PER_ROW % 256 != 0;  // threads without a row
+    static constexpr int STEP = 64 / PER_ROW;                // rows between a lane's vectors
     uint4 v[N];
 
-    // whether a tile of rows `step` elements apart is within 32-bit byte offsets of its first
-    static __device__ __forceinline__ bool near(int64_t step) { return step < (int64_t(1) << 24); }
-    // all rows of p (a row every `step` elements, a tile that is near), whole
-    __device__ __forceinline__ void load_all(const T* p, int64_t step) {
-        const int row = int(threadIdx.x) / PER_ROW, col = int(threadIdx.x) % PER_ROW * R::VE;
-        const uint32_t off = (uint32_t(row) * uint32_t(step) + uint32_t(col)) * uint32_t(sizeof(T));
+    // all rows of p (a row every `step` elements, near), whole
+    __device__ __forceinline__ void load_all(const T* p, int64_t step, int lane) {
+        const uint32_t off = (uint32_t(lane / PER_ROW) * uint32_t(step) + uint32_t(lane % PER_ROW * R::VE)) * uint32_t(sizeof(T));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (PARTIAL && row >= C) continue;
             const typename R::words w = *reinterpret_cast<const typename R::words*>(
                 reinterpret_cast<const char*>(p + int64_t(i * STEP) * step) + off);
             v[i] = make_uint4(w.x, w.y, w.z, w.w);
         }
     }
-    // rows t0 .. of p, dim elements each; rows from `end` on are zero
-    __device__ __forceinline__ void load(const T* p, int64_t step, int64_t t0, int64_t end, int dim) {
+    // the first `rows` rows of p, dim elements each; the others are zero
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int dim, int lane) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int at = int(threadIdx.x) + 256 * i, row = at / PER_ROW, col = at % PER_ROW * R::VE;
-            const int64_t t = t0 + row;
-            v[i] = R::load(p + t * step + col, row < C && t < end ? dim - col : 0);
+            const int row = lane / PER_ROW + i * STEP, col = lane % PER_ROW * R::VE;
+            v[i] = load_part<T, WHOLE>(p + int64_t(row) * step + col, row < rows, dim - col);
         }
     }
     // into the terms' tiles; CHECK: whether an element is infinite or NaN
     template <bool CHECK>
-    __device__ __forceinline__ bool store(uint16_t* tile) const {
+    __device__ __forceinline__ bool store(uint16_t* tile, int lane) const {
         typedef uint16_t h2 __attribute__((ext_vector_type(2)));
         h2 top = {0, 0};                                     // the largest exponents
         const auto look = [&](uint32_t w) {
             if constexpr (CHECK) top = __builtin_elementwise_max(top, __builtin_bit_cast(h2, w & 0x7f807f80u));
         };
-        const int row = int(threadIdx.x) / PER_ROW, col = int(threadIdx.x) % PER_ROW * R::VE;
-        if (PARTIAL && row >= C) return false;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            uint16_t* to = tile + row * STRIDE + col + i * STEP * STRIDE;
+            uint16_t* to = tile + (lane / PER_ROW + i * STEP) * STRIDE + lane % PER_ROW * R::VE;
             if constexpr (TERMS == 1) {
                 look(v[i].x); look(v[i].y); look(v[i].z); look(v[i].w);
                 *reinterpret_cast<uint4*>(to) = v[i];
@@ -219,40 +240,108 @@ struct Stage {
         return top.x >= 0x7f80 || top.y >= 0x7f80;
     }
 };
+// whether a chunk of rows `step` elements apart lies within 32-bit byte offsets
+__device__ __forceinline__ bool near(int64_t step) { return step < (int64_t(1) << 24); }
 
-// The chunk's decays.  Lane t of one wave holds token t's log decay (0 past
-// the row's end).
-template <int C>
+// A chunk's rows of q or k as operands: row 16 i + lane % 16, elements 32 kk + 8 (lane / 16) ..
+template <typename T, int KP>
+struct Rows {
+    using R = rowvec<T>;
+    static constexpr int W = int(sizeof(T)) / 2, STRIDE = KP + 8, TERMS = kTerms<T>, TERM = C * STRIDE;
+    uint4 v[2][KP / 32][W];
+
+    __device__ __forceinline__ void load_all(const T* p, int64_t step, int lane) {
+        const uint32_t off = (uint32_t(lane & 15) * uint32_t(step) + uint32_t(8 * (lane >> 4))) * uint32_t(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int kk = 0; kk < KP / 32; ++kk)
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const typename R::words x = *reinterpret_cast<const typename R::words*>(
+                        reinterpret_cast<const char*>(p + int64_t(16 * i) * step) + off + (32 * kk * int(sizeof(T)) + 16 * w));
+                    v[i][kk][w] = make_uint4(x.x, x.y, x.z, x.w);
+                }
+    }
+    template <bool WHOLE>
+    __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int dim, int lane) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int kk = 0; kk < KP / 32; ++kk)
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const int row = 16 * i + (lane & 15), col = 32 * kk + 8 * (lane >> 4) + w * R::VE;
+                    v[i][kk][w] = load_part<T, WHOLE>(p + int64_t(row) * step + col, row < rows, dim - col);
+                }
+    }
+    __device__ __forceinline__ void terms(int i, int kk, u4 (&t)[TERMS]) const {
+        if constexpr (TERMS == 1) {
+            t[0] = u4{v[i][kk][0].x, v[i][kk][0].y, v[i][kk][0].z, v[i][kk][0].w};
+        } else {
+            float x[8];
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                float y[R::VE];
+                R::unpack(v[i][kk][w], y);
+#pragma unroll
+                for (int e = 0; e < R::VE; ++e) x[w * R::VE + e] = y[e];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t s[TERMS];
+                split<TERMS>(x[2 * k], x[2 * k + 1], s);
+#pragma unroll
+                for (int n = 0; n < TERMS; ++n) t[n][k] = s[n];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uint16_t* tile, int lane) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int kk = 0; kk < KP / 32; ++kk) {
+                u4 t[TERMS];
+                terms(i, kk, t);
+#pragma unroll
+                for (int n = 0; n < TERMS; ++n)
+                    *reinterpret_cast<u4*>(tile + n * TERM + (16 * i + (lane & 15)) * STRIDE + 32 * kk + 8 * (lane >> 4)) = t[n];
+            }
+    }
+};
+
+// The decays of two neighbouring chunks.  Lane t holds token t's log decay (0
+// past the row's end).
 struct __attribute__((aligned(16))) Decays {
-    int I[C];              // integer part of H (G, or -G in reverse)
-    float col[C];          // 2^-F, with the factor of v
-    float row[C];          // 2^F, with the factor of o
-    float in[C];           // the carried state's factor at a token over `row`'s 2^F
-    float upd[C];          // a token's factor in the state's update, with the factor of v
-    float total;           // 2^G_C
+    int I[64];             // integer part of H (G, or -G in reverse)
+    float col[64];         // 2^-F, with the factor of v
+    float row[64];         // 2^F, with the factor of o
+    float in[64];          // the carried state's factor at a token over `row`'s 2^F
+    float upd[64];         // a token's factor in the state's update, with the factor of v
+    float total[2];        // 2^G_C
 
     __device__ __forceinline__ static float exp2_of(double x) {
         const double i = floor(x);
-        return ldexpf(__builtin_amdgcn_exp2f(float(x - i)), i < -2000.0 ? -2000 : i > 2000.0 ? 2000 : int(i));
+        return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(float(x - i)), i < -2000.0 ? -2000 : i > 2000.0 ? 2000 : int(i));
     }
-    __device__ __forceinline__ void fill(int t, float g, bool rev, float vscale, float oscale) {
+    __device__ __forceinline__ void fill(int lane, float g, bool rev, float vscale, float oscale) {
         double h = double(g) * 1.4426950408889634;
         h = h < kDeepest ? double(kDeepest) : h;          // (NaN stays)
+        const int t = lane & 31;
 #pragma unroll
-        for (int m = 1; m < C; m <<= 1) {
-            const double o = __shfl_up(h, m, 64);
+        for (int m = 1; m < 32; m <<= 1) {
+            const double o = __shfl_up(h, m, 32);
             if (t >= m) h += o;
         }
-        const double G = __shfl(h, C - 1, 64);
-        if (t >= C) return;
+        const double G = __shfl(h, 31, 32);
         const double H = rev ? -h : h, fl = floor(H);
         const float F = float(H - fl);
-        I[t] = int(fl);
-        col[t] = vscale * __builtin_amdgcn_exp2f(-F);
-        row[t] = oscale * __builtin_amdgcn_exp2f(F);
-        in[t] = exp2_of((rev ? H + G : H) - double(F));
-        upd[t] = vscale * exp2_of(rev ? -H : G - H);
-        if (t == 0) total = exp2_of(G);
+        I[lane] = int(fl);
+        col[lane] = vscale * __builtin_amdgcn_exp2f(-F);
+        row[lane] = oscale * __builtin_amdgcn_exp2f(F);
+        in[lane] = exp2_of((rev ? H + G : H) - double(F));
+        upd[lane] = vscale * exp2_of(rev ? -H : G - H);
+        if (t == 0) total[lane >> 5] = exp2_of(G);
     }
 };
 
@@ -262,48 +351,69 @@ __device__ __forceinline__ int64_t tokens_of(const int32_t* lens, int64_t b, int
     return n < 0 ? 0 : n < L ? n : L;
 }
 
-// S <- total S + sum over the chunk's tokens of k_t (w_t v_t)^T.  kt: k's tile; vf: v's
-// columns of this wave, 8 tokens a lane and 32-token step.
-template <typename T, int KP, int NT, int C, typename SK>
-__device__ __forceinline__ void update_state(f4 (&S)[KP / 16][NT], const uint16_t* kt, const u4 (&vf)[C / 32][NT][kTerms<T>],
-                                             const Decays<C>& dec, int dims, int lane) {
+// S <- total S + sum over the chunk's tokens of k_t (w_t v_t)^T.  kt: k's tile;
+// vf: v's columns; half: the chunk of the two in dec.
+template <typename T, int KP, int NT, bool WHOLE>
+__device__ __forceinline__ void update_state(f4 (&S)[KP / 16][NT], const uint16_t* kt, const u4 (&vf)[NT][kTerms<T>],
+                                             const Decays& dec, int half, int kdim, int vdim, int lane) {
     constexpr int R = kTerms<T>;
-    const float tot = dec.total;
+    using SK = Rows<T, KP>;
+    const float tot = dec.total[half];
+    const f4 u0 = *reinterpret_cast<const f4*>(dec.upd + 32 * half + 4 * (lane >> 4));
+    const f4 u1 = *reinterpret_cast<const f4*>(dec.upd + 32 * half + 16 + 4 * (lane >> 4));
+    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
     for (int d = 0; d < KP / 16; ++d)
 #pragma unroll
         for (int n = 0; n < NT; ++n) S[d][n] *= tot;
+    // v's columns n, weighted, in 3 terms
+    const auto weighted = [&](int n, u4 (&bv)[3]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int ks = 0; ks < C / 32; ++ks) {
-        const f4* up = reinterpret_cast<const f4*>(dec.upd + 32 * ks + 8 * (lane >> 4));
-        const f4 u0 = up[0], u1 = up[1];
-        const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-        u4 bv[NT][3];
+        for (int w = 0; w < 4; ++w) {
+            float x0 = lo_half(vf[n][R - 1][w]), x1 = hi_half(vf[n][R - 1][w]);
+#pragma unroll
+            for (int r = R - 2; r >= 0; --r) {                // small terms first: the sum is exact
+                x0 += lo_half(vf[n][r][w]);
+                x1 += hi_half(vf[n][r][w]);
+            }
+            uint32_t t[3];
+            split<3>(x0 * u[2 * w], x1 * u[2 * w + 1], t);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) bv[i][w] = t[i];
+        }
+    };
+    const auto rows = [&](int d, u4 (&kf)[R]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            kf[r] = load_tokens<SK::STRIDE>(kt + r * SK::TERM, 32 * (d >> 1) + 8 * (lane & 3) + 4 * (d & 1), lane);
+    };
+    // (whichever of the two takes fewer registers is held)
+    if constexpr (KP / 16 * R <= 3 * NT) {
+        u4 kf[KP / 16][R];
+#pragma unroll
+        for (int d = 0; d < KP / 16; ++d) rows(d, kf[d]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
+            if (!WHOLE && 16 * n >= vdim) continue;
+            u4 bv[3];
+            weighted(n, bv);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                float x0 = lo_half(vf[ks][n][R - 1][w]), x1 = hi_half(vf[ks][n][R - 1][w]);
-#pragma unroll
-                for (int r = R - 2; r >= 0; --r) {            // small terms first: the sum is exact
-                    x0 += lo_half(vf[ks][n][r][w]);
-                    x1 += hi_half(vf[ks][n][r][w]);
-                }
-                uint32_t t[3];
-                split<3>(x0 * u[2 * w], x1 * u[2 * w + 1], t);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) bv[n][i][w] = t[i];
-            }
+            for (int d = 0; d < KP / 16; ++d) S[d][n] = mfma_terms<R, 3, 2>(kf[d], bv, S[d][n]);
+            stage_end();
         }
+    } else {
+        u4 bv[NT][3];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) weighted(n, bv[n]);
 #pragma unroll
         for (int d = 0; d < KP / 16; ++d) {
-            if (16 * d < dims) {
-                u4 kf[R];
+            if (!WHOLE && 32 * (d >> 1) >= kdim) continue;
+            u4 kf[R];
+            rows(d, kf);
 #pragma unroll
-                for (int r = 0; r < R; ++r) kf[r] = load_cols<SK::STRIDE>(kt + r * SK::TERM, 32 * ks, 16 * d, lane);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) S[d][n] = mfma_terms<R, 3, 2>(kf, bv[n], S[d][n]);
-            }
+            for (int n = 0; n < NT; ++n)
+                if (WHOLE || 16 * n < vdim) S[d][n] = mfma_terms<R, 3, 2>(kf, bv[n], S[d][n]);
+            stage_end();
         }
     }
 }
@@ -327,10 +437,11 @@ __device__ __forceinline__ Place place(Params& p, uint32_t segs) {
     id /= jobs;
     r.tile = tiles > 1 ? int(id % tiles) : 0;
     if (tiles > 1) id /= tiles;
+    r.h = id % H;
+    id /= H;
     r.seg = int(id % segs);
-    r.bh = id / segs;
-    r.b = r.bh / H;
-    r.h = r.bh - r.b * H;
+    r.b = id / segs;
+    r.bh = r.b * H + r.h;
     r.shared = p.rep > 1 ? r.h / uint32_t(p.rep) : r.h;      // the group whose q and k head h reads
     return r;
 }
@@ -339,139 +450,151 @@ __device__ __forceinline__ const T* rows_of_head(Row& r, const Place& at) {
     return static_cast<const T*>(r.p) + int64_t(at.b) * r.b + int64_t(r.rep > 1 ? at.shared : at.h) * r.h;
 }
 
-// ------------------------------------------------------- state of a segment --
-// Each segment's state from a zero start, and its decay.
-template <typename T, int KP, int NT>
-__global__ __launch_bounds__(256) void la_local(const LaParams) {
-    Params& p = params();
-    constexpr int C = kChunk<T>, R = kTerms<T>;
-    using SK = Stage<T, C, KP>;
-    using SV = Stage<T, C, 64 * NT>;
-    __shared__ __attribute__((aligned(16))) uint16_t kt[R * SK::TERM], vt[R * SV::TERM];
-    __shared__ Decays<C> dec;
-    const Place at = place(p, p.segs);
-    Job& J = p.job[at.job];
-    const int n0 = at.tile * 64 * NT;
-    if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
-    const int64_t b = at.b, h = at.h, bh = at.bh;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int64_t s0 = at.seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
-    const int64_t len = tokens_of(p.lens, b, p.L), end = len < s1 ? len : s1;
-    const T* kp = rows_of_head<T>(J.k, at);
-    const T* vp = rows_of_head<T>(J.v, at) + n0;
-    const float* gp = p.g + b * p.g_b + h * p.g_h;
-    const int chunks = int((s1 - s0 + C - 1) / C), vdim = J.V - n0;
-    const bool whole = J.K == KP && vdim >= 64 * NT && SK::near(J.k.l) && SV::near(J.v.l);
+// The tokens of a workgroup and what it reads of them, in the walk's order.
+template <typename T, int KP, int NT, bool Q, bool WHOLE>
+struct Walk {
+    Params& p;
+    Job& J;
+    int64_t s0, s1, end;              // tokens: the span, and where the row's own end in it
+    const T* qp; const T* kp; const T* vp; const float* gp;
+    int chunks, vdim, lane;
+    bool rev, whole;
+    Rows<T, KP> q, k;
+    Stage<T, 16 * NT> v;
 
-    f4 S[KP / 16][NT];
-#pragma unroll
-    for (int d = 0; d < KP / 16; ++d)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) S[d][n] = f4{0.f, 0.f, 0.f, 0.f};
-    float decay = 1.f;
-    SK sk;
-    SV sv;
-    float gv = 0.f;
-    const auto fetch = [&](int i) __attribute__((always_inline)) {
-        const int64_t t0 = s0 + int64_t(J.rev ? chunks - 1 - i : i) * C;
-        if (whole && t0 + C <= end) {
-            sk.load_all(kp + t0 * J.k.l, J.k.l);
-            sv.load_all(vp + t0 * J.v.l, J.v.l);
-        } else {
-            sk.load(kp, J.k.l, t0, end, J.K);
-            sv.load(vp, J.v.l, t0, end, vdim);
-        }
-        gv = 0.f;
-        if (wave == 0 && lane < C && t0 + lane < end) gv = gp[(t0 + lane) * p.g_l];
-    };
-    fetch(0);
-    for (int i = 0; i < chunks; ++i) {
-        (void)sk.template store<false>(kt);
-        (void)sv.template store<false>(vt);
-        if (wave == 0) dec.fill(lane, gv, J.rev, J.vscale, 1.f);
-        __syncthreads();
-        if (i + 1 < chunks) fetch(i + 1);
-        u4 vf[C / 32][NT][R];
-#pragma unroll
-        for (int ks = 0; ks < C / 32; ++ks)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int r = 0; r < R; ++r) vf[ks][n][r] = load_cols<SV::STRIDE>(vt + r * SV::TERM, 32 * ks, 16 * (4 * n + wave), lane);
-        decay *= dec.total;
-        update_state<T, KP, NT, C, SK>(S, kt, vf, dec, J.K, lane);
-        __syncthreads();
+    __device__ __forceinline__ Walk(Params& p_, Job& J_, const Place& at, int64_t span, int lane_) : p(p_), J(J_), lane(lane_) {
+        s0 = at.seg * span;
+        s1 = s0 + span < p.L ? s0 + span : p.L;
+        const int64_t len = tokens_of(p.lens, at.b, p.L);
+        end = len < s1 ? len : s1;
+        chunks = int((s1 - s0 + C - 1) / C);
+        const int n0 = at.tile * p.tile;
+        vdim = J.V - n0 < p.tile ? J.V - n0 : p.tile;
+        rev = J.rev;
+        if (Q) qp = rows_of_head<T>(J.q, at);
+        kp = rows_of_head<T>(J.k, at);
+        vp = rows_of_head<T>(J.v, at) + n0;
+        gp = p.g + int64_t(at.b) * p.g_b + int64_t(at.h) * p.g_h;
+        whole = WHOLE || (J.K == KP && vdim == 16 * NT && (!Q || near(J.q.l)) && near(J.k.l) && near(J.v.l));
     }
-    float* to = J.ends + (bh * p.segs + at.seg) * int64_t(J.K) * J.V;
+    __device__ __forceinline__ int chunk(int i) const { return rev ? chunks - 1 - i : i; }
+    __device__ __forceinline__ void fetch(int i) {
+        const int64_t t0 = s0 + int64_t(chunk(i)) * C;
+        if (whole && t0 + C <= end) {
+            if (Q) q.load_all(qp + t0 * J.q.l, J.q.l, lane);
+            k.load_all(kp + t0 * J.k.l, J.k.l, lane);
+            v.load_all(vp + t0 * J.v.l, J.v.l, lane);
+        } else {
+            const int rows = t0 + C <= end ? C : t0 < end ? int(end - t0) : 0;
+            if (Q) q.template load<WHOLE>(qp + t0 * J.q.l, J.q.l, rows, J.K, lane);
+            k.template load<WHOLE>(kp + t0 * J.k.l, J.k.l, rows, J.K, lane);
+            v.template load<WHOLE>(vp + t0 * J.v.l, J.v.l, rows, vdim, lane);
+        }
+    }
+    // the log decays of the two chunks that `pair` names, a token a lane
+    __device__ __forceinline__ float decay(int pair) const {
+        const int64_t t = s0 + int64_t(pair) * 64 + lane;
+        return t < end ? gp[t * p.g_l] : 0.f;
+    }
+};
+
+// the element (register r of tile d, column tile n) of the state, and whether it exists
+template <int KP, int NT, bool WHOLE, typename F>
+__device__ __forceinline__ void each_state(f4 (&S)[KP / 16][NT], Job& J, int n0, int vdim, int lane, F&& f) {
+    const int c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int col = n0 + 16 * (4 * n + wave) + c;
+        const int col = 16 * n + c;
 #pragma unroll
         for (int d = 0; d < KP / 16; ++d)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * d + 4 * g + r;
-                if (row < J.K && col < J.V) to[int64_t(row) * J.st_k + int64_t(col) * J.st_v] = S[d][n][r];
+                const int row = state_row(d, g, r);
+                S[d][n][r] = f(S[d][n][r], WHOLE || (row < J.K && col < vdim), uint32_t(row * J.st_k + (n0 + col) * J.st_v));
             }
     }
-    if (threadIdx.x == 0 && at.tile == 0) J.decays[bh * p.segs + at.seg] = decay;
+}
+template <int KP, int NT, bool WHOLE>
+__device__ __forceinline__ void write_state(f4 (&S)[KP / 16][NT], Job& J, int n0, int vdim, int lane, float* to) {
+    each_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, [&](float s, bool in, uint32_t i) __attribute__((always_inline)) {
+        if (in) to[i] = s;
+        return s;
+    });
+}
+
+template <typename T, int KP, int NT>
+struct Tiles {
+    __attribute__((aligned(16))) uint16_t k[kTerms<T> * Rows<T, KP>::TERM];
+    __attribute__((aligned(16))) uint16_t v[kTerms<T> * Stage<T, 16 * NT>::TERM];
+    Decays dec;
+};
+
+// ------------------------------------------------------- state of a segment --
+// Each segment's state from a zero start, and its decay.
+template <typename T, int KP, int NT, bool WHOLE>
+__global__ __launch_bounds__(64, 2) void la_local(const LaParams) {
+    Params& p = params();
+    constexpr int R = kTerms<T>;
+    using SV = Stage<T, 16 * NT>;
+    __shared__ Tiles<T, KP, NT> m;
+    const Place at = place(p, p.segs);
+    Job& J = p.job[at.job];
+    const int n0 = at.tile * p.tile, lane = int(threadIdx.x);
+    if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
+    const int64_t bh = at.bh;
+    Walk<T, KP, NT, false, WHOLE> w(p, J, at, p.seg_tokens, lane);
+    f4 S[KP / 16][NT];
+    each_state<KP, NT, WHOLE>(S, J, n0, w.vdim, lane, [](float, bool, uint32_t) __attribute__((always_inline)) { return 0.f; });
+    float decay = 1.f;
+    int pair = -1;
+    w.fetch(0);
+    float g = w.decay(w.chunk(0) >> 1);
+    for (int i = 0; i < w.chunks; ++i) {
+        const int ch = w.chunk(i), half = ch & 1;
+        lds_in_order();
+        w.k.store(m.k, lane);
+        (void)w.v.template store<false>(m.v, lane);
+        if (i + 1 < w.chunks) w.fetch(i + 1);
+        if (pair != ch >> 1) {
+            pair = ch >> 1;
+            m.dec.fill(lane, g, w.rev, J.vscale, 1.f);
+            const int next = pair + (w.rev ? -1 : 1);
+            if (next >= 0) g = w.decay(next);
+            lds_in_order();
+            decay *= m.dec.total[0] * m.dec.total[1];
+        }
+        lds_in_order();
+        u4 vf[NT][R];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, 16 * n + 4 * (lane & 3), lane);
+        update_state<T, KP, NT, WHOLE>(S, m.k, vf, m.dec, half, J.K, w.vdim, lane);
+    }
+    write_state<KP, NT, WHOLE>(S, J, n0, w.vdim, lane, J.ends + (bh * p.segs + at.seg) * int64_t(J.K) * J.V);
+    if (lane == 0 && at.tile == 0) J.decays[bh * p.segs + at.seg] = decay;
 }
 
 // ----------------------------------------------------------------- the walk --
-// P's 32 x 32 blocks that hold causal tiles: rows' half + tokens' half is
-// 0, 1 or 2, whichever way the walk goes.
-template <int C, int N>
-struct Causal {
-    static constexpr int STRIDE = 40, BLOCK = 32 * STRIDE, BLOCKS = C / 16 - 1, TERM = BLOCKS * BLOCK;
-    static __device__ __forceinline__ int at(int row, int token) {
-        return ((row >> 5) + (token >> 5)) * BLOCK + (row & 31) * STRIDE + (token & 31);
-    }
-};
-
-// Workgroups per CU that LDS has room for (160 KiB) set the registers a wave may
-// take: up to 3 waves a SIMD, which hide each other's barriers and loads.
-template <typename T, int KP, int NT, int N>
-constexpr int walk_lds() {
-    constexpr int C = kChunk<T>, R = kTerms<T>;
-    return 2 * (2 * R * Stage<T, C, KP>::TERM + R * Stage<T, C, 64 * NT>::TERM + N * Causal<C, N>::TERM) + 2 * int(sizeof(Decays<C>)) +
-           16 * C + 256 * NT + 16;
-}
-template <typename T, int KP, int NT, int N>
-constexpr int kWalkWaves = KP <= 64 && NT == 1 && 3 * walk_lds<T, KP, NT, N>() <= 163840 ? 3 : KP <= 128 && 2 * walk_lds<T, KP, NT, N>() <= 163840 ? 2 : 1;
-
-template <typename T, int KP, int NT, int N>
-__global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const LaParams) {
+template <typename T, int KP, int NT, int N, bool WHOLE>
+__global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams) {
     Params& p = params();
-    constexpr int C = kChunk<T>, R = kTerms<T>, IT = C / 16, TRI = IT * (IT + 1) / 2, kMax = N == 2 ? 1 : 2;
-    using SK = Stage<T, C, KP>;
-    using SV = Stage<T, C, 64 * NT>;
-    using CP = Causal<C, N>;
-    __shared__ __attribute__((aligned(16))) uint16_t qt[R * SK::TERM], kt[R * SK::TERM], vt[R * SV::TERM], pt[N * CP::TERM];
-    __shared__ Decays<C> decs[2];
-    __shared__ float dots[4][C];
-    __shared__ int bad_any, bad_col[64 * NT];
+    constexpr int R = kTerms<T>, kMax = N == 2 ? 1 : 2;
+    using SV = Stage<T, 16 * NT>;
+    __shared__ Tiles<T, KP, NT> m;
+    __shared__ int bad_col[16 * NT];
     const int segs = p.serial ? 1 : p.segs;
     const Place at = place(p, segs);
     Job& J = p.job[at.job];
-    const int n0 = at.tile * 64 * NT;
+    const int n0 = at.tile * p.tile, lane = int(threadIdx.x), c = lane & 15, g = lane >> 4;
     if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
-    const int64_t b = at.b, h = at.h, bh = at.bh;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int64_t span = p.serial ? p.L : p.seg_tokens;
-    const int64_t s0 = at.seg * span, s1 = s0 + span < p.L ? s0 + span : p.L;
-    const int64_t len = tokens_of(p.lens, b, p.L), end = len < s1 ? len : s1;
-    const T* qp = rows_of_head<T>(J.q, at);
-    const T* kp = rows_of_head<T>(J.k, at);
-    const T* vp = rows_of_head<T>(J.v, at) + n0;
+    const int64_t bh = at.bh, KV = int64_t(J.K) * J.V;
+    Walk<T, KP, NT, true, WHOLE> w(p, J, at, p.serial ? p.L : p.seg_tokens, lane);
+    const bool rev = w.rev;
+    const int vdim = w.vdim;
     const T* xp = J.dot ? rows_of_head<T>(J.x, at) + n0 : nullptr;
-    const int64_t op = b * J.o.b + h * J.o.h + n0;
-    const float* gp = p.g + b * p.g_b + h * p.g_h;
-    const int64_t KV = int64_t(J.K) * J.V;
-    const int chunks = int((s1 - s0 + C - 1) / C), vdim = J.V - n0, rev = J.rev;
-    const int64_t seg_mask = p.seg_tokens - 1;
-    const bool whole_v = vdim >= 64 * NT;
-    const bool whole = J.K == KP && whole_v && SK::near(J.q.l) && SK::near(J.k.l) && SV::near(J.v.l);
-    const bool near_o = whole_v && SV::near(J.o.l) && SV::near(J.x.l);
+    const int64_t op = int64_t(at.b) * J.o.b + int64_t(at.h) * J.o.h + n0, seg_mask = p.seg_tokens - 1;
+    const bool near_o = WHOLE || (vdim == 16 * NT && near(J.o.l) && near(J.x.l));
 
     // the state before the walk's first token
     const float* from = J.in ? J.in + bh * KV : nullptr;
@@ -480,215 +603,162 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const
         if (before >= 0 && before < p.segs) from = J.carry + (bh * p.segs + before) * KV;
     }
     f4 S[KP / 16][NT];
-    const auto each_state = [&](auto&& f) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int col = n0 + 16 * (4 * n + wave) + c;
-#pragma unroll
-            for (int d = 0; d < KP / 16; ++d)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * d + 4 * g + r;
-                    S[d][n][r] = f(S[d][n][r], row < J.K && col < J.V, uint32_t(row * J.st_k + col * J.st_v));
-                }
-        }
-    };
-    if (from) each_state([&](float, bool in, uint32_t i) { return in ? from[i] : 0.f; });
-    else each_state([](float, bool, uint32_t) { return 0.f; });
-    const auto write_state = [&](float* to) __attribute__((always_inline)) {
-        each_state([&](float s, bool in, uint32_t i) {
-            if (in) to[i] = s;
-            return s;
-        });
-    };
+    if (from) each_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, [&](float, bool in, uint32_t i) __attribute__((always_inline)) { return in ? from[i] : 0.f; });
+    else each_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, [](float, bool, uint32_t) __attribute__((always_inline)) { return 0.f; });
 
-    SK sq, sk;
-    SV sv;
-    float gv = 0.f;                                   // (wave 3) the decays of the chunk after the staged one
-    const auto start = [&](int i) { return s0 + int64_t(rev ? chunks - 1 - i : i) * C; };
-    const auto fetch = [&](int i) __attribute__((always_inline)) {
-        const int64_t t0 = start(i);
-        if (whole && t0 + C <= end) {
-            sq.load_all(qp + t0 * J.q.l, J.q.l);
-            sk.load_all(kp + t0 * J.k.l, J.k.l);
-            sv.load_all(vp + t0 * J.v.l, J.v.l);
-        } else {
-            sq.load(qp, J.q.l, t0, end, J.K);
-            sk.load(kp, J.k.l, t0, end, J.K);
-            sv.load(vp, J.v.l, t0, end, vdim);
-        }
-    };
-    const auto fetch_decay = [&](int i) __attribute__((always_inline)) {
-        gv = 0.f;
-        if (wave == 3 && i < chunks) {
-            const int64_t t = start(i) + lane;
-            if (lane < C && t < end) gv = gp[t * p.g_l];
-        }
-    };
-    // the tiles of P's blocks above (in reverse: below) the diagonal
-    for (int i = threadIdx.x; i < N * (C / 32) * 64; i += 256) {
-        const int e = i % 64, row = 32 * (i / 64 % (C / 32)) + (rev ? 16 : 0) + e / 4, token = 32 * (i / 64 % (C / 32)) + (rev ? 0 : 16) + 4 * (e % 4);
-        *reinterpret_cast<u2*>(pt + i / (64 * (C / 32)) * CP::TERM + CP::at(row, token)) = u2{0u, 0u};
+    int pair = -1;
+    float decay = 0.f;
+    if (w.chunks > 0) {
+        w.fetch(0);
+        decay = w.decay(w.chunk(0) >> 1);
     }
-    if (threadIdx.x == 0) bad_any = 0;
-    if (chunks > 0) {
-        fetch_decay(0);
-        fetch(0);
-        if (wave == 3) decs[0].fill(lane, gv, rev, J.vscale, J.oscale);
-        fetch_decay(1);
-    }
-    __syncthreads();
-    for (int ci = 0; ci < chunks; ++ci) {
-        const int64_t t0 = start(ci);
-        const Decays<C>& dec = decs[ci & 1];
-        (void)sq.template store<false>(qt);
-        (void)sk.template store<false>(kt);
-        if (sv.template store<true>(vt)) bad_any = 1;
-        __syncthreads();
-        if (ci + 1 < chunks) fetch(ci + 1);
+    for (int ci = 0; ci < w.chunks; ++ci) {
+        const int ch = w.chunk(ci), half = ch & 1;
+        const int64_t t0 = w.s0 + int64_t(ch) * C;
+        const bool last = ci + 1 == w.chunks;
+        lds_in_order();
+        w.k.store(m.k, lane);
         // A sum over tokens multiplies every v, by P's zeros too: infinities and
         // NaN of v are taken out of the tile here and put into the results from
         // their token on.
-        const bool bad = bad_any != 0;
-        if (bad) {
-            __syncthreads();
-            if (threadIdx.x == 0) bad_any = 0;
-            if (int(threadIdx.x) < 64 * NT) {
-                int first = rev ? -1 : C;
-                for (int i = 0; i < C; ++i) {
-                    const int row = rev ? i : C - 1 - i;
-                    if ((vt[row * SV::STRIDE + threadIdx.x] & 0x7f80u) == 0x7f80u) {
-                        first = row;
-                        for (int r = 0; r < R; ++r) vt[r * SV::TERM + row * SV::STRIDE + threadIdx.x] = 0;
-                    }
+        const bool bad = __ballot(w.v.template store<true>(m.v, lane)) != 0;
+        lds_in_order();
+        if (bad && lane < 16 * NT) {
+            int first = rev ? -1 : C;
+            for (int i = 0; i < C; ++i) {
+                const int row = rev ? i : C - 1 - i;
+                if ((m.v[row * SV::STRIDE + lane] & 0x7f80u) == 0x7f80u) {
+                    first = row;
+                    for (int r = 0; r < R; ++r) m.v[r * SV::TERM + row * SV::STRIDE + lane] = 0;
                 }
-                bad_col[threadIdx.x] = first;
             }
-            __syncthreads();
+            bad_col[lane] = first;
         }
-
-        // P's causal tiles, dealt out to the waves
-#pragma unroll
-        for (int s = 0; s < (TRI + 3) / 4; ++s) {
-            const int tile = 4 * s + wave;
-            if (tile < TRI) {
-                int it = tile >= 6 ? 3 : tile >= 3 ? 2 : tile >= 1 ? 1 : 0, jt = tile - it * (it + 1) / 2;
-                if (rev) {
-                    it = IT - 1 - it;
-                    jt = IT - 1 - jt;
-                }
-                f4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kk = 0; kk < KP / 32; ++kk) {
-                    if (32 * kk >= J.K) continue;
-                    u4 kf[R], qf[R];
-#pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        kf[r] = *reinterpret_cast<const u4*>(kt + r * SK::TERM + (16 * jt + c) * SK::STRIDE + 32 * kk + 8 * g);
-                        qf[r] = *reinterpret_cast<const u4*>(qt + r * SK::TERM + (16 * it + c) * SK::STRIDE + 32 * kk + 8 * g);
-                    }
-                    acc = mfma_terms<R, R, 2>(kf, qf, acc);
-                }
-                typedef int i4 __attribute__((ext_vector_type(4)));
-                const i4 Ij = *reinterpret_cast<const i4*>(dec.I + 16 * jt + 4 * g);
-                acc *= *reinterpret_cast<const f4*>(dec.col + 16 * jt + 4 * g);
-                const int Ii = dec.I[16 * it + c];
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = __builtin_amdgcn_ldexpf(acc[r], Ii - Ij[r]);
-                if (it == jt) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = (rev ? 4 * g + r < c : 4 * g + r > c) ? 0.f : v[r];
-                }
-                uint32_t lo[N], hi[N];
-                split<N>(v[0], v[1], lo);
-                split<N>(v[2], v[3], hi);
-#pragma unroll
-                for (int t = 0; t < N; ++t)
-                    *reinterpret_cast<u2*>(pt + t * CP::TERM + CP::at(16 * it + c, 16 * jt + 4 * g)) = u2{lo[t], hi[t]};
-            }
+        if (pair != ch >> 1) {
+            pair = ch >> 1;
+            m.dec.fill(lane, decay, rev, J.vscale, J.oscale);
+            const int next = pair + (rev ? -1 : 1);
+            if (next >= 0) decay = w.decay(next);
         }
-        // the next chunk's decays, by the wave with the fewest tiles
-        if (wave == 3 && ci + 1 < chunks) decs[(ci + 1) & 1].fill(lane, gv, rev, J.vscale, J.oscale);
-        fetch_decay(ci + 2);
-        __syncthreads();
+        lds_in_order();
+        const int d0 = 32 * half;
 
-        // o^T: q S with the carried state's factor, then P V
-        f4 o[IT][NT];
+        // P^T's causal tiles (tokens j, rows i), and o^T = S^T q
+        f4 o[2][NT], P[3];                                   // P: (0, 0), (0, 1) or in reverse (1, 0), (1, 1)
 #pragma unroll
-        for (int it = 0; it < IT; ++it)
+        for (int it = 0; it < 2; ++it)
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[it][n] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
+        for (int i = 0; i < 3; ++i) P[i] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
         for (int kk = 0; kk < KP / 32; ++kk) {
-            if (32 * kk >= J.K) continue;
-            u4 sf[NT][N];
+            if (!WHOLE && 32 * kk >= J.K) continue;
+            u4 qf[2][R], kf[2][R];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int i = 0; i < 2; ++i) {
+                w.q.terms(i, kk, qf[i]);
+                w.k.terms(i, kk, kf[i]);
+            }
+            P[0] = mfma_terms<R, R, 2>(kf[0], qf[0], P[0]);
+            P[2] = mfma_terms<R, R, 2>(kf[1], qf[1], P[2]);
+            if (rev) P[1] = mfma_terms<R, R, 2>(kf[1], qf[0], P[1]);
+            else P[1] = mfma_terms<R, R, 2>(kf[0], qf[1], P[1]);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+            for (int n = 0; n < NT; ++n) {
+                if (!WHOLE && 16 * n >= vdim) continue;
+                u4 sf[N];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
                     uint32_t t[N];
-                    const f4& s = S[2 * kk + (w >> 1)][n];
-                    split<N>(s[2 * (w & 1)], s[2 * (w & 1) + 1], t);
+                    const f4& s = S[2 * kk + (x >> 1)][n];
+                    split<N>(s[2 * (x & 1)], s[2 * (x & 1) + 1], t);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) sf[n][i][w] = t[i];
+                    for (int i = 0; i < N; ++i) sf[i][x] = t[i];
                 }
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
-                u4 qf[R];
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const uint16_t* q = qt + r * SK::TERM + (16 * it + c) * SK::STRIDE + 32 * kk + 4 * g;
-                    const u2 a = *reinterpret_cast<const u2*>(q), d = *reinterpret_cast<const u2*>(q + 16);
-                    qf[r] = u4{a.x, a.y, d.x, d.y};
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) o[it][n] = mfma_terms<N, R, kMax>(sf[n], qf, o[it][n]);
+                for (int it = 0; it < 2; ++it) o[it][n] = mfma_terms<N, R, kMax>(sf, qf[it], o[it][n]);
             }
+            stage_end();
         }
-        u4 vf[C / 32][NT][R];
+        uint2 x4[2][NT][int(sizeof(T)) / 2];
+        const bool whole_o = near_o && t0 + C <= w.end && !bad;
+        if (J.dot && whole_o) {
+            const uint32_t off = (uint32_t(c) * uint32_t(J.x.l) + uint32_t(4 * g)) * uint32_t(sizeof(T));
 #pragma unroll
-        for (int ks = 0; ks < C / 32; ++ks)
+            for (int it = 0; it < 2; ++it)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int r = 0; r < R; ++r) vf[ks][n][r] = load_cols<SV::STRIDE>(vt + r * SV::TERM, 32 * ks, 16 * (4 * n + wave), lane);
-#pragma unroll
-        for (int it = 0; it < IT; ++it) {
-            const float f = dec.in[16 * it + c];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[it][n] *= f;
-#pragma unroll
-            for (int ks = 0; ks < C / 32; ++ks) {
-                if (rev ? 32 * ks + 31 < 16 * it : 32 * ks > 16 * it + 15) continue;
-                u4 pf[N];
-#pragma unroll
-                for (int t = 0; t < N; ++t) pf[t] = *reinterpret_cast<const u4*>(pt + t * CP::TERM + CP::at(16 * it + c, 32 * ks + 8 * g));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) o[it][n] = mfma_terms<R, N, kMax>(vf[ks][n], pf, o[it][n]);
-            }
-            const float last = dec.row[16 * it + c];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[it][n] *= last;
+                    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
+                        const half4_at2 h = *reinterpret_cast<const half4_at2*>(reinterpret_cast<const char*>(xp + (t0 + 16 * it) * J.x.l) +
+                                                                                off + (16 * n * int(sizeof(T)) + 8 * i));
+                        x4[it][n][i] = make_uint2(h.x, h.y);
+                    }
         }
-        const bool last = ci + 1 == chunks;
-        if (!last || J.ends || J.out_state) update_state<T, KP, NT, C, SK>(S, kt, vf, dec, J.K, lane);
+        u4 vf[NT][R];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, 16 * n + 4 * (lane & 3), lane);
 
-        float dot[IT] = {};
-        if (near_o && t0 + C <= end && !bad) {
-            const int64_t first = op + t0 * J.o.l;
+        // P's decays and split, and o^T <- 2^G o^T + V^T P^T
+        typedef int i4 __attribute__((ext_vector_type(4)));
+        i4 Ij[2];
+        f4 cj[2];
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
-                const uint32_t row = uint32_t(c) * uint32_t(J.o.l), xrow = uint32_t(c) * uint32_t(J.x.l);
+        for (int j = 0; j < 2; ++j) {
+            Ij[j] = *reinterpret_cast<const i4*>(m.dec.I + d0 + 16 * j + 4 * g);
+            cj[j] = *reinterpret_cast<const f4*>(m.dec.col + d0 + 16 * j + 4 * g);
+        }
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+            const int Ii = m.dec.I[d0 + 16 * it + c];
+            u4 pf[N];
+#pragma unroll
+            for (int t = 0; t < N; ++t) pf[t] = u4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (it == j || (rev ? j > it : j < it)) {
+                    f4 v = (it == j ? P[2 * it] : P[1]) * cj[j];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        v[r] = __builtin_amdgcn_ldexpf(v[r], Ii - Ij[j][r]);
+                        if (it == j) v[r] = (rev ? 4 * g + r < c : 4 * g + r > c) ? 0.f : v[r];
+                    }
+                    uint32_t lo[N], hi[N];
+                    split<N>(v[0], v[1], lo);
+                    split<N>(v[2], v[3], hi);
+#pragma unroll
+                    for (int t = 0; t < N; ++t) {
+                        pf[t][2 * j] = lo[t];
+                        pf[t][2 * j + 1] = hi[t];
+                    }
+                }
+            }
+            const float carried = m.dec.in[d0 + 16 * it + c], out = m.dec.row[d0 + 16 * it + c];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                if (!WHOLE && 16 * n >= vdim) continue;
+                o[it][n] = mfma_terms<R, N, kMax>(vf[n], pf, o[it][n] * carried);
+                o[it][n] *= out;
+            }
+        }
+
+        float dot[2] = {0.f, 0.f};
+        if (whole_o) {
+            const uint32_t row = uint32_t(c) * uint32_t(J.o.l) + uint32_t(4 * g);
+#pragma unroll
+            for (int it = 0; it < 2; ++it) {
+                const int64_t first = op + (t0 + 16 * it) * J.o.l;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint32_t col = uint32_t(16 * (4 * n + wave) + 4 * g);
                     const float v[4] = {o[it][n][0], o[it][n][1], o[it][n][2], o[it][n][3]};
-                    if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + (first + 16 * it * J.o.l) + (row + col), v, 4);
-                    else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + (first + 16 * it * J.o.l) + (row + col), v, 4);
+                    if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 16 * n), v, 4);
+                    else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + first + (row + 16 * n), v, 4);
                     if (J.dot) {
                         float x[4];
-                        load4<T>(xp + (t0 + 16 * it) * J.x.l + (xrow + col), x, 4);
+                        load4<T>(reinterpret_cast<const T*>(&x4[it][n]), x, 4);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) dot[it] = __builtin_fmaf(v[r], x[r], dot[it]);
                     }
@@ -696,13 +766,13 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const
             }
         } else {
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
+            for (int it = 0; it < 2; ++it) {
                 const int i = 16 * it + c;
                 const int64_t t = t0 + i;
-                const bool live = t < len;
+                const bool live = t < w.end;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int col = 16 * (4 * n + wave) + 4 * g, cnt = t < s1 ? vdim - col : 0;
+                    const int col = 16 * n + 4 * g, cnt = t < w.s1 ? vdim - col : 0;
                     float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -725,19 +795,25 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const
         }
         if (J.dot) {
 #pragma unroll
-            for (int it = 0; it < IT; ++it) {
+            for (int it = 0; it < 2; ++it) {
                 // over the lanes of the token's other columns: g = 0 .. 3
                 auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(dot[it]), __float_as_uint(dot[it]), false, false);
                 float d = __uint_as_float(s[0]) + __uint_as_float(s[1]);
                 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(d), __float_as_uint(d), false, false);
                 d = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-                if (g == 0) dots[wave][16 * it + c] = d;
+                const int64_t t = t0 + 16 * it + c;
+                if (g == 0 && t < w.s1) J.dot[(int64_t(at.tile) * p.B * p.H + bh) * p.L + t] = d;
             }
         }
+        // (the next rows are requested only here: in flight any earlier, they and
+        // the results together would not fit the registers)
+        if (!last) w.fetch(ci + 1);
+        stage_end();
+        if (!last || J.ends || J.out_state) update_state<T, KP, NT, WHOLE>(S, m.k, vf, m.dec, half, J.K, vdim, lane);
         if (bad) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int first = bad_col[16 * (4 * n + wave) + c];
+                const int first = bad_col[16 * n + c];
                 if (first >= 0 && first < C) {
 #pragma unroll
                     for (int d = 0; d < KP / 16; ++d)
@@ -747,31 +823,26 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KP, NT, N>)) void la_walk(const
             }
         }
         if (J.ends && ((rev ? t0 & seg_mask : (t0 + C) & seg_mask) == 0 || (!rev && last)))
-            write_state(J.ends + (bh * p.segs + (t0 >> p.seg_shift)) * KV);
-        __syncthreads();
-        if (J.dot && int(threadIdx.x) < C && t0 + threadIdx.x < s1)
-            J.dot[(int64_t(at.tile) * p.B * p.H + bh) * p.L + t0 + threadIdx.x] =
-                (dots[0][threadIdx.x] + dots[1][threadIdx.x]) + (dots[2][threadIdx.x] + dots[3][threadIdx.x]);
+            write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + (bh * p.segs + (t0 >> p.seg_shift)) * KV);
     }
-    if (chunks == 0 && J.ends) write_state(J.ends + bh * p.segs * KV);
-    if (J.out_state) write_state(J.out_state + bh * KV);
+    if (w.chunks == 0 && J.ends) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + bh * p.segs * KV);
+    if (J.out_state) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.out_state + bh * KV);
 }
 
 }  // namespace la
 
-// Launches over J.K <= KP, J.V in column tiles of 64 NT (see la_tile).
-template <typename F>
+// f(KP, NT): the padded width of q and k, and the 16-column tiles of a wave
+template <typename T, typename F>
 hipError_t la_for_dims(const LaParams& p, F&& f) {
-    using std::integral_constant;
     int k = 0;
     for (int j = 0; j < p.njobs; ++j) k = p.job[j].K > k ? p.job[j].K : k;
     const auto with = [&](auto kp) {
-        return p.tile == 64 ? f(kp, integral_constant<int, 1>{}) : f(kp, integral_constant<int, 2>{});
+        return f(kp, std::integral_constant<int, la_cols(decltype(kp)::value, sizeof(T)) / 16>{});
     };
-    if (k <= 32) return with(integral_constant<int, 32>{});
-    if (k <= 64) return with(integral_constant<int, 64>{});
-    if (k <= 128) return with(integral_constant<int, 128>{});
-    return with(integral_constant<int, 256>{});
+    if (k <= 32) return with(std::integral_constant<int, 32>{});
+    if (k <= 64) return with(std::integral_constant<int, 64>{});
+    if (k <= 128) return with(std::integral_constant<int, 128>{});
+    return with(std::integral_constant<int, 256>{});
 }
 // (a multiple of the XCDs, so that a segment's workgroups share one)
 inline dim3 la_grid(const LaParams& p, int segs) {
@@ -779,26 +850,41 @@ inline dim3 la_grid(const LaParams& p, int segs) {
     return dim3(unsigned((n + kXcds - 1) / kXcds * kXcds));
 }
 
+// every tile of every job is full, and rows are near
+template <int KP, int NT>
+bool la_whole(const LaParams& p) {
+    const auto near = [](const LaRows& r) { return r.l < (int64_t(1) << 24); };
+    for (int j = 0; j < p.njobs; ++j) {
+        const LaJob& J = p.job[j];
+        if (J.K != KP || p.tile != 16 * NT || J.V % p.tile != 0 || !near(J.q) || !near(J.k) || !near(J.v) || !near(J.o) || !near(J.x)) return false;
+    }
+    return true;
+}
 template <typename T>
 hipError_t la_local_launch(const LaParams& p, hipStream_t stream) {
-    return la_for_dims(p, [&](auto kp, auto nt) {
-        hipLaunchKernelGGL((la::la_local<T, decltype(kp)::value, decltype(nt)::value>), la_grid(p, p.segs), dim3(256), 0, stream, p);
+    return la_for_dims<T>(p, [&](auto kp, auto nt) {
+        constexpr int KP = decltype(kp)::value, NT = decltype(nt)::value;
+        const dim3 grid = la_grid(p, p.segs);
+        if (la_whole<KP, NT>(p)) hipLaunchKernelGGL((la::la_local<T, KP, NT, true>), grid, dim3(64), 0, stream, p);
+        else hipLaunchKernelGGL((la::la_local<T, KP, NT, false>), grid, dim3(64), 0, stream, p);
         return hipGetLastError();
     });
 }
 template <typename T>
 hipError_t la_walk_launch(const LaParams& p, bool fine, hipStream_t stream) {
-    return la_for_dims(p, [&](auto kp, auto nt) {
+    return la_for_dims<T>(p, [&](auto kp, auto nt) {
         constexpr int KP = decltype(kp)::value, NT = decltype(nt)::value;
         const dim3 grid = la_grid(p, p.serial ? 1 : p.segs);
+        const auto run = [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            if (la_whole<KP, NT>(p)) hipLaunchKernelGGL((la::la_walk<T, KP, NT, N, true>), grid, dim3(64), 0, stream, p);
+            else hipLaunchKernelGGL((la::la_walk<T, KP, NT, N, false>), grid, dim3(64), 0, stream, p);
+            return hipGetLastError();
+        };
         if constexpr (sizeof(T) == 2) {
-            if (!fine) {
-                hipLaunchKernelGGL((la::la_walk<T, KP, NT, 2>), grid, dim3(256), 0, stream, p);
-                return hipGetLastError();
-            }
+            if (!fine) return run(std::integral_constant<int, 2>{});
         }
-        hipLaunchKernelGGL((la::la_walk<T, KP, NT, 3>), grid, dim3(256), 0, stream, p);
-        return hipGetLastError();
+        return run(std::integral_constant<int, 3>{});
     });
 }
 
