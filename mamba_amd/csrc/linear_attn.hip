@@ -215,7 +215,7 @@ LaParams common(const ss_linear_attn_args& a) {
     p.g = a.g; p.g_b = a.g_batch_stride; p.g_l = a.g_len_stride; p.g_h = a.g_head_stride;
     p.lens = a.lengths;
     p.seg_tokens = linear_attn_segment(&a);
-    while ((int64_t(1) << p.seg_shift) < p.seg_tokens) ++p.seg_shift;
+    p.seg_chunks = int(p.seg_tokens / 32);
     p.segs = int(linear_attn_segs(&a));
     p.rep = int(a.heads / a.groups);
     return p;
@@ -247,10 +247,9 @@ hipError_t walk(int dtype, const LaParams& p, bool fine, hipStream_t stream) {
 
 int64_t linear_attn_segment(const ss_linear_attn_args* a) {
     const int64_t bh = a->batch * a->heads;
-    const int64_t segs = bh > 0 ? (kSegsWanted + bh - 1) / bh : 1, want = (a->seqlen + segs - 1) / segs;
-    int64_t n = kSegTokMin;
-    while (n < want && n < kSegTokMax) n *= 2;
-    return n;
+    const int64_t segs = bh > 0 && bh < kSegsWanted ? kSegsWanted / bh : 1;
+    const int64_t n = ((a->seqlen + segs - 1) / segs + 63) / 64 * 64;
+    return n < kSegTokMin ? kSegTokMin : n > kSegTokMax ? kSegTokMax : n;
 }
 int64_t linear_attn_segs(const ss_linear_attn_args* a) {
     const int64_t n = linear_attn_segment(a);

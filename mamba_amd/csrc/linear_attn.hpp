@@ -49,8 +49,8 @@ struct LaParams {
     const float* g;
     int64_t g_b, g_l, g_h;
     const int32_t* lens;
-    int64_t seg_tokens;               // a power of two, 2^seg_shift
-    int segs, seg_shift, rep;         // rep: heads per group
+    int64_t seg_tokens;               // a multiple of 64: seg_chunks chunks of 32
+    int segs, seg_chunks, rep;        // rep: heads per group
     int serial;                       // a workgroup walks a whole row (else a segment, from its carry)
     int tile, tiles;                  // value columns per workgroup, and tiles of the widest job
 };

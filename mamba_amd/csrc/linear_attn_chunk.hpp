@@ -65,27 +65,26 @@ __device__ __forceinline__ f4 mfma(const u4& a, const u4& b, const f4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// x0, x1 as N bf16 terms each, packed (x0 low): the first N - 1 by cutting
-// bits off, so what is left over is exact; the last of 2 rounded, of 3 exact
-template <int N>
-__device__ __forceinline__ void split(float x0, float x1, uint32_t (&t)[N]) {
-    const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
-    t[0] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-    if constexpr (N > 1) {
-        const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
-        if constexpr (N == 2) {
-            t[1] = io<bf16_t>::pack2(r0, r1);
-        } else {
-            const uint32_t m0 = __float_as_uint(r0), m1 = __float_as_uint(r1);
-            t[1] = __builtin_amdgcn_perm(m1, m0, 0x07060302u);
-            const float s0 = r0 - __uint_as_float(m0 & 0xffff0000u), s1 = r1 - __uint_as_float(m1 & 0xffff0000u);
-            t[2] = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
-        }
-    }
-}
-
 __device__ __forceinline__ float lo_half(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_half(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// x0, x1 as N bf16 terms each, packed (x0 low).  2 terms: both rounded, 2^-18 off
+// at most.  3 terms: cut, so what is left over is exact and the third holds it.
+template <int N>
+__device__ __forceinline__ void split(float x0, float x1, uint32_t (&t)[N]) {
+    if constexpr (N <= 2) {
+        t[0] = io<bf16_t>::pack2(x0, x1);
+        if constexpr (N == 2) t[1] = io<bf16_t>::pack2(x0 - lo_half(t[0]), x1 - hi_half(t[0]));
+    } else {
+        const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
+        t[0] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+        const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
+        const uint32_t m0 = __float_as_uint(r0), m1 = __float_as_uint(r1);
+        t[1] = __builtin_amdgcn_perm(m1, m0, 0x07060302u);
+        const float s0 = r0 - __uint_as_float(m0 & 0xffff0000u), s1 = r1 - __uint_as_float(m1 & 0xffff0000u);
+        t[2] = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
+    }
+}
 
 // LDS of a wave: its accesses run in order; this keeps the compiler's order.
 __device__ __forceinline__ void lds_in_order() { __asm__ volatile("" ::: "memory"); }
@@ -94,19 +93,29 @@ __device__ __forceinline__ void lds_in_order() { __asm__ volatile("" ::: "memory
 // splits of all steps to the front and runs out of registers.
 __device__ __forceinline__ void stage_end() { __builtin_amdgcn_sched_barrier(0); }
 
-// c += sum of the products of a's NA and b's NB terms whose order is at most
-// kMax (2: down to 2^-24; 1: to 2^-16), small ones first
-template <int NA, int NB, int kMax>
-__device__ __forceinline__ f4 mfma_terms(const u4 (&a)[NA], const u4 (&b)[NB], f4 c) {
+// The lane again, unknown to the compiler: what a rarely taken path derives from it
+// is then computed there, and not once ahead of the loop and kept in registers.
+__device__ __forceinline__ int late(int lane) {
+    __asm__ volatile("" : "+v"(lane));
+    return lane;
+}
+
+// c[i] += sum of the products of a[i]'s NA and b[i]'s NB terms whose order is at
+// most kMax (2: down to 2^-24; 1: to 2^-16), small ones first.  I independent sums
+// at once: a product then need not wait for the one before it.  ai, bi: which operand
+// the sums take (a stride of 0 shares one).
+template <int I, int SA, int SB, int NA, int NB, int kMax>
+__device__ __forceinline__ void mfma_terms(const u4 (*a)[NA], const u4 (*b)[NB], f4* const (&c)[I]) {
 #pragma unroll
     for (int o = kMax; o >= 0; --o) {
 #pragma unroll
-        for (int i = 0; i < NA; ++i) {
-            const int j = o - i;
-            if (j >= 0 && j < NB) c = mfma(a[i], b[j], c);
+        for (int x = 0; x < NA; ++x) {
+            const int y = o - x;
+            if (y < 0 || y >= NB) continue;
+#pragma unroll
+            for (int i = 0; i < I; ++i) *c[i] = mfma(a[SA * i][x], b[SB * i][y], *c[i]);
         }
     }
-    return c;
 }
 
 constexpr int C = 32;                     // tokens per chunk
@@ -123,6 +132,18 @@ __device__ __forceinline__ u4 load_tokens(const uint16_t* tile, int block, int l
     const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 16 * STRIDE)));
     return u4{lo.x, lo.y, hi.x, hi.y};
 }
+
+// Column m of a wave's column tile n: as the state's rows, so that a lane's
+// registers of two tiles are 8 neighbouring columns of the result (NT 1: 4).
+template <int NT> constexpr __device__ __forceinline__ int value_col(int n, int m) {
+    return NT == 1 ? m : 32 * (n >> 1) + 8 * (m >> 2) + 4 * (n & 1) + (m & 3);
+}
+// first column of the 4 that a lane reads of tile n for its group (load_tokens)
+template <int NT> constexpr __device__ __forceinline__ int value_block(int n, int lane) {
+    return NT == 1 ? 4 * (lane & 3) : 32 * (n >> 1) + 8 * (lane & 3) + 4 * (n & 1);
+}
+// whether the tile has columns below vdim
+template <int NT> constexpr __device__ __forceinline__ bool tile_in(int n, int vdim) { return 32 * (n >> 1) < vdim; }
 
 // The state's tile t (16 rows), register r of lane group g: row of the state
 __device__ __forceinline__ int state_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
@@ -165,6 +186,38 @@ __device__ __forceinline__ void load4(const T* p, float (&v)[4], int cnt) {
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = i < cnt ? io<T>::load(p + i) : 0.f;
+}
+
+// 8-byte words at any element alignment; a lane's 4 or 8 columns of a result
+typedef uint32_t words4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+template <int W>
+__device__ __forceinline__ void load_words(const char* p, uint2 (&w)[W]) {
+    if constexpr (W == 1) {
+        const half4_at2 x = *reinterpret_cast<const half4_at2*>(p);
+        w[0] = make_uint2(x.x, x.y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; i += 2) {
+            const words4_at2 x = *reinterpret_cast<const words4_at2*>(p + 8 * i);
+            w[i] = make_uint2(x.x, x.y);
+            w[i + 1] = make_uint2(x.z, x.w);
+        }
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_cols(T* p, const float (&v)[N]) {
+    using R = rowvec<T>;
+    if constexpr (N < R::VE) {
+        store4<T>(p, v, 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += R::VE) {
+            float x[R::VE];
+#pragma unroll
+            for (int e = 0; e < R::VE; ++e) x[e] = v[i + e];
+            R::store(p + i, x, R::VE);
+        }
+    }
 }
 
 // a vector of a row that may not exist, and (unless WHOLE) may end inside it
@@ -316,7 +369,7 @@ struct __attribute__((aligned(16))) Decays {
     int I[64];             // integer part of H (G, or -G in reverse)
     float col[64];         // 2^-F, with the factor of v
     float row[64];         // 2^F, with the factor of o
-    float in[64];          // the carried state's factor at a token over `row`'s 2^F
+    float in[64];          // the carried state's factor at a token, with the factor of o
     float upd[64];         // a token's factor in the state's update, with the factor of v
     float total[2];        // 2^G_C
 
@@ -339,7 +392,7 @@ struct __attribute__((aligned(16))) Decays {
         I[lane] = int(fl);
         col[lane] = vscale * __builtin_amdgcn_exp2f(-F);
         row[lane] = oscale * __builtin_amdgcn_exp2f(F);
-        in[lane] = exp2_of((rev ? H + G : H) - double(F));
+        in[lane] = oscale * exp2_of(rev ? H + G : H);
         upd[lane] = vscale * exp2_of(rev ? -H : G - H);
         if (t == 0) total[lane >> 5] = exp2_of(G);
     }
@@ -394,11 +447,13 @@ __device__ __forceinline__ void update_state(f4 (&S)[KP / 16][NT], const uint16_
         for (int d = 0; d < KP / 16; ++d) rows(d, kf[d]);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            if (!WHOLE && 16 * n >= vdim) continue;
+            if (!WHOLE && !tile_in<NT>(n, vdim)) continue;
             u4 bv[3];
             weighted(n, bv);
+            f4* to[KP / 16];
 #pragma unroll
-            for (int d = 0; d < KP / 16; ++d) S[d][n] = mfma_terms<R, 3, 2>(kf[d], bv, S[d][n]);
+            for (int d = 0; d < KP / 16; ++d) to[d] = &S[d][n];
+            mfma_terms<KP / 16, 1, 0, R, 3, 2>(kf, &bv, to);
             stage_end();
         }
     } else {
@@ -410,9 +465,10 @@ __device__ __forceinline__ void update_state(f4 (&S)[KP / 16][NT], const uint16_
             if (!WHOLE && 32 * (d >> 1) >= kdim) continue;
             u4 kf[R];
             rows(d, kf);
+            f4* to[NT];                                       // (tiles past vdim: v's columns are zero)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                if (WHOLE || 16 * n < vdim) S[d][n] = mfma_terms<R, 3, 2>(kf, bv[n], S[d][n]);
+            for (int n = 0; n < NT; ++n) to[n] = &S[d][n];
+            mfma_terms<NT, 0, 1, R, 3, 2>(&kf, bv, to);
             stage_end();
         }
     }
@@ -458,7 +514,7 @@ struct Walk {
     int64_t s0, s1, end;              // tokens: the span, and where the row's own end in it
     const T* qp; const T* kp; const T* vp; const float* gp;
     int chunks, vdim, lane;
-    bool rev, whole;
+    bool whole, rev;
     Rows<T, KP> q, k;
     Stage<T, 16 * NT> v;
 
@@ -486,9 +542,10 @@ struct Walk {
             v.load_all(vp + t0 * J.v.l, J.v.l, lane);
         } else {
             const int rows = t0 + C <= end ? C : t0 < end ? int(end - t0) : 0;
-            if (Q) q.template load<WHOLE>(qp + t0 * J.q.l, J.q.l, rows, J.K, lane);
-            k.template load<WHOLE>(kp + t0 * J.k.l, J.k.l, rows, J.K, lane);
-            v.template load<WHOLE>(vp + t0 * J.v.l, J.v.l, rows, vdim, lane);
+            const int l = late(lane);
+            if (Q) q.template load<WHOLE>(qp + t0 * J.q.l, J.q.l, rows, J.K, l);
+            k.template load<WHOLE>(kp + t0 * J.k.l, J.k.l, rows, J.K, l);
+            v.template load<WHOLE>(vp + t0 * J.v.l, J.v.l, rows, vdim, l);
         }
     }
     // the log decays of the two chunks that `pair` names, a token a lane
@@ -504,7 +561,7 @@ __device__ __forceinline__ void each_state(f4 (&S)[KP / 16][NT], Job& J, int n0,
     const int c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int col = 16 * n + c;
+        const int col = value_col<NT>(n, c);
 #pragma unroll
         for (int d = 0; d < KP / 16; ++d)
 #pragma unroll
@@ -516,7 +573,7 @@ __device__ __forceinline__ void each_state(f4 (&S)[KP / 16][NT], Job& J, int n0,
 }
 template <int KP, int NT, bool WHOLE>
 __device__ __forceinline__ void write_state(f4 (&S)[KP / 16][NT], Job& J, int n0, int vdim, int lane, float* to) {
-    each_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, [&](float s, bool in, uint32_t i) __attribute__((always_inline)) {
+    each_state<KP, NT, WHOLE>(S, J, n0, vdim, late(lane), [&](float s, bool in, uint32_t i) __attribute__((always_inline)) {
         if (in) to[i] = s;
         return s;
     });
@@ -531,16 +588,11 @@ struct Tiles {
 
 // ------------------------------------------------------- state of a segment --
 // Each segment's state from a zero start, and its decay.
-template <typename T, int KP, int NT, bool WHOLE>
-__global__ __launch_bounds__(64, 2) void la_local(const LaParams) {
-    Params& p = params();
+template <typename T, int KP, int NT, bool WHOLE, bool rev>
+__device__ __forceinline__ void local_rows(Params& p, Job& J, const Place& at, Tiles<T, KP, NT>& m) {
     constexpr int R = kTerms<T>;
     using SV = Stage<T, 16 * NT>;
-    __shared__ Tiles<T, KP, NT> m;
-    const Place at = place(p, p.segs);
-    Job& J = p.job[at.job];
     const int n0 = at.tile * p.tile, lane = int(threadIdx.x);
-    if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
     const int64_t bh = at.bh;
     Walk<T, KP, NT, false, WHOLE> w(p, J, at, p.seg_tokens, lane);
     f4 S[KP / 16][NT];
@@ -557,8 +609,8 @@ __global__ __launch_bounds__(64, 2) void la_local(const LaParams) {
         if (i + 1 < w.chunks) w.fetch(i + 1);
         if (pair != ch >> 1) {
             pair = ch >> 1;
-            m.dec.fill(lane, g, w.rev, J.vscale, 1.f);
-            const int next = pair + (w.rev ? -1 : 1);
+            m.dec.fill(lane, g, rev, J.vscale, 1.f);
+            const int next = pair + (rev ? -1 : 1);
             if (next >= 0) g = w.decay(next);
             lds_in_order();
             decay *= m.dec.total[0] * m.dec.total[1];
@@ -568,32 +620,35 @@ __global__ __launch_bounds__(64, 2) void la_local(const LaParams) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, 16 * n + 4 * (lane & 3), lane);
+            for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, value_block<NT>(n, lane), lane);
         update_state<T, KP, NT, WHOLE>(S, m.k, vf, m.dec, half, J.K, w.vdim, lane);
     }
     write_state<KP, NT, WHOLE>(S, J, n0, w.vdim, lane, J.ends + (bh * p.segs + at.seg) * int64_t(J.K) * J.V);
     if (lane == 0 && at.tile == 0) J.decays[bh * p.segs + at.seg] = decay;
 }
 
+template <typename T, int KP, int NT, bool WHOLE>
+__global__ __launch_bounds__(64, 2) void la_local(const LaParams) {
+    Params& p = params();
+    __shared__ Tiles<T, KP, NT> m;
+    const Place at = place(p, p.segs);
+    Job& J = p.job[at.job];
+    if (at.tile * p.tile >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
+    if (J.rev) local_rows<T, KP, NT, WHOLE, true>(p, J, at, m);
+    else local_rows<T, KP, NT, WHOLE, false>(p, J, at, m);
+}
+
 // ----------------------------------------------------------------- the walk --
 template <typename T, int KP, int NT, int N, bool WHOLE>
-__global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams) {
-    Params& p = params();
+__device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Tiles<T, KP, NT>& m, int* bad_col, bool rev) {
     constexpr int R = kTerms<T>, kMax = N == 2 ? 1 : 2;
     using SV = Stage<T, 16 * NT>;
-    __shared__ Tiles<T, KP, NT> m;
-    __shared__ int bad_col[16 * NT];
-    const int segs = p.serial ? 1 : p.segs;
-    const Place at = place(p, segs);
-    Job& J = p.job[at.job];
     const int n0 = at.tile * p.tile, lane = int(threadIdx.x), c = lane & 15, g = lane >> 4;
-    if (n0 >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
     const int64_t bh = at.bh, KV = int64_t(J.K) * J.V;
     Walk<T, KP, NT, true, WHOLE> w(p, J, at, p.serial ? p.L : p.seg_tokens, lane);
-    const bool rev = w.rev;
     const int vdim = w.vdim;
     const T* xp = J.dot ? rows_of_head<T>(J.x, at) + n0 : nullptr;
-    const int64_t op = int64_t(at.b) * J.o.b + int64_t(at.h) * J.o.h + n0, seg_mask = p.seg_tokens - 1;
+    const int64_t op = int64_t(at.b) * J.o.b + int64_t(at.h) * J.o.h + n0;
     const bool near_o = WHOLE || (vdim == 16 * NT && near(J.o.l) && near(J.x.l));
 
     // the state before the walk's first token
@@ -660,13 +715,16 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
                 w.q.terms(i, kk, qf[i]);
                 w.k.terms(i, kk, kf[i]);
             }
-            P[0] = mfma_terms<R, R, 2>(kf[0], qf[0], P[0]);
-            P[2] = mfma_terms<R, R, 2>(kf[1], qf[1], P[2]);
-            if (rev) P[1] = mfma_terms<R, R, 2>(kf[1], qf[0], P[1]);
-            else P[1] = mfma_terms<R, R, 2>(kf[0], qf[1], P[1]);
+            {
+                f4* const diagonal[2] = {&P[0], &P[2]};
+                f4* const beside[1] = {&P[1]};
+                mfma_terms<2, 1, 1, R, R, 2>(kf, qf, diagonal);
+                if (rev) mfma_terms<1, 0, 0, R, R, 2>(kf + 1, qf, beside);
+                else mfma_terms<1, 0, 0, R, R, 2>(kf, qf + 1, beside);
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                if (!WHOLE && 16 * n >= vdim) continue;
+                if (!WHOLE && !tile_in<NT>(n, vdim)) continue;
                 u4 sf[N];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -676,31 +734,29 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
 #pragma unroll
                     for (int i = 0; i < N; ++i) sf[i][x] = t[i];
                 }
-#pragma unroll
-                for (int it = 0; it < 2; ++it) o[it][n] = mfma_terms<N, R, kMax>(sf, qf[it], o[it][n]);
+                f4* const to[2] = {&o[0][n], &o[1][n]};
+                mfma_terms<2, 0, 1, N, R, kMax>(&sf, qf, to);
             }
             stage_end();
         }
-        uint2 x4[2][NT][int(sizeof(T)) / 2];
+        // 8 columns (NT 1: 4) a lane: of the result, and of x for dot
+        constexpr int COLS = NT == 1 ? 4 : 8, VECS = (16 * NT + 4 * COLS - 1) / (4 * COLS);
+        constexpr int WORDS = COLS * int(sizeof(T)) / 8;       // 8-byte words of a row a vector
+        uint2 xv[2][VECS][WORDS];
         const bool whole_o = near_o && t0 + C <= w.end && !bad;
         if (J.dot && whole_o) {
-            const uint32_t off = (uint32_t(c) * uint32_t(J.x.l) + uint32_t(4 * g)) * uint32_t(sizeof(T));
+            const uint32_t off = (uint32_t(c) * uint32_t(J.x.l) + uint32_t(COLS * g)) * uint32_t(sizeof(T));
 #pragma unroll
             for (int it = 0; it < 2; ++it)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < int(sizeof(T)) / 2; ++i) {
-                        const half4_at2 h = *reinterpret_cast<const half4_at2*>(reinterpret_cast<const char*>(xp + (t0 + 16 * it) * J.x.l) +
-                                                                                off + (16 * n * int(sizeof(T)) + 8 * i));
-                        x4[it][n][i] = make_uint2(h.x, h.y);
-                    }
+                for (int n = 0; n < VECS; ++n)
+                    load_words<WORDS>(reinterpret_cast<const char*>(xp + (t0 + 16 * it) * J.x.l) + off + 4 * COLS * n * int(sizeof(T)), xv[it][n]);
         }
         u4 vf[NT][R];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, 16 * n + 4 * (lane & 3), lane);
+            for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, value_block<NT>(n, lane), lane);
 
         // P's decays and split, and o^T <- 2^G o^T + V^T P^T
         typedef int i4 __attribute__((ext_vector_type(4)));
@@ -714,13 +770,14 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
             const int Ii = m.dec.I[d0 + 16 * it + c];
+            const float row = m.dec.row[d0 + 16 * it + c];
             u4 pf[N];
 #pragma unroll
             for (int t = 0; t < N; ++t) pf[t] = u4{0u, 0u, 0u, 0u};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (it == j || (rev ? j > it : j < it)) {
-                    f4 v = (it == j ? P[2 * it] : P[1]) * cj[j];
+                    f4 v = (it == j ? P[2 * it] : P[1]) * (cj[j] * row);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         v[r] = __builtin_amdgcn_ldexpf(v[r], Ii - Ij[j][r]);
@@ -736,35 +793,42 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
                     }
                 }
             }
-            const float carried = m.dec.in[d0 + 16 * it + c], out = m.dec.row[d0 + 16 * it + c];
+            const float carried = m.dec.in[d0 + 16 * it + c];
+            f4* to[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                if (!WHOLE && 16 * n >= vdim) continue;
-                o[it][n] = mfma_terms<R, N, kMax>(vf[n], pf, o[it][n] * carried);
-                o[it][n] *= out;
+                o[it][n] *= carried;
+                to[n] = &o[it][n];
             }
+            mfma_terms<NT, 1, 0, R, N, kMax>(vf, &pf, to);
         }
 
         float dot[2] = {0.f, 0.f};
         if (whole_o) {
-            const uint32_t row = uint32_t(c) * uint32_t(J.o.l) + uint32_t(4 * g);
+            const uint32_t row = uint32_t(c) * uint32_t(J.o.l) + uint32_t(COLS * g);
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
                 const int64_t first = op + (t0 + 16 * it) * J.o.l;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float v[4] = {o[it][n][0], o[it][n][1], o[it][n][2], o[it][n][3]};
-                    if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 16 * n), v, 4);
-                    else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + first + (row + 16 * n), v, 4);
-                    if (J.dot) {
-                        float x[4];
-                        load4<T>(reinterpret_cast<const T*>(&x4[it][n]), x, 4);
+                for (int n = 0; n < VECS; ++n) {
+                    float v[COLS];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) dot[it] = __builtin_fmaf(v[r], x[r], dot[it]);
+                    for (int e = 0; e < COLS; ++e) v[e] = o[it][COLS / 4 * n + e / 4][e & 3];
+                    if (J.o_f32) store_cols<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
+                    else store_cols<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
+                    if (J.dot) {
+#pragma unroll
+                        for (int e = 0; e < COLS; e += 4) {
+                            float x[4];
+                            load4<T>(reinterpret_cast<const T*>(&xv[it][n][e * int(sizeof(T)) / 8]), x, 4);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) dot[it] = __builtin_fmaf(v[e + r], x[r], dot[it]);
+                        }
                     }
                 }
             }
         } else {
+            const int l = late(lane), c = l & 15, g = l >> 4;
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
                 const int i = 16 * it + c;
@@ -772,7 +836,7 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
                 const bool live = t < w.end;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int col = 16 * n + 4 * g, cnt = t < w.s1 ? vdim - col : 0;
+                    const int col = value_col<NT>(n, 4 * g), cnt = t < w.s1 ? vdim - col : 0;
                     float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -813,7 +877,7 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
         if (bad) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int first = bad_col[16 * n + c];
+                const int first = bad_col[value_col<NT>(n, c)];
                 if (first >= 0 && first < C) {
 #pragma unroll
                     for (int d = 0; d < KP / 16; ++d)
@@ -822,11 +886,23 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
                 }
             }
         }
-        if (J.ends && ((rev ? t0 & seg_mask : (t0 + C) & seg_mask) == 0 || (!rev && last)))
-            write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + (bh * p.segs + (t0 >> p.seg_shift)) * KV);
+        // (a whole row's walk: the state at the end of each segment)
+        const uint32_t seg = uint32_t(ch) / uint32_t(p.seg_chunks), next = uint32_t(rev ? ch - 1 : ch + 1) / uint32_t(p.seg_chunks);
+        if (J.ends && (last || next != seg)) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + (bh * p.segs + seg) * KV);
     }
     if (w.chunks == 0 && J.ends) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + bh * p.segs * KV);
     if (J.out_state) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.out_state + bh * KV);
+}
+
+template <typename T, int KP, int NT, int N, bool WHOLE>
+__global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams) {
+    Params& p = params();
+    __shared__ Tiles<T, KP, NT> m;
+    __shared__ int bad_col[16 * NT];
+    const Place at = place(p, p.serial ? 1 : p.segs);
+    Job& J = p.job[at.job];
+    if (at.tile * p.tile >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
+    walk_rows<T, KP, NT, N, WHOLE>(p, J, at, m, bad_col, J.rev);
 }
 
 }  // namespace la
