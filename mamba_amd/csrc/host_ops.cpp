@@ -31,7 +31,10 @@ std::string shape_str(at::IntArrayRef s) {            // as Python prints a tupl
     for (size_t i = 0; i < s.size(); ++i) r += (i ? ", " : "") + std::to_string(s[i]);
     return r + (s.size() == 1 ? ",)" : ")");
 }
-std::string dtype_str(at::ScalarType t) { return std::string(py::str(py::cast(t))); }
+std::string dtype_str(at::ScalarType t) {
+    const py::gil_scoped_acquire gil;                 // (a backward's checks run without it)
+    return std::string(py::str(py::cast(t)));
+}
 
 // what: the module's prefix of its messages
 #define REQUIRE(what, cond, msg)                                                   \
@@ -50,12 +53,33 @@ template <typename F>
 void launch(const at::Device& dev, const char* what, F&& f) {
     int rc;
     {
-        py::gil_scoped_release nogil;
+        std::optional<py::gil_scoped_release> nogil;
+        if (PyGILState_Check()) nogil.emplace();       // (autograd's thread does not hold it)
         const c10::OptionalDeviceGuard guard(dev);
         rc = f();
     }
     check(rc, what);                 // (the message is this thread's)
 }
+
+// The stream that is current for the device, for nodes of the autograd graph:
+// autograd runs a node's backward on the stream of its forward.
+void* current_stream(const at::Device& dev) {
+    if (!dev.is_cuda()) return nullptr;                // (refused by the call)
+    const py::gil_scoped_acquire gil;
+    static const py::handle get = py::object(py::module_::import("torch._C").attr("_cuda_getCurrentRawStream")).release();
+    return reinterpret_cast<void*>(get(int(dev.index())).cast<int64_t>());
+}
+// whether an operator's node will be asked for a backward
+bool wants_grad(std::initializer_list<const Tensor*> inputs) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : inputs)
+        if (t && t->defined() && t->requires_grad()) return true;
+    return false;
+}
+Tensor given(const OptT& t) { return t ? *t : Tensor(); }
+OptT maybe(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 bool itype_of(at::ScalarType t, int32_t* out) {
     switch (t) {
@@ -698,9 +722,9 @@ int64_t lin_segs(const ss_linear_attn_args& a) {
     return std::max<int64_t>(1, (a.seqlen + n - 1) / n);
 }
 
-// (out, last_state or None, ends or None, the tensors as read: q, k, v, g, initial_state, lengths)
-py::tuple lin_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
-                  const OptT& lengths, double scale, bool want_last, bool want_ends, int64_t stream) {
+struct LinOut { Tensor out; OptT last, ends; LinIn in; };     // in: the tensors as read
+LinOut lin_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
+               const OptT& lengths, double scale, bool want_last, bool want_ends, void* stream) {
     ss_linear_attn_args a;
     const LinIn in = fill_linear(a, q, k, v, g, initial, lengths, scale);
     const Tensor out = at::empty({a.batch, a.seqlen, a.heads, a.d_value}, in.v.options());
@@ -716,14 +740,14 @@ py::tuple lin_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
         ws = bytes_on(n, in.v);
         a.workspace = ptr(*ws); a.workspace_bytes = n;
     }
-    launch(in.v.device(), "linear_attn forward", [&] { return ss_linear_attn_fwd(&a, reinterpret_cast<void*>(stream)); });
-    return py::make_tuple(out, last, ends, py::make_tuple(in.q, in.k, in.v, in.g, in.initial, in.lengths));
+    launch(in.v.device(), "linear_attn forward", [&] { return ss_linear_attn_fwd(&a, stream); });
+    return {out, last, ends, in};
 }
 
-// (dq, dk, dv, dg fp32, dinitial_state or None)
-py::tuple lin_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
+struct LinGrads { Tensor dq, dk, dv, dg; OptT dinitial; };    // dg: fp32
+LinGrads lin_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
                   const OptT& lengths, const Tensor& ends, double scale, bool g_per_head, const Tensor& dout_,
-                  const OptT& dlast_, bool want_dinitial, int64_t stream) {
+                  const OptT& dlast_, bool want_dinitial, void* stream) {
     ss_linear_attn_bwd_args b{};
     const LinIn in = fill_linear(b.f, q, k, v, g, initial, lengths, scale);
     const ss_linear_attn_args& a = b.f;
@@ -756,9 +780,57 @@ py::tuple lin_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
             ws = bytes_on(n, in.v);
             b.f.workspace = ptr(*ws); b.f.workspace_bytes = n;
         }
-        launch(dev, "linear_attn backward", [&] { return ss_linear_attn_bwd(&b, reinterpret_cast<void*>(stream)); });
+        launch(dev, "linear_attn backward", [&] { return ss_linear_attn_bwd(&b, stream); });
     }
-    return py::make_tuple(dq, dk, dv, dg, dinitial);
+    return {dq, dk, dv, dg, dinitial};
+}
+
+// The autograd node, native like the rest of a call's host side: a forward +
+// backward of a small layer is bound by it (as a Python node, a border of 2047
+// x 1001 rows took 128 us for 38 of kernels).
+struct LinAttn : torch::autograd::Function<LinAttn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                 const OptT& initial, const OptT& lengths, double scale, bool want_last, bool need) {
+        const LinOut r = lin_fwd(q, k, v, g, initial, lengths, scale, want_last, need, current_stream(v.device()));
+        if (need) {
+            ctx->save_for_backward({r.in.q, r.in.k, r.in.v, r.in.g, given(r.in.initial), given(r.in.lengths), given(r.ends)});
+            ctx->saved_data["scale"] = scale;
+            ctx->saved_data["g_type"] = int64_t(g.scalar_type());
+            ctx->saved_data["per_head"] = g.dim() == 1;
+            ctx->set_materialize_grads(false);
+        }
+        variable_list out{r.out};
+        if (want_last) out.push_back(*r.last);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list r(9);
+        const Tensor dlast = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grads[0].defined() && !dlast.defined()) return r;
+        const auto t = ctx->get_saved_variables();
+        const Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(t[2]);
+        const bool has_initial = t[4].defined();
+        const LinGrads d = lin_bwd(t[0], t[1], t[2], t[3], maybe(t[4]), maybe(t[5]), t[6], ctx->saved_data["scale"].toDouble(),
+                                   ctx->saved_data["per_head"].toBool(), dout, maybe(dlast),
+                                   has_initial && ctx->needs_input_grad(4), current_stream(t[2].device()));
+        if (ctx->needs_input_grad(0)) r[0] = d.dq;
+        if (ctx->needs_input_grad(1)) r[1] = d.dk;
+        if (ctx->needs_input_grad(2)) r[2] = d.dv;
+        if (ctx->needs_input_grad(3)) r[3] = d.dg.to(at::ScalarType(ctx->saved_data["g_type"].toInt()));
+        r[4] = given(d.dinitial);
+        return r;
+    }
+};
+// (out, last_state or None)
+py::tuple linear_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
+                      const OptT& lengths, double scale, bool want_last) {
+    const bool need = wants_grad({&q, &k, &v, &g, initial ? &*initial : nullptr});
+    if (!need) {
+        const LinOut r = lin_fwd(q, k, v, g, initial, lengths, scale, want_last, false, current_stream(v.device()));
+        return py::make_tuple(r.out, r.last);
+    }
+    const variable_list r = LinAttn::apply(q, k, v, g, initial, lengths, scale, want_last, need);
+    return py::make_tuple(r[0], want_last ? OptT(r[1]) : OptT());
 }
 
 constexpr const char* kLinUp = "linear_attn_update";
@@ -845,9 +917,10 @@ void norm_x(const char* what, const Tensor& x, int32_t* dtype) {
     REQUIRE(what, x.dim() >= 1, "x must have at least one dimension");
 }
 
-// (out, s, rstd or None, the tensors as read: x, residual, gate, post, pre, scale_vec), rows as (rows, dim)
-py::tuple block_norm_fwd(const Tensor& x_, const Tensor& residual_, const OptT& gate_, const Tensor& post, const Tensor& pre,
-                         const OptT& scale_vec, double scale, double eps, bool want_rstd, int64_t stream) {
+// (rows as (rows, dim); read: x, residual, gate, post, pre, scale_vec)
+struct BorderOut { Tensor out, s; OptT rstd; variable_list read; };
+BorderOut block_norm_fwd(const Tensor& x_, const Tensor& residual_, const OptT& gate_, const Tensor& post, const Tensor& pre,
+                         const OptT& scale_vec, double scale, double eps, bool want_rstd, void* stream) {
     ss_block_norm_args a{};
     norm_x(kBlockNorm, x_, &a.dtype);
     const Tensor x = any_rows(x_), residual = like_rows(kBlockNorm, "residual", residual_, x_);
@@ -865,14 +938,15 @@ py::tuple block_norm_fwd(const Tensor& x_, const Tensor& residual_, const OptT& 
     a.x = ptr(x); a.residual = ptr(residual); a.gate = ptr(gate);
     a.post = ptr(w.w[0]); a.pre = ptr(w.w[1]); a.scale_vec = ptr(w.w[2]);
     a.out = ptr(out); a.residual_out = ptr(s); a.rstd = fptr<float>(rstd);
-    launch(x.device(), "block_norm forward", [&] { return ss_block_norm_fwd(&a, reinterpret_cast<void*>(stream)); });
-    return py::make_tuple(out, s, rstd, py::make_tuple(x, residual, gate, w.w[0], w.w[1], w.w[2]));
+    launch(x.device(), "block_norm forward", [&] { return ss_block_norm_fwd(&a, stream); });
+    return {out, s, rstd, {x, residual, given(gate), given(w.w[0]), given(w.w[1]), given(w.w[2])}};
 }
 
-// (dx, dresidual or None, dgate or None, dpost, dpre, dscale or None) from the forward's tensors as read
-py::tuple block_norm_bwd(const Tensor& x, const Tensor& residual, const OptT& gate, const Tensor& post, const Tensor& pre,
+// from the forward's tensors as read
+struct BorderGrads { Tensor dx; OptT dresidual, dgate; Tensor dpost, dpre; OptT dscale; };
+BorderGrads block_norm_bwd(const Tensor& x, const Tensor& residual, const OptT& gate, const Tensor& post, const Tensor& pre,
                          const OptT& scale_vec, const Tensor& rstd, double scale, const OptT& dout_, const OptT& ds_,
-                         bool want_dresidual, int64_t stream) {
+                         bool want_dresidual, void* stream) {
     ss_block_norm_bwd_args g{};
     norm_x(kBlockNorm, x, &g.dtype);
     REQUIRE(kBlockNorm, x.dim() == 2, "x must be (rows, dim)");
@@ -900,13 +974,58 @@ py::tuple block_norm_bwd(const Tensor& x, const Tensor& residual, const OptT& ga
     g.scale_vec = ptr(scale_vec); g.rstd = static_cast<float*>(ptr(rstd)); g.dout = ptr(dout); g.dresidual_out = ptr(ds);
     g.dx = ptr(dx); g.dresidual = ptr(dresidual); g.dgate = ptr(dgate); g.dpost = ptr(dpost); g.dpre = ptr(dpre);
     g.dscale = ptr(dscale); g.workspace = ptr(ws); g.workspace_bytes = n;
-    launch(x.device(), "block_norm backward", [&] { return ss_block_norm_bwd(&g, reinterpret_cast<void*>(stream)); });
-    return py::make_tuple(dx, dresidual, dgate, dpost, dpre, dscale);
+    launch(x.device(), "block_norm backward", [&] { return ss_block_norm_bwd(&g, stream); });
+    return {dx, dresidual, dgate, dpost, dpre, dscale};
+}
+
+struct BlockNorm : torch::autograd::Function<BlockNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& post, const Tensor& pre,
+                                 const OptT& gate, const OptT& scale_vec, double scale, double eps) {
+        const BorderOut r = block_norm_fwd(x, residual, gate, post, pre, scale_vec, scale, eps, true, current_stream(x.device()));
+        variable_list saved = r.read;
+        saved.push_back(*r.rstd);
+        ctx->save_for_backward(saved);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["types"] = std::vector<int64_t>{int64_t(post.scalar_type()), int64_t(pre.scalar_type()),
+                                                        scale_vec ? int64_t(scale_vec->scalar_type()) : 0};
+        ctx->set_materialize_grads(false);
+        return {r.out.view(x.sizes()), r.s.view(x.sizes())};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list r(8);
+        if (!grads[0].defined() && !grads[1].defined()) return r;
+        const auto t = ctx->get_saved_variables();
+        const auto rows = [&](const Tensor& g) { return g.defined() ? OptT(g.reshape(t[0].sizes())) : OptT(); };
+        const BorderGrads d = block_norm_bwd(t[0], t[1], maybe(t[2]), t[3], t[4], maybe(t[5]), t[6], ctx->saved_data["scale"].toDouble(),
+                                             rows(grads[0]), rows(grads[1]), ctx->needs_input_grad(1), current_stream(t[0].device()));
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        const auto typed = [&](const Tensor& w, int i) { return w.to(at::ScalarType(types[i])); };
+        const size_t at_gate = 4, at_scale = t[2].defined() ? 5 : 4;      // (an absent gate is no input)
+        if (ctx->needs_input_grad(0)) r[0] = d.dx.view(shape);
+        if (ctx->needs_input_grad(1)) r[1] = d.dresidual->view(shape);
+        if (ctx->needs_input_grad(2)) r[2] = typed(d.dpost, 0);
+        if (ctx->needs_input_grad(3)) r[3] = typed(d.dpre, 1);
+        if (t[2].defined() && ctx->needs_input_grad(at_gate)) r[4] = d.dgate->view(shape);
+        if (t[5].defined() && ctx->needs_input_grad(at_scale)) r[5] = typed(*d.dscale, 2);
+        return r;
+    }
+};
+// (out, s)
+py::tuple block_norm(const Tensor& x, const Tensor& residual, const Tensor& post, const Tensor& pre, const OptT& gate,
+                     const OptT& scale_vec, double scale, double eps) {
+    if (!wants_grad({&x, &residual, &post, &pre, gate ? &*gate : nullptr, scale_vec ? &*scale_vec : nullptr})) {
+        const BorderOut r = block_norm_fwd(x, residual, gate, post, pre, scale_vec, scale, eps, false, current_stream(x.device()));
+        return py::make_tuple(r.out.view(x.sizes()), r.s.view(x.sizes()));
+    }
+    const variable_list r = BlockNorm::apply(x, residual, post, pre, gate, scale_vec, scale, eps);
+    return py::make_tuple(r[0], r[1]);
 }
 
 // (out, x, gate, weight as read), rows as (rows, dim)
-py::tuple gated_norm_fwd(const Tensor& x_, const Tensor& gate_, const Tensor& weight, int64_t groups, double eps,
-                         int64_t stream) {
+variable_list gated_norm_fwd(const Tensor& x_, const Tensor& gate_, const Tensor& weight, int64_t groups, double eps,
+                             void* stream) {
     ss_gated_norm_args a{};
     norm_x(kGatedNorm, x_, &a.dtype);
     const Tensor x = any_rows(x_), gate = like_rows(kGatedNorm, "gate", gate_, x_);
@@ -917,13 +1036,13 @@ py::tuple gated_norm_fwd(const Tensor& x_, const Tensor& gate_, const Tensor& we
     const Tensor out = at::empty(x.sizes(), x.options());
     a.x_row_stride = x.stride(0); a.gate_row_stride = gate.stride(0); a.out_row_stride = out.stride(0);
     a.x = ptr(x); a.gate = ptr(gate); a.weight = ptr(w.w[0]); a.out = ptr(out);
-    launch(x.device(), "gated_rms_norm forward", [&] { return ss_gated_norm_fwd(&a, reinterpret_cast<void*>(stream)); });
-    return py::make_tuple(out, x, gate, w.w[0]);
+    launch(x.device(), "gated_rms_norm forward", [&] { return ss_gated_norm_fwd(&a, stream); });
+    return {out, x, gate, *w.w[0]};
 }
 
 // (dx, dgate, dweight)
-py::tuple gated_norm_bwd(const Tensor& x, const Tensor& gate, const Tensor& weight, const Tensor& dout_, int64_t groups,
-                         double eps, int64_t stream) {
+variable_list gated_norm_bwd(const Tensor& x, const Tensor& gate, const Tensor& weight, const Tensor& dout_, int64_t groups,
+                             double eps, void* stream) {
     ss_gated_norm_bwd_args g{};
     norm_x(kGatedNorm, x, &g.dtype);
     REQUIRE(kGatedNorm, x.dim() == 2, "x must be (rows, dim)");
@@ -939,8 +1058,36 @@ py::tuple gated_norm_bwd(const Tensor& x, const Tensor& gate, const Tensor& weig
     g.x_row_stride = x.stride(0); g.gate_row_stride = gate.stride(0); g.dout_row_stride = dout.stride(0);
     g.x = ptr(x); g.gate = ptr(gate); g.weight = ptr(weight); g.dout = ptr(dout);
     g.dx = ptr(dx); g.dgate = ptr(dgate); g.dweight = ptr(dw); g.workspace = ptr(ws); g.workspace_bytes = n;
-    launch(x.device(), "gated_rms_norm backward", [&] { return ss_gated_norm_bwd(&g, reinterpret_cast<void*>(stream)); });
-    return py::make_tuple(dx, dgate, dw);
+    launch(x.device(), "gated_rms_norm backward", [&] { return ss_gated_norm_bwd(&g, stream); });
+    return {dx, dgate, dw};
+}
+
+struct GatedNorm : torch::autograd::Function<GatedNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
+        const variable_list r = gated_norm_fwd(x, gate, weight, groups, eps, current_stream(x.device()));
+        ctx->save_for_backward({r[1], r[2], r[3]});
+        ctx->saved_data["groups"] = groups;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["type"] = int64_t(weight.scalar_type());
+        return r[0].view(x.sizes());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto t = ctx->get_saved_variables();
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const variable_list d = gated_norm_bwd(t[0], t[1], t[2], grads[0].reshape(t[0].sizes()), ctx->saved_data["groups"].toInt(),
+                                               ctx->saved_data["eps"].toDouble(), current_stream(t[0].device()));
+        variable_list r(5);
+        if (ctx->needs_input_grad(0)) r[0] = d[0].view(shape);
+        if (ctx->needs_input_grad(1)) r[1] = d[1].view(shape);
+        if (ctx->needs_input_grad(2)) r[2] = d[2].to(at::ScalarType(ctx->saved_data["type"].toInt()));
+        return r;
+    }
+};
+Tensor gated_norm(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
+    if (!wants_grad({&x, &gate, &weight}))
+        return gated_norm_fwd(x, gate, weight, groups, eps, current_stream(x.device()))[0].view(x.sizes());
+    return GatedNorm::apply(x, gate, weight, groups, eps);
 }
 
 // -------------------------------------------------------------- clipping --
@@ -1014,13 +1161,10 @@ PYBIND11_MODULE(mamba_host, m) {
     m.def("linear_ws_bytes", &linear_ws_bytes);
     m.def("linear", &linear);
     m.def("state_update", &state_update);
-    m.def("lin_fwd", &lin_fwd);
-    m.def("lin_bwd", &lin_bwd);
+    m.def("linear_attn", &linear_attn);
     m.def("lin_update", &lin_update);
-    m.def("block_norm_fwd", &block_norm_fwd);
-    m.def("block_norm_bwd", &block_norm_bwd);
-    m.def("gated_norm_fwd", &gated_norm_fwd);
-    m.def("gated_norm_bwd", &gated_norm_bwd);
+    m.def("block_norm", &block_norm);
+    m.def("gated_norm", &gated_norm);
     m.def("clip_grads", &clip_grads);
     m.def("abi", [] { return py::make_tuple(SS_ABI_VERSION, sizeof(ss_fwd_args), sizeof(ss_bwd_args)); });
 }

@@ -28,45 +28,15 @@ d_key), v (batch, heads, d_value), g (batch, heads) or (heads,); returns out
 (batch, heads, d_value).  The state after a prompt is linear_attn_fn's
 last_state.
 """
-import torch
-
 from .. import _native as nat
 from ..selective_scan import _raw_stream
-
-
-class LinearAttnFn(torch.autograd.Function):
-    """Autograd of linear_attn_fn; returns (out, last_state or None)."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, g, initial_state, lengths, scale, want_last):
-        need = any(ctx.needs_input_grad[:5])
-        out, last, ends, read = nat.host().lin_fwd(q, k, v, g, initial_state, lengths, scale, want_last, need,
-                                                   _raw_stream(v.device))
-        if need:
-            ctx.save_for_backward(*read, ends)
-        ctx.scale, ctx.g_dtype, ctx.g_per_head = scale, g.dtype, g.dim() == 1
-        ctx.set_materialize_grads(False)
-        return out, last
-
-    @staticmethod
-    def backward(ctx, dout, dlast=None):
-        if dout is None and dlast is None:
-            return (None,) * 8
-        q, k, v, g, initial, lengths, ends = ctx.saved_tensors
-        if dout is None:
-            dout = torch.zeros_like(v)
-        need = ctx.needs_input_grad
-        dq, dk, dv, dg, dinitial = nat.host().lin_bwd(q, k, v, g, initial, lengths, ends, ctx.scale, ctx.g_per_head, dout,
-                                                      dlast, initial is not None and need[4], _raw_stream(v.device))
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None,
-                dg.to(ctx.g_dtype) if need[3] else None, dinitial, None, None, None)
 
 
 def linear_attn_fn(q, k, v, g, scale=None, initial_state=None, lengths=None, return_last_state=False):
     """Linear attention with a decay for each head; see the module docstring."""
     if scale is None:
         scale = max(1, q.shape[-1]) ** -0.5
-    out, last = LinearAttnFn.apply(q, k, v, g, initial_state, lengths, float(scale), bool(return_last_state))
+    out, last = nat.host().linear_attn(q, k, v, g, initial_state, lengths, float(scale), bool(return_last_state))
     return (out, last) if return_last_state else out
 
 
