@@ -47,7 +47,8 @@ namespace ss {
 
 namespace {
 
-constexpr int kMaxParts = 512;                // workgroups (rows of column sums) of a backward
+constexpr int kMaxParts = 512;                // workgroups (rows of column sums) of a border's backward
+constexpr int kHeadParts = 1024, kHeadBlocks = 4096;   // workgroups of the heads' backward and forward
 constexpr int kSumWaves = 16;                 // column sums: waves per workgroup
 
 struct BorderParams {
@@ -72,6 +73,29 @@ struct GatedParams {
     void* out;
     const void* dout; void* dx; void* dgate;
     float* part;                                             // (row blocks, dim)
+};
+
+// a lane's weights in their own type
+template <typename T, typename TW>
+struct PackedWeights {
+    static constexpr int VE = rowvec<T>::VE, PER = rowvec<TW>::VE, N = VE / PER;
+    uint4 v[N];
+    __device__ __forceinline__ void load(const TW* p, int n) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = rowvec<TW>::load(p + i * PER, n - i * PER);
+    }
+    // (unpacked at each use: the compiler would do it once, ahead of the rows)
+    __device__ __forceinline__ void get(float (&o)[VE]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float t[PER];
+            uint4 w = v[i];
+            __asm__ volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
+            rowvec<TW>::unpack(w, t);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) o[i * PER + e] = t[e];
+        }
+    }
 };
 
 // sums over the waves of a row's team; red: two buffers, used in turn, so one
@@ -173,26 +197,25 @@ __global__ __launch_bounds__(kBlock<WPR>) void block_norm_fwd(const BorderParams
 }
 
 template <typename T, typename TW, int WPR, int EPT>
-__global__ __launch_bounds__(kBlock<WPR>) void block_norm_bwd(const BorderParams p) {
+__global__ __launch_bounds__(kBlock<WPR>, kBlock<WPR> / 256 > 2 ? kBlock<WPR> / 256 : 2) void block_norm_bwd(const BorderParams p) {
     using R = rowvec<T>;
     constexpr int VE = R::VE, NV = EPT / VE, TEAM = 64 * WPR, ROWS = kBlock<WPR> / TEAM;
     __shared__ float red[2][WPR][3];
     __shared__ float cols[ROWS > 1 ? 3 * TEAM * EPT : 1];
     const int u = int(threadIdx.x) % TEAM, wave = u >> 6;
     int col[NV], cnt[NV];
-    float wpost[NV][VE], wpre[NV][VE], wsc[NV][VE], apost[NV][VE], apre[NV][VE], asc[NV][VE];
+    // (weights stay in their own type: as fp32 they and the sums would leave room for one wave a SIMD)
+    PackedWeights<T, TW> kpost[NV], kpre[NV], ksc[NV];
+    float apost[NV][VE], apre[NV][VE], asc[NV][VE];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         col[k] = (k * TEAM + u) * VE;
         cnt[k] = p.dim - col[k];
-        R::template weights<TW>(static_cast<const TW*>(p.post) + col[k], cnt[k], wpost[k]);
-        R::template weights<TW>(static_cast<const TW*>(p.pre) + col[k], cnt[k], wpre[k]);
-        if (p.wscale) R::template weights<TW>(static_cast<const TW*>(p.wscale) + col[k], cnt[k], wsc[k]);
+        kpost[k].load(static_cast<const TW*>(p.post) + col[k], cnt[k]);
+        kpre[k].load(static_cast<const TW*>(p.pre) + col[k], cnt[k]);
+        ksc[k].load(static_cast<const TW*>(p.wscale) + col[k], p.wscale ? cnt[k] : 0);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            if (!p.wscale) wsc[k][e] = p.scale;
-            apost[k][e] = apre[k][e] = asc[k][e] = 0.f;
-        }
+        for (int e = 0; e < VE; ++e) apost[k][e] = apre[k][e] = asc[k][e] = 0.f;
     }
     const float inv = 1.f / float(p.dim);
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
@@ -211,7 +234,10 @@ __global__ __launch_bounds__(kBlock<WPR>) void block_norm_bwd(const BorderParams
         float sig[NV][VE], sum[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            float x[VE], r[VE], z[VE], o[VE], d[VE];
+            float x[VE], r[VE], z[VE], o[VE], d[VE], wpost[VE], wpre[VE], wsc[VE];
+            kpost[k].get(wpost);
+            kpre[k].get(wpre);
+            ksc[k].get(wsc);
             R::unpack(cx[k], x);
             R::unpack(cr[k], r);
             R::unpack(cz[k], z);
@@ -219,13 +245,14 @@ __global__ __launch_bounds__(kBlock<WPR>) void block_norm_bwd(const BorderParams
             R::unpack(cs[k], d);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
+                if (!p.wscale) wsc[e] = p.scale;
                 float sil = 1.f;
                 if (p.gate) {
                     sig[k][e] = sigmoid(z[e]);
                     sil = z[e] * sig[k][e];
                 }
-                const float c = wsc[k][e] * sil * (1.f + wpost[k][e]) * x[e], s = __builtin_fmaf(n1, c, r[e]);
-                const float ow = o[e] * (1.f + wpre[k][e]), h = __builtin_fmaf(n2, ow, d[e]);
+                const float c = wsc[e] * sil * (1.f + wpost[e]) * x[e], s = __builtin_fmaf(n1, c, r[e]);
+                const float ow = o[e] * (1.f + wpre[e]), h = __builtin_fmaf(n2, ow, d[e]);
                 sum[0] = __builtin_fmaf(ow, s, sum[0]);
                 sum[1] = __builtin_fmaf(h, c, sum[1]);
                 sum[2] = __builtin_fmaf(s, c, sum[2]);
@@ -237,7 +264,10 @@ __global__ __launch_bounds__(kBlock<WPR>) void block_norm_bwd(const BorderParams
         const float k1 = n1 * n1 * n1 * (sum[1] - k2 * sum[2]) * inv;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            float x[VE], r[VE], z[VE], o[VE], d[VE], gz[VE];
+            float x[VE], r[VE], z[VE], o[VE], d[VE], gz[VE], wpost[VE], wpre[VE], wsc[VE];
+            kpost[k].get(wpost);
+            kpre[k].get(wpre);
+            ksc[k].get(wsc);
             R::unpack(cx[k], x);
             R::unpack(cr[k], r);
             R::unpack(cz[k], z);
@@ -245,11 +275,12 @@ __global__ __launch_bounds__(kBlock<WPR>) void block_norm_bwd(const BorderParams
             R::unpack(cs[k], d);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
-                const float w1 = 1.f + wpost[k][e], sil = p.gate ? z[e] * sig[k][e] : 1.f;
-                const float c = wsc[k][e] * sil * w1 * x[e], s = __builtin_fmaf(n1, c, r[e]);
-                const float ow = o[e] * (1.f + wpre[k][e]);
+                if (!p.wscale) wsc[e] = p.scale;
+                const float w1 = 1.f + wpost[e], sil = p.gate ? z[e] * sig[k][e] : 1.f;
+                const float c = wsc[e] * sil * w1 * x[e], s = __builtin_fmaf(n1, c, r[e]);
+                const float ow = o[e] * (1.f + wpre[e]);
                 const float dr = __builtin_fmaf(n2, ow, d[e]) - k2 * s;
-                const float xn = x[e] * n1, dt = dr * wsc[k][e];
+                const float xn = x[e] * n1, dt = dr * wsc[e];
                 apre[k][e] = __builtin_fmaf(o[e], s * n2, apre[k][e]);
                 apost[k][e] = __builtin_fmaf(dt * sil, xn, apost[k][e]);
                 asc[k][e] = __builtin_fmaf(dr, xn * w1 * sil, asc[k][e]);
@@ -483,7 +514,7 @@ int64_t border_parts(int64_t rows, int64_t dim) {
 
 // the teams' places in a workgroup, and the row blocks of a launch
 struct HeadGrid { int gpw, rpw, threads; int64_t sets, blocks; };
-HeadGrid head_grid(int64_t rows, int64_t groups, int64_t n) {
+HeadGrid head_grid(int64_t rows, int64_t groups, int64_t n, bool bwd) {
     HeadGrid h{};
     int L = 2;
     (void)for_group(n, [&](auto l, auto) { L = decltype(l)::value; return hipSuccess; });
@@ -493,15 +524,15 @@ HeadGrid head_grid(int64_t rows, int64_t groups, int64_t n) {
     if (h.rpw > rows && rows > 0) h.rpw = int(rows);
     h.threads = (h.gpw * h.rpw * L + 63) / 64 * 64;
     h.sets = (groups + h.gpw - 1) / h.gpw;
-    const int64_t want = (rows + h.rpw - 1) / h.rpw, most = (4 * kMaxParts + h.sets - 1) / h.sets;
+    // (the backward's row blocks are rows of column sums: fewer of them)
+    const int64_t want = (rows + h.rpw - 1) / h.rpw, all = bwd ? kHeadParts : kHeadBlocks, most = (all + h.sets - 1) / h.sets;
     h.blocks = want < most ? want : most;
-    if (h.blocks > kMaxParts) h.blocks = kMaxParts;
     return h;
 }
 
 template <bool BWD>
 hipError_t gated_launch(GatedParams p, int dtype, int w_dtype, void* dweight, hipStream_t stream) {
-    const HeadGrid h = head_grid(p.rows, p.groups, p.n);
+    const HeadGrid h = head_grid(p.rows, p.groups, p.n, BWD);
     p.gpw = h.gpw; p.rpw = h.rpw;
     return for_types(dtype, w_dtype, [&](auto t, auto tw) {
         using T = decltype(t);
@@ -526,7 +557,7 @@ hipError_t gated_launch(GatedParams p, int dtype, int w_dtype, void* dweight, hi
 
 int64_t block_norm_bwd_space(int64_t rows, int64_t dim) { return border_parts(rows, dim) * 3 * dim * 4; }
 int64_t gated_norm_bwd_space(int64_t rows, int64_t dim, int64_t groups) {
-    return groups > 0 && rows > 0 ? head_grid(rows, groups, dim / groups).blocks * dim * 4 : 0;
+    return groups > 0 && rows > 0 ? head_grid(rows, groups, dim / groups, true).blocks * dim * 4 : 0;
 }
 
 hipError_t block_norm_fwd_launch(const ss_block_norm_args* a, hipStream_t stream) {
