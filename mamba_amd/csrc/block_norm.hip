@@ -75,21 +75,30 @@ struct GatedParams {
     float* part;                                             // (row blocks, dim)
 };
 
-// a lane's weights in their own type
-template <typename T, typename TW>
+// a lane's weights in their own type; HOLD: in registers, else read at each use
+// (from the caches: 16 fp32 weights a lane of three vectors would spill)
+template <typename T, typename TW, bool HOLD>
 struct PackedWeights {
     static constexpr int VE = rowvec<T>::VE, PER = rowvec<TW>::VE, N = VE / PER;
-    uint4 v[N];
-    __device__ __forceinline__ void load(const TW* p, int n) {
+    uint4 v[HOLD ? N : 1];
+    const TW* at;
+    int n;
+    __device__ __forceinline__ void load(const TW* p, int n_) {
+        at = p;
+        n = n_;
+        if constexpr (HOLD) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = rowvec<TW>::load(p + i * PER, n - i * PER);
+            for (int i = 0; i < N; ++i) v[i] = rowvec<TW>::load(p + i * PER, n - i * PER);
+        }
     }
     // (unpacked at each use: the compiler would do it once, ahead of the rows)
     __device__ __forceinline__ void get(float (&o)[VE]) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float t[PER];
-            uint4 w = v[i];
+            uint4 w;
+            if constexpr (HOLD) w = v[i];
+            else w = rowvec<TW>::load(at + i * PER, n - i * PER);
             __asm__ volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
             rowvec<TW>::unpack(w, t);
 #pragma unroll
@@ -205,7 +214,7 @@ __global__ __launch_bounds__(kBlock<WPR>, kBlock<WPR> / 256 > 2 ? kBlock<WPR> / 
     const int u = int(threadIdx.x) % TEAM, wave = u >> 6;
     int col[NV], cnt[NV];
     // (weights stay in their own type: as fp32 they and the sums would leave room for one wave a SIMD)
-    PackedWeights<T, TW> kpost[NV], kpre[NV], ksc[NV];
+    PackedWeights<T, TW, EPT * sizeof(TW) <= 32> kpost[NV], kpre[NV], ksc[NV];
     float apost[NV][VE], apre[NV][VE], asc[NV][VE];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -476,7 +485,7 @@ hipError_t for_row(int64_t dim, F&& f) {
     if (dim <= 1024) return f(I(integral_constant<int, 1>{}), I(integral_constant<int, 16>{}));
     if (dim <= 2048) return f(I(integral_constant<int, 4>{}), I(integral_constant<int, 8>{}));
     if (dim <= 4096) return f(I(integral_constant<int, 4>{}), I(integral_constant<int, 16>{}));
-    if (dim <= 8192) return f(I(integral_constant<int, 16>{}), I(integral_constant<int, 8>{}));
+    if (dim <= 8192) return f(I(integral_constant<int, 8>{}), I(integral_constant<int, 16>{}));
     return f(I(integral_constant<int, 16>{}), I(integral_constant<int, 16>{}));
 }
 int border_rows_at_once(int64_t dim) { return dim <= 1024 ? 4 : 1; }

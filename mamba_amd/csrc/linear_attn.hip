@@ -19,6 +19,7 @@
 #include <cstdint>
 
 #include "linear_attn.hpp"
+#include "norm_rows.hpp"
 #include "ss_device.hpp"
 #include "ss_kernels.hpp"
 
@@ -61,33 +62,27 @@ __global__ __launch_bounds__(256) void la_carry(const LaParams p) {
     if (J.out_state) J.out_state[bh * KV + i] = s;
 }
 
+// Sum over the 4 waves of a workgroup, in every thread.
+__device__ __forceinline__ double sum_all(double v, double (&red)[4]) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 // dg of one segment: the inner product of the two states at its end, and the
-// sums of D from its last token down.  256 threads, up to 4 tokens each.
+// sums of D from its last token down.  256 threads, up to 4 tokens each.  Bound
+// by the states' bytes.
 constexpr int kDgTok = 4;
 
 __global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
     const int64_t bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-    const int seg = int(blockIdx.y), tid = int(threadIdx.x);
+    const int seg = int(blockIdx.y), tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const int64_t s0 = seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
     const int64_t len = row_len(p.lens, b, p.L);
-    __shared__ double red[256];
-
-    double f = 0.0;
-    const float* dS = seg + 1 < p.segs ? p.rends + (bh * p.segs + seg + 1) * int64_t(p.KV)
-                                       : p.dlast ? p.dlast + bh * int64_t(p.KV) : nullptr;
-    if (dS) {
-        const float* S = p.ends + (bh * p.segs + seg) * int64_t(p.KV);
-#pragma unroll 8
-        for (int i = tid; i < p.KV; i += 256) f += double(S[i]) * double(dS[i]);
-    }
-    red[tid] = f;
-    __syncthreads();
-    for (int m = 128; m >= 1; m >>= 1) {
-        if (tid < m) red[tid] += red[tid + m];
-        __syncthreads();
-    }
-    const double F = red[0];
-    __syncthreads();
+    __shared__ double red[4];
 
     // this thread's tokens, from the segment's end down
     double d[kDgTok], sum = 0.0;
@@ -99,19 +94,39 @@ __global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
             for (int q = 0; q < p.qtiles; ++q) v += p.dotq[(int64_t(q) * p.B * p.H + bh) * p.L + t];
             for (int k = 0; k < p.ktiles; ++k) v -= p.dotk[(int64_t(k) * p.B * p.H + bh) * p.L + t];
         }
-        sum += v;
+        d[i] = v;
+    }
+    double f = 0.0;
+    const float* dS = seg + 1 < p.segs ? p.rends + (bh * p.segs + seg + 1) * int64_t(p.KV)
+                                       : p.dlast ? p.dlast + bh * int64_t(p.KV) : nullptr;
+    if (dS) {
+        const float* S = p.ends + (bh * p.segs + seg) * int64_t(p.KV);
+#pragma unroll 4
+        for (int i = 4 * tid; i < p.KV; i += 1024) {
+            float x[4], y[4];
+            rowvec<float>::unpack(rowvec<float>::load(S + i, p.KV - i), x);
+            rowvec<float>::unpack(rowvec<float>::load(dS + i, p.KV - i), y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f += double(x[e]) * double(y[e]);
+        }
+    }
+    const double F = sum_all(f, red);
+#pragma unroll
+    for (int i = 0; i < kDgTok; ++i) {
+        sum += d[i];
         d[i] = sum;
     }
-    red[tid] = sum;
-    __syncthreads();
-    for (int m = 1; m < 256; m <<= 1) {                 // sums over the threads up to this one
-        const double o = tid >= m ? red[tid - m] : 0.0;
-        __syncthreads();
-        red[tid] += o;
-        __syncthreads();
+    double upto = sum;                                  // sums over the threads up to this one
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const double o = __shfl_up(upto, m, 64);
+        if (lane >= m) upto += o;
     }
-    const double base = F + (tid ? red[tid - 1] : 0.0);
     __syncthreads();
+    if (lane == 63) red[wave] = upto;
+    __syncthreads();
+    double base = F + (upto - sum);
+    for (int w = 0; w < wave; ++w) base += red[w];
     double mine = 0.0;
 #pragma unroll
     for (int i = 0; i < kDgTok; ++i) {
@@ -123,13 +138,8 @@ __global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
         }
     }
     if (!p.part) return;
-    red[tid] = mine;
-    __syncthreads();
-    for (int m = 128; m >= 1; m >>= 1) {
-        if (tid < m) red[tid] += red[tid + m];
-        __syncthreads();
-    }
-    if (tid == 0) p.part[bh * p.segs + seg] = red[0];
+    mine = sum_all(mine, red);
+    if (tid == 0) p.part[bh * p.segs + seg] = mine;
 }
 
 // dg of a head with one decay: the sum over batch rows and segments
@@ -167,12 +177,12 @@ constexpr int64_t kFull = 1024, kSegsWanted = 1536, kSegTokMin = 64, kSegTokMax 
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
-int64_t type_size(const ss_linear_attn_args& a) { return a.dtype == SS_F32 ? 4 : 2; }
+int terms(const ss_linear_attn_args& a) { return a.dtype == SS_F32 ? 3 : a.dtype == SS_BF16 ? 1 : 2; }
 int64_t tile_count(int64_t dim, int tile) { return (dim + tile - 1) / tile; }
 // the backward's passes share a launch: the tile of the widest
 int bwd_tile(const ss_linear_attn_args& a) {
     const int64_t d = a.d_key > a.d_value ? a.d_key : a.d_value;
-    return la_tile(d, d, type_size(a));
+    return la_tile(d, d, terms(a));
 }
 
 struct BwdSpace { int64_t dotq, dotk, rends, decays, part, dq, dk, bytes; };
@@ -202,7 +212,7 @@ bool serial(const ss_linear_attn_args& a, int64_t tiles) {
 struct FwdSpace { int64_t ends, decays, bytes; };
 FwdSpace fwd_space(const ss_linear_attn_args& a) {
     FwdSpace s{};
-    if (serial(a, tile_count(a.d_value, la_tile(a.d_key, a.d_value, type_size(a))))) return s;
+    if (serial(a, tile_count(a.d_value, la_tile(a.d_key, a.d_value, terms(a))))) return s;
     const int64_t n = a.batch * a.heads * linear_attn_segs(&a);
     s.decays = a.ends ? 0 : round16(n * a.d_key * a.d_value * 4);
     s.bytes = s.decays + round16(n * 4);
@@ -239,8 +249,8 @@ hipError_t carries(int dtype, const LaParams& local, hipStream_t stream) {
     hipLaunchKernelGGL(la_carry, dim3(unsigned((KV + 255) / 256), unsigned(bh), unsigned(local.njobs)), dim3(256), 0, stream, local);
     return hipGetLastError();
 }
-hipError_t walk(int dtype, const LaParams& p, bool fine, hipStream_t stream) {
-    return for_type(dtype, [&](auto t) { return la_walk_launch<decltype(t)>(p, fine, stream); });
+hipError_t walk(int dtype, const LaParams& p, bool backward, hipStream_t stream) {
+    return for_type(dtype, [&](auto t) { return la_walk_launch<decltype(t)>(p, backward, stream); });
 }
 
 }  // namespace
@@ -263,7 +273,7 @@ hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stre
     LaParams p = common(*a);
     const int rep = int(a->heads / a->groups);
     p.njobs = 1;
-    p.tile = la_tile(a->d_key, a->d_value, type_size(*a));
+    p.tile = la_tile(a->d_key, a->d_value, terms(*a));
     p.tiles = int(tile_count(a->d_value, p.tile));
     p.serial = serial(*a, p.tiles);
     LaJob& j = p.job[0];

@@ -56,20 +56,20 @@ struct LaParams {
 };
 
 // Most value columns a workgroup takes for q and k of up to k columns, in rows of
-// this element size: the state's share and the rows on their way stay within the
+// so many bf16 terms (bf16 1, fp16 2, fp32 3): the state's share and the rows on their way stay within the
 // 256 registers a lane that let two waves share a SIMD.
-constexpr int la_cols(int64_t k, int64_t size) { return k <= 64 ? (size == 2 ? 64 : 32) : k <= 128 ? 32 : 16; }
+constexpr int la_cols(int64_t k, int terms) { return k <= 64 ? (terms == 1 ? 64 : 32) : k <= 128 ? 32 : 16; }
 // ... and those it takes of v columns: a multiple of 16, the shares even.
-inline int la_tile(int64_t k, int64_t v, int64_t size) {
-    const int64_t most = la_cols(k, size) / 16, cols = (v + 15) / 16, n = (cols + most - 1) / most;
+inline int la_tile(int64_t k, int64_t v, int terms) {
+    const int64_t most = la_cols(k, terms) / 16, cols = (v + 15) / 16, n = (cols + most - 1) / most;
     return int((cols + n - 1) / n * 16);
 }
 
 // The segments' states from a zero start and their decays (job.ends,
-// job.decays); and the walk itself.  fine: 16-bit rows, too, with what is
-// computed in 3 terms.
+// job.decays); and the walk itself (a backward's: what is computed in 3 terms
+// for 16-bit rows too, and job.dot).
 template <typename T> hipError_t la_local_launch(const LaParams& p, hipStream_t stream);
-template <typename T> hipError_t la_walk_launch(const LaParams& p, bool fine, hipStream_t stream);
+template <typename T> hipError_t la_walk_launch(const LaParams& p, bool backward, hipStream_t stream);
 
 // dg of the tokens of one segment (see linear_attn.hip)
 struct LaDgParams {

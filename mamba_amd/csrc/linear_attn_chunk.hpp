@@ -301,14 +301,24 @@ template <typename T, int KP>
 struct Rows {
     using R = rowvec<T>;
     static constexpr int W = int(sizeof(T)) / 2, STRIDE = KP + 8, TERMS = kTerms<T>, TERM = C * STRIDE;
-    uint4 v[2][KP / 32][W];
+    // Rows too wide to wait in registers (KP fp32 256: 128 a lane) are read where they
+    // are used: only where they lie is kept.
+    static constexpr bool STREAM = KP * int(sizeof(T)) > 512;
+    uint4 v[2][STREAM ? 1 : KP / 32][W];
+    const T* from;
+    int64_t step;
+    int rows, dim, lane;
 
+    __device__ __forceinline__ void keep(const T* p, int64_t step_, int rows_, int dim_, int lane_) {
+        from = p; step = step_; rows = rows_; dim = dim_; lane = lane_;
+    }
     __device__ __forceinline__ void load_all(const T* p, int64_t step, int lane) {
+        if constexpr (STREAM) return keep(p, step, C, KP, lane);
         const uint32_t off = (uint32_t(lane & 15) * uint32_t(step) + uint32_t(8 * (lane >> 4))) * uint32_t(sizeof(T));
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int kk = 0; kk < KP / 32; ++kk)
+            for (int kk = 0; kk < (STREAM ? 0 : KP / 32); ++kk)
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     const typename R::words x = *reinterpret_cast<const typename R::words*>(
@@ -318,10 +328,11 @@ struct Rows {
     }
     template <bool WHOLE>
     __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int dim, int lane) {
+        if constexpr (STREAM) return keep(p, step, rows, dim, lane);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int kk = 0; kk < KP / 32; ++kk)
+            for (int kk = 0; kk < (STREAM ? 0 : KP / 32); ++kk)
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     const int row = 16 * i + (lane & 15), col = 32 * kk + 8 * (lane >> 4) + w * R::VE;
@@ -329,14 +340,24 @@ struct Rows {
                 }
     }
     __device__ __forceinline__ void terms(int i, int kk, u4 (&t)[TERMS]) const {
+        uint4 x4[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if constexpr (STREAM) {
+                const int row = 16 * i + (lane & 15), col = 32 * kk + 8 * (lane >> 4) + w * R::VE;
+                x4[w] = R::load(from + int64_t(row) * step + col, row < rows ? dim - col : 0);
+            } else {
+                x4[w] = v[i][kk][w];
+            }
+        }
         if constexpr (TERMS == 1) {
-            t[0] = u4{v[i][kk][0].x, v[i][kk][0].y, v[i][kk][0].z, v[i][kk][0].w};
+            t[0] = u4{x4[0].x, x4[0].y, x4[0].z, x4[0].w};
         } else {
             float x[8];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 float y[R::VE];
-                R::unpack(v[i][kk][w], y);
+                R::unpack(x4[w], y);
 #pragma unroll
                 for (int e = 0; e < R::VE; ++e) x[w * R::VE + e] = y[e];
             }
@@ -356,6 +377,7 @@ struct Rows {
             for (int kk = 0; kk < KP / 32; ++kk) {
                 u4 t[TERMS];
                 terms(i, kk, t);
+                if constexpr (STREAM) stage_end();
 #pragma unroll
                 for (int n = 0; n < TERMS; ++n)
                     *reinterpret_cast<u4*>(tile + n * TERM + (16 * i + (lane & 15)) * STRIDE + 32 * kk + 8 * (lane >> 4)) = t[n];
@@ -639,7 +661,8 @@ __global__ __launch_bounds__(64, 2) void la_local(const LaParams) {
 }
 
 // ----------------------------------------------------------------- the walk --
-template <typename T, int KP, int NT, int N, bool WHOLE>
+// DOT: a pass of the backward (J.dot may be asked for)
+template <typename T, int KP, int NT, int N, bool DOT, bool WHOLE>
 __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Tiles<T, KP, NT>& m, int* bad_col, bool rev) {
     constexpr int R = kTerms<T>, kMax = N == 2 ? 1 : 2;
     using SV = Stage<T, 16 * NT>;
@@ -647,7 +670,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
     const int64_t bh = at.bh, KV = int64_t(J.K) * J.V;
     Walk<T, KP, NT, true, WHOLE> w(p, J, at, p.serial ? p.L : p.seg_tokens, lane);
     const int vdim = w.vdim;
-    const T* xp = J.dot ? rows_of_head<T>(J.x, at) + n0 : nullptr;
+    const T* xp = DOT && J.dot ? rows_of_head<T>(J.x, at) + n0 : nullptr;
     const int64_t op = int64_t(at.b) * J.o.b + int64_t(at.h) * J.o.h + n0;
     const bool near_o = WHOLE || (vdim == 16 * NT && near(J.o.l) && near(J.x.l));
 
@@ -744,7 +767,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
         constexpr int WORDS = COLS * int(sizeof(T)) / 8;       // 8-byte words of a row a vector
         uint2 xv[2][VECS][WORDS];
         const bool whole_o = near_o && t0 + C <= w.end && !bad;
-        if (J.dot && whole_o) {
+        if (DOT && J.dot && whole_o) {
             const uint32_t off = (uint32_t(c) * uint32_t(J.x.l) + uint32_t(COLS * g)) * uint32_t(sizeof(T));
 #pragma unroll
             for (int it = 0; it < 2; ++it)
@@ -758,6 +781,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
 #pragma unroll
             for (int r = 0; r < R; ++r) vf[n][r] = load_tokens<SV::STRIDE>(m.v + r * SV::TERM, value_block<NT>(n, lane), lane);
 
+        if (!DOT) stage_end();
         // P's decays and split, and o^T <- 2^G o^T + V^T P^T
         typedef int i4 __attribute__((ext_vector_type(4)));
         i4 Ij[2];
@@ -814,9 +838,9 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
                     float v[COLS];
 #pragma unroll
                     for (int e = 0; e < COLS; ++e) v[e] = o[it][COLS / 4 * n + e / 4][e & 3];
-                    if (J.o_f32) store_cols<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
+                    if (DOT && J.o_f32) store_cols<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
                     else store_cols<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
-                    if (J.dot) {
+                    if (DOT && J.dot) {
 #pragma unroll
                         for (int e = 0; e < COLS; e += 4) {
                             float x[4];
@@ -845,9 +869,9 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
                     }
                     if (cnt > 0) {
                         const int64_t to = op + t * J.o.l + col;
-                        if (J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + to, v, cnt);
+                        if (DOT && J.o_f32) store4<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + to, v, cnt);
                         else store4<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + to, v, cnt);
-                        if (J.dot && live) {
+                        if (DOT && J.dot && live) {
                             float x[4];
                             load4<T>(xp + t * J.x.l + col, x, cnt);
 #pragma unroll
@@ -857,7 +881,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
                 }
             }
         }
-        if (J.dot) {
+        if (DOT && J.dot) {
 #pragma unroll
             for (int it = 0; it < 2; ++it) {
                 // over the lanes of the token's other columns: g = 0 .. 3
@@ -894,7 +918,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
     if (J.out_state) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.out_state + bh * KV);
 }
 
-template <typename T, int KP, int NT, int N, bool WHOLE>
+template <typename T, int KP, int NT, int N, bool DOT, bool WHOLE>
 __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams) {
     Params& p = params();
     __shared__ Tiles<T, KP, NT> m;
@@ -902,7 +926,7 @@ __global__ __launch_bounds__(64, KP <= 128 ? 2 : 1) void la_walk(const LaParams)
     const Place at = place(p, p.serial ? 1 : p.segs);
     Job& J = p.job[at.job];
     if (at.tile * p.tile >= J.V || at.bh >= uint32_t(p.B * p.H)) return;
-    walk_rows<T, KP, NT, N, WHOLE>(p, J, at, m, bad_col, J.rev);
+    walk_rows<T, KP, NT, N, DOT, WHOLE>(p, J, at, m, bad_col, J.rev);
 }
 
 }  // namespace la
@@ -913,7 +937,7 @@ hipError_t la_for_dims(const LaParams& p, F&& f) {
     int k = 0;
     for (int j = 0; j < p.njobs; ++j) k = p.job[j].K > k ? p.job[j].K : k;
     const auto with = [&](auto kp) {
-        return f(kp, std::integral_constant<int, la_cols(decltype(kp)::value, sizeof(T)) / 16>{});
+        return f(kp, std::integral_constant<int, la_cols(decltype(kp)::value, la::kTerms<T>) / 16>{});
     };
     if (k <= 32) return with(std::integral_constant<int, 32>{});
     if (k <= 64) return with(std::integral_constant<int, 64>{});
@@ -947,20 +971,19 @@ hipError_t la_local_launch(const LaParams& p, hipStream_t stream) {
     });
 }
 template <typename T>
-hipError_t la_walk_launch(const LaParams& p, bool fine, hipStream_t stream) {
+hipError_t la_walk_launch(const LaParams& p, bool backward, hipStream_t stream) {
     return la_for_dims<T>(p, [&](auto kp, auto nt) {
         constexpr int KP = decltype(kp)::value, NT = decltype(nt)::value;
         const dim3 grid = la_grid(p, p.serial ? 1 : p.segs);
-        const auto run = [&](auto n) {
+        const auto run = [&](auto n, auto dot) {
             constexpr int N = decltype(n)::value;
-            if (la_whole<KP, NT>(p)) hipLaunchKernelGGL((la::la_walk<T, KP, NT, N, true>), grid, dim3(64), 0, stream, p);
-            else hipLaunchKernelGGL((la::la_walk<T, KP, NT, N, false>), grid, dim3(64), 0, stream, p);
+            constexpr bool DOT = decltype(dot)::value;
+            if (la_whole<KP, NT>(p)) hipLaunchKernelGGL((la::la_walk<T, KP, NT, N, DOT, true>), grid, dim3(64), 0, stream, p);
+            else hipLaunchKernelGGL((la::la_walk<T, KP, NT, N, DOT, false>), grid, dim3(64), 0, stream, p);
             return hipGetLastError();
         };
-        if constexpr (sizeof(T) == 2) {
-            if (!fine) return run(std::integral_constant<int, 2>{});
-        }
-        return run(std::integral_constant<int, 3>{});
+        constexpr int kForward = sizeof(T) == 2 ? 2 : 3;
+        return backward ? run(std::integral_constant<int, 3>{}, std::true_type{}) : run(std::integral_constant<int, kForward>{}, std::false_type{});
     });
 }
 
