@@ -494,7 +494,7 @@ int ss_decode_linear(const ss_decode_linear_args* a, void* stream);
  * row b holds lengths[b] tokens (clamped to [0, seqlen]): tokens past them
  * are not read, their outputs are zero, and last_state is the state after
  * the row's own last token.  d_key and d_value: 1 to 256; batch * heads up
- * to 2^21; seqlen up to 2^24.
+ * to 2^20; seqlen up to 2^24.
  * ends: fp32 (batch, heads, segments, d_key, d_value), the state after each
  * segment of ss_linear_attn_segment() tokens, kept for the backward.
  * ------------------------------------------------------------------------ */

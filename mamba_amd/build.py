@@ -22,7 +22,7 @@ HOST_PATH = os.path.join(LIB_DIR, "mamba_host.so")
 ARCH = os.environ.get("MAMBA_AMD_ARCH", "gfx950")
 # the scan kernels are one unit per I/O type (the units without a suffix hold fp32's)
 SOURCES = ["ss_bwd.hip", "ss_bwd_bf16.hip", "ss_bwd_f16.hip", "ss_fwd.hip", "ss_fwd_bf16.hip", "ss_fwd_f16.hip",
-           "ss_api.hip", "conv1d.hip", "rms_norm.hip", "decode.hip", "decode_linear.hip", "linear_attn.hip",
+           "ops_api.hip", "conv1d.hip", "rms_norm.hip", "decode.hip", "decode_linear.hip", "linear_attn.hip",
            "linear_attn_f32.hip", "linear_attn_bf16.hip", "linear_attn_f16.hip", "block_norm.hip", "clip_grads.hip"]
 
 

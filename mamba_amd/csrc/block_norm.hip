@@ -40,8 +40,8 @@
 
 #include "../../include/mamba_ss.h"
 #include "norm_rows.hpp"
+#include "ops_kernels.hpp"
 #include "ss_device.hpp"
-#include "ss_kernels.hpp"
 
 namespace ss {
 
@@ -297,9 +297,9 @@ __global__ __launch_bounds__(kBlock<WPR>, kBlock<WPR> / 256 > 2 ? kBlock<WPR> / 
                 d[e] = dr;
                 x[e] = n1 * (dt * sil * w1) - x[e] * k1;
             }
-            R::store(static_cast<T*>(p.dx) + row * p.dim + col[k], x, cnt[k]);
-            if (p.dres) R::store(static_cast<T*>(p.dres) + row * p.dim + col[k], d, cnt[k]);
             if (p.gate) R::store(static_cast<T*>(p.dgate) + row * p.dim + col[k], gz, cnt[k]);
+            if (p.dres) R::store(static_cast<T*>(p.dres) + row * p.dim + col[k], d, cnt[k]);
+            R::store(static_cast<T*>(p.dx) + row * p.dim + col[k], x, cnt[k]);
         }
     }
     // the workgroup's column sums, its rows' teams in order

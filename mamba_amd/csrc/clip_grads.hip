@@ -17,8 +17,8 @@
 
 #include "../../include/mamba_ss.h"
 #include "norm_rows.hpp"
+#include "ops_kernels.hpp"
 #include "ss_device.hpp"
-#include "ss_kernels.hpp"
 
 namespace ss {
 

@@ -20,8 +20,8 @@
 
 #include "linear_attn.hpp"
 #include "norm_rows.hpp"
+#include "ops_kernels.hpp"
 #include "ss_device.hpp"
-#include "ss_kernels.hpp"
 
 namespace ss {
 
