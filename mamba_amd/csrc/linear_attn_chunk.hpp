@@ -4,8 +4,9 @@
 // A wave walks the chunks (32 tokens) of one segment, or of a whole row, for
 // one (batch, head) and up to 16 NT value columns, and holds the state of its
 // columns in registers.  Waves do not meet: a workgroup is one wave, and the 6 to
-// 12 of a CU hide each other's loads.  (Four waves that shared a 64-token chunk
-// and met at three barriers in it spent half their time waiting.)
+// 8 of a CU hide each other's loads.  (Four waves that shared a 64-token chunk and
+// met at three barriers in it spent half their time waiting: 429 us for the
+// training step below, 303 now.)
 // With G the sum of the log2 decays from the chunk's start up to a token
 // (itself included), the forward chunk is
 //
@@ -37,6 +38,15 @@
 //  - P's registers are an operand as they are, in the token order of tok();
 //  - sums over tokens read k and v in that order through the transposing LDS
 //    load, where 16 lanes read 4 rows of 16 elements and get a column of 4 each.
+//
+// Measured, 8 x 2048 tokens x 24 heads of 64 x 64, bf16: the forward's walk 56 us
+// (225 MB: 4.0 TB/s, where plain reads of the same rows reach 6.5), the three
+// passes of the backward together 158 us (about 1180 vector and 120 matrix
+// instructions a chunk: a lane's vector instructions alone are 74 us; two waves a
+// SIMD, which wait for memory 38 % of the time), a segment's states 28 us.  What
+// bounds it is issue: splitting P, S and the weighted rows, and the decays.  With
+// 2 terms in the backward as well it runs 5 % faster, and the decay's gradient is
+// off by 7e-6 instead of 6e-7.
 #pragma once
 
 #include <hip/hip_runtime.h>
