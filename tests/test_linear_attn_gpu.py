@@ -66,6 +66,15 @@ def test_one_decay_per_head(shape, dtype):
     compare(x, run(x))
 
 
+@pytest.mark.parametrize("shape", [(600, 1100, 2, 1, 8, 8), (1100, 70, 1, 1, 16, 16)], ids=lambda s: "x".join(map(str, s)))
+def test_many_rows(shape):
+    """Enough rows to fill the GPU: each is walked whole, through one segment or several."""
+    lengths = [(7 * i) % (shape[1] + 1) for i in range(shape[0])]
+    x = make(*shape, BF16, seed=30, initial=True, lengths=lengths)
+    x["g"] = x["g"] * 0.1
+    compare(x, run(x))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
 def test_lengths(dtype):
     x = make(6, 150, 4, 2, 64, 64, dtype, seed=4, initial=True, lengths=[0, 1, 64, 65, 150, 149])
