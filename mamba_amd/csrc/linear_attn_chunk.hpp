@@ -200,8 +200,22 @@ __device__ __forceinline__ void load4(const T* p, float (&v)[4], int cnt) {
 
 // 8-byte words at any element alignment; a lane's 4 or 8 columns of a result
 typedef uint32_t words4_at2 __attribute__((ext_vector_type(4), aligned(2)));
-template <int W>
-__device__ __forceinline__ void load_words(const char* p, uint2 (&w)[W]) {
+template <typename T, int W, bool WHOLE>
+__device__ __forceinline__ void load_words(const char* p, uint2 (&w)[W], int cnt) {
+    constexpr int COLS = 8 * W / int(sizeof(T));
+    if (!WHOLE && cnt < COLS) {                             // (the first cnt elements, zero past them)
+        uint32_t x[2 * W] = {};
+#pragma unroll
+        for (int e = 0; e < COLS - 1; ++e) {
+            if (e < cnt) {
+                if constexpr (sizeof(T) == 4) x[e] = *reinterpret_cast<const uint32_t*>(p + 4 * e);
+                else x[e >> 1] |= uint32_t(*reinterpret_cast<const uint16_t*>(p + 2 * e)) << (16 * (e & 1));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = make_uint2(x[2 * i], x[2 * i + 1]);
+        return;
+    }
     if constexpr (W == 1) {
         const half4_at2 x = *reinterpret_cast<const half4_at2*>(p);
         w[0] = make_uint2(x.x, x.y);
@@ -214,18 +228,18 @@ __device__ __forceinline__ void load_words(const char* p, uint2 (&w)[W]) {
         }
     }
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_cols(T* p, const float (&v)[N]) {
+template <typename T, int N, bool WHOLE>
+__device__ __forceinline__ void store_cols(T* p, const float (&v)[N], int cnt) {
     using R = rowvec<T>;
     if constexpr (N < R::VE) {
-        store4<T>(p, v, 4);
+        store4<T>(p, v, WHOLE ? 4 : cnt);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += R::VE) {
             float x[R::VE];
 #pragma unroll
             for (int e = 0; e < R::VE; ++e) x[e] = v[i + e];
-            R::store(p + i, x, R::VE);
+            R::store(p + i, x, WHOLE ? int(R::VE) : cnt - i);
         }
     }
 }
@@ -240,6 +254,32 @@ __device__ __forceinline__ uint4 load_part(const T* p, bool in, int n) {
     } else {
         return rowvec<T>::load(p, in ? n : 0);
     }
+}
+
+// Whether kernels for other than whole tiles read and write rows of any width by
+// vectors (load_any).  4 x 2048 tokens, 16 heads of 61 x 61, forward + backward: bf16 227 us
+// with it and 284 without, fp16 257 and 306; but fp32 347 and 341, bf16 97 x 97 528 and 496.
+template <typename T, int KP> constexpr bool kAny = sizeof(T) == 2 && KP <= 64;
+
+// Elements col .. of a row of dim (at least a vector's) elements, zero past its end:
+// the vector that ends with the row, shifted, where the one at col would cross it.
+template <typename T>
+__device__ __forceinline__ uint4 load_any(const char* row, int col, int dim) {
+    using R = rowvec<T>;
+    const int start = col < dim - R::VE ? col : dim - R::VE, cut = col - start;
+    const typename R::words w = *reinterpret_cast<const typename R::words*>(row + start * int(sizeof(T)));
+    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    if (cut > 0) {
+        const int half = int(sizeof(T)) == 2 ? 1 : 0, words = cut >> half;
+        if (words & 2) { x[0] = x[2]; x[1] = x[3]; x[2] = x[3] = 0u; }
+        if (words & 1) { x[0] = x[1]; x[1] = x[2]; x[2] = x[3]; x[3] = 0u; }
+        if (half && (cut & 1)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (x[i] >> 16) | (i < 3 ? x[i < 3 ? i + 1 : 3] << 16 : 0u);
+        }
+        if (cut >= R::VE) x[0] = x[1] = x[2] = x[3] = 0u;
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // A chunk's rows of v on their way from global memory to LDS.
@@ -260,6 +300,13 @@ struct Stage {
                 reinterpret_cast<const char*>(p + int64_t(i * STEP) * step) + off);
             v[i] = make_uint4(w.x, w.y, w.z, w.w);
         }
+    }
+    // all rows, of dim elements (at least a vector's)
+    __device__ __forceinline__ void load_dim(const T* p, int64_t step, int dim, int lane) {
+        const uint32_t off = uint32_t(lane / PER_ROW) * uint32_t(step) * uint32_t(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = load_any<T>(reinterpret_cast<const char*>(p + int64_t(i * STEP) * step) + off, lane % PER_ROW * R::VE, dim);
     }
     // the first `rows` rows of p, dim elements each; the others are zero
     template <bool WHOLE>
@@ -335,6 +382,18 @@ struct Rows {
                         reinterpret_cast<const char*>(p + int64_t(16 * i) * step) + off + (32 * kk * int(sizeof(T)) + 16 * w));
                     v[i][kk][w] = make_uint4(x.x, x.y, x.z, x.w);
                 }
+    }
+    __device__ __forceinline__ void load_dim(const T* p, int64_t step, int dim, int lane) {
+        if constexpr (STREAM) return keep(p, step, C, dim, lane);
+        const uint32_t off = uint32_t(lane & 15) * uint32_t(step) * uint32_t(sizeof(T));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int kk = 0; kk < (STREAM ? 0 : KP / 32); ++kk)
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+                    v[i][kk][w] = load_any<T>(reinterpret_cast<const char*>(p + int64_t(16 * i) * step) + off,
+                                              32 * kk + 8 * (lane >> 4) + w * R::VE, dim);
     }
     template <bool WHOLE>
     __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int dim, int lane) {
@@ -563,15 +622,19 @@ struct Walk {
         kp = rows_of_head<T>(J.k, at);
         vp = rows_of_head<T>(J.v, at) + n0;
         gp = p.g + int64_t(at.b) * p.g_b + int64_t(at.h) * p.g_h;
-        whole = WHOLE || (J.K == KP && vdim == 16 * NT && (!Q || near(J.q.l)) && near(J.k.l) && near(J.v.l));
+        whole = WHOLE || ((kAny<T, KP> ? J.K >= rowvec<T>::VE && vdim >= rowvec<T>::VE : J.K == KP && vdim == 16 * NT) && (!Q || near(J.q.l)) && near(J.k.l) && near(J.v.l));
     }
     __device__ __forceinline__ int chunk(int i) const { return rev ? chunks - 1 - i : i; }
     __device__ __forceinline__ void fetch(int i) {
         const int64_t t0 = s0 + int64_t(chunk(i)) * C;
-        if (whole && t0 + C <= end) {
+        if ((WHOLE || (!kAny<T, KP> && whole)) && t0 + C <= end) {
             if (Q) q.load_all(qp + t0 * J.q.l, J.q.l, lane);
             k.load_all(kp + t0 * J.k.l, J.k.l, lane);
             v.load_all(vp + t0 * J.v.l, J.v.l, lane);
+        } else if (!WHOLE && kAny<T, KP> && whole && t0 + C <= end) {
+            if (Q) q.load_dim(qp + t0 * J.q.l, J.q.l, J.K, lane);
+            k.load_dim(kp + t0 * J.k.l, J.k.l, J.K, lane);
+            v.load_dim(vp + t0 * J.v.l, J.v.l, vdim, lane);
         } else {
             const int rows = t0 + C <= end ? C : t0 < end ? int(end - t0) : 0;
             const int l = late(lane);
@@ -682,7 +745,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
     const int vdim = w.vdim;
     const T* xp = DOT && J.dot ? rows_of_head<T>(J.x, at) + n0 : nullptr;
     const int64_t op = int64_t(at.b) * J.o.b + int64_t(at.h) * J.o.h + n0;
-    const bool near_o = WHOLE || (vdim == 16 * NT && near(J.o.l) && near(J.x.l));
+    const bool near_o = WHOLE || ((kAny<T, KP> || vdim == 16 * NT) && near(J.o.l) && near(J.x.l));
 
     // the state before the walk's first token
     const float* from = J.in ? J.in + bh * KV : nullptr;
@@ -783,7 +846,8 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
             for (int it = 0; it < 2; ++it)
 #pragma unroll
                 for (int n = 0; n < VECS; ++n)
-                    load_words<WORDS>(reinterpret_cast<const char*>(xp + (t0 + 16 * it) * J.x.l) + off + 4 * COLS * n * int(sizeof(T)), xv[it][n]);
+                    load_words<T, WORDS, WHOLE || !kAny<T, KP>>(reinterpret_cast<const char*>(xp + (t0 + 16 * it) * J.x.l) + off + 4 * COLS * n * int(sizeof(T)), xv[it][n],
+                                                vdim - COLS * (4 * n + g));
         }
         u4 vf[NT][R];
 #pragma unroll
@@ -848,8 +912,9 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
                     float v[COLS];
 #pragma unroll
                     for (int e = 0; e < COLS; ++e) v[e] = o[it][COLS / 4 * n + e / 4][e & 3];
-                    if (DOT && J.o_f32) store_cols<float>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
-                    else store_cols<T>(static_cast<T*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v);
+                    const int cnt = vdim - COLS * (4 * n + g);
+                    if (DOT && J.o_f32) store_cols<float, COLS, WHOLE || !kAny<T, KP>>(static_cast<float*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v, cnt);
+                    else store_cols<T, COLS, WHOLE || !kAny<T, KP>>(static_cast<T*>(const_cast<void*>(J.o.p)) + first + (row + 4 * COLS * n), v, cnt);
                     if (DOT && J.dot) {
 #pragma unroll
                         for (int e = 0; e < COLS; e += 4) {
