@@ -61,8 +61,9 @@ void launch(const at::Device& dev, const char* what, F&& f) {
     check(rc, what);                 // (the message is this thread's)
 }
 
-// The stream that is current for the device, for nodes of the autograd graph:
-// autograd runs a node's backward on the stream of its forward.
+// The stream that is current for the device.  A node's backward takes its
+// forward's (kept in the node): autograd makes that one current for it, and its
+// thread need not take the GIL to ask.
 void* current_stream(const at::Device& dev) {
     if (!dev.is_cuda()) return nullptr;                // (refused by the call)
     const py::gil_scoped_acquire gil;
@@ -80,6 +81,7 @@ Tensor given(const OptT& t) { return t ? *t : Tensor(); }
 OptT maybe(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+void* node_stream(AutogradContext* ctx) { return reinterpret_cast<void*>(ctx->saved_data["stream"].toInt()); }
 
 bool itype_of(at::ScalarType t, int32_t* out) {
     switch (t) {
@@ -791,8 +793,10 @@ LinGrads lin_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
 struct LinAttn : torch::autograd::Function<LinAttn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
                                  const OptT& initial, const OptT& lengths, double scale, bool want_last, bool need) {
-        const LinOut r = lin_fwd(q, k, v, g, initial, lengths, scale, want_last, need, current_stream(v.device()));
+        void* const stream = current_stream(v.device());
+        const LinOut r = lin_fwd(q, k, v, g, initial, lengths, scale, want_last, need, stream);
         if (need) {
+            ctx->saved_data["stream"] = reinterpret_cast<int64_t>(stream);
             ctx->save_for_backward({r.in.q, r.in.k, r.in.v, r.in.g, given(r.in.initial), given(r.in.lengths), given(r.ends)});
             ctx->saved_data["scale"] = scale;
             ctx->saved_data["g_type"] = int64_t(g.scalar_type());
@@ -812,7 +816,7 @@ struct LinAttn : torch::autograd::Function<LinAttn> {
         const bool has_initial = t[4].defined();
         const LinGrads d = lin_bwd(t[0], t[1], t[2], t[3], maybe(t[4]), maybe(t[5]), t[6], ctx->saved_data["scale"].toDouble(),
                                    ctx->saved_data["per_head"].toBool(), dout, maybe(dlast),
-                                   has_initial && ctx->needs_input_grad(4), current_stream(t[2].device()));
+                                   has_initial && ctx->needs_input_grad(4), node_stream(ctx));
         if (ctx->needs_input_grad(0)) r[0] = d.dq;
         if (ctx->needs_input_grad(1)) r[1] = d.dk;
         if (ctx->needs_input_grad(2)) r[2] = d.dv;
@@ -981,7 +985,9 @@ BorderGrads block_norm_bwd(const Tensor& x, const Tensor& residual, const OptT& 
 struct BlockNorm : torch::autograd::Function<BlockNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const Tensor& post, const Tensor& pre,
                                  const OptT& gate, const OptT& scale_vec, double scale, double eps) {
-        const BorderOut r = block_norm_fwd(x, residual, gate, post, pre, scale_vec, scale, eps, true, current_stream(x.device()));
+        void* const stream = current_stream(x.device());
+        const BorderOut r = block_norm_fwd(x, residual, gate, post, pre, scale_vec, scale, eps, true, stream);
+        ctx->saved_data["stream"] = reinterpret_cast<int64_t>(stream);
         variable_list saved = r.read;
         saved.push_back(*r.rstd);
         ctx->save_for_backward(saved);
@@ -998,7 +1004,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         const auto t = ctx->get_saved_variables();
         const auto rows = [&](const Tensor& g) { return g.defined() ? OptT(g.reshape(t[0].sizes())) : OptT(); };
         const BorderGrads d = block_norm_bwd(t[0], t[1], maybe(t[2]), t[3], t[4], maybe(t[5]), t[6], ctx->saved_data["scale"].toDouble(),
-                                             rows(grads[0]), rows(grads[1]), ctx->needs_input_grad(1), current_stream(t[0].device()));
+                                             rows(grads[0]), rows(grads[1]), ctx->needs_input_grad(1), node_stream(ctx));
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const auto types = ctx->saved_data["types"].toIntVector();
         const auto typed = [&](const Tensor& w, int i) { return w.to(at::ScalarType(types[i])); };
@@ -1064,7 +1070,9 @@ variable_list gated_norm_bwd(const Tensor& x, const Tensor& gate, const Tensor& 
 
 struct GatedNorm : torch::autograd::Function<GatedNorm> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
-        const variable_list r = gated_norm_fwd(x, gate, weight, groups, eps, current_stream(x.device()));
+        void* const stream = current_stream(x.device());
+        const variable_list r = gated_norm_fwd(x, gate, weight, groups, eps, stream);
+        ctx->saved_data["stream"] = reinterpret_cast<int64_t>(stream);
         ctx->save_for_backward({r[1], r[2], r[3]});
         ctx->saved_data["groups"] = groups;
         ctx->saved_data["eps"] = eps;
@@ -1076,7 +1084,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
         const auto t = ctx->get_saved_variables();
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const variable_list d = gated_norm_bwd(t[0], t[1], t[2], grads[0].reshape(t[0].sizes()), ctx->saved_data["groups"].toInt(),
-                                               ctx->saved_data["eps"].toDouble(), current_stream(t[0].device()));
+                                               ctx->saved_data["eps"].toDouble(), node_stream(ctx));
         variable_list r(5);
         if (ctx->needs_input_grad(0)) r[0] = d[0].view(shape);
         if (ctx->needs_input_grad(1)) r[1] = d[1].view(shape);
