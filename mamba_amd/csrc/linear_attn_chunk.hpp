@@ -15,16 +15,15 @@
 //
 // and the reverse walk the same with G negated, j >= i, the factors
 // 2^(G_C - G_i) at o and 2^G_j at k_j.  G is summed in 64 bits and kept as an
-// integer I and a fraction F, so P's factor is 2^-F_j (a column), 2^F_i (a row,
-// applied to o at the end) and an exact shift by I_i - I_j: however far the sums
-// run, no factor loses bits, overflows by itself or needs an exponential for
-// each pair.
+// integer I and a fraction F, so P's factor is 2^-F_j (a column), 2^F_i (a row)
+// and an exact shift by I_i - I_j: however far the sums run, no factor loses
+// bits, overflows by itself or needs an exponential for each pair.
 //
 // Products run on bf16 matrix instructions with 32-bit sums.  A row of type
 // T is a sum of R bf16 terms, exactly: 1 (bf16), 2 (fp16, 11 bits) or 3
 // (fp32); what is computed (P, S, the weighted rows of the state's update) is
-// split into 2 or 3 terms, and of the products of terms those below 2^-24
-// (2 terms: 2^-16) are left out.  2 terms are enough where the result is rounded
+// split into 2 or 3 terms (2^-18 off at most, or exact), and of the products of
+// terms those below 2^-24 (2 terms: 2^-16) are left out.  2 terms are enough where the result is rounded
 // to 16 bits; states, and gradients that the decay's gradient is summed from,
 // take 3.
 //
@@ -35,7 +34,7 @@
 //  - q and k come from global memory as operands, 8 elements of a row a lane;
 //  - the state's rows are numbered so that the registers a lane holds are the 8
 //    elements of q that it multiplies (state_row);
-//  - P's registers are an operand as they are, in the token order of tok();
+//  - P's registers are an operand as they are, in the token order of load_tokens;
 //  - sums over tokens read k and v in that order through the transposing LDS
 //    load, where 16 lanes read 4 rows of 16 elements and get a column of 4 each.
 //
