@@ -77,6 +77,11 @@ bool wants_grad(std::initializer_list<const Tensor*> inputs) {
         if (t && t->defined() && t->requires_grad()) return true;
     return false;
 }
+// A tensor that the library wrote in place: autograd then refuses a backward that
+// saved what it held (tensors made in inference mode are never saved).
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Tensor given(const OptT& t) { return t ? *t : Tensor(); }
 OptT maybe(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 using torch::autograd::AutogradContext;
@@ -859,7 +864,8 @@ Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const
     REQUIRE(kLinUp, state.numel() == 0 || ((V <= 1 || state.stride(3) == 1) && (K <= 1 || state.stride(2) == V)),
             "state must be contiguous along its last two dims (it is updated in place)");
     const Tensor q = seq_unit(q_), k = seq_unit(k_), v = seq_unit(v_), g = decays(kLinUp, g_, B, -1, H, v_);
-    if (out)
+    const bool own_out = out.has_value();
+    if (own_out)
         REQUIRE(kLinUp, out->sizes() == v.sizes() && out->scalar_type() == v.scalar_type() && out->device() == dev && unit(*out),
                 "out must match v, with unit stride along the last dim");
     else out = at::empty({B, H, V}, v.options());
@@ -874,6 +880,8 @@ Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const
     a.state = static_cast<float*>(ptr(state)); a.q = ptr(q); a.k = ptr(k); a.v = ptr(v);
     a.g = static_cast<float*>(ptr(g)); a.out = ptr(*out);
     launch(dev, kLinUp, [&] { return ss_linear_attn_update(&a, reinterpret_cast<void*>(stream)); });
+    written(state);
+    if (own_out) written(*out);
     return *out;
 }
 
@@ -1135,7 +1143,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& o
     const Tensor ws = at::empty({bytes}, options.dtype(at::kByte));
     a.norm = static_cast<float*>(ptr(norm)); a.workspace = ptr(ws); a.workspace_bytes = bytes;
     launch(dev, kClip, [&] { return ss_clip_grads(&a, reinterpret_cast<void*>(stream)); });
-    for (const Tensor& o : outs) o.unsafeGetTensorImpl()->bump_version();
+    for (const Tensor& o : outs) written(o);
     return norm;
 }
 
