@@ -856,6 +856,8 @@ Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const
     const int64_t G = q_.size(1), K = q_.size(2);
     REQUIRE(kLinUp, H == 0 || (G > 0 && H % G == 0),
             "heads " + std::to_string(H) + " is not a multiple of groups " + std::to_string(G));
+    REQUIRE(kLinUp, !wants_grad({&state, &q_, &k_, &v_, &g_}),
+            "a token's update has no backward; call it under torch.no_grad(), or linear_attn_fn for gradients");
     on_device(kLinUp, "q", q_, dev); on_device(kLinUp, "k", k_, dev); on_device(kLinUp, "state", state, dev);
     of_type(kLinUp, "q", q_, v_.scalar_type()); of_type(kLinUp, "k", k_, v_.scalar_type());
     of_type(kLinUp, "state", state, at::kFloat);

@@ -65,8 +65,9 @@ class LinearAttnLM(nn.Module):
     def allocate_states(self, batch_size, device=None):
         return [m.allocate_state(batch_size, device) for m in self.mixers]
 
+    @torch.no_grad()
     def step(self, input_ids, states):
-        """One token per sequence: input_ids (batch,) -> logits (batch, vocab); the states advance in place."""
+        """One token per sequence: input_ids (batch,) -> logits (batch, vocab); the states advance in place.  No gradients flow."""
         return self.lm_head(self._blocks(self.embedding(input_ids), lambda i, normed: self.mixers[i].step(normed, states[i])))
 
     @torch.no_grad()

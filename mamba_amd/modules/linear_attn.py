@@ -6,7 +6,8 @@
     out = output_proj(gated_rms_norm_fn(o, z, norm))    each head's norm and gate (ops/block_norm.py)
 
 ``forward`` runs prompts and training, over rows of different ``lengths`` and
-from a ``state`` of earlier tokens; ``step`` advances the state by one token.
+from a ``state`` of earlier tokens; ``step`` advances the state by one token,
+without gradients.
 All on the HIP library: tensors on a ROCm device.
 """
 import math
@@ -58,8 +59,9 @@ class LinearAttn(nn.Module):
         device = self.input_proj.weight.device if device is None else device
         return torch.zeros(batch_size, self.n_heads, self.key_dim, self.head_dim, device=device)
 
+    @torch.no_grad()
     def step(self, hidden_states, state):
-        """One token: (batch, model_dim) -> the same shape; the state advances in place."""
+        """One token: (batch, model_dim) -> the same shape; the state advances in place.  No gradients flow."""
         q, k, v, z, g = self._split(hidden_states)
         o = linear_attn_update(state, q, k, v, g)
         return self.output_proj(gated_rms_norm_fn(o.flatten(1), z, self.norm, n_groups=self.n_heads, eps=self.eps))
