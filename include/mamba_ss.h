@@ -554,7 +554,9 @@ int ss_linear_attn_bwd(const ss_linear_attn_bwd_args* a, void* stream);
 /* One token: state <- exp(g) state + k v^T in place, out = scale q^T state.
  * q, k: (batch, groups, d_key); v, out: (batch, heads, d_value), unit stride
  * along the last dim; g: fp32 (batch, heads); state: fp32 (batch, heads,
- * d_key, d_value), the last two dims contiguous. */
+ * d_key, d_value), the last two dims contiguous.  No two elements of state or
+ * of out may share memory (refused), and neither may lie over another tensor
+ * of the call. */
 typedef struct ss_linear_attn_update_args {
     int64_t batch, heads, groups, d_key, d_value;
     int32_t dtype;                       /* enum ss_dtype */

@@ -4,6 +4,7 @@
 #include "ss_api.hip"
 
 #include "ops_kernels.hpp"
+#include "overlap.hpp"
 
 extern "C" {
 
@@ -129,6 +130,12 @@ int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream) {
     if (!aligned(a->state, 4) || !aligned(a->g, 4) || !aligned(a->q, es) || !aligned(a->k, es) || !aligned(a->v, es) ||
         !aligned(a->out, es))
         return fail(SS_ERR_INVALID, "state / q / k / v / g / out is misaligned");
+    if (ss::blocks_overlap(a->batch, a->state_batch_stride, a->heads, a->state_head_stride, a->d_key * a->d_value))
+        return fail(SS_ERR_INVALID, "state's elements overlap (strides %lld, %lld): it is updated in place",
+                    (long long)a->state_batch_stride, (long long)a->state_head_stride);
+    if (ss::blocks_overlap(a->batch, a->out_batch_stride, a->heads, a->out_head_stride, a->d_value))
+        return fail(SS_ERR_INVALID, "out's elements overlap (strides %lld, %lld)", (long long)a->out_batch_stride,
+                    (long long)a->out_head_stride);
     const hipError_t e = ss::linear_attn_update_launch(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(SS_ERR_HIP, "linear attention update launch failed: %s", hipGetErrorString(e));
     return ok();

@@ -26,8 +26,9 @@ A token's infinities or NaN reach the outputs of its own and later tokens.
 (batch, heads, d_key, d_value) by one token in place: q, k (batch, groups,
 d_key), v (batch, heads, d_value), g (batch, heads) or (heads,); returns out
 (batch, heads, d_value).  The state after a prompt is linear_attn_fn's
-last_state.  It has no backward: with grad mode on, inputs that require a
-gradient are refused.
+last_state.  Elements of state or of out that share memory (an expanded state)
+are refused; neither may lie over another tensor of the call.  It has no
+backward: with grad mode on, inputs that require a gradient are refused.
 """
 from .. import _native as nat
 from ..selective_scan import _raw_stream

@@ -43,3 +43,25 @@ def test_inference_mode():
         assert torch.equal(linear_attn_update(held, q[:, 0], k[:, 0], v[:, 0], g[:, 0]), want)
         held.copy_(state)
     assert torch.equal(linear_attn_update(held, q[:, 0], k[:, 0], v[:, 0], g[:, 0]), want)
+
+
+def test_overlapping_states_are_refused():
+    q, k, v, g, state = inputs(3)
+    t = q[:, 0], k[:, 0], v[:, 0], g[:, 0]
+    for bad in (state[:1].expand_as(state), state[:, :1].expand_as(state)):
+        before = bad.clone()
+        with pytest.raises(ValueError, match="state's elements overlap"):
+            linear_attn_update(bad, *t)
+        assert torch.equal(bad, before)
+    with pytest.raises(ValueError, match="out's elements overlap"):
+        linear_attn_update(state, *t, out=torch.empty_like(v[:1, 0]).expand(2, 4, 24))
+    # rows apart, heads in the other order of memory, and one row whose stride is anything
+    want = state.clone()
+    linear_attn_update(want, *t)
+    for held in (torch.zeros(4, 2, 32, 24, device=DEV).transpose(0, 1), torch.zeros(2, 9, 32, 24, device=DEV)[:, 1::2]):
+        held.copy_(state)
+        linear_attn_update(held, *t)
+        assert torch.equal(held, want)
+    one = state[:1].clone()
+    linear_attn_update(one.as_strided(one.shape, (0, *one.stride()[1:])), *(x[:1] for x in t))
+    assert torch.equal(one, want[:1])
