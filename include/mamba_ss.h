@@ -523,8 +523,9 @@ typedef struct ss_linear_attn_args {
 /* dq, dk: (batch, seqlen, groups, d_key), dv: (batch, seqlen, heads,
  * d_value), contiguous, dtype (the sums over the heads of a group in fp32,
  * rounded once).  dg: fp32 (batch, seqlen, heads) contiguous, or (heads)
- * when g_per_head (the sum over batch and tokens).  Every sum has a fixed
- * order: the same bits on every run. */
+ * when g_per_head (the sum over batch and tokens); zero where exp(g) is, and
+ * with an error that has the factor exp(g) where g is below -8.3.  Every sum has a
+ * fixed order: the same bits on every run. */
 typedef struct ss_linear_attn_bwd_args {
     ss_linear_attn_args f;               /* as for the forward; f.ends from it */
     int64_t dout_batch_stride, dout_len_stride, dout_head_stride;

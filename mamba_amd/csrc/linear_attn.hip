@@ -13,7 +13,9 @@
 //        = <S_e, dS_e> + sum of D_s over t <= s < e
 // for any e >= t: S_e the state before token e, dS_e the gradient arriving at
 // it from token e on.  e is the end of t's segment, so the sum, which cancels,
-// runs over one segment and not the whole row.
+// runs over one segment and not the whole row.  Its terms lack the factor exp(g_t)
+// that dg_t has, so where that is small dg_t is formed without it
+// (la_decay_grad_strong), and e of the tokens before is that token.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -74,73 +76,386 @@ __device__ __forceinline__ double sum_all(double v, double (&red)[4]) {
 }
 
 // dg of one segment: the inner product of the two states at its end, and the
-// sums of D from its last token down.  256 threads, up to 4 tokens each.  16 us for
+// sums of D from its last token down.  256 threads, up to 4 tokens each.  15 us for
 // 1536 segments of 256 tokens: the states' 50 MB, and dg's stores of 4 bytes a row.
-constexpr int kDgTok = 4;
+constexpr int kDgTok = 4, kDgSegMax = 256 * kDgTok;
+
+// A segment's tokens and, token top - i a thread's i-th, dg by the sums of D
+struct DgSeg {
+    int64_t bh, b, h, s0, s1;
+    int seg, n, top;                                    // n: the row's own tokens in it
+    const float* dS;                                    // what arrives at its end, or null
+    double d[kDgTok];                                   // dg
+    __device__ __forceinline__ DgSeg(const LaDgParams& p, int64_t bh_, int seg_, double (&red)[4]) : bh(bh_), seg(seg_) {
+        const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+        const int64_t KV = int64_t(p.K) * p.V;
+        b = bh / p.H;
+        h = bh % p.H;
+        s0 = seg * p.seg_tokens;
+        s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
+        const int64_t len = row_len(p.lens, b, p.L);
+        n = int((len < s1 ? len : s1) - s0);
+        top = int(s1 - s0) - 1 - tid * kDgTok;
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kDgTok; ++i) {
+            const int64_t t = s0 + (top - i);
+            double v = 0.0;
+            if (t >= s0 && t < len) {
+                for (int q = 0; q < p.qtiles; ++q) v += p.dotq[(int64_t(q) * p.B * p.H + bh) * p.L + t];
+                for (int k = 0; k < p.ktiles; ++k) v -= p.dotk[(int64_t(k) * p.B * p.H + bh) * p.L + t];
+            }
+            d[i] = v;
+        }
+        double f = 0.0;
+        dS = seg + 1 < p.segs ? p.rends + (bh * p.segs + seg + 1) * KV : p.dlast ? p.dlast + bh * KV : nullptr;
+        if (dS) {
+            const float* S = p.ends + (bh * p.segs + seg) * KV;
+#pragma unroll 4
+            for (int i = 4 * tid; i < KV; i += 1024) {
+                float x[4], y[4];
+                rowvec<float>::unpack(rowvec<float>::load(S + i, int(KV) - i), x);
+                rowvec<float>::unpack(rowvec<float>::load(dS + i, int(KV) - i), y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f += double(x[e]) * double(y[e]);
+            }
+        }
+        const double F = sum_all(f, red);
+#pragma unroll
+        for (int i = 0; i < kDgTok; ++i) {
+            sum += d[i];
+            d[i] = sum;
+        }
+        double upto = sum;                              // sums over the threads up to this one
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const double o = __shfl_up(upto, m, 64);
+            if (lane >= m) upto += o;
+        }
+        __syncthreads();
+        if (lane == 63) red[wave] = upto;
+        __syncthreads();
+        double base = F + (upto - sum);
+        for (int w = 0; w < wave; ++w) base += red[w];
+#pragma unroll
+        for (int i = 0; i < kDgTok; ++i) d[i] += base;
+    }
+    __device__ __forceinline__ void store(const LaDgParams& p, double (&red)[4]) const {
+        double mine = 0.0;
+#pragma unroll
+        for (int i = 0; i < kDgTok; ++i) {
+            const int t = top - i;
+            if (t >= 0) {
+                const double v = t < n ? d[i] : 0.0;
+                if (p.dg) p.dg[(b * p.L + s0 + t) * p.H + h] = float(v);
+                mine += v;
+            }
+        }
+        if (!p.part) return;
+        mine = sum_all(mine, red);
+        if (threadIdx.x == 0) p.part[bh * p.segs + seg] = mine;
+    }
+};
 
 __global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
-    const int64_t bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-    const int seg = int(blockIdx.y), tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    const int64_t s0 = seg * p.seg_tokens, s1 = s0 + p.seg_tokens < p.L ? s0 + p.seg_tokens : p.L;
-    const int64_t len = row_len(p.lens, b, p.L);
     __shared__ double red[4];
+    const DgSeg s(p, blockIdx.x, int(blockIdx.y), red);
+    s.store(p, red);
+}
 
-    // this thread's tokens, from the segment's end down
-    double d[kDgTok], sum = 0.0;
+// The segments with strong decays once more: dg of those is formed by itself, and the
+// sums of D start at the next one.  With a chunk of 32 tokens c0 .. c1-1 around token t, S the
+// state before c0, R the gradient arriving at c1 and M_ij = scale (q_i . k_j) (dout_i . v_j),
+// each times the decays on its way,
+//   dg_t = R . S + sum over i >= t of scale q_i^T S dout_i + sum over j < t of k_j^T R v_j
+//          + sum over i >= t > j of M_ij        (i, j in the chunk)
+// has the factor exp(g_t) in every term.  S is walked once from the segment's start; R is
+// summed for each chunk that has a strong decay, over the tokens after it as far as
+// their factors matter.  256 threads hold 4 x 4 elements each of a 64 x 64 part of both.
+// Bound by its vector instructions (about 5,000 a wave and chunk).  Forward + backward of 8 x 2048 tokens x 24 heads of
+// 64 x 64, bf16: 340 us without a strong decay (5 of them this launch's), 760 with one
+// token in 256 strong, 1,060 with one in 32, 1,000 with all.
+constexpr float kVanished = 0x1p-60f;
+constexpr int kStrongBlocks = 512;                     // (two a CU, by their LDS)
+constexpr int kDgChunk = 32, kDgPart = 64;
+
+struct StrongShared {
+    // a chunk's rows, a part of their columns: (q, dout, k, v); A and B: the sums over S and R, without their factors
+    __attribute__((aligned(16))) float rows[4][kDgChunk][kDgPart + 4];
+    double red[4], alone[kDgSegMax], across[kDgSegMax / kDgChunk];
+    float dec[kDgSegMax], A[kDgSegMax], B[kDgSegMax], M[kDgChunk][kDgChunk + 1], in[kDgChunk], out[kDgChunk], sums[4][kDgChunk];
+    uint32_t flags[kDgSegMax / kDgChunk], live[kDgSegMax / kDgChunk];     // a bit a token: strong; and with a factor above 0
+    uint64_t found[4];
+};
+
+template <typename T>
+__device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, StrongShared& m) {
+    constexpr int C = kDgChunk, W = kDgPart;
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, ti = 4 * (tid >> 4), tj = 4 * (tid & 15);
+    DgSeg s(p, id / p.segs, int(id % p.segs), m.red);
+    const int n = s.n;
+    float g[kDgTok];
+    if (tid < kDgSegMax / C) {
+        m.flags[tid] = m.live[tid] = 0u;
+        m.across[tid] = 0.0;
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kDgTok; ++i) {
-        const int64_t t = s1 - 1 - (int64_t(tid) * kDgTok + i);
-        double v = 0.0;
-        if (t >= s0 && t < len) {
-            for (int q = 0; q < p.qtiles; ++q) v += p.dotq[(int64_t(q) * p.B * p.H + bh) * p.L + t];
-            for (int k = 0; k < p.ktiles; ++k) v -= p.dotk[(int64_t(k) * p.B * p.H + bh) * p.L + t];
-        }
-        d[i] = v;
+        const int t = s.top - i;
+        g[i] = 0.f;
+        if (t < 0 || t >= n) continue;
+        g[i] = p.g[s.b * p.g_b + (s.s0 + t) * p.g_l + s.h * p.g_h];
+        m.dec[t] = expf(g[i]);
+        m.A[t] = m.B[t] = 0.f;
+        m.alone[t] = 0.0;
+        if (!(g[i] < kLaStrong)) continue;
+        atomicOr(&m.flags[t / C], 1u << (t % C));
+        if (m.dec[t] > 0.f) atomicOr(&m.live[t / C], 1u << (t % C));
     }
-    double f = 0.0;
-    const float* dS = seg + 1 < p.segs ? p.rends + (bh * p.segs + seg + 1) * int64_t(p.KV)
-                                       : p.dlast ? p.dlast + bh * int64_t(p.KV) : nullptr;
-    if (dS) {
-        const float* S = p.ends + (bh * p.segs + seg) * int64_t(p.KV);
+    __syncthreads();
+    int last = -1;
+    for (int c = 0; c * C < n; ++c)
+        if (m.live[c]) last = c;
+
+    const int64_t KV = int64_t(p.K) * p.V;
+    const auto head = [&](const LaRows& r) { return static_cast<const T*>(r.p) + s.b * r.b + s.s0 * r.l + s.h / r.rep * r.h; };
+    const T *q = head(p.q), *k = head(p.k), *v = head(p.v), *dout = head(p.dout);
+    // columns from `col` on of the tokens c0 .. c1-1 (zero past both ends)
+    const auto stage = [&](int to, const T* rows, int64_t step, int dim, int col, int c0, int c1) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = (tid >> 4) + 16 * h;
+            float x[4];
+            load4<T>(rows + int64_t(c0 + r) * step + col + tj, x, c0 + r < c1 ? dim - col - tj : 0);
+            *reinterpret_cast<float4*>(&m.rows[to][r][tj]) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+    };
+    const auto quad = [&](int from, int r, int at, float (&x)[4]) __attribute__((always_inline)) {
+        const float4 w = *reinterpret_cast<const float4*>(&m.rows[from][r][at]);
+        x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+    };
+    // a <- f a + x y^T, and the wave's sums of x^T a y for the rows of xs and ys
+    const auto add = [](float (&a)[4][4], float f, const float (&x)[4], const float (&y)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[i][j] = __builtin_fmaf(x[i], y[j], f * a[i][j]);
+    };
+    const auto products = [&](const float (&a)[4][4], int xs, int ys, int cnt) __attribute__((always_inline)) {
+        for (int t = 0; t < cnt; t += 4) {                  // (4 sums at a time; rows past cnt are zero)
+            float f[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float x[4], y[4];
+                quad(xs, t + u, ti, x);
+                quad(ys, t + u, tj, y);
+                f[u] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float r = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) r = __builtin_fmaf(a[i][j], y[j], r);
+                    f[u] = __builtin_fmaf(x[i], r, f[u]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) f[u] = lanes_sum<64>(f[u]);
+            if (lane == 0) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) m.sums[wave][t + u] = f[u];
+            }
+        }
+    };
+    const auto gather = [&](float* to, int cnt) __attribute__((always_inline)) {        // the 4 waves' sums
+        __syncthreads();
+        if (tid < cnt) to[tid] += (m.sums[0][tid] + m.sums[1][tid]) + (m.sums[2][tid] + m.sums[3][tid]);
+    };
+    const float* S0 = s.seg > 0 ? p.ends + (s.bh * p.segs + s.seg - 1) * KV : p.first ? p.first + s.bh * KV : nullptr;
+    for (int k0 = 0; k0 < p.K; k0 += W) {
+        for (int v0 = 0; v0 < p.V; v0 += W) {
+            const auto state = [&](const float* from, int i, int j) {
+                return from && k0 + ti + i < p.K && v0 + tj + j < p.V ? from[(k0 + ti + i) * p.V + v0 + tj + j] : 0.f;
+            };
+            float S[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) S[i][j] = state(S0, i, j);
+            for (int c = 0; c <= last; ++c) {
+                const int c0 = c * C, c1 = c0 + C < n ? c0 + C : n;
+                const bool here = m.live[c] != 0u;
+                float R[4][4] = {};
+                if (here) {
+                    float w = c1 < n ? m.dec[c1] : 1.f;     // the decays from c1 to the token
+                    int t = c1;
+                    for (; t < n && !(w < kVanished); t += C) {
+                        const int cnt = t + C < n ? C : n - t;
+                        __syncthreads();
+                        stage(0, q, p.q.l, p.K, k0, t, n);
+                        stage(1, dout, p.dout.l, p.V, v0, t, n);
+                        __syncthreads();
 #pragma unroll 4
-        for (int i = 4 * tid; i < p.KV; i += 1024) {
-            float x[4], y[4];
-            rowvec<float>::unpack(rowvec<float>::load(S + i, p.KV - i), x);
-            rowvec<float>::unpack(rowvec<float>::load(dS + i, p.KV - i), y);
+                        for (int i = 0; i < cnt; ++i) {
+                            float x[4], y[4];
+                            quad(0, i, ti, x);
+                            quad(1, i, tj, y);
+                            const float f = w * p.scale;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f += double(x[e]) * double(y[e]);
+                            for (int e = 0; e < 4; ++e) x[e] *= f;
+                            add(R, 1.f, x, y);
+                            if (t + i + 1 < n) w *= m.dec[t + i + 1];
+                        }
+                    }
+                    double f = 0.0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (t >= n) R[i][j] = __builtin_fmaf(w, state(s.dS, i, j), R[i][j]);
+                            f = __builtin_fma(double(S[i][j]), double(R[i][j]), f);
+                        }
+                    f = sum_all(f, m.red);
+                    if (tid == 0) m.across[c] += f;
+                }
+                __syncthreads();
+                if (here) {
+                    stage(0, q, p.q.l, p.K, k0, c0, c1);
+                    stage(1, dout, p.dout.l, p.V, v0, c0, c1);
+                }
+                stage(2, k, p.k.l, p.K, k0, c0, c1);
+                stage(3, v, p.v.l, p.V, v0, c0, c1);
+                __syncthreads();
+                if (here) {
+                    products(S, 0, 1, c1 - c0);
+                    gather(m.A + c0, c1 - c0);
+                    __syncthreads();
+                    products(R, 2, 3, c1 - c0);
+                    gather(m.B + c0, c1 - c0);
+                }
+#pragma unroll 4
+                for (int t = c0; t < c1; ++t) {
+                    float x[4], y[4];
+                    quad(2, t - c0, ti, x);
+                    quad(3, t - c0, tj, y);
+                    add(S, m.dec[t], x, y);
+                }
+            }
         }
     }
-    const double F = sum_all(f, red);
+    // the chunks' own pairs, and the sums
+    for (int c = 0; c <= last; ++c) {
+        if (!m.live[c]) continue;
+        const int c0 = c * C, c1 = c0 + C < n ? c0 + C : n, cnt = c1 - c0;
+        // 4 pairs a thread: row i, and j, j + 8 ..
+        const int i = tid >> 3, j0 = tid & 7;
+        const auto pairs = [&](const T* xs, int64_t xl, const T* ys, int64_t yl, int dim, float (&o)[4]) __attribute__((always_inline)) {
+            for (int col = 0; col < dim; col += W) {
+                __syncthreads();
+                stage(0, xs, xl, dim, col, c0, c1);
+                stage(1, ys, yl, dim, col, c0, c1);
+                __syncthreads();
+#pragma unroll 4
+                for (int e = 0; e < W; e += 4) {
+                    float x[4], y[4];
+                    quad(0, i, e, x);
 #pragma unroll
-    for (int i = 0; i < kDgTok; ++i) {
-        sum += d[i];
-        d[i] = sum;
-    }
-    double upto = sum;                                  // sums over the threads up to this one
+                    for (int j = 0; j < 4; ++j) {
+                        quad(1, j0 + 8 * j, e, y);
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double o = __shfl_up(upto, m, 64);
-        if (lane >= m) upto += o;
+                        for (int a = 0; a < 4; ++a) o[j] = __builtin_fmaf(x[a], y[a], o[j]);
+                    }
+                }
+            }
+        };
+        float qk[4] = {}, dv[4] = {};
+        pairs(q, p.q.l, k, p.k.l, p.K, qk);
+        pairs(dout, p.dout.l, v, p.v.l, p.V, dv);
+        // log2 of the decays from c0 to a token, in every wave (a reset far below any other)
+        double G = 0.0;
+        if (lane < cnt) {
+            const float gt = p.g[s.b * p.g_b + (s.s0 + c0 + lane) * p.g_l + s.h * p.g_h];
+            G = gt < -1e6f ? -1e6 : double(gt) * 1.4426950408889634;
+        }
+#pragma unroll
+        for (int x = 1; x < C; x <<= 1) {
+            const double o = __shfl_up(G, x, 64);
+            if (lane >= x) G += o;
+        }
+        const auto factor = [](double x) {                  // 2^x
+            const double w = floor(x);
+            return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(float(x - w)), w < -2000.0 ? -2000 : w > 2000.0 ? 2000 : int(w));
+        };
+        const double Gi = __shfl(G, i, 64), Gm = __shfl(G, cnt - 1, 64);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double Gj = __shfl(G, j0 + 8 * j, 64);
+            if (i < cnt && j0 + 8 * j < i) m.M[i][j0 + 8 * j] = p.scale * factor(Gi - Gj) * qk[j] * dv[j];
+        }
+        if (tid < cnt) {
+            m.in[tid] = factor(G);                          // the decays from c0 to the token
+            m.out[tid] = factor(Gm - G);                    // ... and after it
+        }
+        __syncthreads();
+        const int t = i, l = j0;                            // 8 lanes a token
+        const bool mine = m.live[c] >> t & 1;
+        double f = 0.0;
+        if (mine) {
+            for (int r = t + l; r < cnt; r += 8) {
+                f += double(p.scale * m.in[r]) * m.A[c0 + r];
+#pragma unroll 8
+                for (int j = 0; j < t; ++j) f += double(m.M[r][j]);
+            }
+            for (int j = l; j < t; j += 8) f += double(m.out[j]) * m.B[c0 + j];
+            if (l == 0) f += double(m.in[cnt - 1]) * m.across[c];
+        }
+#pragma unroll
+        for (int x = 4; x >= 1; x >>= 1) f += __shfl_xor(f, x, 64);
+        if (l == 0 && mine) m.alone[c0 + t] = f;
     }
     __syncthreads();
-    if (lane == 63) red[wave] = upto;
-    __syncthreads();
-    double base = F + (upto - sum);
-    for (int w = 0; w < wave; ++w) base += red[w];
-    double mine = 0.0;
+    // the tokens before a strong decay start at it: alone <- what it is more than the sum was
+    double own[kDgTok];
 #pragma unroll
     for (int i = 0; i < kDgTok; ++i) {
-        const int64_t t = s1 - 1 - (int64_t(tid) * kDgTok + i);
-        if (t >= s0) {
-            const double v = t < len ? base + d[i] : 0.0;
-            if (p.dg) p.dg[(b * p.L + t) * p.H + h] = float(v);
-            mine += v;
+        own[i] = 0.0;
+        if (!(g[i] < kLaStrong)) continue;
+        own[i] = m.alone[s.top - i];
+        m.alone[s.top - i] -= s.d[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kDgTok; ++i) {
+        const int t = s.top - i;
+        if (t < 0 || t >= n) continue;
+        int word = t / C;
+        uint32_t next = m.flags[word] & (~0u << (t % C));
+        while (!next && ++word < kDgSegMax / C) next = m.flags[word];
+        if (g[i] < kLaStrong) s.d[i] = own[i];
+        else if (next) s.d[i] += m.alone[C * word + __builtin_ctz(next)];
+    }
+    s.store(p, m.red);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void la_decay_grad_strong(const LaDgParams p) {
+    __shared__ StrongShared m;
+    const int tid = int(threadIdx.x);
+    // this workgroup's segments, a thread looks at one
+    const int64_t all = p.B * p.H * p.segs, step = gridDim.x;
+    for (int64_t first = blockIdx.x; first < all; first += 256 * step) {
+        const int64_t mine = first + tid * step;
+        const uint64_t found = __ballot(mine < all && p.strong[mine]);
+        __syncthreads();
+        if ((tid & 63) == 0) m.found[tid >> 6] = found;
+        __syncthreads();
+        for (int w = 0; w < 4; ++w) {
+            for (uint64_t left = m.found[w]; left; left &= left - 1) {
+                strong_segment<T>(p, first + (64 * w + __builtin_ctzll(left)) * step, m);
+                __syncthreads();
+            }
         }
     }
-    if (!p.part) return;
-    mine = sum_all(mine, red);
-    if (tid == 0) p.part[bh * p.segs + seg] = mine;
 }
 
 // dg of a head with one decay: the sum over batch rows and segments
@@ -178,7 +493,7 @@ __global__ __launch_bounds__(256) void la_group_sum(const float* part0, T* out0,
 // KB a segment of 64 x 64): a prompt of 32768 tokens, 24 heads of 64 x 64, takes 193,
 // 181 and 219 us with 1024, 1536 and 2112 of them, a training step of 8 x 2048
 // tokens 311, 304 and 315.
-constexpr int64_t kFull = 1024, kSegsWanted = 1536, kSegTokMin = 64, kSegTokMax = 1024;
+constexpr int64_t kFull = 1024, kSegsWanted = 1536, kSegTokMin = 64, kSegTokMax = kDgSegMax;
 
 int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
@@ -190,7 +505,7 @@ int bwd_tile(const ss_linear_attn_args& a) {
     return la_tile(d, d, terms(a));
 }
 
-struct BwdSpace { int64_t dotq, dotk, rends, decays, part, dq, dk, bytes; };
+struct BwdSpace { int64_t dotq, dotk, rends, decays, part, strong, dq, dk, bytes; };
 BwdSpace bwd_space(const ss_linear_attn_bwd_args* g) {
     const ss_linear_attn_args& a = g->f;
     const int64_t bh = a.batch * a.heads, segs = linear_attn_segs(&a);
@@ -203,6 +518,7 @@ BwdSpace bwd_space(const ss_linear_attn_bwd_args* g) {
     s.rends = take(bh * segs * a.d_key * a.d_value * 4);
     s.decays = take(bh * segs * 4);
     s.part = take(g->g_per_head ? bh * segs * 8 : 0);
+    s.strong = take(bh * segs * 4);
     const int64_t shared = a.heads > a.groups ? a.batch * a.seqlen * a.heads * a.d_key * 4 : 0;
     s.dq = take(shared);
     s.dk = take(shared);
@@ -322,6 +638,7 @@ hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t 
     p.tile = bwd_tile(a);
     p.tiles = int(tile_count(K > V ? K : V, p.tile));
     p.serial = serial(a, p.tiles);
+    p.strong = reinterpret_cast<int32_t*>(ws + sp.strong);
     LaJob& jq = p.job[0];
     jq.q = dout; jq.k = v; jq.v = k; jq.x = q;
     jq.o = grad(part ? ws + sp.dq : g->dq, K);
@@ -366,12 +683,22 @@ hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t 
     d.B = a.batch; d.L = a.seqlen; d.H = a.heads;
     d.lens = a.lengths; d.seg_tokens = p.seg_tokens; d.segs = p.segs;
     d.qtiles = d.ktiles = int(tile_count(K, p.tile));
-    d.KV = K * V;
+    d.K = K; d.V = V;
+    d.g = p.g; d.g_b = p.g_b; d.g_l = p.g_l; d.g_h = p.g_h;
+    d.strong = p.strong;
+    d.q = q; d.k = k; d.v = v; d.dout = dout;
+    d.scale = a.scale; d.first = a.initial_state;
     d.dotq = jq.dot; d.dotk = jk.dot; d.ends = a.ends; d.rends = rends; d.dlast = g->dlast_state;
     d.dg = g->g_per_head ? nullptr : g->dg;
     d.part = g->g_per_head ? reinterpret_cast<double*>(ws + sp.part) : nullptr;
     hipLaunchKernelGGL(la_decay_grad, dim3(unsigned(a.batch * a.heads), unsigned(p.segs)), dim3(256), 0, stream, d);
     e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    e = for_type(a.dtype, [&](auto t) {
+        const int64_t n = a.batch * a.heads * p.segs;
+        hipLaunchKernelGGL((la_decay_grad_strong<decltype(t)>), dim3(unsigned(n < kStrongBlocks ? n : kStrongBlocks)), dim3(256), 0, stream, d);
+        return hipGetLastError();
+    });
     if (e != hipSuccess) return e;
     if (g->g_per_head) {
         hipLaunchKernelGGL(la_decay_grad_heads, dim3(unsigned(a.heads)), dim3(256), 0, stream, d.part, g->dg, a.batch,

@@ -53,7 +53,12 @@ struct LaParams {
     int segs, seg_chunks, rep;        // rep: heads per group
     int serial;                       // a workgroup walks a whole row (else a segment, from its carry)
     int tile, tiles;                  // value columns per workgroup, and tiles of the widest job
+    int32_t* strong;                  // written by a backward's walk: (B, H, segs), whether the segment has a strong decay
 };
+
+// A log decay below it (2^-12) is a strong one: the decay's gradient is a sum that holds to
+// about 2^-21 of terms without the decay's factor, which would leave it fewer than 9 bits.
+constexpr float kLaStrong = -8.317766f;
 
 // Most value columns a workgroup takes for q and k of up to k columns, in rows of
 // so many bf16 terms (bf16 1, fp16 2, fp32 3): the state's share and the rows on their way stay within the
@@ -76,13 +81,20 @@ struct LaDgParams {
     int64_t B, L, H;
     const int32_t* lens;
     int64_t seg_tokens;
-    int segs, qtiles, ktiles, KV;
+    int segs, qtiles, ktiles, K, V;
+    const float* g;
+    int64_t g_b, g_l, g_h;
     const float* dotq; const float* dotk;   // (tiles, B, H, L)
     const float* ends;                      // S after each segment (B, H, segs, K, V)
     const float* rends;                     // dS after each segment's walk (before it in time), same layout
     const float* dlast;                     // (B, H, K, V) or null
     float* dg;                              // (B, L, H), or null with part
     double* part;                           // (B, H, segs) sums over the segment's tokens, or null
+    const int32_t* strong;                  // LaParams'
+    // read only for those segments: the forward's rows, out's gradient, scale and the state before the first token
+    LaRows q, k, v, dout;
+    float scale;
+    const float* first;                     // (B, H, K, V) or null
 };
 
 }  // namespace ss

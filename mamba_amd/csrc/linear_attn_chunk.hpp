@@ -158,7 +158,6 @@ template <int NT> constexpr __device__ __forceinline__ bool tile_in(int n, int v
 __device__ __forceinline__ int state_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
 
 // 4 consecutive elements, the first cnt of them
-typedef uint32_t half4_at2 __attribute__((ext_vector_type(2), aligned(2)));
 template <typename T>
 __device__ __forceinline__ void store4(T* p, const float (&v)[4], int cnt) {
     if (cnt >= 4) {
@@ -175,28 +174,6 @@ __device__ __forceinline__ void store4(T* p, const float (&v)[4], int cnt) {
     for (int i = 0; i < 3; ++i)
         if (i < cnt) io<T>::store(p + i, v[i]);
 }
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4], int cnt) {
-    if (cnt >= 4) {
-        if constexpr (sizeof(T) == 4) {
-            const words_at4 w = *reinterpret_cast<const words_at4*>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
-        } else {
-            const half4_at2 w = *reinterpret_cast<const half4_at2*>(p);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t u = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
-                if constexpr (__is_same(T, bf16_t)) v[i] = __uint_as_float(u << 16);
-                else v[i] = float(__builtin_bit_cast(_Float16, uint16_t(u)));
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < cnt ? io<T>::load(p + i) : 0.f;
-}
-
 // 8-byte words at any element alignment; a lane's 4 or 8 columns of a result
 typedef uint32_t words4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T, int W, bool WHOLE>
@@ -757,6 +734,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
     else each_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, [](float, bool, uint32_t) __attribute__((always_inline)) { return 0.f; });
 
     int pair = -1;
+    bool strong = false;                                     // (a lane's tokens, of the segment so far)
     float decay = 0.f;
     if (w.chunks > 0) {
         w.fetch(0);
@@ -787,6 +765,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
         if (pair != ch >> 1) {
             pair = ch >> 1;
             m.dec.fill(lane, decay, rev, J.vscale, J.oscale);
+            if (DOT) strong |= decay < kLaStrong;
             const int next = pair + (rev ? -1 : 1);
             if (next >= 0) decay = w.decay(next);
         }
@@ -986,6 +965,11 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
         }
         // (a whole row's walk: the state at the end of each segment)
         const uint32_t seg = uint32_t(ch) / uint32_t(p.seg_chunks), next = uint32_t(rev ? ch - 1 : ch + 1) / uint32_t(p.seg_chunks);
+        if (DOT && at.job == 0 && at.tile == 0 && (last || next != seg)) {
+            const bool any = __ballot(strong) != 0;
+            if (lane == 0) p.strong[bh * p.segs + (p.serial ? seg : uint32_t(at.seg))] = any;
+            strong = false;
+        }
         if (J.ends && (last || next != seg)) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + (bh * p.segs + seg) * KV);
     }
     if (w.chunks == 0 && J.ends) write_state<KP, NT, WHOLE>(S, J, n0, vdim, lane, J.ends + bh * p.segs * KV);

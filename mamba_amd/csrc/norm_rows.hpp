@@ -93,6 +93,30 @@ struct rowvec {
     }
 };
 
+// 4 consecutive elements at any element alignment, the first cnt of them and zero past them
+typedef uint32_t half4_at2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float (&v)[4], int cnt) {
+    if (cnt >= 4) {
+        if constexpr (sizeof(T) == 4) {
+            const words_at4 w = *reinterpret_cast<const words_at4*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+        } else {
+            const half4_at2 w = *reinterpret_cast<const half4_at2*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+                if constexpr (__is_same(T, bf16_t)) v[i] = __uint_as_float(u << 16);
+                else v[i] = float(__builtin_bit_cast(_Float16, uint16_t(u)));
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < cnt ? io<T>::load(p + i) : 0.f;
+}
+
 // Sum over each aligned set of N lanes (N a power of two up to 64), in every
 // lane of it.  Within 16 lanes by DPP: once quads agree, a half-row mirror
 // brings the other quad of 8 lanes, and a rotation by 8 the other half row.

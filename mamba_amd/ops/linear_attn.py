@@ -20,6 +20,9 @@ row's last state is the one after its own last token (a row of length 0 keeps
 its initial state).  Returns out (batch, seqlen, heads, d_value), or (out,
 last_state) with ``return_last_state``.  Gradients flow to q, k, v, g and
 initial_state; their sums have a fixed order, so the same bits on every run.
+dg of a token is zero where exp(g) is, and within a small part of exp(g) |S| |dS|
+(the states on its two sides) where g is below -8.3; above, it is a difference of
+sums over up to 1024 tokens, and within about 2^-21 of their size.
 A token's infinities or NaN reach the outputs of its own and later tokens.
 
 ``linear_attn_update(state, q, k, v, g, scale=None, out=None)`` advances state
