@@ -77,6 +77,12 @@ bool wants_grad(std::initializer_list<const Tensor*> inputs) {
         if (t && t->defined() && t->requires_grad()) return true;
     return false;
 }
+// A forward-mode tangent would be lost: the operators have none.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        REQUIRE(what, !t || !t->defined() || !t->_fw_grad(0).defined(), "forward-mode derivatives are not implemented");
+}
+const Tensor* at_opt(const OptT& t) { return t ? &*t : nullptr; }
 // A tensor that the library wrote in place: autograd then refuses a backward that
 // saved what it held (tensors made in inference mode are never saved).
 void written(const Tensor& t) {
@@ -833,7 +839,8 @@ struct LinAttn : torch::autograd::Function<LinAttn> {
 // (out, last_state or None)
 py::tuple linear_attn(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptT& initial,
                       const OptT& lengths, double scale, bool want_last) {
-    const bool need = wants_grad({&q, &k, &v, &g, initial ? &*initial : nullptr});
+    no_tangents(kLin, {&q, &k, &v, &g, at_opt(initial)});
+    const bool need = wants_grad({&q, &k, &v, &g, at_opt(initial)});
     if (!need) {
         const LinOut r = lin_fwd(q, k, v, g, initial, lengths, scale, want_last, false, current_stream(v.device()));
         return py::make_tuple(r.out, r.last);
@@ -856,6 +863,7 @@ Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const
     const int64_t G = q_.size(1), K = q_.size(2);
     REQUIRE(kLinUp, H == 0 || (G > 0 && H % G == 0),
             "heads " + std::to_string(H) + " is not a multiple of groups " + std::to_string(G));
+    no_tangents(kLinUp, {&state, &q_, &k_, &v_, &g_});
     REQUIRE(kLinUp, !wants_grad({&state, &q_, &k_, &v_, &g_}),
             "a token's update has no backward; call it under torch.no_grad(), or linear_attn_fn for gradients");
     on_device(kLinUp, "q", q_, dev); on_device(kLinUp, "k", k_, dev); on_device(kLinUp, "state", state, dev);
@@ -1031,7 +1039,8 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 // (out, s)
 py::tuple block_norm(const Tensor& x, const Tensor& residual, const Tensor& post, const Tensor& pre, const OptT& gate,
                      const OptT& scale_vec, double scale, double eps) {
-    if (!wants_grad({&x, &residual, &post, &pre, gate ? &*gate : nullptr, scale_vec ? &*scale_vec : nullptr})) {
+    no_tangents(kBlockNorm, {&x, &residual, &post, &pre, at_opt(gate), at_opt(scale_vec)});
+    if (!wants_grad({&x, &residual, &post, &pre, at_opt(gate), at_opt(scale_vec)})) {
         const BorderOut r = block_norm_fwd(x, residual, gate, post, pre, scale_vec, scale, eps, false, current_stream(x.device()));
         return py::make_tuple(r.out.view(x.sizes()), r.s.view(x.sizes()));
     }
@@ -1103,6 +1112,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     }
 };
 Tensor gated_norm(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
+    no_tangents(kGatedNorm, {&x, &gate, &weight});
     if (!wants_grad({&x, &gate, &weight}))
         return gated_norm_fwd(x, gate, weight, groups, eps, current_stream(x.device()))[0].view(x.sizes());
     return GatedNorm::apply(x, gate, weight, groups, eps);
@@ -1127,6 +1137,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, const std::vector<Tensor>& o
         const Tensor &g = grads[i], &o = outs[i];
         const auto at_i = [&] { return " of tensor " + std::to_string(i); };
         REQUIRE(kClip, g.device() == dev && o.device() == dev, "all tensors must be on one device");
+        no_tangents(kClip, {&g, &o});
         REQUIRE(kClip, itype_of(g.scalar_type(), &dtypes[i]), "unsupported dtype " + dtype_str(g.scalar_type()) + at_i());
         REQUIRE(kClip, g.is_non_overlapping_and_dense(), "gaps or overlaps in the elements" + at_i());
         if (!o.is_same(g))
