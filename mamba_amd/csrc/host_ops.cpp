@@ -92,6 +92,41 @@ Tensor given(const OptT& t) { return t ? *t : Tensor(); }
 OptT maybe(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+// The operators' gradients have no derivative of their own.  With create_graph they
+// come out of a node that says so when a second backward reaches it; the values are of
+// use as they are.
+struct FinalGrads : torch::autograd::Function<FinalGrads> {
+    static variable_list forward(AutogradContext* ctx, const Tensor&, const variable_list& grads, const std::string& what) {
+        ctx->saved_data["what"] = what;
+        variable_list r;
+        for (const Tensor& g : grads) r.push_back(g.variable_data());
+        return r;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list) {
+        throw std::runtime_error(ctx->saved_data["what"].toStringRef() + ": second derivatives are not implemented");
+    }
+};
+variable_list final_grads(const char* what, variable_list grads) {
+    if (!at::GradMode::is_enabled()) return grads;
+    variable_list some;
+    for (const Tensor& g : grads)
+        if (g.defined()) some.push_back(g);
+    if (some.empty()) return grads;
+    // (a node needs an input that requires a gradient)
+    const Tensor anchor = at::empty({0}, some[0].options().dtype(at::kFloat)).requires_grad_();
+    const variable_list r = FinalGrads::apply(anchor, some, std::string(what));
+    size_t at = 0;
+    for (Tensor& g : grads)
+        if (g.defined()) g = r[at++];
+    return grads;
+}
+std::vector<OptT> final_grads_py(const std::string& what, const std::vector<OptT>& grads) {
+    variable_list r;
+    for (const OptT& g : grads) r.push_back(given(g));
+    std::vector<OptT> out;
+    for (const Tensor& g : final_grads(what.c_str(), r)) out.push_back(maybe(g));
+    return out;
+}
 void* node_stream(AutogradContext* ctx) { return reinterpret_cast<void*>(ctx->saved_data["stream"].toInt()); }
 
 bool itype_of(at::ScalarType t, int32_t* out) {
@@ -833,7 +868,7 @@ struct LinAttn : torch::autograd::Function<LinAttn> {
         if (ctx->needs_input_grad(2)) r[2] = d.dv;
         if (ctx->needs_input_grad(3)) r[3] = d.dg.to(at::ScalarType(ctx->saved_data["g_type"].toInt()));
         r[4] = given(d.dinitial);
-        return r;
+        return final_grads(kLin, r);
     }
 };
 // (out, last_state or None)
@@ -1033,7 +1068,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         if (ctx->needs_input_grad(3)) r[3] = typed(d.dpre, 1);
         if (t[2].defined() && ctx->needs_input_grad(at_gate)) r[4] = d.dgate->view(shape);
         if (t[5].defined() && ctx->needs_input_grad(at_scale)) r[5] = typed(*d.dscale, 2);
-        return r;
+        return final_grads(kBlockNorm, r);
     }
 };
 // (out, s)
@@ -1108,7 +1143,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
         if (ctx->needs_input_grad(0)) r[0] = d[0].view(shape);
         if (ctx->needs_input_grad(1)) r[1] = d[1].view(shape);
         if (ctx->needs_input_grad(2)) r[2] = d[2].to(at::ScalarType(ctx->saved_data["type"].toInt()));
-        return r;
+        return final_grads(kGatedNorm, r);
     }
 };
 Tensor gated_norm(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
@@ -1195,5 +1230,6 @@ PYBIND11_MODULE(mamba_host, m) {
     m.def("block_norm", &block_norm);
     m.def("gated_norm", &gated_norm);
     m.def("clip_grads", &clip_grads);
+    m.def("final_grads", &final_grads_py);
     m.def("abi", [] { return py::make_tuple(SS_ABI_VERSION, sizeof(ss_fwd_args), sizeof(ss_bwd_args)); });
 }

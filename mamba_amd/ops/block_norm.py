@@ -24,7 +24,8 @@ of n_groups equal parts of a row (the heads of a block) by itself:
     out = rms(part of x) * (1 + weight) * silu(gate)
 
 Gradients flow to x, gate and weight.  Weight gradients are summed over rows
-in a fixed order, so they have the same bits on every run.
+in a fixed order, so they have the same bits on every run.  Forward-mode and
+second derivatives are refused.
 """
 import torch
 

@@ -24,6 +24,7 @@ dg of a token is zero where exp(g) is, and within a small part of exp(g) |S| |dS
 (the states on its two sides) where g is below -8.3; above, it is a difference of
 sums over up to 1024 tokens, and within about 2^-21 of their size.
 A token's infinities or NaN reach the outputs of its own and later tokens.
+Forward-mode and second derivatives are refused.
 
 ``linear_attn_update(state, q, k, v, g, scale=None, out=None)`` advances state
 (batch, heads, d_key, d_value) by one token in place: q, k (batch, groups,

@@ -51,3 +51,21 @@ def test_tangents_are_refused_in_place():
             linear_attn_update(state, fwad.make_dual(t, t), t, v, g)
         with pytest.raises(ValueError, match="forward-mode"):
             clip_grads([fwad.make_dual(t, t)], 1.0)
+
+
+@pytest.mark.parametrize("name", ["linear_attn", "border", "heads"])
+def test_second_derivatives_are_refused(name):
+    call, x = calls()[name]
+    for n in range(len(x)):
+        y = [t.clone() for t in x]
+        y[n].requires_grad_()
+        first, = torch.autograd.grad(call(*y).sum(), [y[n]])
+        graph, = torch.autograd.grad(call(*y).sum(), [y[n]], create_graph=True)
+        assert torch.equal(first, graph)
+        with pytest.raises(RuntimeError, match="second"):
+            (graph.square().sum() + y[n].square().sum()).backward()
+        y[n].grad = None                       # (the other term's share)
+        # a gradient kept with its graph is of use as it is
+        call(*y).sum().backward(create_graph=True)
+        assert torch.equal(y[n].grad.detach(), first)
+        y[n].grad = None
