@@ -24,6 +24,7 @@ import torch
 
 from .. import _native as nat
 from ..selective_scan import _ITYPES, _ptr, _raw_stream, _require, _stream
+from ..utils.final_backward import final_backward
 
 
 def _weight2d(weight, dim):
@@ -97,6 +98,7 @@ class CausalConv1dFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @final_backward("causal_conv1d")
     def backward(ctx, dout):
         x, weight, bias = ctx.saved_tensors
         dx, dw, db = _conv_bwd_typed(x, weight, bias, dout, ctx.silu)

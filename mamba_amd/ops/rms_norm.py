@@ -20,6 +20,7 @@ import torch
 
 from .. import _native as nat
 from ..selective_scan import _ITYPES, _ptr, _raw_stream, _stream
+from ..utils.final_backward import final_backward
 
 
 def _require(cond, msg):
@@ -134,6 +135,7 @@ class RMSNormFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @final_backward("rms_norm")
     def backward(ctx, dout, dres=None):
         s, weight, rstd = ctx.saved_tensors
         if dout is None:

@@ -19,6 +19,7 @@ import torch
 
 from .. import _native as nat
 from .. import selective_scan
+from ..utils.final_backward import final_backward
 from ..utils.tensor_utils import ensure_contiguous
 
 
@@ -50,6 +51,7 @@ class SelectiveScanFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @final_backward("selective_scan")
     def backward(ctx, dout):
         dout = ensure_contiguous(dout)
         u, delta, A, B, C, D, delta_bias, x = ctx.saved_tensors
@@ -87,6 +89,7 @@ class SelectiveScanZFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @final_backward("selective_scan")
     def backward(ctx, dout, *unused):
         u, delta, A, B, C, D, delta_bias, z, x, y = ctx.saved_tensors
         if not _seq_ok(dout) or dout.dtype != delta.dtype:
@@ -243,6 +246,7 @@ class MambaInnerFn(torch.autograd.Function):
         return res
 
     @staticmethod
+    @final_backward("mamba_inner")
     def backward(ctx, dres):
         from .causal_conv1d import _conv_bwd_typed
         (xz, conv1d_weight, conv1d_bias, x_proj_weight, delta_proj_weight, out_proj_weight,
