@@ -22,10 +22,12 @@
 // Products run on bf16 matrix instructions with 32-bit sums.  A row of type
 // T is a sum of R bf16 terms, exactly: 1 (bf16), 2 (fp16, 11 bits) or 3
 // (fp32); what is computed (P, S, the weighted rows of the state's update) is
-// split into 2 or 3 terms (2^-18 off at most, or exact), and of the products of
-// terms those below 2^-24 (2 terms: 2^-16) are left out.  2 terms are enough where the result is rounded
-// to 16 bits; states, and gradients that the decay's gradient is summed from,
-// take 3.
+// split into 2 or 3 terms (2^-18 off at most, or exact).  Of the products of terms
+// those of the second with the third (2 terms: the second with the second) and beyond
+// are left out: of 3 terms at most 2^-22 of a product, 2^-25 rms and of either sign,
+// so a sum's share of them shrinks; of 2 terms 2^-16.  2 terms are enough where the
+// result is rounded to 16 bits; states, and gradients that the decay's gradient is
+// summed from, take 3.
 //
 // Layouts.  A 16x16x32 instruction takes 8 summands a lane (lane l: row or
 // column l % 16, summands 8 (l / 16) ..) and returns 4 consecutive rows of a
@@ -78,8 +80,10 @@ __device__ __forceinline__ float lo_half(uint32_t v) { return __uint_as_float(v 
 __device__ __forceinline__ float hi_half(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
 // x0, x1 as N bf16 terms each, packed (x0 low).  2 terms: both rounded, 2^-18 off
-// at most.  3 terms: cut, so what is left over is exact and the third holds it.
-template <int N>
+// at most.  3 terms, exact: the first cut (so that none of a finite value is
+// infinite), 16 bits left over; the second rounded, so that the third, what is left, has either
+// sign.  CUT: the second cut as well, where no product of terms is left out.
+template <int N, bool CUT = false>
 __device__ __forceinline__ void split(float x0, float x1, uint32_t (&t)[N]) {
     if constexpr (N <= 2) {
         t[0] = io<bf16_t>::pack2(x0, x1);
@@ -88,9 +92,9 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&t)[N]) {
         const uint32_t u0 = __float_as_uint(x0), u1 = __float_as_uint(x1);
         t[0] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
         const float r0 = x0 - __uint_as_float(u0 & 0xffff0000u), r1 = x1 - __uint_as_float(u1 & 0xffff0000u);
-        const uint32_t m0 = __float_as_uint(r0), m1 = __float_as_uint(r1);
-        t[1] = __builtin_amdgcn_perm(m1, m0, 0x07060302u);
-        const float s0 = r0 - __uint_as_float(m0 & 0xffff0000u), s1 = r1 - __uint_as_float(m1 & 0xffff0000u);
+        if constexpr (CUT) t[1] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+        else t[1] = io<bf16_t>::pack2(r0, r1);
+        const float s0 = r0 - lo_half(t[1]), s1 = r1 - hi_half(t[1]);
         t[2] = __builtin_amdgcn_perm(__float_as_uint(s1), __float_as_uint(s0), 0x07060302u);
     }
 }
@@ -497,7 +501,7 @@ __device__ __forceinline__ void update_state(f4 (&S)[KP / 16][NT], const uint16_
                 x1 += hi_half(vf[n][r][w]);
             }
             uint32_t t[3];
-            split<3>(x0 * u[2 * w], x1 * u[2 * w + 1], t);
+            split<3, R == 1>(x0 * u[2 * w], x1 * u[2 * w + 1], t);
 #pragma unroll
             for (int i = 0; i < 3; ++i) bv[i][w] = t[i];
         }
@@ -804,7 +808,7 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
                 for (int x = 0; x < 4; ++x) {
                     uint32_t t[N];
                     const f4& s = S[2 * kk + (x >> 1)][n];
-                    split<N>(s[2 * (x & 1)], s[2 * (x & 1) + 1], t);
+                    split<N, R == 1>(s[2 * (x & 1)], s[2 * (x & 1) + 1], t);
 #pragma unroll
                     for (int i = 0; i < N; ++i) sf[i][x] = t[i];
                 }
@@ -860,8 +864,8 @@ __device__ __forceinline__ void walk_rows(Params& p, Job& J, const Place& at, Ti
                         if (it == j) v[r] = (rev ? 4 * g + r < c : 4 * g + r > c) ? 0.f : v[r];
                     }
                     uint32_t lo[N], hi[N];
-                    split<N>(v[0], v[1], lo);
-                    split<N>(v[2], v[3], hi);
+                    split<N, R == 1>(v[0], v[1], lo);
+                    split<N, R == 1>(v[2], v[3], hi);
 #pragma unroll
                     for (int t = 0; t < N; ++t) {
                         pf[t][2 * j] = lo[t];
