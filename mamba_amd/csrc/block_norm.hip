@@ -8,22 +8,23 @@
 //   out = rms(s) (1 + pre)                   (of the unrounded s)
 //
 // Backward, with n1, n2 the two reciprocal roots (kept by the forward),
-// c = scale silu(gate) (1 + post) x (so s = residual + n1 c) and
+// c = scale silu(gate) (1 + post) n1 x (so s = residual + c) and
 // h = ds + n2 dout (1 + pre):
 //
-//   k2 = n2^3 mean(dout (1 + pre) s),   dr = h - k2 s = dresidual
-//   dx = n1 dr scale silu(gate) (1 + post) - x n1^3 mean(dr c)
+//   a2 = n2 mean(n2 dout (1 + pre) s),   dr = h - a2 n2 s = dresidual
+//   dx = n1 dr scale silu(gate) (1 + post) - n1 x a1,   a1 = n1 mean(dr c)
 //   dgate = dr scale x n1 (1 + post) silu'(gate)
 //   dpost, dpre, dscale: sums over rows of dr scale silu(gate) x n1,
 //                        dout s n2, dr x n1 (1 + post) silu(gate)
 //
-// mean(dr c) = mean(h c) - k2 mean(s c), so a row needs one reduction (of
-// three sums) and is read once.
+// mean(dr c) = mean(h c) - a2 n2 mean(s c), so a row needs one reduction (of
+// three sums) and is read once.  No product holds a root's square alone: rows of
+// 1e-15 or 1e15 keep their gradients.
 //
 // Heads (gated_norm), each row in groups of n elements with a norm of its own:
 //
 //   out = rms_group(x) (1 + weight) silu(gate)
-//   with g = dout silu(gate):  dx = r g (1 + weight) - x r^3 mean(g (1 + weight) x),
+//   with g = dout silu(gate):  dx = r g (1 + weight) - x r (r mean(r g (1 + weight) x)),
 //   dgate = dout x r (1 + weight) silu'(gate),  dweight = sum over rows of g x r
 //
 // (r recomputed in the backward: its sum rides with the other one.)
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(kBlock<WPR>, kBlock<WPR> / 256 > 2 ? kBlock<WPR> / 
                     sig[k][e] = sigmoid(z[e]);
                     sil = z[e] * sig[k][e];
                 }
-                const float c = wsc[e] * sil * (1.f + wpost[e]) * x[e], s = __builtin_fmaf(n1, c, r[e]);
+                const float c = wsc[e] * sil * (1.f + wpost[e]) * (x[e] * n1), s = r[e] + c;
                 const float ow = o[e] * (1.f + wpre[e]), h = __builtin_fmaf(n2, ow, d[e]);
                 sum[0] = __builtin_fmaf(ow, s, sum[0]);
                 sum[1] = __builtin_fmaf(h, c, sum[1]);
@@ -272,8 +273,8 @@ __global__ __launch_bounds__(kBlock<WPR>, kBlock<WPR> / 256 > 2 ? kBlock<WPR> / 
         }
         team_sum<WPR>(sum, red[turn], wave);
         turn ^= 1;
-        const float k2 = n2 * n2 * n2 * sum[0] * inv;
-        const float k1 = n1 * n1 * n1 * (sum[1] - k2 * sum[2]) * inv;
+        const float a2 = n2 * (n2 * sum[0] * inv);
+        const float a1 = n1 * ((sum[1] - a2 * (n2 * sum[2])) * inv);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             float x[VE], r[VE], z[VE], o[VE], d[VE], gz[VE], wpost[VE], wpre[VE], wsc[VE];
@@ -288,17 +289,17 @@ __global__ __launch_bounds__(kBlock<WPR>, kBlock<WPR> / 256 > 2 ? kBlock<WPR> / 
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 if (!p.wscale) wsc[e] = p.scale;
-                const float w1 = 1.f + wpost[e], sil = p.gate ? z[e] * sig[k][e] : 1.f;
-                const float c = wsc[e] * sil * w1 * x[e], s = __builtin_fmaf(n1, c, r[e]);
+                const float w1 = 1.f + wpost[e], sil = p.gate ? z[e] * sig[k][e] : 1.f, xn = x[e] * n1;
+                const float c = wsc[e] * sil * w1 * xn, sn = (r[e] + c) * n2;
                 const float ow = o[e] * (1.f + wpre[e]);
-                const float dr = __builtin_fmaf(n2, ow, d[e]) - k2 * s;
-                const float xn = x[e] * n1, dt = dr * wsc[e];
-                apre[k][e] = __builtin_fmaf(o[e], s * n2, apre[k][e]);
+                const float dr = __builtin_fmaf(n2, ow, d[e]) - a2 * sn;
+                const float dt = dr * wsc[e];
+                apre[k][e] = __builtin_fmaf(o[e], sn, apre[k][e]);
                 apost[k][e] = __builtin_fmaf(dt * sil, xn, apost[k][e]);
                 asc[k][e] = __builtin_fmaf(dr, xn * w1 * sil, asc[k][e]);
                 gz[e] = p.gate ? dt * (xn * w1) * sig[k][e] * __builtin_fmaf(z[e], 1.f - sig[k][e], 1.f) : 0.f;
                 d[e] = dr;
-                x[e] = n1 * (dt * sil * w1) - x[e] * k1;
+                x[e] = n1 * (dt * sil * w1) - xn * a1;
             }
             if (p.gate) R::store(static_cast<T*>(p.dgate) + row * p.dim + col[k], gz, cnt[k]);
             if (p.dres) R::store(static_cast<T*>(p.dres) + row * p.dim + col[k], d, cnt[k]);
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(kHeadBlock<L>) void gated_norm(const GatedParams p)
             if constexpr (BWD) sum[1] = lanes_sum<L>(sum[1]);
         }
         const float r = rsqrtf(sum[0] * inv + p.eps);
-        const float k1 = r * r * r * sum[1] * inv;
+        const float a = r * (r * sum[1] * inv);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int n = live ? cnt[k] : 0;
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(kHeadBlock<L>) void gated_norm(const GatedParams p)
                     const float gr = o[e] * sil;
                     acc[k][e] = __builtin_fmaf(gr, xr, acc[k][e]);
                     gz[e] = o[e] * (xr * w1) * sig[k][e] * __builtin_fmaf(z[e], 1.f - sig[k][e], 1.f);
-                    x[e] = r * (gr * w1) - x[e] * k1;
+                    x[e] = r * (gr * w1) - xr * a;
                 } else {
                     x[e] = xr * w1 * sil;
                 }
