@@ -72,11 +72,21 @@ class LinearAttnLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids, max_new_tokens, lengths=None):
-        """Greedy continuation, (batch, max_new_tokens); rows of input_ids hold lengths[b] tokens."""
+        """Greedy continuation, (batch, max_new_tokens); rows of input_ids hold lengths[b] tokens
+        (at least one, all of a row's where lengths[b] is larger)."""
         batch, seqlen = input_ids.shape
+        if lengths is None:
+            at = torch.full((batch,), seqlen, device=input_ids.device)
+        else:
+            if lengths.shape != (batch,):
+                raise ValueError(f"generate: lengths has shape {tuple(lengths.shape)}, expected {(batch,)}")
+            at = lengths.long().clamp(max=seqlen)
+        if seqlen == 0 or bool((at < 1).any()):
+            raise ValueError("generate: a row without a token has nothing to continue")
+        if max_new_tokens < 1:
+            return input_ids.new_empty(batch, 0)
         states = self.allocate_states(batch, input_ids.device)
         logits = self(input_ids, lengths=lengths, states=states)
-        at = torch.full((batch,), seqlen, device=input_ids.device) if lengths is None else lengths.long()
         logits = logits[torch.arange(batch, device=input_ids.device), at - 1]
         out = []
         for i in range(max_new_tokens):
