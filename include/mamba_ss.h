@@ -676,7 +676,7 @@ int64_t ss_gated_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t gro
  *   norm = sqrt(sum g^2),  outs[i] = grads[i] * min(1, max_norm / (norm + eps))
  * (squares summed in 64 bits, in a fixed order; the product in fp32, rounded
  * to the tensor's type).  The arrays are host memory, read before the call
- * returns.  outs[i] may be grads[i]; other overlaps are not allowed.
+ * returns.  outs[i] may be grads[i]; other overlaps of an output are refused.
  * ------------------------------------------------------------------------ */
 typedef struct ss_clip_grads_args {
     int64_t count;                       /* tensors */

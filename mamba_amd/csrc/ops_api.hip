@@ -3,6 +3,8 @@
 // last error (per thread) it shares.
 #include "ss_api.hip"
 
+#include <new>
+
 #include "ops_kernels.hpp"
 #include "overlap.hpp"
 
@@ -288,6 +290,24 @@ static int check_clip_grads(const ss_clip_grads_args* a) {
     return ok();
 }
 
+// Two workgroups must not write, or write and read, one element.
+static int check_clip_overlap(const ss_clip_grads_args* a) try {
+    std::vector<ss::Span> ins, outs;
+    outs.reserve(a->count);
+    for (int64_t i = 0; i < a->count; ++i) {
+        if (a->numels[i] == 0) continue;
+        const uintptr_t bytes = uintptr_t(a->numels[i]) * elem_size(a->dtypes[i]);
+        const uintptr_t in = reinterpret_cast<uintptr_t>(a->grads[i]), out = reinterpret_cast<uintptr_t>(a->outs[i]);
+        outs.push_back({out, out + bytes, i});
+        if (in != out) ins.push_back({in, in + bytes, i});
+    }
+    const int64_t at = ss::outputs_clash(ins, outs);
+    if (at >= 0) return fail(SS_ERR_INVALID, "the output of tensor %lld lies over another tensor", (long long)at);
+    return SS_OK;
+} catch (const std::bad_alloc&) {
+    return fail(SS_ERR_INVALID, "out of host memory");
+}
+
 int64_t ss_clip_grads_workspace_bytes(const ss_clip_grads_args* a) {
     return check_clip_grads(a) == SS_OK ? 16 + 8 * ss::clip_grads_chunks(a) : -1;
 }
@@ -298,6 +318,7 @@ int ss_clip_grads(const ss_clip_grads_args* a, void* stream) {
     if (!(a->max_norm >= 0.f) || !(a->eps >= 0.f)) return fail(SS_ERR_INVALID, "max_norm and eps must be >= 0");
     if (!a->norm || !aligned(a->norm, 4)) return fail(SS_ERR_INVALID, "norm is NULL or misaligned");
     rc = check_space(a->workspace, a->workspace_bytes, 16 + 8 * ss::clip_grads_chunks(a));
+    if (rc == SS_OK) rc = check_clip_overlap(a);
     if (rc != SS_OK) return rc;
     const hipError_t e = ss::clip_grads_launch(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(SS_ERR_HIP, "gradient clipping launch failed: %s", hipGetErrorString(e));

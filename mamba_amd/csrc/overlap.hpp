@@ -1,8 +1,10 @@
 // Whether tensors that a launch writes share elements.  Plain C++, so that the
 // checks and a host program share the rule.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 #include <utility>
+#include <vector>
 
 namespace ss {
 
@@ -22,6 +24,25 @@ inline bool blocks_overlap(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64
         if (j + 1 < n2 && (j + 1) * s2 - d < size) return true;
     }
     return false;
+}
+
+struct Span { uintptr_t from, to; int64_t at; };      // bytes [from, to) of tensor `at`, not empty
+
+// The first output (of `outs`, sorted here) that lies over another one, or over an
+// input that is not its own in whole, by its `at`; -1: none.
+inline int64_t outputs_clash(const std::vector<Span>& ins, std::vector<Span>& outs) {
+    const auto before = [](const Span& a, const Span& b) { return a.from < b.from; };
+    if (!std::is_sorted(outs.begin(), outs.end(), before)) std::sort(outs.begin(), outs.end(), before);
+    for (size_t i = 1; i < outs.size(); ++i)
+        if (outs[i].from < outs[i - 1].to) return outs[i].at;
+    for (const Span& in : ins) {
+        if (outs.empty() || in.to <= outs.front().from || in.from >= outs.back().to) continue;
+        // outputs are apart, so the first that ends past the input's start is the one that may reach into it
+        auto o = std::upper_bound(outs.begin(), outs.end(), in.from, [](uintptr_t v, const Span& s) { return v < s.to; });
+        for (; o != outs.end() && o->from < in.to; ++o)
+            if (o->at != in.at || o->from != in.from || o->to != in.to) return o->at;
+    }
+    return -1;
 }
 
 }  // namespace ss

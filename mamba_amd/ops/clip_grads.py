@@ -8,7 +8,9 @@ parameters without a gradient, are left out):
     out  = grad * min(1, max_norm / (norm + eps))   (fp32, rounded to the tensor's dtype)
 
 The gradients are scaled in place, or written to ``out``, tensors of the same
-shapes, strides and dtypes (None where grads holds None).  Returns norm, a 0-d
+shapes, strides and dtypes (None where grads holds None).  An output that lies
+over another tensor than its own gradient (one gradient given twice, in place) is
+refused.  Returns norm, a 0-d
 fp32 tensor on the device: nothing waits for the GPU.  Sums have a fixed
 order, the same bits on every run.  An infinity or NaN among the gradients
 makes the norm infinite or NaN, and the gradients zero (and NaN at the

@@ -65,3 +65,57 @@ def test_update_refused(which, batch, heads, strides):
         setattr(a, n, FAKE + 65536 * i)
     assert lib.ss_linear_attn_update(ctypes.byref(a), None) == nat.SS_ERR_INVALID
     assert f"{which}'s elements overlap" in lib.ss_last_error().decode()
+
+
+SPANS = """
+#include <cstdio>
+#include <cstdlib>
+#include "overlap.hpp"
+int main() {
+    int bad = 0;
+    std::srand(1);
+    for (int turn = 0; turn < 200000; ++turn) {
+        std::vector<ss::Span> ins, outs;
+        const int n = 1 + std::rand() % 4;
+        for (int64_t i = 0; i < n; ++i) {
+            const uintptr_t size = 1 + std::rand() % 6, in = std::rand() % 40;
+            const uintptr_t out = std::rand() % 3 ? in : std::rand() % 40;
+            if (in != out) ins.push_back({in, in + size, i});
+            outs.push_back({out, out + size, i});
+        }
+        bool want = false;
+        const auto meet = [](const ss::Span& a, const ss::Span& b) { return a.from < b.to && b.from < a.to; };
+        for (size_t i = 0; i < outs.size(); ++i) {
+            for (size_t j = 0; j < i; ++j) want |= meet(outs[i], outs[j]);
+            for (const ss::Span& in : ins) want |= meet(outs[i], in);
+        }
+        const int64_t at = ss::outputs_clash(ins, outs);
+        if ((at >= 0) != want || at >= n) ++bad, std::printf("turn %d\\n", turn);
+    }
+    return bad != 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no host compiler")
+def test_the_rule_of_spans(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(SPANS)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-I", CSRC, str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert run.returncode == 0, run.stdout[-2000:]
+
+
+# (grads, outs) as offsets in bytes of two tensors of 100 bf16 elements: one tensor twice, two that overlap, an output
+# over another's gradient, one that slides over its own
+@pytest.mark.parametrize("grads,outs", [((0, 0), (0, 0)), ((0, 198), (0, 198)), ((0, 0), (4096, 4096)), ((0, 4096), (4096, 8192)),
+                                        ((0, 4096), (2, 8192)), ((8192, 4096), (0, 4294))], ids=str)
+def test_clip_refused(grads, outs):
+    lib = nat.load()
+    a = nat.ClipGradsArgs()
+    a.count, a.max_norm, a.eps, a.norm, a.workspace, a.workspace_bytes = 2, 1.0, 1e-6, FAKE, FAKE, 1 << 20
+    keep = ((ctypes.c_void_p * 2)(*(2 * FAKE + x for x in grads)), (ctypes.c_void_p * 2)(*(2 * FAKE + x for x in outs)),
+            (ctypes.c_int64 * 2)(100, 100), (ctypes.c_int32 * 2)(nat.SS_BF16, nat.SS_BF16))
+    a.grads, a.outs, a.numels, a.dtypes = (ctypes.cast(k, ctypes.c_void_p) for k in keep)
+    assert lib.ss_clip_grads(ctypes.byref(a), None) == nat.SS_ERR_INVALID
+    assert "lies over another tensor" in lib.ss_last_error().decode()
