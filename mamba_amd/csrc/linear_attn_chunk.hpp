@@ -553,8 +553,8 @@ __device__ __forceinline__ Params& params() { return *(Params*)__builtin_amdgcn_
 
 // Workgroup order: the jobs of a segment (they read the same rows), then its column
 // tiles, side by side on one XCD.
-// (32-bit divisions: a launch holds fewer than 2^24 workgroups, and the 64-bit
-// ones cost a short walk a tenth of its time.)
+// (32-bit divisions: a launch holds fewer than 2^26 workgroups of 64 threads, and the
+// 64-bit ones cost a short walk a tenth of its time.)
 struct Place { int job, tile, seg; uint32_t bh, b, h, shared; };      // (bh past the last one: nothing to do)
 __device__ __forceinline__ Place place(Params& p, uint32_t segs) {
     uint32_t id = uint32_t(xcd_block_id());
