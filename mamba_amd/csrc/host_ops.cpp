@@ -974,7 +974,7 @@ void norm_x(const char* what, const Tensor& x, int32_t* dtype) {
     REQUIRE(what, x.dim() >= 1, "x must have at least one dimension");
 }
 
-// (rows as (rows, dim); read: x, residual, gate, post, pre, scale_vec)
+// (out, s: of x's shape; read: x, residual, gate, post, pre, scale_vec, rows as (rows, dim))
 struct BorderOut { Tensor out, s; OptT rstd; variable_list read; };
 BorderOut block_norm_fwd(const Tensor& x_, const Tensor& residual_, const OptT& gate_, const Tensor& post, const Tensor& pre,
                          const OptT& scale_vec, double scale, double eps, bool want_rstd, void* stream) {
@@ -986,12 +986,13 @@ BorderOut block_norm_fwd(const Tensor& x_, const Tensor& residual_, const OptT& 
     a.w_dtype = w.dtype;
     a.rows = x.size(0); a.dim = x.size(1);
     a.eps = float(eps); a.scale = float(scale);
-    const Tensor out = at::empty(x.sizes(), x.options()), s = at::empty(x.sizes(), x.options());
+    // (of x's shape, not views: what autograd returns can then be changed in place)
+    const Tensor out = at::empty(x_.sizes(), x.options()), s = at::empty(x_.sizes(), x.options());
     OptT rstd;
     if (want_rstd) rstd = f32_like({a.rows, 2}, x);
     a.x_row_stride = x.stride(0); a.residual_row_stride = residual.stride(0);
     if (gate) a.gate_row_stride = gate->stride(0);
-    a.out_row_stride = out.stride(0); a.residual_out_row_stride = s.stride(0);
+    a.out_row_stride = a.residual_out_row_stride = a.dim;
     a.x = ptr(x); a.residual = ptr(residual); a.gate = ptr(gate);
     a.post = ptr(w.w[0]); a.pre = ptr(w.w[1]); a.scale_vec = ptr(w.w[2]);
     a.out = ptr(out); a.residual_out = ptr(s); a.rstd = fptr<float>(rstd);
@@ -1049,7 +1050,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
         ctx->saved_data["types"] = std::vector<int64_t>{int64_t(post.scalar_type()), int64_t(pre.scalar_type()),
                                                         scale_vec ? int64_t(scale_vec->scalar_type()) : 0};
         ctx->set_materialize_grads(false);
-        return {r.out.view(x.sizes()), r.s.view(x.sizes())};
+        return {r.out, r.s};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list r(8);
@@ -1077,13 +1078,13 @@ py::tuple block_norm(const Tensor& x, const Tensor& residual, const Tensor& post
     no_tangents(kBlockNorm, {&x, &residual, &post, &pre, at_opt(gate), at_opt(scale_vec)});
     if (!wants_grad({&x, &residual, &post, &pre, at_opt(gate), at_opt(scale_vec)})) {
         const BorderOut r = block_norm_fwd(x, residual, gate, post, pre, scale_vec, scale, eps, false, current_stream(x.device()));
-        return py::make_tuple(r.out.view(x.sizes()), r.s.view(x.sizes()));
+        return py::make_tuple(r.out, r.s);
     }
     const variable_list r = BlockNorm::apply(x, residual, post, pre, gate, scale_vec, scale, eps);
     return py::make_tuple(r[0], r[1]);
 }
 
-// (out, x, gate, weight as read), rows as (rows, dim)
+// (out of x's shape; x, gate, weight as read, rows as (rows, dim))
 variable_list gated_norm_fwd(const Tensor& x_, const Tensor& gate_, const Tensor& weight, int64_t groups, double eps,
                              void* stream) {
     ss_gated_norm_args a{};
@@ -1093,8 +1094,8 @@ variable_list gated_norm_fwd(const Tensor& x_, const Tensor& gate_, const Tensor
     const Weights w = weights_of(kGatedNorm, x_, {{"weight", &ow}});
     a.w_dtype = w.dtype;
     a.rows = x.size(0); a.dim = x.size(1); a.groups = groups; a.eps = float(eps);
-    const Tensor out = at::empty(x.sizes(), x.options());
-    a.x_row_stride = x.stride(0); a.gate_row_stride = gate.stride(0); a.out_row_stride = out.stride(0);
+    const Tensor out = at::empty(x_.sizes(), x.options());
+    a.x_row_stride = x.stride(0); a.gate_row_stride = gate.stride(0); a.out_row_stride = a.dim;
     a.x = ptr(x); a.gate = ptr(gate); a.weight = ptr(w.w[0]); a.out = ptr(out);
     launch(x.device(), "gated_rms_norm forward", [&] { return ss_gated_norm_fwd(&a, stream); });
     return {out, x, gate, *w.w[0]};
@@ -1132,7 +1133,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["shape"] = x.sizes().vec();
         ctx->saved_data["type"] = int64_t(weight.scalar_type());
-        return r[0].view(x.sizes());
+        return r[0];
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto t = ctx->get_saved_variables();
@@ -1149,7 +1150,7 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
 Tensor gated_norm(const Tensor& x, const Tensor& gate, const Tensor& weight, int64_t groups, double eps) {
     no_tangents(kGatedNorm, {&x, &gate, &weight});
     if (!wants_grad({&x, &gate, &weight}))
-        return gated_norm_fwd(x, gate, weight, groups, eps, current_stream(x.device()))[0].view(x.sizes());
+        return gated_norm_fwd(x, gate, weight, groups, eps, current_stream(x.device()))[0];
     return GatedNorm::apply(x, gate, weight, groups, eps);
 }
 
