@@ -813,6 +813,10 @@ LinGrads lin_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
                  dv = at::empty(in.v.sizes(), in.v.options());
     const Tensor dg = g_per_head ? f32_like({a.heads}, in.v) : f32_like({a.batch, a.seqlen, a.heads}, in.v);
     if (a.batch == 0) dg.zero_();
+    if (a.heads == 0) {                                // (q and k reach no output)
+        dq.zero_();
+        dk.zero_();
+    }
     b.f.ends = static_cast<float*>(ptr(ends));
     b.dout_batch_stride = dout.stride(0); b.dout_len_stride = dout.stride(1); b.dout_head_stride = dout.stride(2);
     b.dout = ptr(dout); b.dlast_state = fptr<float>(dlast);
