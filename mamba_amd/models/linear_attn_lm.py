@@ -49,7 +49,9 @@ class LinearAttnLM(nn.Module):
         """mix(i, normed) -> block i's output; returns the head's input."""
         normed = rms_norm_fn(s, self.pre[0], eps=self.config.eps)
         for i in range(len(self.mixers)):
-            normed, s = block_norm_fn(mix(i, normed), s, self.post[i], self.pre[i + 1], scale=self.scale[i], eps=self.config.eps)
+            # (under autocast the mixer's output has 16 bits; the residual stream keeps its type)
+            y = mix(i, normed).to(s.dtype)
+            normed, s = block_norm_fn(y, s, self.post[i], self.pre[i + 1], scale=self.scale[i], eps=self.config.eps)
         return normed
 
     def forward(self, input_ids, lengths=None, states=None):
