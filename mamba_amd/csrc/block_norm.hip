@@ -32,7 +32,7 @@
 // A row (a group) lies in the registers of a team of lanes, 8 or 16 elements
 // a lane, between its one load and its one store: the kernels are bound by
 // HBM.  16384 x 768 bf16 with gate and scale: forward 26 us (126 MB, 4.8 TB/s),
-// backward 56 us (201 MB, 3.6 TB/s: 253 registers leave two waves a SIMD; with the
+// backward 56 us (201 MB, 3.6 TB/s: 246 registers leave two waves a SIMD; with the
 // weights as fp32 there was one, 80 us).  16384 x 24 heads of 64: forward 27 us
 // (5.6 TB/s), backward 51 us (4.9 TB/s).  Weights and column sums stay in the team's registers over its rows.
 // The column sums leave as one fp32 row per workgroup, summed by a second

@@ -61,8 +61,10 @@ struct LaParams {
 constexpr float kLaStrong = -8.317766f;
 
 // Most value columns a workgroup takes for q and k of up to k columns, in rows of
-// so many bf16 terms (bf16 1, fp16 2, fp32 3): the state's share and the rows on their way stay within the
-// 256 registers a lane that let two waves share a SIMD.
+// so many bf16 terms (bf16 1, fp16 2, fp32 3): the state's share and the rows on their way about fill the
+// 256 registers a lane that let two waves share a SIMD.  Spilled beyond them, of bf16 heads: 10
+// registers by the 64 x 64 forward's walk (18 where tiles are not whole), 3 and 10 at 128 x 128, none and 6
+// by the 64 x 64 backward's; of fp16 heads up to 19; fp32 rows of 128 take 512 registers and one wave.
 constexpr int la_cols(int64_t k, int terms) { return k <= 64 ? (terms == 1 ? 64 : 32) : k <= 128 ? 32 : 16; }
 // ... and those it takes of v columns: a multiple of 16, the shares even.
 inline int la_tile(int64_t k, int64_t v, int terms) {

@@ -40,13 +40,15 @@
 //  - sums over tokens read k and v in that order through the transposing LDS
 //    load, where 16 lanes read 4 rows of 16 elements and get a column of 4 each.
 //
-// Measured, 8 x 2048 tokens x 24 heads of 64 x 64, bf16: the forward's walk 56 us
-// (225 MB: 4.0 TB/s, where plain reads of the same rows reach 6.5), the three
-// passes of the backward together 158 us (about 1180 vector and 120 matrix
-// instructions a chunk: a lane's vector instructions alone are 74 us; two waves a
-// SIMD, which wait for memory 38 % of the time), a segment's states 28 us.  What
-// bounds it is issue: splitting P, S and the weighted rows, and the decays.  With
-// 2 terms in the backward as well it runs 5 % faster, and the decay's gradient is
+// Measured, 8 x 2048 tokens x 24 heads of 64 x 64, bf16 (the best and the median of ten
+// launches): the forward's walk 56 and 61 us (225 MB: 4.0 TB/s, where plain reads of the
+// same rows reach 6.5), the three passes of the backward together 159 and 173 us (about 1180 vector
+// and 120 matrix instructions a chunk), a segment's states 27 and 29 us.  Vector instructions
+// alone would take 19 of the forward's 56 us and 71 of the backward's 159.  With two
+// waves a SIMD, the forward's waves issue for 37 % of their time, wait for their turn or an
+// earlier instruction for 20 and for memory for 43; the backward's for 43, 31 and 26.  So it is bound by
+// latency at that occupancy as much as by issue: splitting P, S and the weighted rows, and
+// the decays.  With 2 terms in the backward as well it runs 5 % faster, and the decay's gradient is
 // off by 7e-6 instead of 6e-7.
 #pragma once
 
@@ -114,7 +116,7 @@ __device__ __forceinline__ int late(int lane) {
 }
 
 // c[i] += sum of the products of a[i]'s NA and b[i]'s NB terms whose order is at
-// most kMax (2: down to 2^-24; 1: to 2^-16), small ones first.  I independent sums
+// most kMax (left out: with 2 up to 2^-22 of a product, with 1 2^-16), small ones first.  I independent sums
 // at once: a product then need not wait for the one before it.  ai, bi: which operand
 // the sums take (a stride of 0 shares one).
 template <int I, int SA, int SB, int NA, int NB, int kMax>

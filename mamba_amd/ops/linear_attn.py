@@ -23,7 +23,8 @@ initial_state; their sums have a fixed order, so the same bits on every run.
 dg of a token is zero where exp(g) is, and within a small part of exp(g) |S| |dS|
 (the states on its two sides) where g is below -8.3; above, it is a difference of
 sums over up to 1024 tokens, and within about 2^-21 of their size.
-A token's infinities or NaN reach the outputs of its own and later tokens.
+A token's infinities or NaN reach the outputs of its own and later tokens (and,
+of the gradients, dg of earlier tokens too).
 Forward-mode and second derivatives are refused.
 
 ``linear_attn_update(state, q, k, v, g, scale=None, out=None)`` advances state
