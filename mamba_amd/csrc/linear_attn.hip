@@ -172,18 +172,20 @@ __global__ __launch_bounds__(256) void la_decay_grad(const LaDgParams p) {
 // has the factor exp(g_t) in every term.  S is walked once from the segment's start; R is
 // summed for each chunk that has a strong decay, over the tokens after it as far as
 // their factors matter.  256 threads hold 4 x 4 elements each of a 64 x 64 part of both.
-// Bound by its vector instructions (about 5,000 a wave and chunk).  Forward + backward of 8 x 2048 tokens x 24 heads of
-// 64 x 64, bf16: 340 us without a strong decay (5 of them this launch's), 760 with one
-// token in 256 strong, 1,060 with one in 32, 1,000 with all.
+// The rows get their factors on the way into LDS, so a token costs S and R 16 products each.
+// Bound by the latency of its rows and barriers at two workgroups a CU and by its vector instructions.  Forward +
+// backward of 8 x 2048 tokens x 24 heads of 64 x 64, bf16: 340 us without a strong decay (5
+// of them this launch's), 700 with one token in 256 strong, 950 with one in 32 or with all.
 constexpr float kVanished = 0x1p-60f;
 constexpr int kStrongBlocks = 512;                     // (two a CU, by their LDS)
 constexpr int kDgChunk = 32, kDgPart = 64;
 
 struct StrongShared {
-    // a chunk's rows, a part of their columns: (q, dout, k, v); A and B: the sums over S and R, without their factors
+    // a chunk's rows, a part of their columns, with their factors: (q, dout, k, v); [2] holds M afterwards
     __attribute__((aligned(16))) float rows[4][kDgChunk][kDgPart + 4];
-    double red[4], alone[kDgSegMax], across[kDgSegMax / kDgChunk];
-    float dec[kDgSegMax], A[kDgSegMax], B[kDgSegMax], M[kDgChunk][kDgChunk + 1], in[kDgChunk], out[kDgChunk], sums[4][kDgChunk];
+    double red[4], alone[kDgSegMax], across[kDgSegMax / kDgChunk];      // across: <S, R> of a chunk
+    float upto[kDgSegMax], after[kDgSegMax];               // the decays from a token's chunk's start to it, and after it to the end
+    float A[kDgSegMax], B[kDgSegMax], sums[4][kDgChunk];   // the tokens' sums over S and over R
     uint32_t flags[kDgSegMax / kDgChunk], live[kDgSegMax / kDgChunk];     // a bit a token: strong; and with a factor above 0
     uint64_t found[4];
 };
@@ -206,12 +208,34 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
         g[i] = 0.f;
         if (t < 0 || t >= n) continue;
         g[i] = p.g[s.b * p.g_b + (s.s0 + t) * p.g_l + s.h * p.g_h];
-        m.dec[t] = expf(g[i]);
         m.A[t] = m.B[t] = 0.f;
         m.alone[t] = 0.0;
         if (!(g[i] < kLaStrong)) continue;
         atomicOr(&m.flags[t / C], 1u << (t % C));
-        if (m.dec[t] > 0.f) atomicOr(&m.live[t / C], 1u << (t % C));
+        if (expf(g[i]) > 0.f) atomicOr(&m.live[t / C], 1u << (t % C));
+    }
+    // log2 of the decays from the chunk's start to a token, a chunk 32 lanes (a reset far below any other)
+    const auto logs = [&](int t) __attribute__((always_inline)) {
+        double G = 0.0;
+        if (t < n) {
+            const float gt = p.g[s.b * p.g_b + (s.s0 + t) * p.g_l + s.h * p.g_h];
+            G = gt < -1e6f ? -1e6 : double(gt) * 1.4426950408889634;
+        }
+#pragma unroll
+        for (int x = 1; x < C; x <<= 1) {
+            const double o = __shfl_up(G, x, C);
+            if ((lane & (C - 1)) >= x) G += o;
+        }
+        return G;
+    };
+    const auto factor = [](double x) {                      // 2^x
+        const double w = floor(x);
+        return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(float(x - w)), w < -2000.0 ? -2000 : w > 2000.0 ? 2000 : int(w));
+    };
+    for (int t = tid; t < (n + C - 1) / C * C; t += 256) {
+        const double G = logs(t);
+        m.upto[t] = factor(G);
+        m.after[t] = factor(__shfl(G, C - 1, C) - G);
     }
     __syncthreads();
     int last = -1;
@@ -221,29 +245,39 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
     const int64_t KV = int64_t(p.K) * p.V;
     const auto head = [&](const LaRows& r) { return static_cast<const T*>(r.p) + s.b * r.b + s.s0 * r.l + s.h / r.rep * r.h; };
     const T *q = head(p.q), *k = head(p.k), *v = head(p.v), *dout = head(p.dout);
-    // columns from `col` on of the tokens c0 .. c1-1 (zero past both ends)
-    const auto stage = [&](int to, const T* rows, int64_t step, int dim, int col, int c0, int c1) __attribute__((always_inline)) {
+    // columns from `col` on of the tokens from c0 on (zero past both ends), times f and the tokens' factors
+    const auto stage = [&](int to, const T* rows, int64_t step, int dim, int col, int c0, const float* factors = nullptr, float f = 1.f)
+                           __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = (tid >> 4) + 16 * h;
             float x[4];
-            load4<T>(rows + int64_t(c0 + r) * step + col + tj, x, c0 + r < c1 ? dim - col - tj : 0);
-            *reinterpret_cast<float4*>(&m.rows[to][r][tj]) = make_float4(x[0], x[1], x[2], x[3]);
+            load4<T>(rows + int64_t(c0 + r) * step + col + tj, x, c0 + r < n ? dim - col - tj : 0);
+            const float w = factors ? f * factors[c0 + r] : f;
+            *reinterpret_cast<float4*>(&m.rows[to][r][tj]) = make_float4(w * x[0], w * x[1], w * x[2], w * x[3]);
         }
     };
     const auto quad = [&](int from, int r, int at, float (&x)[4]) __attribute__((always_inline)) {
         const float4 w = *reinterpret_cast<const float4*>(&m.rows[from][r][at]);
         x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
     };
-    // a <- f a + x y^T, and the wave's sums of x^T a y for the rows of xs and ys
-    const auto add = [](float (&a)[4][4], float f, const float (&x)[4], const float (&y)[4]) __attribute__((always_inline)) {
+    // a <- a + x y^T summed over the rows of xs and ys (those past cnt are zero), and the wave's sums of x^T a y for each
+    const auto add = [&](float (&a)[4][4], int xs, int ys, int cnt) __attribute__((always_inline)) {
+        for (int t = 0; t < cnt; t += 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int u = 0; u < 4; ++u) {
+                float x[4], y[4];
+                quad(xs, t + u, ti, x);
+                quad(ys, t + u, tj, y);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[i][j] = __builtin_fmaf(x[i], y[j], f * a[i][j]);
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[i][j] = __builtin_fmaf(x[i], y[j], a[i][j]);
+            }
+        }
     };
     const auto products = [&](const float (&a)[4][4], int xs, int ys, int cnt) __attribute__((always_inline)) {
-        for (int t = 0; t < cnt; t += 4) {                  // (4 sums at a time; rows past cnt are zero)
+        for (int t = 0; t < cnt; t += 4) {
             float f[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
@@ -287,25 +321,16 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
                 const bool here = m.live[c] != 0u;
                 float R[4][4] = {};
                 if (here) {
-                    float w = c1 < n ? m.dec[c1] : 1.f;     // the decays from c1 to the token
+                    float w = 1.f;                          // the decays from c1 to the chunk at t
                     int t = c1;
                     for (; t < n && !(w < kVanished); t += C) {
                         const int cnt = t + C < n ? C : n - t;
                         __syncthreads();
-                        stage(0, q, p.q.l, p.K, k0, t, n);
-                        stage(1, dout, p.dout.l, p.V, v0, t, n);
+                        stage(0, q, p.q.l, p.K, k0, t, m.upto, w * p.scale);
+                        stage(1, dout, p.dout.l, p.V, v0, t);
                         __syncthreads();
-#pragma unroll 4
-                        for (int i = 0; i < cnt; ++i) {
-                            float x[4], y[4];
-                            quad(0, i, ti, x);
-                            quad(1, i, tj, y);
-                            const float f = w * p.scale;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) x[e] *= f;
-                            add(R, 1.f, x, y);
-                            if (t + i + 1 < n) w *= m.dec[t + i + 1];
-                        }
+                        add(R, 0, 1, cnt);
+                        w *= m.upto[t + cnt - 1];
                     }
                     double f = 0.0;
 #pragma unroll
@@ -320,11 +345,11 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
                 }
                 __syncthreads();
                 if (here) {
-                    stage(0, q, p.q.l, p.K, k0, c0, c1);
-                    stage(1, dout, p.dout.l, p.V, v0, c0, c1);
+                    stage(0, q, p.q.l, p.K, k0, c0, m.upto, p.scale);
+                    stage(1, dout, p.dout.l, p.V, v0, c0);
                 }
-                stage(2, k, p.k.l, p.K, k0, c0, c1);
-                stage(3, v, p.v.l, p.V, v0, c0, c1);
+                stage(2, k, p.k.l, p.K, k0, c0, m.after);
+                stage(3, v, p.v.l, p.V, v0, c0);
                 __syncthreads();
                 if (here) {
                     products(S, 0, 1, c1 - c0);
@@ -333,13 +358,12 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
                     products(R, 2, 3, c1 - c0);
                     gather(m.B + c0, c1 - c0);
                 }
-#pragma unroll 4
-                for (int t = c0; t < c1; ++t) {
-                    float x[4], y[4];
-                    quad(2, t - c0, ti, x);
-                    quad(3, t - c0, tj, y);
-                    add(S, m.dec[t], x, y);
-                }
+                const float total = m.upto[c1 - 1];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) S[i][j] *= total;
+                add(S, 2, 3, c1 - c0);
             }
         }
     }
@@ -352,8 +376,8 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
         const auto pairs = [&](const T* xs, int64_t xl, const T* ys, int64_t yl, int dim, float (&o)[4]) __attribute__((always_inline)) {
             for (int col = 0; col < dim; col += W) {
                 __syncthreads();
-                stage(0, xs, xl, dim, col, c0, c1);
-                stage(1, ys, yl, dim, col, c0, c1);
+                stage(0, xs, xl, dim, col, c0);
+                stage(1, ys, yl, dim, col, c0);
                 __syncthreads();
 #pragma unroll 4
                 for (int e = 0; e < W; e += 4) {
@@ -371,30 +395,11 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
         float qk[4] = {}, dv[4] = {};
         pairs(q, p.q.l, k, p.k.l, p.K, qk);
         pairs(dout, p.dout.l, v, p.v.l, p.V, dv);
-        // log2 of the decays from c0 to a token, in every wave (a reset far below any other)
-        double G = 0.0;
-        if (lane < cnt) {
-            const float gt = p.g[s.b * p.g_b + (s.s0 + c0 + lane) * p.g_l + s.h * p.g_h];
-            G = gt < -1e6f ? -1e6 : double(gt) * 1.4426950408889634;
-        }
-#pragma unroll
-        for (int x = 1; x < C; x <<= 1) {
-            const double o = __shfl_up(G, x, 64);
-            if (lane >= x) G += o;
-        }
-        const auto factor = [](double x) {                  // 2^x
-            const double w = floor(x);
-            return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(float(x - w)), w < -2000.0 ? -2000 : w > 2000.0 ? 2000 : int(w));
-        };
-        const double Gi = __shfl(G, i, 64), Gm = __shfl(G, cnt - 1, 64);
+        const double G = logs(c0 + (lane & (C - 1))), Gi = __shfl(G, i, C);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const double Gj = __shfl(G, j0 + 8 * j, 64);
-            if (i < cnt && j0 + 8 * j < i) m.M[i][j0 + 8 * j] = p.scale * factor(Gi - Gj) * qk[j] * dv[j];
-        }
-        if (tid < cnt) {
-            m.in[tid] = factor(G);                          // the decays from c0 to the token
-            m.out[tid] = factor(Gm - G);                    // ... and after it
+            const double Gj = __shfl(G, j0 + 8 * j, C);
+            if (i < cnt && j0 + 8 * j < i) m.rows[2][i][j0 + 8 * j] = p.scale * factor(Gi - Gj) * qk[j] * dv[j];
         }
         __syncthreads();
         const int t = i, l = j0;                            // 8 lanes a token
@@ -402,12 +407,12 @@ __device__ __forceinline__ void strong_segment(const LaDgParams& p, int64_t id, 
         double f = 0.0;
         if (mine) {
             for (int r = t + l; r < cnt; r += 8) {
-                f += double(p.scale * m.in[r]) * m.A[c0 + r];
+                f += m.A[c0 + r];
 #pragma unroll 8
-                for (int j = 0; j < t; ++j) f += double(m.M[r][j]);
+                for (int j = 0; j < t; ++j) f += m.rows[2][r][j];
             }
-            for (int j = l; j < t; j += 8) f += double(m.out[j]) * m.B[c0 + j];
-            if (l == 0) f += double(m.in[cnt - 1]) * m.across[c];
+            for (int j = l; j < t; j += 8) f += m.B[c0 + j];
+            if (l == 0) f += double(m.upto[c1 - 1]) * m.across[c];
         }
 #pragma unroll
         for (int x = 4; x >= 1; x >>= 1) f += __shfl_xor(f, x, 64);
