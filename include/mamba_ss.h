@@ -578,6 +578,92 @@ typedef struct ss_linear_attn_update_args {
 int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The gated delta rule.  No counterpart in the reference.  Per (batch b,
+ * head h), with group j = h / (heads / groups) and a = exp(g[b, t, h]):
+ *   e   = v[b, t, h] - a S_{t-1}^T k[b, t, j]
+ *   S_t = a S_{t-1} + beta[b, t, h] k[b, t, j] e^T                 (d_key x d_value, fp32)
+ *   out[b, t, h] = scale * S_t^T q[b, t, j]
+ * Shapes, strides, lengths and states as for the linear attention above; g and
+ * beta: fp32 (batch, seqlen, heads), any strides (0 too).  d_key and d_value: 1
+ * to 256; batch * heads up to 2^20; seqlen up to 2^24; batch * heads * seqlen
+ * below 2^28 (fp32 keys above 64, fp16 above 128) or 2^29.
+ * saved: what the backward takes from the forward (ss_delta_rule_saved_bytes() bytes,
+ * 16-byte aligned), or NULL.
+ * ------------------------------------------------------------------------ */
+typedef struct ss_delta_rule_args {
+    int64_t batch, seqlen, heads, groups, d_key, d_value;
+    int32_t dtype;                       /* enum ss_dtype */
+    float scale;
+    int64_t q_batch_stride, q_len_stride, q_head_stride;
+    int64_t k_batch_stride, k_len_stride, k_head_stride;
+    int64_t v_batch_stride, v_len_stride, v_head_stride;
+    int64_t out_batch_stride, out_len_stride, out_head_stride;
+    int64_t g_batch_stride, g_len_stride, g_head_stride;
+    int64_t beta_batch_stride, beta_len_stride, beta_head_stride;
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* g;
+    const float* beta;
+    const float* initial_state;          /* may be NULL */
+    const int32_t* lengths;              /* may be NULL: every row holds seqlen tokens */
+    void* out;                           /* ignored by ss_delta_rule_bwd */
+    float* last_state;                   /* may be NULL (not written); ignored by ss_delta_rule_bwd */
+    void* saved;                         /* written by the forward unless NULL, read by the backward */
+    void* workspace;                     /* the entry point's workspace_bytes, 16-byte aligned; NULL iff 0 */
+    int64_t saved_bytes, workspace_bytes;
+} ss_delta_rule_args;
+
+/* dq, dk: (batch, seqlen, groups, d_key), dv: (batch, seqlen, heads,
+ * d_value), contiguous, dtype (the sums over the heads of a group in fp32,
+ * rounded once).  dg, dbeta: fp32 (batch, seqlen, heads) contiguous.  Every term
+ * of dg has the factor exp(g).  Every sum has a fixed order. */
+typedef struct ss_delta_rule_bwd_args {
+    ss_delta_rule_args f;                /* as for the forward; f.saved from it */
+    int64_t dout_batch_stride, dout_len_stride, dout_head_stride;
+    const void* dout;
+    const float* dlast_state;            /* may be NULL: zero */
+    void* dq;
+    void* dk;
+    void* dv;
+    float* dg;
+    float* dbeta;
+    float* dinitial_state;               /* may be NULL (not written) */
+} ss_delta_rule_bwd_args;
+
+/* Bytes of `saved` and of workspace that the calls need (0: none), or -1 (with
+   ss_last_error set) on failing checks.  The forward's workspace is smaller with saved given.
+   No device work. */
+int64_t ss_delta_rule_saved_bytes(const ss_delta_rule_args* a);
+int64_t ss_delta_rule_fwd_workspace_bytes(const ss_delta_rule_args* a);
+int64_t ss_delta_rule_bwd_workspace_bytes(const ss_delta_rule_bwd_args* a);
+int ss_delta_rule_fwd(const ss_delta_rule_args* a, void* stream);
+int ss_delta_rule_bwd(const ss_delta_rule_bwd_args* a, void* stream);
+
+/* One token: the state advances in place and out is read from it.  Shapes and
+ * overlaps as for ss_linear_attn_update; beta: fp32 (batch, heads). */
+typedef struct ss_delta_rule_update_args {
+    int64_t batch, heads, groups, d_key, d_value;
+    int32_t dtype;                       /* enum ss_dtype */
+    float scale;
+    int64_t state_batch_stride, state_head_stride;
+    int64_t q_batch_stride, q_head_stride;
+    int64_t k_batch_stride, k_head_stride;
+    int64_t v_batch_stride, v_head_stride;
+    int64_t out_batch_stride, out_head_stride;
+    int64_t g_batch_stride, g_head_stride;
+    int64_t beta_batch_stride, beta_head_stride;
+    float* state;
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* g;
+    const float* beta;
+    void* out;
+} ss_delta_rule_update_args;
+int ss_delta_rule_update(const ss_delta_rule_update_args* a, void* stream);
+
+/* ------------------------------------------------------------------------
  * The norms around a block.  No counterpart in the reference, whose block
  * has the norm in front only (models/causal_lm.py:30-35).  With rms(v) =
  * v * rsqrt(mean(v^2) + eps) over a row, in fp32:

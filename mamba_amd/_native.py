@@ -187,6 +187,33 @@ class LinearAttnUpdateArgs(ctypes.Structure):
     ]
 
 
+class DeltaRuleArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("seqlen", _i64), ("heads", _i64), ("groups", _i64), ("d_key", _i64), ("d_value", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+    ] + [(f"{t}_{d}_stride", _i64) for t in ("q", "k", "v", "out", "g", "beta") for d in ("batch", "len", "head")] + [
+        ("q", _p), ("k", _p), ("v", _p), ("g", _p), ("beta", _p), ("initial_state", _p), ("lengths", _p),
+        ("out", _p), ("last_state", _p), ("saved", _p), ("workspace", _p), ("saved_bytes", _i64), ("workspace_bytes", _i64),
+    ]
+
+
+class DeltaRuleBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("f", DeltaRuleArgs),
+        ("dout_batch_stride", _i64), ("dout_len_stride", _i64), ("dout_head_stride", _i64),
+        ("dout", _p), ("dlast_state", _p), ("dq", _p), ("dk", _p), ("dv", _p), ("dg", _p), ("dbeta", _p), ("dinitial_state", _p),
+    ]
+
+
+class DeltaRuleUpdateArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", _i64), ("heads", _i64), ("groups", _i64), ("d_key", _i64), ("d_value", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+    ] + [(f"{t}_{d}_stride", _i64) for t in ("state", "q", "k", "v", "out", "g", "beta") for d in ("batch", "head")] + [
+        ("state", _p), ("q", _p), ("k", _p), ("v", _p), ("g", _p), ("beta", _p), ("out", _p),
+    ]
+
+
 class BlockNormArgs(ctypes.Structure):
     _fields_ = [("rows", _i64), ("dim", _i64), ("dtype", _i32), ("w_dtype", _i32), ("eps", ctypes.c_float),
                 ("scale", ctypes.c_float)] + [
@@ -285,12 +312,14 @@ def load():
         lib.ss_bwd_noalloc.argtypes = [ctypes.POINTER(BwdArgs), _p]
         lib.ss_bwd_noalloc.restype = ctypes.c_int
         for name, T in (("ss_linear_attn_segment", LinearAttnArgs), ("ss_linear_attn_fwd_workspace_bytes", LinearAttnArgs),
-                        ("ss_linear_attn_bwd_workspace_bytes", LinearAttnBwdArgs)):
+                        ("ss_linear_attn_bwd_workspace_bytes", LinearAttnBwdArgs), ("ss_delta_rule_saved_bytes", DeltaRuleArgs),
+                        ("ss_delta_rule_fwd_workspace_bytes", DeltaRuleArgs), ("ss_delta_rule_bwd_workspace_bytes", DeltaRuleBwdArgs)):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(T)]
             fn.restype = _i64
         for name, T in (("ss_linear_attn_fwd", LinearAttnArgs), ("ss_linear_attn_bwd", LinearAttnBwdArgs),
-                        ("ss_linear_attn_update", LinearAttnUpdateArgs)):
+                        ("ss_linear_attn_update", LinearAttnUpdateArgs), ("ss_delta_rule_fwd", DeltaRuleArgs),
+                        ("ss_delta_rule_bwd", DeltaRuleBwdArgs), ("ss_delta_rule_update", DeltaRuleUpdateArgs)):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(T), _p]
             fn.restype = ctypes.c_int

@@ -1,0 +1,403 @@
+// The gated delta rule on gfx950: the launches of a prompt or a training step
+// (kernels in delta_rule_chunk.hpp), and the recurrence for one token.
+//
+// A pass is two launches, the chunks' inverses and the walk over the chunks; the
+// backward is the walk back and the gradients of all chunks side by side.  A walk is
+// serial along a row, so with few rows it is cut into segments that run side by side:
+// over a segment a state S becomes M S + N, with M and N the same walk's result from the
+// identity and from zero; they are joined along the row (dr_join), and each
+// segment is then walked from the state it starts with.  Back, dS becomes M^T dS + N'.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "bf16_terms.hpp"
+#include "delta_rule.hpp"
+#include "norm_rows.hpp"
+#include "ops_kernels.hpp"
+#include "ss_device.hpp"
+
+namespace ss {
+
+namespace {
+
+using namespace la;
+
+// The states that the segments start from, in place of their own: S <- M S + N along the
+// row (REV: M^T, from the last segment on).  A wave 16 value columns, which do not meet.
+template <int KP, bool REV>
+__global__ __launch_bounds__(256) void dr_join(const DrParams p) {
+    constexpr int NS = KP / 16, NK = KP / 32;
+    const int lane = int(threadIdx.x) & 63, g = lane >> 4, c = lane & 15;
+    const int64_t bh = blockIdx.x;
+    const int col = int(blockIdx.y) * 64 + 16 * (int(threadIdx.x) >> 6) + c, Kp = dr_round16(p.K);
+    if (col - c >= p.V) return;
+    f4 S[NS];
+#pragma unroll
+    for (int t = 0; t < NS; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int key = state_row(t, g, r);
+            S[t][r] = p.init && key < p.K && col < p.V ? p.init[(bh * p.K + key) * p.V + col] : 0.f;
+        }
+    for (int i = 0; i < p.segs; ++i) {
+        const int64_t s = bh * p.segs + (REV ? p.segs - 1 - i : i);
+        float* add = p.seg_add + s * p.K * p.Vp + col;
+        const float* mul = p.seg_mul + s * p.K * Kp;
+        u4 sf[NK][3];
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const f4& x = S[2 * k + (h >> 1)];
+                uint32_t t[3];
+                split<3>(x[2 * (h & 1)], x[2 * (h & 1) + 1], t);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) sf[k][n][h] = t[n];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+            f4 own;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = state_row(t, g, r);
+                own[r] = key < p.K ? add[int64_t(key) * p.Vp] : 0.f;
+                if (key < p.K) add[int64_t(key) * p.Vp] = S[t][r];
+            }
+            S[t] = own;
+        }
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+            const int row = 32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3);
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                u4 a[3];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const int from = 32 * k + 8 * g + 2 * h;
+                    float x0 = 0.f, x1 = 0.f;
+                    if (row < p.K && from < p.K) {
+                        x0 = REV ? mul[int64_t(from) * Kp + row] : mul[int64_t(row) * Kp + from];
+                        if (from + 1 < p.K) x1 = REV ? mul[int64_t(from + 1) * Kp + row] : mul[int64_t(row) * Kp + from + 1];
+                    }
+                    uint32_t w[3];
+                    split<3>(x0, x1, w);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) a[n][h] = w[n];
+                }
+                f4* const to[1] = {&S[t]};
+                mfma_terms<1, 0, 0, 3, 3, 2>(&a, &sf[k], to);
+            }
+        }
+    }
+}
+
+// The heads of a group share q and k: out[r, j, :] = sum over i of part[r, j * rep + i, :]
+template <typename T>
+__global__ __launch_bounds__(256) void dr_group_sum(const float* dq, T* outq, const float* dk, T* outk, int64_t n, int rep, int dim) {
+    const float* part = blockIdx.y ? dk : dq;
+    T* out = blockIdx.y ? outk : outq;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        const int64_t g = i / dim, c = i % dim;
+        float s = 0.f;
+        for (int r = 0; r < rep; ++r) s += part[(g * rep + r) * dim + c];
+        io<T>::store(out + i, s);
+    }
+}
+
+template <typename F>
+hipError_t for_type(int32_t dtype, F&& f) {
+    switch (dtype) {
+        case SS_F32: return f(float{});
+        case SS_BF16: return f(bf16_t{});
+        default: return f(_Float16{});
+    }
+}
+
+int terms(int32_t dtype) { return dtype == SS_F32 ? 3 : dtype == SS_BF16 ? 1 : 2; }
+
+// Rows are cut into segments where fewer than half the 256 compute units would walk, and a
+// segment keeps at least 8 chunks.
+constexpr int64_t kUnits = 256, kSegChunksMin = 8;
+
+struct Plan {
+    int64_t bh, nch, tri, state, rows, mul;      // (batch, head) pairs, chunks; floats of a chunk's inverse, a state, a chunk's rows, an M
+    int segs, seg_chunks, chunk;
+};
+Plan plan_of(const ss_delta_rule_args& a) {
+    Plan p{};
+    p.chunk = dr_chunk(a.d_key, terms(a.dtype));
+    p.bh = a.batch * a.heads;
+    p.nch = (a.seqlen + p.chunk - 1) / p.chunk;
+    const int64_t nr = p.chunk / 16, vp = dr_round16(a.d_value);
+    p.tri = nr * (nr + 1) / 2 * 256;
+    p.state = a.d_key * vp;
+    p.rows = p.chunk * vp;
+    p.mul = a.d_key * dr_round16(a.d_key);
+    const int64_t walks = p.bh * ((a.d_value + 63) / 64);
+    int64_t segs = walks > 0 ? kUnits / walks : 1;
+    if (segs > p.nch / kSegChunksMin) segs = p.nch / kSegChunksMin;
+    if (segs < 1) segs = 1;
+    const int64_t per = p.nch > 0 ? (p.nch + segs - 1) / segs : 1;
+    p.segs = p.nch > 0 ? int((p.nch + per - 1) / per) : 1;
+    p.seg_chunks = int(per);
+    return p;
+}
+
+// floats at offsets of one buffer, each part 16-byte aligned
+struct Parts {
+    int64_t bytes = 0;
+    int64_t take(int64_t floats) {
+        const int64_t at = bytes;
+        bytes += (floats * 4 + 15) / 16 * 16;
+        return at;
+    }
+};
+struct Saved { int64_t tri, states, err, mul, bytes; };
+Saved saved_of(const Plan& p) {
+    Saved s{};
+    Parts parts;
+    s.tri = parts.take(p.bh * p.nch * p.tri);
+    s.states = parts.take(p.bh * p.nch * p.state);
+    s.err = parts.take(p.bh * p.nch * p.rows);
+    s.mul = p.segs > 1 ? parts.take(p.bh * p.segs * p.mul) : 0;
+    s.bytes = parts.bytes;
+    return s;
+}
+struct FwdSpace { int64_t add, tri, mul, bytes; };
+FwdSpace fwd_space(const ss_delta_rule_args& a, const Plan& p) {
+    FwdSpace s{};
+    Parts parts;
+    if (p.segs > 1) s.add = parts.take(p.bh * p.segs * p.state);
+    if (!a.saved) {
+        s.tri = parts.take(p.bh * p.nch * p.tri);
+        if (p.segs > 1) s.mul = parts.take(p.bh * p.segs * p.mul);
+    }
+    s.bytes = parts.bytes;
+    return s;
+}
+struct BwdSpace { int64_t dstates, derr, add, dq, dk, bytes; };
+BwdSpace bwd_space(const ss_delta_rule_args& a, const Plan& p) {
+    BwdSpace s{};
+    Parts parts;
+    s.dstates = parts.take(p.bh * p.nch * p.state);
+    s.derr = parts.take(p.bh * p.nch * p.rows);
+    if (p.segs > 1) s.add = parts.take(p.bh * p.segs * p.state);
+    if (a.groups != a.heads) {
+        s.dq = parts.take(p.bh * a.seqlen * a.d_key);
+        s.dk = parts.take(p.bh * a.seqlen * a.d_key);
+    }
+    s.bytes = parts.bytes;
+    return s;
+}
+
+DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
+    DrParams p{};
+    p.B = a.batch; p.L = a.seqlen; p.H = a.heads;
+    p.K = int(a.d_key); p.V = int(a.d_value); p.Vp = dr_round16(a.d_value);
+    p.rep = int(a.heads / a.groups); p.nch = int(plan.nch);
+    p.scale = a.scale;
+    p.q = {a.q, a.q_batch_stride, a.q_len_stride, a.q_head_stride, p.rep};
+    p.k = {a.k, a.k_batch_stride, a.k_len_stride, a.k_head_stride, p.rep};
+    p.v = {a.v, a.v_batch_stride, a.v_len_stride, a.v_head_stride, 1};
+    p.g = a.g; p.g_b = a.g_batch_stride; p.g_l = a.g_len_stride; p.g_h = a.g_head_stride;
+    p.beta = a.beta; p.be_b = a.beta_batch_stride; p.be_l = a.beta_len_stride; p.be_h = a.beta_head_stride;
+    p.lens = a.lengths;
+    p.segs = plan.segs; p.seg_chunks = plan.seg_chunks;
+    return p;
+}
+
+float* at(void* base, int64_t bytes) { return reinterpret_cast<float*>(static_cast<char*>(base) + bytes); }
+
+// the walk, of segments side by side after what they start from
+hipError_t walk(int32_t dtype, DrParams p, bool rev, hipStream_t stream) {
+    const auto launch = [&](const DrParams& q) {
+        return for_type(dtype, [&](auto t) { return dr_walk_launch<decltype(t)>(q, rev, stream); });
+    };
+    if (p.segs > 1) {
+        DrParams own = p;
+        own.local = 1;
+        hipError_t e = launch(own);
+        if (e != hipSuccess) return e;
+        const dim3 grid(unsigned(p.B * p.H), unsigned(p.V + 63) / 64);
+        const auto join = [&](auto kp) {
+            constexpr int KP = decltype(kp)::value;
+            if (rev) hipLaunchKernelGGL((dr_join<KP, true>), grid, dim3(256), 0, stream, p);
+            else hipLaunchKernelGGL((dr_join<KP, false>), grid, dim3(256), 0, stream, p);
+            return hipGetLastError();
+        };
+        const int64_t kp = dr_keys(p.K);
+        e = kp == 64 ? join(std::integral_constant<int, 64>{}) : kp == 128 ? join(std::integral_constant<int, 128>{})
+                                                                          : join(std::integral_constant<int, 256>{});
+        if (e != hipSuccess) return e;
+    }
+    return launch(p);
+}
+
+}  // namespace
+
+int64_t delta_rule_chunks(const ss_delta_rule_args* a) {
+    const Plan p = plan_of(*a);
+    return p.bh * p.nch;
+}
+int64_t delta_rule_saved_bytes(const ss_delta_rule_args* a) { return saved_of(plan_of(*a)).bytes; }
+int64_t delta_rule_fwd_space(const ss_delta_rule_args* a) { return fwd_space(*a, plan_of(*a)).bytes; }
+int64_t delta_rule_bwd_space(const ss_delta_rule_bwd_args* g) { return bwd_space(g->f, plan_of(g->f)).bytes; }
+
+hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream) {
+    const Plan plan = plan_of(*a);
+    const FwdSpace sp = fwd_space(*a, plan);
+    const Saved sv = saved_of(plan);
+    DrParams p = params_of(*a, plan);
+    p.o = {a->out, a->out_batch_stride, a->out_len_stride, a->out_head_stride, 1};
+    p.init = a->initial_state; p.last = a->last_state;
+    p.seg_add = at(a->workspace, sp.add);
+    if (a->saved) {
+        p.tri = at(a->saved, sv.tri); p.states = at(a->saved, sv.states); p.err = at(a->saved, sv.err);
+        p.seg_mul = at(a->saved, sv.mul);
+    } else {
+        p.tri = at(a->workspace, sp.tri);
+        p.seg_mul = at(a->workspace, sp.mul);
+    }
+    if (plan.nch > 0) {
+        const hipError_t e = for_type(a->dtype, [&](auto t) { return dr_prep_launch<decltype(t)>(p, stream); });
+        if (e != hipSuccess) return e;
+    }
+    return walk(a->dtype, p, false, stream);
+}
+
+hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t stream) {
+    const ss_delta_rule_args& a = g->f;
+    const Plan plan = plan_of(a);
+    const BwdSpace sp = bwd_space(a, plan);
+    const Saved sv = saved_of(plan);
+    DrParams p = params_of(a, plan);
+    p.o = {g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1};
+    p.init = g->dlast_state; p.last = g->dinitial_state;
+    p.tri = at(a.saved, sv.tri); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = at(a.saved, sv.mul);
+    p.dstates = at(a.workspace, sp.dstates); p.derr = at(a.workspace, sp.derr); p.seg_add = at(a.workspace, sp.add);
+    hipError_t e = walk(a.dtype, p, true, stream);
+    if (e != hipSuccess || plan.nch == 0) return e;
+    const bool part = p.rep > 1;
+    p.dq = part ? at(a.workspace, sp.dq) : g->dq; p.dk = part ? at(a.workspace, sp.dk) : g->dk; p.dv = g->dv;
+    p.dg = g->dg; p.dbeta = g->dbeta;
+    e = for_type(a.dtype, [&](auto t) { return dr_grads_launch<decltype(t)>(p, stream); });
+    if (e != hipSuccess || !part) return e;
+    return for_type(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        const int64_t n = a.batch * a.seqlen * a.groups * a.d_key, want = (n + 255) / 256;
+        hipLaunchKernelGGL((dr_group_sum<T>), dim3(unsigned(want < 65536 ? want : 65536), 2), dim3(256), 0, stream,
+                           static_cast<const float*>(p.dq), static_cast<T*>(g->dq), static_cast<const float*>(p.dk),
+                           static_cast<T*>(g->dk), n, p.rep, p.K);
+        return hipGetLastError();
+    });
+}
+
+namespace {
+
+// One token.  With the state S before it, u = beta (v - a S^T k) and
+// q^T (a S + k u^T) = a S^T q + (q . k) u, so both sums over the state's rows are taken
+// together and the state is read once: bound by its bytes.  A workgroup owns 64 value
+// columns of one (batch, head); thread (i, c) holds 4 neighbouring columns (1 where rows are not
+// 16-byte aligned) of up to RPT rows i, i + RG ... in registers.
+template <typename T, int RPT, bool VEC>
+__global__ __launch_bounds__(256) void dr_update(const ss_delta_rule_update_args a) {
+    constexpr int W = VEC ? 4 : 1, CT = 64 / W, RG = 256 / CT;
+    const int64_t bh = blockIdx.x, b = bh / a.heads, h = bh % a.heads, j = h / (a.heads / a.groups);
+    const int tid = int(threadIdx.x), c = tid % CT, rg = tid / CT, n = int(blockIdx.y) * 64 + c * W;
+    const int K = int(a.d_key), V = int(a.d_value);
+    __shared__ float qs[256], ks[256];
+    __shared__ __attribute__((aligned(16))) float redk[4][64], redq[4][64], redqk[4];
+    float* S = a.state + b * a.state_batch_stride + h * a.state_head_stride;
+    float s[RPT][W];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int d = rg + i * RG;
+        const bool in = d < K && n < V;
+        if constexpr (VEC) {
+            const float4 t = in ? *reinterpret_cast<const float4*>(S + int64_t(d) * V + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+            s[i][0] = t.x; s[i][1] = t.y; s[i][2] = t.z; s[i][3] = t.w;
+        } else {
+            s[i][0] = in ? S[int64_t(d) * V + n] : 0.f;
+        }
+    }
+    qs[tid] = tid < K ? io<T>::load(static_cast<const T*>(a.q) + b * a.q_batch_stride + j * a.q_head_stride + tid) : 0.f;
+    ks[tid] = tid < K ? io<T>::load(static_cast<const T*>(a.k) + b * a.k_batch_stride + j * a.k_head_stride + tid) : 0.f;
+    const float dec = expf(a.g[b * a.g_batch_stride + h * a.g_head_stride]), beta = a.beta[b * a.beta_batch_stride + h * a.beta_head_stride];
+    float v[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        v[w] = n + w < V ? io<T>::load(static_cast<const T*>(a.v) + b * a.v_batch_stride + h * a.v_head_stride + n + w) : 0.f;
+    __syncthreads();
+    // a wave's 64 lanes: CT columns (or all 64) by 64 / CT rows
+    float kS[W] = {}, qS[W] = {};
+    const float qk = lanes_sum<64>(qs[tid] * ks[tid]);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int d = rg + i * RG;
+        const float kd = d < K ? ks[d] : 0.f, qd = d < K ? qs[d] : 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            s[i][w] *= dec;
+            kS[w] = __builtin_fmaf(kd, s[i][w], kS[w]);
+            qS[w] = __builtin_fmaf(qd, s[i][w], qS[w]);
+        }
+    }
+    const int wave = tid >> 6, lane = tid & 63;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        if constexpr (VEC) {
+            kS[w] += __shfl_xor(kS[w], 16, 64); kS[w] += __shfl_xor(kS[w], 32, 64);
+            qS[w] += __shfl_xor(qS[w], 16, 64); qS[w] += __shfl_xor(qS[w], 32, 64);
+        }
+        if (!VEC || lane < 16) {
+            redk[wave][c * W + w] = kS[w];
+            redq[wave][c * W + w] = qS[w];
+        }
+    }
+    if (lane == 0) redqk[wave] = qk;
+    __syncthreads();
+    const float dot = (redqk[0] + redqk[1]) + (redqk[2] + redqk[3]);
+    float u[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const int m = c * W + w;
+        const float kx = (redk[0][m] + redk[1][m]) + (redk[2][m] + redk[3][m]), qx = (redq[0][m] + redq[1][m]) + (redq[2][m] + redq[3][m]);
+        u[w] = beta * (v[w] - kx);
+        if (rg == 0 && n + w < V)
+            io<T>::store(static_cast<T*>(a.out) + b * a.out_batch_stride + h * a.out_head_stride + n + w, a.scale * __builtin_fmaf(dot, u[w], qx));
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const int d = rg + i * RG;
+        if (d >= K || n >= V) continue;
+        const float kd = ks[d];
+#pragma unroll
+        for (int w = 0; w < W; ++w) s[i][w] = __builtin_fmaf(kd, u[w], s[i][w]);
+        if constexpr (VEC) *reinterpret_cast<float4*>(S + int64_t(d) * V + n) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+        else S[int64_t(d) * V + n] = s[i][0];
+    }
+}
+
+template <typename T>
+hipError_t update_t(const ss_delta_rule_update_args* a, hipStream_t stream) {
+    const bool vec = a->d_value % 4 == 0 && a->state_batch_stride % 4 == 0 && a->state_head_stride % 4 == 0 &&
+                     (reinterpret_cast<uintptr_t>(a->state) & 15) == 0;
+    const dim3 grid(unsigned(a->batch * a->heads), unsigned(a->d_value + 63) / 64);
+    if (vec && a->d_key <= 64) hipLaunchKernelGGL((dr_update<T, 4, true>), grid, dim3(256), 0, stream, *a);
+    else if (vec && a->d_key <= 128) hipLaunchKernelGGL((dr_update<T, 8, true>), grid, dim3(256), 0, stream, *a);
+    else if (vec) hipLaunchKernelGGL((dr_update<T, 16, true>), grid, dim3(256), 0, stream, *a);
+    else if (a->d_key <= 128) hipLaunchKernelGGL((dr_update<T, 32, false>), grid, dim3(256), 0, stream, *a);
+    else hipLaunchKernelGGL((dr_update<T, 64, false>), grid, dim3(256), 0, stream, *a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t delta_rule_update_launch(const ss_delta_rule_update_args* a, hipStream_t stream) {
+    return for_type(a->dtype, [&](auto t) { return update_t<decltype(t)>(a, stream); });
+}
+
+}  // namespace ss

@@ -1,0 +1,54 @@
+// The gated delta rule: what its host and device sides share.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/mamba_ss.h"
+#include "linear_attn.hpp"
+
+namespace ss {
+
+// Key columns of the kernels' tiles, and tokens a chunk: the backward's tiles of
+// a chunk (q, k and 64 value columns of dout, the errors and their gradients in 3 terms)
+// fit the 160 KB of LDS.  terms: bf16 terms of a row's element (bf16 1, fp16 2, fp32 3).
+constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
+constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 ? 64 : 32; }
+constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
+
+// Per (batch, head) pair and chunk, what the kernels hand on (fp32):
+//   tri     the lower 16 x 16 tiles of the chunk's triangular inverse, tile (i, j) at i (i + 1) / 2 + j, row-major
+//   states  the state before the chunk, (K, Vp)
+//   err     the tokens' prediction errors, (chunk, Vp)
+//   dstates the gradient of the state after the chunk;  derr: of the errors, as err
+// Vp: value columns rounded up to 16, zero past the last.
+struct DrParams {
+    int64_t B, L, H;
+    int K, V, Vp, rep, nch;               // rep: heads per group; nch: chunks of a row of L tokens
+    float scale;
+    LaRows q, k, v, o;                    // o: out, or the backward's dout
+    const float* g; int64_t g_b, g_l, g_h;
+    const float* beta; int64_t be_b, be_l, be_h;
+    const int32_t* lens;
+    const float* init; float* last;       // (B, H, K, V) before and after the walk (backward: dlast, dinitial), or null
+    float* tri;
+    float* states;                        // null: not kept
+    float* err;
+    float* dstates;
+    float* derr;
+    // a row's segments of seg_chunks chunks side by side (segs 1: the whole row)
+    int segs, seg_chunks;
+    int local;                            // the segments' own states from zero and what becomes of a state over one
+    float* seg_add;                       // (B, H, segs, K, Vp): their states; then the states that they start from
+    float* seg_mul;                       // (B, H, segs, K, Kp): over a segment S becomes seg_mul S + its own; Kp: K rounded up to 16
+    // gradients
+    void* dq; void* dk; void* dv;         // contiguous; dq and dk in fp32 per head with rep > 1
+    float* dg; float* dbeta;              // (B, L, H)
+};
+
+// The chunks' triangular inverses; the walk over the chunks, forward or (rev) back; the gradients.
+template <typename T> hipError_t dr_prep_launch(const DrParams& p, hipStream_t stream);
+template <typename T> hipError_t dr_walk_launch(const DrParams& p, bool rev, hipStream_t stream);
+template <typename T> hipError_t dr_grads_launch(const DrParams& p, hipStream_t stream);
+
+}  // namespace ss

@@ -934,6 +934,220 @@ Tensor lin_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const
     return *out;
 }
 
+// -------------------------------------------------------- gated delta rule --
+constexpr const char* kDelta = "delta_rule";
+
+// a factor per token and head (g, beta) as the library reads it: fp32
+Tensor per_token(const char* what, const char* name, const Tensor& t, at::IntArrayRef shape, const Tensor& v) {
+    on_device(what, name, t, v.device());
+    REQUIRE(what, t.scalar_type() == at::kFloat || t.scalar_type() == v.scalar_type(),
+            std::string(name) + " has dtype " + dtype_str(t.scalar_type()) + ", expected float32 or v's");
+    REQUIRE(what, t.sizes() == shape, std::string(name) + " has shape " + shape_str(t.sizes()) + ", expected " + shape_str(shape));
+    return t.to(at::kFloat);
+}
+Tensor delta_state(const char* name, const Tensor& t, at::IntArrayRef shape, const at::Device& dev) {
+    on_device(kDelta, name, t, dev);
+    of_type(kDelta, name, t, at::kFloat);
+    REQUIRE(kDelta, t.sizes() == shape, std::string(name) + " has shape " + shape_str(t.sizes()) + ", expected " + shape_str(shape));
+    return t.contiguous();
+}
+
+struct DeltaIn { Tensor q, k, v, g, beta; OptT initial, lengths; };
+
+DeltaIn fill_delta(ss_delta_rule_args& a, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& beta_,
+                   const OptT& initial, const OptT& lengths, double scale) {
+    a = ss_delta_rule_args{};
+    REQUIRE(kDelta, v_.dim() == 4, "v must be (batch, seqlen, heads, d_value), got shape " + shape_str(v_.sizes()));
+    const at::Device dev = v_.device();
+    REQUIRE(kDelta, dev.is_cuda(), "tensors must be on a ROCm GPU device (no CPU path)");
+    REQUIRE(kDelta, itype_of(v_.scalar_type(), &a.dtype), "unsupported dtype " + dtype_str(v_.scalar_type()));
+    const int64_t B = v_.size(0), L = v_.size(1), H = v_.size(2), V = v_.size(3);
+    REQUIRE(kDelta, q_.dim() == 4 && q_.size(0) == B && q_.size(1) == L,
+            "q must be (batch, seqlen, groups, d_key), got shape " + shape_str(q_.sizes()));
+    REQUIRE(kDelta, k_.sizes() == q_.sizes(), "k has shape " + shape_str(k_.sizes()) + ", expected " + shape_str(q_.sizes()));
+    const int64_t G = q_.size(2), K = q_.size(3);
+    REQUIRE(kDelta, H == 0 || (G > 0 && H % G == 0),
+            "heads " + std::to_string(H) + " is not a multiple of groups " + std::to_string(G));
+    on_device(kDelta, "q", q_, dev); on_device(kDelta, "k", k_, dev);
+    of_type(kDelta, "q", q_, v_.scalar_type()); of_type(kDelta, "k", k_, v_.scalar_type());
+    DeltaIn in{seq_unit(q_), seq_unit(k_), seq_unit(v_), per_token(kDelta, "g", g_, {B, L, H}, v_),
+               per_token(kDelta, "beta", beta_, {B, L, H}, v_), {}, {}};
+    if (initial) in.initial = delta_state("initial_state", *initial, {B, H, K, V}, dev);
+    if (lengths) {
+        on_device(kDelta, "lengths", *lengths, dev);
+        REQUIRE(kDelta, same_shape(*lengths, {B}) && (lengths->scalar_type() == at::kInt || lengths->scalar_type() == at::kLong),
+                "lengths must be a (batch,) integer tensor, got " + shape_str(lengths->sizes()) + " " + dtype_str(lengths->scalar_type()));
+        in.lengths = (lengths->scalar_type() == at::kInt ? *lengths : lengths->clamp(0, L).to(at::kInt)).contiguous();
+    }
+    a.batch = B; a.seqlen = L; a.heads = H; a.groups = G; a.d_key = K; a.d_value = V;
+    a.scale = float(scale);
+    a.q_batch_stride = in.q.stride(0); a.q_len_stride = in.q.stride(1); a.q_head_stride = in.q.stride(2);
+    a.k_batch_stride = in.k.stride(0); a.k_len_stride = in.k.stride(1); a.k_head_stride = in.k.stride(2);
+    a.v_batch_stride = in.v.stride(0); a.v_len_stride = in.v.stride(1); a.v_head_stride = in.v.stride(2);
+    a.g_batch_stride = in.g.stride(0); a.g_len_stride = in.g.stride(1); a.g_head_stride = in.g.stride(2);
+    a.beta_batch_stride = in.beta.stride(0); a.beta_len_stride = in.beta.stride(1); a.beta_head_stride = in.beta.stride(2);
+    a.q = ptr(in.q); a.k = ptr(in.k); a.v = ptr(in.v); a.g = static_cast<float*>(ptr(in.g)); a.beta = static_cast<float*>(ptr(in.beta));
+    a.initial_state = fptr<float>(in.initial); a.lengths = fptr<int32_t>(in.lengths);
+    return in;
+}
+
+struct DeltaOut { Tensor out; OptT last, saved; DeltaIn in; };     // in: the tensors as read
+DeltaOut delta_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const OptT& initial,
+                   const OptT& lengths, double scale, bool want_last, bool need, void* stream) {
+    ss_delta_rule_args a;
+    const DeltaIn in = fill_delta(a, q, k, v, g, beta, initial, lengths, scale);
+    const Tensor out = at::empty({a.batch, a.seqlen, a.heads, a.d_value}, in.v.options());
+    OptT last, saved, ws;
+    if (want_last) last = f32_like({a.batch, a.heads, a.d_key, a.d_value}, in.v);
+    a.out_batch_stride = out.stride(0); a.out_len_stride = out.stride(1); a.out_head_stride = out.stride(2);
+    a.out = ptr(out); a.last_state = fptr<float>(last);
+    if (need) {
+        const int64_t n = ss_delta_rule_saved_bytes(&a);
+        if (n < 0) check(SS_ERR_INVALID, kDelta);
+        saved = bytes_on(n, in.v);
+        a.saved = ptr(*saved); a.saved_bytes = n;
+    }
+    const int64_t n = ss_delta_rule_fwd_workspace_bytes(&a);
+    if (n < 0) check(SS_ERR_INVALID, kDelta);
+    if (n > 0) {
+        ws = bytes_on(n, in.v);
+        a.workspace = ptr(*ws); a.workspace_bytes = n;
+    }
+    launch(in.v.device(), "delta_rule forward", [&] { return ss_delta_rule_fwd(&a, stream); });
+    return {out, last, saved, in};
+}
+
+struct DeltaGrads { Tensor dq, dk, dv, dg, dbeta; OptT dinitial; };    // dg, dbeta: fp32
+DeltaGrads delta_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const OptT& initial,
+                     const OptT& lengths, const Tensor& saved, double scale, const Tensor& dout_, const OptT& dlast_,
+                     bool want_dinitial, void* stream) {
+    ss_delta_rule_bwd_args b{};
+    const DeltaIn in = fill_delta(b.f, q, k, v, g, beta, initial, lengths, scale);
+    const ss_delta_rule_args& a = b.f;
+    const at::Device dev = in.v.device();
+    REQUIRE(kDelta, dout_.sizes() == in.v.sizes() && dout_.scalar_type() == in.v.scalar_type() && dout_.device() == dev,
+            "dout must match v, got " + shape_str(dout_.sizes()) + " " + dtype_str(dout_.scalar_type()));
+    const Tensor dout = seq_unit(dout_);
+    OptT dlast, dinitial, ws;
+    if (dlast_) dlast = delta_state("dlast_state", *dlast_, {a.batch, a.heads, a.d_key, a.d_value}, dev);
+    if (want_dinitial) dinitial = f32_like({a.batch, a.heads, a.d_key, a.d_value}, in.v);
+    const Tensor dq = at::empty(in.q.sizes(), in.q.options()), dk = at::empty(in.q.sizes(), in.q.options()),
+                 dv = at::empty(in.v.sizes(), in.v.options());
+    const Tensor dg = f32_like({a.batch, a.seqlen, a.heads}, in.v), dbeta = f32_like({a.batch, a.seqlen, a.heads}, in.v);
+    if (a.heads == 0) {                                // (q and k reach no output)
+        dq.zero_();
+        dk.zero_();
+    }
+    b.f.saved = ptr(saved); b.f.saved_bytes = saved.numel();
+    b.dout_batch_stride = dout.stride(0); b.dout_len_stride = dout.stride(1); b.dout_head_stride = dout.stride(2);
+    b.dout = ptr(dout); b.dlast_state = fptr<float>(dlast);
+    b.dq = ptr(dq); b.dk = ptr(dk); b.dv = ptr(dv);
+    b.dg = static_cast<float*>(ptr(dg)); b.dbeta = static_cast<float*>(ptr(dbeta)); b.dinitial_state = fptr<float>(dinitial);
+    if (a.batch > 0 && a.heads > 0) {
+        const int64_t n = ss_delta_rule_bwd_workspace_bytes(&b);
+        if (n < 0) check(SS_ERR_INVALID, kDelta);
+        if (n > 0) {
+            ws = bytes_on(n, in.v);
+            b.f.workspace = ptr(*ws); b.f.workspace_bytes = n;
+        }
+        launch(dev, "delta_rule backward", [&] { return ss_delta_rule_bwd(&b, stream); });
+    }
+    return {dq, dk, dv, dg, dbeta, dinitial};
+}
+
+struct DeltaRule : torch::autograd::Function<DeltaRule> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                 const Tensor& beta, const OptT& initial, const OptT& lengths, double scale, bool want_last) {
+        void* const stream = current_stream(v.device());
+        const DeltaOut r = delta_fwd(q, k, v, g, beta, initial, lengths, scale, want_last, true, stream);
+        ctx->saved_data["stream"] = reinterpret_cast<int64_t>(stream);
+        ctx->save_for_backward({r.in.q, r.in.k, r.in.v, r.in.g, r.in.beta, given(r.in.initial), given(r.in.lengths), *r.saved});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["types"] = std::vector<int64_t>{int64_t(g.scalar_type()), int64_t(beta.scalar_type())};
+        ctx->set_materialize_grads(false);
+        variable_list out{r.out};
+        if (want_last) out.push_back(*r.last);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list r(9);
+        const Tensor dlast = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grads[0].defined() && !dlast.defined()) return r;
+        const auto t = ctx->get_saved_variables();
+        const Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(t[2]);
+        const bool has_initial = t[5].defined();
+        const DeltaGrads d = delta_bwd(t[0], t[1], t[2], t[3], t[4], maybe(t[5]), maybe(t[6]), t[7], ctx->saved_data["scale"].toDouble(),
+                                       dout, maybe(dlast), has_initial && ctx->needs_input_grad(5), node_stream(ctx));
+        const auto types = ctx->saved_data["types"].toIntVector();
+        if (ctx->needs_input_grad(0)) r[0] = d.dq;
+        if (ctx->needs_input_grad(1)) r[1] = d.dk;
+        if (ctx->needs_input_grad(2)) r[2] = d.dv;
+        if (ctx->needs_input_grad(3)) r[3] = d.dg.to(at::ScalarType(types[0]));
+        if (ctx->needs_input_grad(4)) r[4] = d.dbeta.to(at::ScalarType(types[1]));
+        r[5] = given(d.dinitial);
+        return final_grads(kDelta, r);
+    }
+};
+// (out, last_state or None)
+py::tuple delta_rule(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const OptT& initial,
+                     const OptT& lengths, double scale, bool want_last) {
+    no_tangents(kDelta, {&q, &k, &v, &g, &beta, at_opt(initial)});
+    if (!wants_grad({&q, &k, &v, &g, &beta, at_opt(initial)})) {
+        const DeltaOut r = delta_fwd(q, k, v, g, beta, initial, lengths, scale, want_last, false, current_stream(v.device()));
+        return py::make_tuple(r.out, r.last);
+    }
+    const variable_list r = DeltaRule::apply(q, k, v, g, beta, initial, lengths, scale, want_last);
+    return py::make_tuple(r[0], want_last ? OptT(r[1]) : OptT());
+}
+
+constexpr const char* kDeltaUp = "delta_rule_update";
+
+Tensor delta_update(const Tensor& state, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& beta_,
+                    double scale, OptT out, int64_t stream) {
+    REQUIRE(kDeltaUp, v_.dim() == 3 && v_.is_cuda(), "v must be (batch, heads, d_value) on a ROCm GPU device (no CPU path)");
+    ss_delta_rule_update_args a{};
+    REQUIRE(kDeltaUp, itype_of(v_.scalar_type(), &a.dtype), "unsupported dtype " + dtype_str(v_.scalar_type()));
+    const at::Device dev = v_.device();
+    const int64_t B = v_.size(0), H = v_.size(1), V = v_.size(2);
+    REQUIRE(kDeltaUp, q_.dim() == 3 && q_.size(0) == B, "q must be (batch, groups, d_key), got shape " + shape_str(q_.sizes()));
+    REQUIRE(kDeltaUp, k_.sizes() == q_.sizes(), "k has shape " + shape_str(k_.sizes()) + ", expected " + shape_str(q_.sizes()));
+    const int64_t G = q_.size(1), K = q_.size(2);
+    REQUIRE(kDeltaUp, H == 0 || (G > 0 && H % G == 0),
+            "heads " + std::to_string(H) + " is not a multiple of groups " + std::to_string(G));
+    no_tangents(kDeltaUp, {&state, &q_, &k_, &v_, &g_, &beta_});
+    REQUIRE(kDeltaUp, !wants_grad({&state, &q_, &k_, &v_, &g_, &beta_}),
+            "a token's update has no backward; call it under torch.no_grad(), or delta_rule_fn for gradients");
+    on_device(kDeltaUp, "q", q_, dev); on_device(kDeltaUp, "k", k_, dev); on_device(kDeltaUp, "state", state, dev);
+    of_type(kDeltaUp, "q", q_, v_.scalar_type()); of_type(kDeltaUp, "k", k_, v_.scalar_type());
+    of_type(kDeltaUp, "state", state, at::kFloat);
+    REQUIRE(kDeltaUp, same_shape(state, {B, H, K, V}),
+            "state has shape " + shape_str(state.sizes()) + ", expected " + shape_str({B, H, K, V}));
+    REQUIRE(kDeltaUp, state.numel() == 0 || ((V <= 1 || state.stride(3) == 1) && (K <= 1 || state.stride(2) == V)),
+            "state must be contiguous along its last two dims (it is updated in place)");
+    const Tensor q = seq_unit(q_), k = seq_unit(k_), v = seq_unit(v_), g = per_token(kDeltaUp, "g", g_, {B, H}, v_),
+                 beta = per_token(kDeltaUp, "beta", beta_, {B, H}, v_);
+    const bool own_out = out.has_value();
+    if (own_out)
+        REQUIRE(kDeltaUp, out->sizes() == v.sizes() && out->scalar_type() == v.scalar_type() && out->device() == dev && unit(*out),
+                "out must match v, with unit stride along the last dim");
+    else out = at::empty({B, H, V}, v.options());
+    a.batch = B; a.heads = H; a.groups = G; a.d_key = K; a.d_value = V;
+    a.scale = float(scale);
+    a.state_batch_stride = state.stride(0); a.state_head_stride = state.stride(1);
+    a.q_batch_stride = q.stride(0); a.q_head_stride = q.stride(1);
+    a.k_batch_stride = k.stride(0); a.k_head_stride = k.stride(1);
+    a.v_batch_stride = v.stride(0); a.v_head_stride = v.stride(1);
+    a.out_batch_stride = out->stride(0); a.out_head_stride = out->stride(1);
+    a.g_batch_stride = g.stride(0); a.g_head_stride = g.stride(1);
+    a.beta_batch_stride = beta.stride(0); a.beta_head_stride = beta.stride(1);
+    a.state = static_cast<float*>(ptr(state)); a.q = ptr(q); a.k = ptr(k); a.v = ptr(v);
+    a.g = static_cast<float*>(ptr(g)); a.beta = static_cast<float*>(ptr(beta)); a.out = ptr(*out);
+    launch(dev, kDeltaUp, [&] { return ss_delta_rule_update(&a, reinterpret_cast<void*>(stream)); });
+    written(state);
+    if (own_out) written(*out);
+    return *out;
+}
+
 // ------------------------------------------------------------ block norms --
 constexpr const char* kBlockNorm = "block_norm";
 constexpr const char* kGatedNorm = "gated_rms_norm";
@@ -1232,6 +1446,8 @@ PYBIND11_MODULE(mamba_host, m) {
     m.def("state_update", &state_update);
     m.def("linear_attn", &linear_attn);
     m.def("lin_update", &lin_update);
+    m.def("delta_rule", &delta_rule);
+    m.def("delta_update", &delta_update);
     m.def("block_norm", &block_norm);
     m.def("gated_norm", &gated_norm);
     m.def("clip_grads", &clip_grads);

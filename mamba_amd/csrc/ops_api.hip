@@ -143,6 +143,144 @@ int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream) {
     return ok();
 }
 
+// Checks shared by the delta rule's calls.
+static int check_delta_rule(const ss_delta_rule_args* a, bool bwd) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    const int64_t sizes[] = {a->batch, a->seqlen, a->heads, a->groups};
+    for (int64_t n : sizes)
+        if (n < 0)
+            return fail(SS_ERR_INVALID, "negative size (batch=%lld seqlen=%lld heads=%lld groups=%lld)", (long long)a->batch,
+                        (long long)a->seqlen, (long long)a->heads, (long long)a->groups);
+    if (a->dtype != SS_F32 && a->dtype != SS_BF16 && a->dtype != SS_F16)
+        return fail(SS_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->d_key < 1 || a->d_key > ss::kDeltaRuleMaxDim || a->d_value < 1 || a->d_value > ss::kDeltaRuleMaxDim)
+        return fail(SS_ERR_UNSUPPORTED, "d_key=%lld, d_value=%lld outside [1, %lld]", (long long)a->d_key,
+                    (long long)a->d_value, (long long)ss::kDeltaRuleMaxDim);
+    if (a->heads > 0 && (a->groups < 1 || a->heads % a->groups != 0))
+        return fail(SS_ERR_INVALID, "heads=%lld is not a multiple of groups=%lld", (long long)a->heads, (long long)a->groups);
+    if (a->batch > 0 && a->heads > ss::kLinearAttnMaxRows / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
+    if (a->seqlen > (int64_t(1) << 24)) return fail(SS_ERR_UNSUPPORTED, "seqlen=%lld above 2^24", (long long)a->seqlen);
+    if (a->batch > 0 && a->heads > 0 && ss::delta_rule_chunks(a) > ss::kDeltaRuleMaxChunks)
+        return fail(SS_ERR_UNSUPPORTED, "batch * heads * seqlen too large");
+    const int64_t st[] = {a->q_batch_stride, a->q_len_stride, a->q_head_stride, a->k_batch_stride, a->k_len_stride,
+                          a->k_head_stride, a->v_batch_stride, a->v_len_stride, a->v_head_stride, a->g_batch_stride,
+                          a->g_len_stride, a->g_head_stride, a->beta_batch_stride, a->beta_len_stride, a->beta_head_stride};
+    for (int64_t v : st)
+        if (v < 0) return fail(SS_ERR_INVALID, "negative stride");
+    if (a->batch == 0 || a->heads == 0) return ok();
+    const size_t es = elem_size(a->dtype);
+    if (a->seqlen > 0) {
+        if (!a->q || !a->k || !a->v || !a->g || !a->beta) return fail(SS_ERR_INVALID, "q / k / v / g / beta is NULL");
+        if (!aligned(a->q, es) || !aligned(a->k, es) || !aligned(a->v, es) || !aligned(a->g, 4) || !aligned(a->beta, 4))
+            return fail(SS_ERR_INVALID, "q / k / v / g / beta is misaligned");
+    }
+    if (!aligned(a->initial_state, 4) || !aligned(a->lengths, 4)) return fail(SS_ERR_INVALID, "initial_state / lengths is misaligned");
+    if (!bwd) {
+        if (a->out_batch_stride < 0 || a->out_len_stride < 0 || a->out_head_stride < 0)
+            return fail(SS_ERR_INVALID, "negative stride");
+        if (a->seqlen > 0 && !a->out) return fail(SS_ERR_INVALID, "out is NULL");
+        if (!aligned(a->out, es) || !aligned(a->last_state, 4))
+            return fail(SS_ERR_INVALID, "out / last_state is misaligned");
+    }
+    return ok();
+}
+
+static int check_delta_rule_bwd(const ss_delta_rule_bwd_args* g) {
+    const int rc = check_delta_rule(g ? &g->f : nullptr, true);
+    if (rc != SS_OK || g->f.batch == 0 || g->f.heads == 0) return rc;
+    if (g->dout_batch_stride < 0 || g->dout_len_stride < 0 || g->dout_head_stride < 0)
+        return fail(SS_ERR_INVALID, "negative stride");
+    if (g->f.seqlen > 0 && (!g->dout || !g->dq || !g->dk || !g->dv || !g->dg || !g->dbeta))
+        return fail(SS_ERR_INVALID, "dout / dq / dk / dv / dg / dbeta is NULL");
+    const size_t es = elem_size(g->f.dtype);
+    if (!aligned(g->dout, es) || !aligned(g->dq, es) || !aligned(g->dk, es) || !aligned(g->dv, es) ||
+        !aligned(g->dg, 4) || !aligned(g->dbeta, 4) || !aligned(g->dlast_state, 4) || !aligned(g->dinitial_state, 4))
+        return fail(SS_ERR_INVALID, "a gradient is misaligned");
+    return ok();
+}
+
+// what the forward keeps for the backward
+static int check_saved(const ss_delta_rule_args* a, bool need) {
+    const int64_t n = ss::delta_rule_saved_bytes(a);
+    if ((need && n > 0 && !a->saved) || (a->saved && a->saved_bytes < n))
+        return fail(SS_ERR_INVALID, "saved of %lld bytes needed (got %lld)", (long long)n, (long long)(a->saved ? a->saved_bytes : 0));
+    if (!aligned(a->saved, 16)) return fail(SS_ERR_INVALID, "saved must be 16-byte aligned");
+    return SS_OK;
+}
+
+int64_t ss_delta_rule_saved_bytes(const ss_delta_rule_args* a) {
+    if (check_delta_rule(a, true) != SS_OK) return -1;
+    return a->batch == 0 || a->heads == 0 ? 0 : ss::delta_rule_saved_bytes(a);
+}
+
+int64_t ss_delta_rule_fwd_workspace_bytes(const ss_delta_rule_args* a) {
+    if (check_delta_rule(a, false) != SS_OK) return -1;
+    return a->batch == 0 || a->heads == 0 ? 0 : ss::delta_rule_fwd_space(a);
+}
+
+int64_t ss_delta_rule_bwd_workspace_bytes(const ss_delta_rule_bwd_args* g) {
+    if (check_delta_rule_bwd(g) != SS_OK) return -1;
+    return g->f.batch == 0 || g->f.heads == 0 ? 0 : ss::delta_rule_bwd_space(g);
+}
+
+int ss_delta_rule_fwd(const ss_delta_rule_args* a, void* stream) {
+    int rc = check_delta_rule(a, false);
+    if (rc != SS_OK || a->batch == 0 || a->heads == 0) return rc;
+    rc = check_saved(a, false);
+    if (rc == SS_OK) rc = check_space(a->workspace, a->workspace_bytes, ss::delta_rule_fwd_space(a));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::delta_rule_fwd_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "delta rule forward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_delta_rule_bwd(const ss_delta_rule_bwd_args* g, void* stream) {
+    int rc = check_delta_rule_bwd(g);
+    if (rc != SS_OK || g->f.batch == 0 || g->f.heads == 0) return rc;
+    rc = check_saved(&g->f, true);
+    if (rc == SS_OK) rc = check_space(g->f.workspace, g->f.workspace_bytes, ss::delta_rule_bwd_space(g));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::delta_rule_bwd_launch(g, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "delta rule backward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_delta_rule_update(const ss_delta_rule_update_args* a, void* stream) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    if (a->batch < 0 || a->heads < 0 || a->groups < 0)
+        return fail(SS_ERR_INVALID, "negative size (batch=%lld heads=%lld groups=%lld)", (long long)a->batch,
+                    (long long)a->heads, (long long)a->groups);
+    if (a->dtype != SS_F32 && a->dtype != SS_BF16 && a->dtype != SS_F16)
+        return fail(SS_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->d_key < 1 || a->d_key > ss::kDeltaRuleMaxDim || a->d_value < 1 || a->d_value > ss::kDeltaRuleMaxDim)
+        return fail(SS_ERR_UNSUPPORTED, "d_key=%lld, d_value=%lld outside [1, %lld]", (long long)a->d_key,
+                    (long long)a->d_value, (long long)ss::kDeltaRuleMaxDim);
+    if (a->heads > 0 && (a->groups < 1 || a->heads % a->groups != 0))
+        return fail(SS_ERR_INVALID, "heads=%lld is not a multiple of groups=%lld", (long long)a->heads, (long long)a->groups);
+    if (a->batch > 0 && a->heads > ss::kLinearAttnMaxRows / a->batch) return fail(SS_ERR_UNSUPPORTED, "batch * heads too large");
+    const int64_t st[] = {a->state_batch_stride, a->state_head_stride, a->q_batch_stride, a->q_head_stride, a->k_batch_stride,
+                          a->k_head_stride, a->v_batch_stride, a->v_head_stride, a->out_batch_stride, a->out_head_stride,
+                          a->g_batch_stride, a->g_head_stride, a->beta_batch_stride, a->beta_head_stride};
+    for (int64_t v : st)
+        if (v < 0) return fail(SS_ERR_INVALID, "negative stride");
+    if (a->batch == 0 || a->heads == 0) return ok();
+    if (!a->state || !a->q || !a->k || !a->v || !a->g || !a->beta || !a->out)
+        return fail(SS_ERR_INVALID, "state / q / k / v / g / beta / out is NULL");
+    const size_t es = elem_size(a->dtype);
+    if (!aligned(a->state, 4) || !aligned(a->g, 4) || !aligned(a->beta, 4) || !aligned(a->q, es) || !aligned(a->k, es) ||
+        !aligned(a->v, es) || !aligned(a->out, es))
+        return fail(SS_ERR_INVALID, "state / q / k / v / g / beta / out is misaligned");
+    if (ss::blocks_overlap(a->batch, a->state_batch_stride, a->heads, a->state_head_stride, a->d_key * a->d_value))
+        return fail(SS_ERR_INVALID, "state's elements overlap (strides %lld, %lld): it is updated in place",
+                    (long long)a->state_batch_stride, (long long)a->state_head_stride);
+    if (ss::blocks_overlap(a->batch, a->out_batch_stride, a->heads, a->out_head_stride, a->d_value))
+        return fail(SS_ERR_INVALID, "out's elements overlap (strides %lld, %lld)", (long long)a->out_batch_stride,
+                    (long long)a->out_head_stride);
+    const hipError_t e = ss::delta_rule_update_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "delta rule update launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
 static int check_block_norm(int64_t rows, int64_t dim, int dtype, int w_dtype) {
     if (rows < 0 || dim < 0)
         return fail(SS_ERR_INVALID, "negative size (rows=%lld dim=%lld)", (long long)rows, (long long)dim);

@@ -18,6 +18,15 @@ hipError_t linear_attn_fwd_launch(const ss_linear_attn_args* a, hipStream_t stre
 hipError_t linear_attn_bwd_launch(const ss_linear_attn_bwd_args* g, hipStream_t stream);
 hipError_t linear_attn_update_launch(const ss_linear_attn_update_args* a, hipStream_t stream);
 constexpr int64_t kLinearAttnMaxDim = 256, kLinearAttnMaxRows = int64_t(1) << 20;   // rows: batch * heads
+// the gated delta rule (delta_rule.hip)
+int64_t delta_rule_saved_bytes(const ss_delta_rule_args* a);
+int64_t delta_rule_fwd_space(const ss_delta_rule_args* a);
+int64_t delta_rule_bwd_space(const ss_delta_rule_bwd_args* g);
+hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream);
+hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t stream);
+hipError_t delta_rule_update_launch(const ss_delta_rule_update_args* a, hipStream_t stream);
+int64_t delta_rule_chunks(const ss_delta_rule_args* a);             // of all rows
+constexpr int64_t kDeltaRuleMaxDim = 256, kDeltaRuleMaxChunks = (int64_t(1) << 23) - 1;   // (a launch holds 2^32 threads, a chunk up to 512)
 // the norms around a block and the gated norm of each head (block_norm.hip)
 int64_t block_norm_bwd_space(int64_t rows, int64_t dim);
 int64_t gated_norm_bwd_space(int64_t rows, int64_t dim, int64_t groups);
