@@ -6,7 +6,7 @@ gated norms of the heads, the border norms and the clipping of the gradients
 by their global norm; the answers come from prompts of different lengths and
 then one token at a time.
 
-    python examples/train_linear_attn_lm.py [--steps 300] [--symbols 8] [--length 12]
+    python examples/train_linear_attn_lm.py [--steps 300] [--symbols 8] [--length 12] [--mixer delta_rule]
 """
 import argparse
 import os
@@ -26,11 +26,13 @@ def batch_of(n, symbols, length, gen, device):
     return torch.cat([x, torch.zeros(n, 1, dtype=x.dtype, device=device), x], 1)
 
 
-def train(steps=300, symbols=8, length=12, batch=64, lr=3e-3, max_norm=1.0, seed=0, log=print, device="cuda"):
+def train(steps=300, symbols=8, length=12, batch=64, lr=3e-3, max_norm=1.0, seed=0, log=print, device="cuda",
+          mixer="linear_attn"):
     """Returns (model, losses)."""
     torch.manual_seed(seed)
     gen = torch.Generator(device=device).manual_seed(seed)
-    model = LinearAttnLM(LinearAttnLMConfig(vocab_size=symbols + 1, model_dim=64, num_layers=2, head_dim=32), device=device)
+    model = LinearAttnLM(LinearAttnLMConfig(vocab_size=symbols + 1, model_dim=64, num_layers=2, head_dim=32, mixer=mixer),
+                         device=device)
     params = list(model.parameters())
     opt = torch.optim.AdamW(params, lr=lr)
     losses = []
@@ -53,8 +55,9 @@ def main():
     ap.add_argument("--steps", type=int, default=300)
     ap.add_argument("--symbols", type=int, default=8)
     ap.add_argument("--length", type=int, default=12)
+    ap.add_argument("--mixer", choices=["linear_attn", "delta_rule"], default="linear_attn")
     a = ap.parse_args()
-    model, _ = train(a.steps, a.symbols, a.length)
+    model, _ = train(a.steps, a.symbols, a.length, mixer=a.mixer)
     gen = torch.Generator(device="cuda").manual_seed(1)
     # prompts of different lengths in one batch: symbols and the separator
     full = batch_of(4, a.symbols, a.length, gen, "cuda")

@@ -758,6 +758,65 @@ int ss_gated_norm_bwd(const ss_gated_norm_bwd_args* a, void* stream);
 int64_t ss_gated_norm_bwd_workspace_bytes(int64_t rows, int64_t dim, int64_t groups);
 
 /* ------------------------------------------------------------------------
+ * Layer norm with the residual add in front of it.  No counterpart in the reference
+ * (its norm is the RMSNorm above).  With s = x + residual, rounded to dtype (s = x when
+ * residual is NULL):
+ *   out = (s - mean(s)) * rsqrt(mean((s - mean(s))^2) + eps) * weight (+ bias)
+ * Rows of `dim` (1 to 16384) elements with unit column stride and free row
+ * strides, element type dtype; weight, bias: (dim) contiguous, w_dtype =
+ * dtype or SS_F32.  Outputs must not overlap inputs.
+ * ------------------------------------------------------------------------ */
+typedef struct ss_layer_norm_args {
+    int64_t rows, dim;
+    int32_t dtype, w_dtype;              /* enum ss_dtype */
+    float eps;
+    int32_t pad_;
+    int64_t x_row_stride, residual_row_stride, out_row_stride, residual_out_row_stride;
+    const void* x;
+    const void* residual;                /* may be NULL */
+    const void* weight;
+    const void* bias;                    /* may be NULL */
+    void* out;
+    void* residual_out;                  /* s; may be NULL (not written), ignored without residual */
+    float* stats;                        /* fp32 (rows, 2), mean and reciprocal root; may be NULL (not written); kept for the backward */
+} ss_layer_norm_args;
+
+typedef struct ss_layer_norm_bwd_args {
+    int64_t rows, dim;
+    int32_t dtype, w_dtype;
+    int64_t s_row_stride, dout_row_stride, dresidual_out_row_stride;
+    const void* s;                       /* the normalised rows */
+    const void* weight;
+    const float* stats;                  /* from the forward */
+    const void* dout;                    /* may be NULL: zero */
+    const void* dresidual_out;           /* may be NULL: zero */
+    void* dx;                            /* (rows, dim) contiguous, dtype: the gradient of x and of residual */
+    void* dweight;                       /* (dim), w_dtype, written (not accumulated); sums of a fixed order */
+    void* dbias;                         /* the same; may be NULL (not written) */
+    void* workspace;                     /* ss_layer_norm_bwd_workspace_bytes(rows, dim) bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+} ss_layer_norm_bwd_args;
+
+int ss_layer_norm_fwd(const ss_layer_norm_args* a, void* stream);
+int ss_layer_norm_bwd(const ss_layer_norm_bwd_args* a, void* stream);
+int64_t ss_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim);
+
+/* Rows scaled to length one, those of a (rows, heads, dim) tensor with unit
+ * stride along dim and free strides between rows and heads:
+ *   out = x * rsqrt(sum(x^2) + eps)
+ * or, with dout, out = the gradient of x.  dim: 1 to 16384; rows * heads below 2^32. */
+typedef struct ss_unit_norm_args {
+    int64_t rows, heads, dim;
+    int32_t dtype;                       /* enum ss_dtype */
+    float eps;
+    int64_t x_row_stride, x_head_stride, dout_row_stride, dout_head_stride;
+    const void* x;
+    const void* dout;                    /* NULL: the forward */
+    void* out;                           /* (rows, heads, dim) contiguous */
+} ss_unit_norm_args;
+int ss_unit_norm(const ss_unit_norm_args* a, void* stream);
+
+/* ------------------------------------------------------------------------
  * The norm over many gradient tensors, and the gradients clipped to it:
  *   norm = sqrt(sum g^2),  outs[i] = grads[i] * min(1, max_norm / (norm + eps))
  * (squares summed in 64 bits, in a fixed order; the product in fp32, rounded

@@ -32,6 +32,9 @@ EXPORTED = (
     "ss_linear_attn_fwd", "ss_linear_attn_bwd", "ss_linear_attn_update",
     "ss_block_norm_fwd", "ss_block_norm_bwd", "ss_block_norm_bwd_workspace_bytes",
     "ss_gated_norm_fwd", "ss_gated_norm_bwd", "ss_gated_norm_bwd_workspace_bytes",
+    "ss_delta_rule_saved_bytes", "ss_delta_rule_fwd_workspace_bytes", "ss_delta_rule_bwd_workspace_bytes",
+    "ss_delta_rule_fwd", "ss_delta_rule_bwd", "ss_delta_rule_update",
+    "ss_layer_norm_fwd", "ss_layer_norm_bwd", "ss_layer_norm_bwd_workspace_bytes", "ss_unit_norm",
     "ss_clip_grads", "ss_clip_grads_workspace_bytes",
 )
 
@@ -243,6 +246,24 @@ class GatedNormBwdArgs(ctypes.Structure):
         ("workspace_bytes", _i64)]
 
 
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("dim", _i64), ("dtype", _i32), ("w_dtype", _i32), ("eps", ctypes.c_float), ("pad_", _i32)] + [
+        (f"{t}_row_stride", _i64) for t in ("x", "residual", "out", "residual_out")] + [
+        (t, _p) for t in ("x", "residual", "weight", "bias", "out", "residual_out", "stats")]
+
+
+class LayerNormBwdArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("dim", _i64), ("dtype", _i32), ("w_dtype", _i32)] + [
+        (f"{t}_row_stride", _i64) for t in ("s", "dout", "dresidual_out")] + [
+        (t, _p) for t in ("s", "weight", "stats", "dout", "dresidual_out", "dx", "dweight", "dbias", "workspace")] + [
+        ("workspace_bytes", _i64)]
+
+
+class UnitNormArgs(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("heads", _i64), ("dim", _i64), ("dtype", _i32), ("eps", ctypes.c_float)] + [
+        (f"{t}_stride", _i64) for t in ("x_row", "x_head", "dout_row", "dout_head")] + [(t, _p) for t in ("x", "dout", "out")]
+
+
 class ClipGradsArgs(ctypes.Structure):
     _fields_ = [("count", _i64), ("grads", _p), ("outs", _p), ("numels", _p), ("dtypes", _p),
                 ("max_norm", ctypes.c_float), ("eps", ctypes.c_float), ("norm", _p), ("workspace", _p),
@@ -325,14 +346,17 @@ def load():
             fn.restype = ctypes.c_int
         for name, T in (("ss_block_norm_fwd", BlockNormArgs), ("ss_block_norm_bwd", BlockNormBwdArgs),
                         ("ss_gated_norm_fwd", GatedNormArgs), ("ss_gated_norm_bwd", GatedNormBwdArgs),
-                        ("ss_clip_grads", ClipGradsArgs)):
+                        ("ss_layer_norm_fwd", LayerNormArgs), ("ss_layer_norm_bwd", LayerNormBwdArgs),
+                        ("ss_unit_norm", UnitNormArgs), ("ss_clip_grads", ClipGradsArgs)):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(T), _p]
             fn.restype = ctypes.c_int
         lib.ss_block_norm_bwd_workspace_bytes.argtypes = [_i64, _i64]
+        lib.ss_layer_norm_bwd_workspace_bytes.argtypes = [_i64, _i64]
         lib.ss_gated_norm_bwd_workspace_bytes.argtypes = [_i64, _i64, _i64]
         lib.ss_clip_grads_workspace_bytes.argtypes = [ctypes.POINTER(ClipGradsArgs)]
-        for name in ("ss_block_norm_bwd_workspace_bytes", "ss_gated_norm_bwd_workspace_bytes", "ss_clip_grads_workspace_bytes"):
+        for name in ("ss_block_norm_bwd_workspace_bytes", "ss_layer_norm_bwd_workspace_bytes", "ss_gated_norm_bwd_workspace_bytes",
+                     "ss_clip_grads_workspace_bytes"):
             getattr(lib, name).restype = _i64
         if lib.ss_abi_version() != ABI_VERSION:
             raise RuntimeError(f"mamba_amd: library ABI {lib.ss_abi_version()} != binding ABI {ABI_VERSION}")

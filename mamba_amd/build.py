@@ -24,7 +24,8 @@ ARCH = os.environ.get("MAMBA_AMD_ARCH", "gfx950")
 SOURCES = ["ss_bwd.hip", "ss_bwd_bf16.hip", "ss_bwd_f16.hip", "ss_fwd.hip", "ss_fwd_bf16.hip", "ss_fwd_f16.hip",
            "ops_api.hip", "conv1d.hip", "rms_norm.hip", "decode.hip", "decode_linear.hip", "linear_attn.hip",
            "linear_attn_f32.hip", "linear_attn_bf16.hip", "linear_attn_f16.hip",
-           "delta_rule.hip", "delta_rule_f32.hip", "delta_rule_bf16.hip", "delta_rule_f16.hip", "block_norm.hip", "clip_grads.hip"]
+           "delta_rule.hip", "delta_rule_f32.hip", "delta_rule_bf16.hip", "delta_rule_f16.hip", "block_norm.hip", "layer_norm.hip",
+           "unit_norm.hip", "clip_grads.hip"]
 
 
 def hipcc():

@@ -1372,6 +1372,165 @@ Tensor gated_norm(const Tensor& x, const Tensor& gate, const Tensor& weight, int
     return GatedNorm::apply(x, gate, weight, groups, eps);
 }
 
+// -------------------------------------------------------------- layer norm --
+constexpr const char* kLayer = "layer_norm";
+
+// (out, s: of x's shape, s null without residual or unless asked for; read: s, weight as read; stats)
+struct LayerOut { Tensor out; OptT s, stats; Tensor rows, weight; };
+LayerOut layer_norm_fwd(const Tensor& x_, const Tensor& weight, const OptT& bias, const OptT& residual_, double eps, bool want_s,
+                        bool need, void* stream) {
+    ss_layer_norm_args a{};
+    norm_x(kLayer, x_, &a.dtype);
+    const Tensor x = any_rows(x_);
+    const OptT residual = residual_ ? OptT(like_rows(kLayer, "residual", *residual_, x_)) : OptT(), ow = weight;
+    const Weights w = weights_of(kLayer, x_, {{"weight", &ow}, {"bias", &bias}});
+    a.w_dtype = w.dtype;
+    a.rows = x.size(0); a.dim = x.size(1); a.eps = float(eps);
+    const Tensor out = at::empty(x_.sizes(), x.options());
+    OptT s, stats;
+    if (residual && (want_s || need)) s = at::empty(x_.sizes(), x.options());
+    if (need) stats = f32_like({a.rows, 2}, x);
+    a.x_row_stride = x.stride(0);
+    if (residual) a.residual_row_stride = residual->stride(0);
+    a.out_row_stride = a.residual_out_row_stride = a.dim;
+    a.x = ptr(x); a.residual = ptr(residual); a.weight = ptr(w.w[0]); a.bias = ptr(w.w[1]);
+    a.out = ptr(out); a.residual_out = ptr(s); a.stats = fptr<float>(stats);
+    launch(x.device(), "layer_norm forward", [&] { return ss_layer_norm_fwd(&a, stream); });
+    return {out, s, stats, s ? any_rows(*s) : x, *w.w[0]};
+}
+
+// (dx, dweight, dbias or none)
+variable_list layer_norm_bwd(const Tensor& s, const Tensor& weight, const Tensor& stats, const OptT& dout_, const OptT& ds_,
+                             bool want_dbias, void* stream) {
+    ss_layer_norm_bwd_args g{};
+    norm_x(kLayer, s, &g.dtype);
+    REQUIRE(kLayer, s.dim() == 2, "s must be (rows, dim)");
+    const int64_t rows = s.size(0), dim = s.size(1);
+    REQUIRE(kLayer, stats.scalar_type() == at::kFloat && same_shape(stats, {rows, 2}) && stats.is_contiguous(),
+            "stats must be fp32 (rows, 2) contiguous");
+    REQUIRE(kLayer, itype_of(weight.scalar_type(), &g.w_dtype), "unsupported dtype " + dtype_str(weight.scalar_type()));
+    OptT dout, ds;
+    if (dout_) dout = like_rows(kLayer, "dout", *dout_, s);
+    if (ds_) ds = like_rows(kLayer, "dresidual_out", *ds_, s);
+    const Tensor dx = at::empty(s.sizes(), s.options()), dw = at::empty({dim}, weight.options());
+    OptT db;
+    if (want_dbias) db = at::empty({dim}, weight.options());
+    const int64_t n = ss_layer_norm_bwd_workspace_bytes(rows, dim);
+    if (n < 0) check(SS_ERR_INVALID, kLayer);
+    const Tensor ws = bytes_on(std::max<int64_t>(n, 1), s);
+    g.rows = rows; g.dim = dim;
+    g.s_row_stride = s.stride(0);
+    if (dout) g.dout_row_stride = dout->stride(0);
+    if (ds) g.dresidual_out_row_stride = ds->stride(0);
+    g.s = ptr(s); g.weight = ptr(weight); g.stats = static_cast<float*>(ptr(stats)); g.dout = ptr(dout); g.dresidual_out = ptr(ds);
+    g.dx = ptr(dx); g.dweight = ptr(dw); g.dbias = ptr(db); g.workspace = ptr(ws); g.workspace_bytes = n;
+    launch(s.device(), "layer_norm backward", [&] { return ss_layer_norm_bwd(&g, stream); });
+    return {dx, dw, given(db)};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptT& bias, const OptT& residual,
+                                 double eps, bool prenorm) {
+        void* const stream = current_stream(x.device());
+        const LayerOut r = layer_norm_fwd(x, weight, bias, residual, eps, prenorm, true, stream);
+        ctx->saved_data["stream"] = reinterpret_cast<int64_t>(stream);
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["types"] = std::vector<int64_t>{int64_t(weight.scalar_type()), bias ? int64_t(bias->scalar_type()) : -1};
+        ctx->saved_data["residual"] = residual.has_value();
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({r.rows, r.weight, *r.stats});
+        variable_list out{r.out};
+        // (without residual x passes through the node, so that its two gradients are summed and rounded in one pass)
+        if (prenorm) out.push_back(r.s ? *r.s : x);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        variable_list r(6);
+        const Tensor ds = grads.size() > 1 ? grads[1] : Tensor();
+        if (!grads[0].defined() && !ds.defined()) return r;
+        const auto t = ctx->get_saved_variables();
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        const bool has_bias = types[1] >= 0, has_residual = ctx->saved_data["residual"].toBool();
+        const auto rows = [&](const Tensor& g) { return g.defined() ? OptT(g.reshape(t[0].sizes())) : OptT(); };
+        const variable_list d = layer_norm_bwd(t[0], t[1], t[2], rows(grads[0]), rows(ds), has_bias, node_stream(ctx));
+        const Tensor dx = d[0].view(shape);
+        const size_t at_bias = 2, at_residual = has_bias ? 3 : 2;        // (an absent bias is no input)
+        if (ctx->needs_input_grad(0)) r[0] = dx;
+        if (ctx->needs_input_grad(1)) r[1] = d[1].to(at::ScalarType(types[0]));
+        if (has_bias && ctx->needs_input_grad(at_bias)) r[2] = d[2].to(at::ScalarType(types[1]));
+        if (has_residual && ctx->needs_input_grad(at_residual)) r[3] = dx;
+        return final_grads(kLayer, r);
+    }
+};
+// (out, s or None: with prenorm, unless s is x)
+py::tuple layer_norm(const Tensor& x, const Tensor& weight, const OptT& bias, const OptT& residual, double eps, bool prenorm) {
+    no_tangents(kLayer, {&x, &weight, at_opt(bias), at_opt(residual)});
+    if (!wants_grad({&x, &weight, at_opt(bias), at_opt(residual)})) {
+        const LayerOut r = layer_norm_fwd(x, weight, bias, residual, eps, prenorm, false, current_stream(x.device()));
+        return py::make_tuple(r.out, r.s);
+    }
+    const variable_list r = LayerNorm::apply(x, weight, bias, residual, eps, prenorm);
+    return py::make_tuple(r[0], r.size() > 1 ? OptT(r[1]) : OptT());
+}
+
+// --------------------------------------------------------------- unit norm --
+constexpr const char* kUnit = "unit_norm";
+
+// t as a (rows, heads, dim) view with unit stride along dim (a copy only where there is none)
+Tensor head_rows(const Tensor& t_) {
+    const int64_t dim = t_.size(-1), nd = t_.dim();
+    if (nd == 3 && (dim <= 1 || t_.stride(2) == 1)) return t_;
+    if (nd <= 2 || t_.numel() == 0) {
+        const Tensor t = any_rows(t_);
+        return t.view({t.size(0), 1, dim});
+    }
+    const Tensor t = dim > 1 && t_.stride(-1) != 1 ? t_.contiguous() : t_;
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 2 < nd; ++i) rows *= t.size(i);
+    const Tensor v = t.reshape({rows, t.size(-2), dim});
+    return dim > 1 && v.stride(2) != 1 ? v.contiguous() : v;
+}
+
+// forward, or the gradient of x from dout; of x's shape
+Tensor unit_norm_call(const Tensor& x_, const OptT& dout_, double eps, void* stream) {
+    ss_unit_norm_args a{};
+    norm_x(kUnit, x_, &a.dtype);
+    const Tensor x = head_rows(x_), out = at::empty(x_.sizes(), x_.options());
+    a.rows = x.size(0); a.heads = x.size(1); a.dim = x.size(2); a.eps = float(eps);
+    a.x_row_stride = x.stride(0); a.x_head_stride = x.stride(1);
+    Tensor d;
+    if (dout_) {
+        REQUIRE(kUnit, dout_->sizes() == x_.sizes() && dout_->scalar_type() == x_.scalar_type() && dout_->device() == x_.device(),
+                "dout must match x, got " + shape_str(dout_->sizes()) + " " + dtype_str(dout_->scalar_type()));
+        d = head_rows(*dout_);
+        a.dout_row_stride = d.stride(0); a.dout_head_stride = d.stride(1);
+        a.dout = ptr(d);
+    }
+    a.x = ptr(x); a.out = ptr(out);
+    if (x.numel() > 0) launch(x.device(), kUnit, [&] { return ss_unit_norm(&a, stream); });
+    return out;
+}
+
+struct UnitNorm : torch::autograd::Function<UnitNorm> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, double eps) {
+        void* const stream = current_stream(x.device());
+        ctx->saved_data["stream"] = reinterpret_cast<int64_t>(stream);
+        ctx->saved_data["eps"] = eps;
+        const Tensor out = unit_norm_call(x, OptT(), eps, stream);
+        ctx->save_for_backward({x});
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto t = ctx->get_saved_variables();
+        return final_grads(kUnit, {unit_norm_call(t[0], OptT(grads[0]), ctx->saved_data["eps"].toDouble(), node_stream(ctx)), Tensor()});
+    }
+};
+Tensor unit_norm(const Tensor& x, double eps) {
+    no_tangents(kUnit, {&x});
+    return wants_grad({&x}) ? UnitNorm::apply(x, eps) : unit_norm_call(x, OptT(), eps, current_stream(x.device()));
+}
+
 // -------------------------------------------------------------- clipping --
 constexpr const char* kClip = "clip_grads";
 
@@ -1450,6 +1609,8 @@ PYBIND11_MODULE(mamba_host, m) {
     m.def("delta_update", &delta_update);
     m.def("block_norm", &block_norm);
     m.def("gated_norm", &gated_norm);
+    m.def("layer_norm", &layer_norm);
+    m.def("unit_norm", &unit_norm);
     m.def("clip_grads", &clip_grads);
     m.def("final_grads", &final_grads_py);
     m.def("abi", [] { return py::make_tuple(SS_ABI_VERSION, sizeof(ss_fwd_args), sizeof(ss_bwd_args)); });

@@ -1,5 +1,5 @@
-// The C ABI of the operators beside the scan: linear attention, the norms
-// around a block, gradient clipping.  One unit with ss_api.hip, whose checks and
+// The C ABI of the operators beside the scan: linear attention, the delta rule, the
+// norms, gradient clipping.  One unit with ss_api.hip, whose checks and
 // last error (per thread) it shares.
 #include "ss_api.hip"
 
@@ -404,6 +404,68 @@ int ss_gated_norm_bwd(const ss_gated_norm_bwd_args* g, void* stream) {
     if (rc != SS_OK) return rc;
     const hipError_t e = ss::gated_norm_bwd_launch(g, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(SS_ERR_HIP, "gated norm backward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int64_t ss_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t dim) {
+    if (rows < 0 || dim < 0 || dim > ss::kBlockNormMaxDim) {
+        fail(SS_ERR_INVALID, "rows=%lld, dim=%lld out of range", (long long)rows, (long long)dim);
+        return -1;
+    }
+    return ss::layer_norm_bwd_space(rows, dim);
+}
+
+int ss_layer_norm_fwd(const ss_layer_norm_args* a, void* stream) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    int rc = check_block_norm(a->rows, a->dim, a->dtype, a->w_dtype);
+    if (rc != SS_OK) return rc;
+    if (!(a->eps >= 0.f)) return fail(SS_ERR_INVALID, "eps must be >= 0");
+    if (a->rows == 0 || a->dim == 0) return ok();
+    rc = check_norm_ptrs({{a->x, a->x_row_stride, true, "x"}, {a->residual, a->residual_row_stride, false, "residual"},
+                          {a->out, a->out_row_stride, true, "out"},
+                          {a->residual_out, a->residual_out_row_stride, false, "residual_out"}}, elem_size(a->dtype));
+    if (rc == SS_OK) rc = check_norm_ptrs({{a->weight, 0, true, "weight"}, {a->bias, 0, false, "bias"}}, elem_size(a->w_dtype));
+    if (rc == SS_OK) rc = check_norm_ptrs({{a->stats, 0, false, "stats"}}, 4);
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::layer_norm_fwd_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "layer norm forward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_layer_norm_bwd(const ss_layer_norm_bwd_args* g, void* stream) {
+    if (!g) return fail(SS_ERR_INVALID, "null argument block");
+    int rc = check_block_norm(g->rows, g->dim, g->dtype, g->w_dtype);
+    if (rc != SS_OK) return rc;
+    if (g->dim == 0) return ok();
+    rc = check_norm_ptrs({{g->weight, 0, true, "weight"}, {g->dweight, 0, true, "dweight"}, {g->dbias, 0, false, "dbias"}},
+                         elem_size(g->w_dtype));
+    if (rc == SS_OK && g->rows > 0) {
+        rc = check_norm_ptrs({{g->s, g->s_row_stride, true, "s"}, {g->dout, g->dout_row_stride, false, "dout"},
+                              {g->dresidual_out, g->dresidual_out_row_stride, false, "dresidual_out"},
+                              {g->dx, 0, true, "dx"}}, elem_size(g->dtype));
+        if (rc == SS_OK) rc = check_norm_ptrs({{g->stats, 0, true, "stats"}}, 4);
+    }
+    if (rc == SS_OK) rc = check_space(g->workspace, g->workspace_bytes, ss::layer_norm_bwd_space(g->rows, g->dim));
+    if (rc != SS_OK) return rc;
+    const hipError_t e = ss::layer_norm_bwd_launch(g, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "layer norm backward launch failed: %s", hipGetErrorString(e));
+    return ok();
+}
+
+int ss_unit_norm(const ss_unit_norm_args* a, void* stream) {
+    if (!a) return fail(SS_ERR_INVALID, "null argument block");
+    const int rc = check_block_norm(a->rows, a->dim, a->dtype, a->dtype);
+    if (rc != SS_OK) return rc;
+    if (a->heads < 0) return fail(SS_ERR_INVALID, "negative size (heads=%lld)", (long long)a->heads);
+    if (!(a->eps >= 0.f)) return fail(SS_ERR_INVALID, "eps must be >= 0");
+    if (a->rows == 0 || a->heads == 0 || a->dim == 0) return ok();
+    if (a->rows > ((int64_t(1) << 32) - 1) / a->heads) return fail(SS_ERR_UNSUPPORTED, "rows * heads too large");
+    const int rp = check_norm_ptrs({{a->x, a->x_row_stride, true, "x"}, {a->x, a->x_head_stride, true, "x"},
+                                    {a->dout, a->dout_row_stride, false, "dout"}, {a->dout, a->dout_head_stride, false, "dout"},
+                                    {a->out, 0, true, "out"}}, elem_size(a->dtype));
+    if (rp != SS_OK) return rp;
+    const hipError_t e = ss::unit_norm_launch(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(SS_ERR_HIP, "unit norm launch failed: %s", hipGetErrorString(e));
     return ok();
 }
 

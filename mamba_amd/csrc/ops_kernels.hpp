@@ -35,6 +35,11 @@ hipError_t block_norm_bwd_launch(const ss_block_norm_bwd_args* g, hipStream_t st
 hipError_t gated_norm_fwd_launch(const ss_gated_norm_args* a, hipStream_t stream);
 hipError_t gated_norm_bwd_launch(const ss_gated_norm_bwd_args* g, hipStream_t stream);
 constexpr int64_t kBlockNormMaxDim = 16384;      // a row lies in the registers of one workgroup
+// layer norm (layer_norm.hip), rows of up to kBlockNormMaxDim; rows scaled to length one (unit_norm.hip)
+int64_t layer_norm_bwd_space(int64_t rows, int64_t dim);
+hipError_t layer_norm_fwd_launch(const ss_layer_norm_args* a, hipStream_t stream);
+hipError_t layer_norm_bwd_launch(const ss_layer_norm_bwd_args* g, hipStream_t stream);
+hipError_t unit_norm_launch(const ss_unit_norm_args* a, hipStream_t stream);
 // the norm over many tensors (clip_grads.hip)
 int64_t clip_grads_chunks(const ss_clip_grads_args* a);
 hipError_t clip_grads_launch(const ss_clip_grads_args* a, hipStream_t stream);

@@ -1,0 +1,133 @@
+// Rows scaled to length one (the queries and keys of the delta rule's heads), on gfx950:
+//
+//   y = x r,  r = (sum x^2 + eps)^-1/2,      dx = r (dy - y (y . dy))
+//
+// L lanes hold a row, 8 elements a lane up to 512 (so that neighbouring lanes read neighbouring
+// vectors), between its one load and its one store: bound by HBM.  Rows are those of a
+// (rows, heads, dim) tensor with strides of their own, so that queries and keys are
+// read where they lie in a projection's output.  The backward sums r anew: its sum rides with the
+// other one, and nothing is kept but x.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/mamba_ss.h"
+#include "norm_rows.hpp"
+#include "norm_teams.hpp"
+#include "ops_kernels.hpp"
+#include "ss_device.hpp"
+
+namespace ss {
+
+namespace {
+
+struct UnitParams {
+    uint32_t rows, heads;                              // rows: all rows of all heads
+    int64_t x_rs, x_hs, d_rs, d_hs;                    // x's and dout's strides between rows and heads
+    int dim;
+    float eps;
+    const void* x; const void* dout;
+    void* out;                                         // (rows, heads, dim) contiguous: y, or dx
+};
+
+template <int L> constexpr int kUnitBlock = L > 256 ? L : 256;
+
+template <typename T, int L, int EPT, bool BWD>
+__global__ __launch_bounds__(kUnitBlock<L>) void unit_norm(const UnitParams p) {
+    using R = rowvec<T>;
+    constexpr int VE = R::VE, NV = EPT / VE, WPR = L > 64 ? L / 64 : 1, TEAMS = kUnitBlock<L> / L;
+    __shared__ float red[2][WPR][2];
+    const int u = int(threadIdx.x) % L, wave = u >> 6;
+    int turn = 0;
+    for (int64_t row = int64_t(blockIdx.x) * TEAMS + threadIdx.x / L; row < p.rows; row += int64_t(gridDim.x) * TEAMS) {
+        const uint32_t at = uint32_t(row) / p.heads, head = uint32_t(row) - at * p.heads;
+        const T* x = static_cast<const T*>(p.x) + at * p.x_rs + head * p.x_hs;
+        const T* d = static_cast<const T*>(p.dout) + at * p.d_rs + head * p.d_hs;
+        uint4 cx[NV], cd[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * L + u) * VE;
+            cx[k] = R::load(x + c, p.dim - c);
+            if constexpr (BWD) cd[k] = R::load(d + c, p.dim - c);
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float v[VE], o[VE];
+            R::unpack(cx[k], v);
+            if constexpr (BWD) R::unpack(cd[k], o);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                sum[0] = __builtin_fmaf(v[e], v[e], sum[0]);
+                if constexpr (BWD) sum[1] = __builtin_fmaf(v[e], o[e], sum[1]);
+            }
+        }
+        if constexpr (L > 64) {
+            team_sum<WPR>(sum, red[turn], wave);
+            turn ^= 1;
+        } else {
+            sum[0] = lanes_sum<L>(sum[0]);
+            if constexpr (BWD) sum[1] = lanes_sum<L>(sum[1]);
+        }
+        const float r = rsqrtf(sum[0] + p.eps), yd = r * sum[1];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * L + u) * VE;
+            float v[VE], o[VE];
+            R::unpack(cx[k], v);
+            if constexpr (BWD) R::unpack(cd[k], o);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float y = v[e] * r;
+                v[e] = BWD ? r * __builtin_fmaf(-y, yd, o[e]) : y;
+            }
+            R::store(static_cast<T*>(p.out) + row * p.dim + c, v, p.dim - c);
+        }
+    }
+}
+
+template <typename F>
+hipError_t for_length(int64_t n, F&& f) {
+    using std::integral_constant;
+    const integral_constant<int, 8> e8{};
+    const integral_constant<int, 16> e16{};
+    if (n <= 16) return f(integral_constant<int, 2>{}, e8);
+    if (n <= 32) return f(integral_constant<int, 4>{}, e8);
+    if (n <= 64) return f(integral_constant<int, 8>{}, e8);
+    if (n <= 128) return f(integral_constant<int, 16>{}, e8);
+    if (n <= 256) return f(integral_constant<int, 32>{}, e8);
+    if (n <= 512) return f(integral_constant<int, 64>{}, e8);
+    if (n <= 4096) return f(integral_constant<int, 256>{}, e16);
+    return f(integral_constant<int, 1024>{}, e16);
+}
+
+template <bool BWD>
+hipError_t launch(const UnitParams& p, int dtype, hipStream_t stream) {
+    return for_types(dtype, dtype, [&](auto t, auto) {
+        return for_length(p.dim, [&](auto l, auto ept) {
+            constexpr int L = decltype(l)::value, TEAMS = kUnitBlock<L> / L;
+            const int64_t want = (int64_t(p.rows) + TEAMS - 1) / TEAMS;
+            hipLaunchKernelGGL((unit_norm<decltype(t), L, decltype(ept)::value, BWD>), dim3(unsigned(want < 8192 ? want : 8192)),
+                               dim3(kUnitBlock<L>), 0, stream, p);
+            return hipGetLastError();
+        });
+    });
+}
+
+UnitParams params_of(const ss_unit_norm_args* a) {
+    UnitParams p{};
+    p.rows = uint32_t(a->rows * a->heads); p.heads = uint32_t(a->heads);
+    p.x_rs = a->x_row_stride; p.x_hs = a->x_head_stride; p.d_rs = a->dout_row_stride; p.d_hs = a->dout_head_stride;
+    p.dim = int(a->dim); p.eps = a->eps;
+    p.x = a->x; p.dout = a->dout; p.out = a->out;
+    return p;
+}
+
+}  // namespace
+
+hipError_t unit_norm_launch(const ss_unit_norm_args* a, hipStream_t stream) {
+    return a->dout ? launch<true>(params_of(a), a->dtype, stream) : launch<false>(params_of(a), a->dtype, stream);
+}
+
+}  // namespace ss

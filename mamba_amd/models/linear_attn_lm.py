@@ -1,4 +1,5 @@
-"""LinearAttnLM: a language model of LinearAttn mixers with a norm on both sides of each block.
+"""LinearAttnLM: a language model of LinearAttn or DeltaRule mixers (``mixer`` of the
+configuration) with a norm on both sides of each block.
 
 Block i computes y = mixer_i(normed); the border to the next one is a single
 call, block_norm_fn: the norm after the block, its residual scale, and the
@@ -14,6 +15,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 
+from ..modules.delta_rule import DeltaRule
 from ..modules.linear_attn import LinearAttn
 from ..ops.block_norm import block_norm_fn
 from ..ops.rms_norm import rms_norm_fn
@@ -29,6 +31,10 @@ class LinearAttnLMConfig:
     expansion_factor: int = 2
     residual_scale: float = 0.5
     eps: float = 1e-6
+    mixer: str = "linear_attn"      # or "delta_rule"
+
+
+MIXERS = {"linear_attn": LinearAttn, "delta_rule": DeltaRule}
 
 
 class LinearAttnLM(nn.Module):
@@ -37,9 +43,12 @@ class LinearAttnLM(nn.Module):
         self.config = config
         fk = {"device": device, "dtype": dtype}
         d, n = config.model_dim, config.num_layers
+        if config.mixer not in MIXERS:
+            raise ValueError(f"LinearAttnLM: unknown mixer {config.mixer!r}, expected one of {sorted(MIXERS)}")
+        Mixer = MIXERS[config.mixer]
         self.embedding = nn.Embedding(config.vocab_size, d, **fk)
-        self.mixers = nn.ModuleList([LinearAttn(d, config.head_dim, n_groups=config.n_groups, eps=config.eps,
-                                                expansion_factor=config.expansion_factor, **fk) for _ in range(n)])
+        self.mixers = nn.ModuleList([Mixer(d, config.head_dim, n_groups=config.n_groups, eps=config.eps,
+                                           expansion_factor=config.expansion_factor, **fk) for _ in range(n)])
         self.pre = nn.ParameterList([nn.Parameter(torch.zeros(d, **fk)) for _ in range(n + 1)])
         self.post = nn.ParameterList([nn.Parameter(torch.zeros(d, **fk)) for _ in range(n)])
         self.scale = nn.ParameterList([nn.Parameter(torch.full((d,), config.residual_scale, **fk)) for _ in range(n)])

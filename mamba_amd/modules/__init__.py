@@ -1,3 +1,5 @@
+from .delta_rule import DeltaRule
+from .layer_norm import LayerNorm
 from .linear_attn import LinearAttn
 from .mamba_simple import MambaSimple
 from .rms_norm import RMSNorm
