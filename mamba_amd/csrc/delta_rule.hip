@@ -25,15 +25,18 @@ namespace {
 using namespace la;
 
 // The states that the segments start from, in place of their own: S <- M S + N along the
-// row (REV: M^T, from the last segment on).  A wave 16 value columns, which do not meet.
+// row (REV: M^T, from the last segment on).  A wave 16 value columns, which do not meet; M comes
+// through LDS in 3 terms (in halves of its columns past 128 keys), the next one on its way meanwhile.
 template <int KP, bool REV>
 __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
-    constexpr int NS = KP / 16, NK = KP / 32;
-    const int lane = int(threadIdx.x) & 63, g = lane >> 4, c = lane & 15;
+    constexpr int NS = KP / 16, NK = KP / 32, CW = KP < 128 ? KP : KP == 128 ? 64 : 32, MST = KP + 8, TERM = CW * MST, N = CW * KP / 4 / 256;
+    __shared__ __attribute__((aligned(16))) uint16_t ms[3 * TERM];       // CW columns of M, a row each
+    const int tid = int(threadIdx.x), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int64_t bh = blockIdx.x;
-    const int col = int(blockIdx.y) * 64 + 16 * (int(threadIdx.x) >> 6) + c, Kp = dr_round16(p.K);
-    if (col - c >= p.V) return;
-    f4 S[NS];
+    const int col = int(blockIdx.y) * 64 + 16 * (tid >> 6) + c;
+    const bool live = col - c < p.V;
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 S[NS], in[N];
 #pragma unroll
     for (int t = 0; t < NS; ++t)
 #pragma unroll
@@ -41,10 +44,18 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
             const int key = state_row(t, g, r);
             S[t][r] = p.init && key < p.K && col < p.V ? p.init[(bh * p.K + key) * p.V + col] : 0.f;
         }
+    const auto seg_of = [&](int i) { return bh * p.segs + (REV ? p.segs - 1 - i : i); };
+    const auto fetch = [&](int i, int c0) {
+        if (i >= p.segs) return;
+        const float* mul = p.seg_mul + seg_of(i) * p.Kp * p.Kp;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int x = tid + k * 256, at = c0 + x / (KP / 4), key = x % (KP / 4) * 4;
+            in[k] = at < p.Kp && key < p.Kp ? *reinterpret_cast<const f4*>(mul + int64_t(at) * p.Kp + key) : zero;
+        }
+    };
+    fetch(0, 0);
     for (int i = 0; i < p.segs; ++i) {
-        const int64_t s = bh * p.segs + (REV ? p.segs - 1 - i : i);
-        float* add = p.seg_add + s * p.K * p.Vp + col;
-        const float* mul = p.seg_mul + s * p.K * Kp;
         u4 sf[NK][3];
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
@@ -57,38 +68,66 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
                 for (int n = 0; n < 3; ++n) sf[k][n][h] = t[n];
             }
         }
+        if (live) {
+            float* add = p.seg_add + (seg_of(i) * p.Vp + col) * p.Kp;
 #pragma unroll
-        for (int t = 0; t < NS; ++t) {
-            f4 own;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = state_row(t, g, r);
-                own[r] = key < p.K ? add[int64_t(key) * p.Vp] : 0.f;
-                if (key < p.K) add[int64_t(key) * p.Vp] = S[t][r];
+            for (int t = 0; t < NS; ++t) {
+                const int key = state_row(t, g, 0);
+                if (key >= p.Kp) continue;
+                const f4 own = *reinterpret_cast<const f4*>(add + key);
+                *reinterpret_cast<f4*>(add + key) = S[t];
+                S[t] = own;
             }
-            S[t] = own;
         }
 #pragma unroll
-        for (int t = 0; t < NS; ++t) {
-            const int row = 32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3);
+        for (int c0 = 0; c0 < KP; c0 += CW) {
+            lds_barrier();
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                u4 a[3];
+            for (int k = 0; k < N; ++k) {
+                const int x = tid + k * 256;
+                uint32_t a[3], b[3];
+                split<3>(in[k][0], in[k][1], a);
+                split<3>(in[k][2], in[k][3], b);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int from = 32 * k + 8 * g + 2 * h;
-                    float x0 = 0.f, x1 = 0.f;
-                    if (row < p.K && from < p.K) {
-                        x0 = REV ? mul[int64_t(from) * Kp + row] : mul[int64_t(row) * Kp + from];
-                        if (from + 1 < p.K) x1 = REV ? mul[int64_t(from + 1) * Kp + row] : mul[int64_t(row) * Kp + from + 1];
+                for (int n = 0; n < 3; ++n)
+                    *reinterpret_cast<uint2*>(ms + n * TERM + x / (KP / 4) * MST + x % (KP / 4) * 4) = make_uint2(a[n], b[n]);
+            }
+            lds_barrier();
+            if (c0 + CW < KP) fetch(i, c0 + CW);
+            else fetch(i + 1, 0);
+            if (!live) continue;
+            f4* to[1];
+            if constexpr (REV) {                          // rows of M^T: these columns, all keys
+#pragma unroll
+                for (int t = c0 / 16; t < (c0 + CW) / 16; ++t) {
+                    const uint16_t* row = ms + (32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3) - c0) * MST + 8 * g;
+                    to[0] = &S[t];
+#pragma unroll
+                    for (int k = 0; k < NK; ++k) {
+                        u4 a[3];
+#pragma unroll
+                        for (int n = 0; n < 3; ++n) a[n] = *reinterpret_cast<const u4*>(row + n * TERM + 32 * k);
+                        mfma_terms<1, 0, 0, 3, 3, 2>(&a, &sf[k], to);
                     }
-                    uint32_t w[3];
-                    split<3>(x0, x1, w);
-#pragma unroll
-                    for (int n = 0; n < 3; ++n) a[n][h] = w[n];
                 }
-                f4* const to[1] = {&S[t]};
-                mfma_terms<1, 0, 0, 3, 3, 2>(&a, &sf[k], to);
+            } else {                                      // all rows of M, these columns
+                typedef __attribute__((address_space(3))) s4 lds_s4;
+#pragma unroll
+                for (int t = 0; t < NS; ++t) {
+                    to[0] = &S[t];
+#pragma unroll
+                    for (int k = c0 / 32; k < (c0 + CW) / 32; ++k) {
+                        const uint16_t* at = ms + (32 * k - c0 + 8 * g + (c >> 2)) * MST + 32 * (t >> 1) + 8 * (c & 3) + 4 * (t & 1);
+                        u4 a[3];
+#pragma unroll
+                        for (int n = 0; n < 3; ++n) {
+                            const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM)));
+                            const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM + 4 * MST)));
+                            a[n] = u4{lo.x, lo.y, hi.x, hi.y};
+                        }
+                        mfma_terms<1, 0, 0, 3, 3, 2>(&a, &sf[k], to);
+                    }
+                }
             }
         }
     }
@@ -123,7 +162,7 @@ int terms(int32_t dtype) { return dtype == SS_F32 ? 3 : dtype == SS_BF16 ? 1 : 2
 constexpr int64_t kUnits = 256, kSegChunksMin = 8;
 
 struct Plan {
-    int64_t bh, nch, tri, state, rows, mul;      // (batch, head) pairs, chunks; floats of a chunk's inverse, a state, a chunk's rows, an M
+    int64_t bh, nch, plan, state, rows, mul;     // (batch, head) pairs, chunks; floats of a chunk's plan, a state, a chunk's rows, an M
     int segs, seg_chunks, chunk;
 };
 Plan plan_of(const ss_delta_rule_args& a) {
@@ -131,11 +170,11 @@ Plan plan_of(const ss_delta_rule_args& a) {
     p.chunk = dr_chunk(a.d_key, terms(a.dtype));
     p.bh = a.batch * a.heads;
     p.nch = (a.seqlen + p.chunk - 1) / p.chunk;
-    const int64_t nr = p.chunk / 16, vp = dr_round16(a.d_value);
-    p.tri = nr * (nr + 1) / 2 * 256;
-    p.state = a.d_key * vp;
+    const int64_t kp = dr_round16(a.d_key), vp = dr_round16(a.d_value);
+    p.plan = dr_plan_bytes(p.chunk) / 4;
+    p.state = kp * vp;
     p.rows = p.chunk * vp;
-    p.mul = a.d_key * dr_round16(a.d_key);
+    p.mul = kp * kp;
     const int64_t walks = p.bh * ((a.d_value + 63) / 64);
     int64_t segs = walks > 0 ? kUnits / walks : 1;
     if (segs > p.nch / kSegChunksMin) segs = p.nch / kSegChunksMin;
@@ -155,24 +194,24 @@ struct Parts {
         return at;
     }
 };
-struct Saved { int64_t tri, states, err, mul, bytes; };
+struct Saved { int64_t plan, states, err, mul, bytes; };
 Saved saved_of(const Plan& p) {
     Saved s{};
     Parts parts;
-    s.tri = parts.take(p.bh * p.nch * p.tri);
+    s.plan = parts.take(p.bh * p.nch * p.plan);
     s.states = parts.take(p.bh * p.nch * p.state);
     s.err = parts.take(p.bh * p.nch * p.rows);
     s.mul = p.segs > 1 ? parts.take(p.bh * p.segs * p.mul) : 0;
     s.bytes = parts.bytes;
     return s;
 }
-struct FwdSpace { int64_t add, tri, mul, bytes; };
+struct FwdSpace { int64_t add, plan, mul, bytes; };
 FwdSpace fwd_space(const ss_delta_rule_args& a, const Plan& p) {
     FwdSpace s{};
     Parts parts;
     if (p.segs > 1) s.add = parts.take(p.bh * p.segs * p.state);
     if (!a.saved) {
-        s.tri = parts.take(p.bh * p.nch * p.tri);
+        s.plan = parts.take(p.bh * p.nch * p.plan);
         if (p.segs > 1) s.mul = parts.take(p.bh * p.segs * p.mul);
     }
     s.bytes = parts.bytes;
@@ -196,7 +235,7 @@ BwdSpace bwd_space(const ss_delta_rule_args& a, const Plan& p) {
 DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
     DrParams p{};
     p.B = a.batch; p.L = a.seqlen; p.H = a.heads;
-    p.K = int(a.d_key); p.V = int(a.d_value); p.Vp = dr_round16(a.d_value);
+    p.K = int(a.d_key); p.V = int(a.d_value); p.Kp = dr_round16(a.d_key); p.Vp = dr_round16(a.d_value);
     p.rep = int(a.heads / a.groups); p.nch = int(plan.nch);
     p.scale = a.scale;
     p.q = {a.q, a.q_batch_stride, a.q_len_stride, a.q_head_stride, p.rep};
@@ -255,10 +294,10 @@ hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream
     p.init = a->initial_state; p.last = a->last_state;
     p.seg_add = at(a->workspace, sp.add);
     if (a->saved) {
-        p.tri = at(a->saved, sv.tri); p.states = at(a->saved, sv.states); p.err = at(a->saved, sv.err);
+        p.plan = at(a->saved, sv.plan); p.states = at(a->saved, sv.states); p.err = at(a->saved, sv.err);
         p.seg_mul = at(a->saved, sv.mul);
     } else {
-        p.tri = at(a->workspace, sp.tri);
+        p.plan = at(a->workspace, sp.plan);
         p.seg_mul = at(a->workspace, sp.mul);
     }
     if (plan.nch > 0) {
@@ -276,7 +315,7 @@ hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t st
     DrParams p = params_of(a, plan);
     p.o = {g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1};
     p.init = g->dlast_state; p.last = g->dinitial_state;
-    p.tri = at(a.saved, sv.tri); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = at(a.saved, sv.mul);
+    p.plan = at(a.saved, sv.plan); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = at(a.saved, sv.mul);
     p.dstates = at(a.workspace, sp.dstates); p.derr = at(a.workspace, sp.derr); p.seg_add = at(a.workspace, sp.add);
     hipError_t e = walk(a.dtype, p, true, stream);
     if (e != hipSuccess || plan.nch == 0) return e;

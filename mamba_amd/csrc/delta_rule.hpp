@@ -17,21 +17,22 @@ constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
 
 // Per (batch, head) pair and chunk, what the kernels hand on (fp32):
-//   tri     the lower 16 x 16 tiles of the chunk's triangular inverse, tile (i, j) at i (i + 1) / 2 + j, row-major
-//   states  the state before the chunk, (K, Vp)
-//   err     the tokens' prediction errors, (chunk, Vp)
+//   plan    the chunk's gates and triangular inverse (delta_rule_chunk.hpp), dr_plan_bytes()
+//   states  the state before the chunk, (Vp, Kp): a value column's keys side by side
+//   err     the tokens' prediction errors, (Vp, chunk)
 //   dstates the gradient of the state after the chunk;  derr: of the errors, as err
-// Vp: value columns rounded up to 16, zero past the last.
+// Kp, Vp: keys and value columns rounded up to 16, zero past the last.
+constexpr int64_t dr_plan_bytes(int64_t chunk) { return chunk * 20 + 16 + chunk / 16 * (chunk / 16 + 1) / 2 * 1024; }
 struct DrParams {
     int64_t B, L, H;
-    int K, V, Vp, rep, nch;               // rep: heads per group; nch: chunks of a row of L tokens
+    int K, V, Kp, Vp, rep, nch;               // rep: heads per group; nch: chunks of a row of L tokens
     float scale;
     LaRows q, k, v, o;                    // o: out, or the backward's dout
     const float* g; int64_t g_b, g_l, g_h;
     const float* beta; int64_t be_b, be_l, be_h;
     const int32_t* lens;
     const float* init; float* last;       // (B, H, K, V) before and after the walk (backward: dlast, dinitial), or null
-    float* tri;
+    void* plan;
     float* states;                        // null: not kept
     float* err;
     float* dstates;
@@ -39,8 +40,8 @@ struct DrParams {
     // a row's segments of seg_chunks chunks side by side (segs 1: the whole row)
     int segs, seg_chunks;
     int local;                            // the segments' own states from zero and what becomes of a state over one
-    float* seg_add;                       // (B, H, segs, K, Vp): their states; then the states that they start from
-    float* seg_mul;                       // (B, H, segs, K, Kp): over a segment S becomes seg_mul S + its own; Kp: K rounded up to 16
+    float* seg_add;                       // (B, H, segs, Vp, Kp): their states; then the states that they start from
+    float* seg_mul;                       // (B, H, segs, Kp, Kp): over a segment S becomes M S + its own; column i of M at i Kp
     // gradients
     void* dq; void* dk; void* dv;         // contiguous; dq and dk in fp32 per head with rep > 1
     float* dg; float* dbeta;              // (B, L, H)

@@ -66,11 +66,12 @@ template <typename T, int KP>
 struct Dims {
     static constexpr int KT = kTerms<T>, C = dr_chunk(KP, KT), NR = C / 16, NP = C / 32, NK = KP / 32, NS = KP / 16;
     static constexpr int NT = NR * (NR + 1) / 2;             // lower tiles of a chunk's square
-    static constexpr int KST = KP + 8, CST = C + 8;          // row strides in LDS, elements
-    static constexpr int VST = 64 + 8;
+    static constexpr int KST = KP + 8;                       // row stride of q and k in LDS, elements
+    static constexpr int VST = sizeof(T) == 4 ? 68 : 72;     // of 64 value columns as they are
     static constexpr int OT = sizeof(T) == 4 ? 3 : 2;        // terms of what only a result of type T is formed from
+    // dr_grads: value columns and keys of the states that it takes at a time (tiles of q, k and these fill the LDS)
+    static constexpr int VW = 32, KW = KP <= 128 ? KP : KT == 3 ? 64 : 128;
 };
-
 template <typename T, int KP> constexpr int kPrepThreads = 64 * Dims<T, KP>::NR;
 template <typename T, int KP> constexpr int kGradThreads = 128 * Dims<T, KP>::NR;
 
@@ -94,66 +95,144 @@ __device__ __forceinline__ void pack(const f4& lo, const f4& hi, u4 (&t)[N]) {
         for (int n = 0; n < N; ++n) t[n][h] = s[n];
     }
 }
-// operands from N term tiles TERM elements apart: 8 neighbouring elements; 4 and the 4 that lie 16 further on
+// 4 neighbouring elements in N term tiles TERM elements apart
+template <int N, int TERM>
+__device__ __forceinline__ void put4(uint16_t* to, const f4& x) {
+    uint32_t a[N], b[N];
+    split<N>(x[0], x[1], a);
+    split<N>(x[2], x[3], b);
+#pragma unroll
+    for (int n = 0; n < N; ++n) *reinterpret_cast<uint2*>(to + n * TERM) = make_uint2(a[n], b[n]);
+}
+
+// Operands from N term tiles.  Of a row: 8 neighbouring elements.
 template <int N, int TERM>
 __device__ __forceinline__ void frag8(const uint16_t* at, u4 (&t)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) t[n] = *reinterpret_cast<const u4*>(at + n * TERM);
 }
-template <int N, int TERM>
-__device__ __forceinline__ void frag44(const uint16_t* at, u4 (&t)[N]) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        const u2 lo = *reinterpret_cast<const u2*>(at + n * TERM), hi = *reinterpret_cast<const u2*>(at + n * TERM + 16);
-        t[n] = u4{lo.x, lo.y, hi.x, hi.y};
-    }
-}
-// the same of a column: 32 rows of the tile from `at` on
+// Of a column (the transposing load): rows 4 g .. and 16 + 4 g .. of `at`, the order of two result tiles; or
+// 8 neighbouring rows, 8 g ..
 template <int N, int TERM, int STRIDE>
 __device__ __forceinline__ void frag_col(const uint16_t* at, int block, int lane, u4 (&t)[N]) {
 #pragma unroll
     for (int n = 0; n < N; ++n) t[n] = load_tokens<STRIDE>(at + n * TERM, block, lane);
 }
+typedef __attribute__((address_space(3))) s4 lds_s4;
+__device__ __forceinline__ u2 load_tr(const uint16_t* p) {
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)p));
+}
+template <int N, int TERM, int STRIDE>
+__device__ __forceinline__ void frag_col8(const uint16_t* at, int block, int lane, u4 (&t)[N]) {
+    const uint16_t* p = at + (8 * (lane >> 4) + ((lane & 15) >> 2)) * STRIDE + block;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const u2 lo = load_tr(p + n * TERM), hi = load_tr(p + n * TERM + 4 * STRIDE);
+        t[n] = u4{lo.x, lo.y, hi.x, hi.y};
+    }
+}
+// Of two 16 x 16 tiles that lie as 256 elements each (a wave's reads of one are the whole of it, in
+// order): a row of both, or with TR a column.  A tile below 0 is zero.
+template <int N, int TERM, bool TR>
+__device__ __forceinline__ void frag_tiles(const uint16_t* at, int lo, int hi, int lane, u4 (&t)[N]) {
+    const int g = lane >> 4, c = lane & 15;
+    const uint16_t* p = at + (TR ? 16 * (4 * g + (c >> 2)) + 4 * (c & 3) : 16 * c + 4 * g);
+    const auto get = [&](int tile, int n) {
+        if (tile < 0) return u2{0u, 0u};
+        if constexpr (TR) return load_tr(p + n * TERM + tile * 256);
+        else return *reinterpret_cast<const u2*>(p + n * TERM + tile * 256);
+    };
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const u2 a = get(lo, n), b = get(hi, n);
+        t[n] = u4{a.x, a.y, b.x, b.y};
+    }
+}
+// place of the lower tile (i, j); none above the diagonal
+constexpr __device__ __forceinline__ int tile_at(int i, int j) { return j <= i ? i * (i + 1) / 2 + j : -1; }
 // first of the 4 columns a lane reads for its group: of 16 neighbouring ones, and of the state's tile t
 __device__ __forceinline__ int block16(int t, int lane) { return 16 * t + 4 * (lane & 3); }
 __device__ __forceinline__ int state_block(int t, int lane) { return 32 * (t >> 1) + 8 * (lane & 3) + 4 * (t & 1); }
 
-// A chunk's rows (C x KP of type T) from global memory into term tiles, by NTH threads.
-template <typename T, int KP, int C, int NTH>
+// A chunk's rows (C x W of type T) from global memory by NTH threads: into term tiles, or as they are.
+template <typename T, int W, int C, int NTH>
 struct Tile {
     using R = rowvec<T>;
-    static constexpr int PER = KP / R::VE, N = C * PER / NTH, KT = kTerms<T>, KST = KP + 8, TERM = C * KST;
-    static_assert(C * PER % NTH == 0, "whole vectors a thread");
+    static constexpr int PER = W / R::VE, ALL = C * PER, N = (ALL + NTH - 1) / NTH, KT = kTerms<T>;
     uint4 v[N];
+    // the first `rows` rows and `dim` columns; zero past them
     __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int dim) {
+        const int row = int(threadIdx.x) / PER, col = int(threadIdx.x) % PER * R::VE;
+        if (rows == C && dim > 0 && dim % R::VE == 0 && step < (int64_t(1) << 24)) {
+            // whole vectors: a lane past the row's end reads its first, for nothing
+            const bool in = col < dim;
+            const uint32_t off = (uint32_t(row) * uint32_t(step) + uint32_t(in ? col : 0)) * uint32_t(sizeof(T));
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = int(threadIdx.x) + i * NTH, row = at / PER, col = at % PER * R::VE;
-            v[i] = R::load(p + int64_t(row) * step + col, row < rows ? dim - col : 0);
+            for (int i = 0; i < N; ++i) {
+                if (ALL % NTH != 0 && int(threadIdx.x) + i * NTH >= ALL) continue;
+                const typename R::words w = *reinterpret_cast<const typename R::words*>(
+                    reinterpret_cast<const char*>(p + int64_t(i * (NTH / PER)) * step) + off);
+                v[i] = in ? make_uint4(w.x, w.y, w.z, w.w) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < N; ++i) {
+                const int r = row + i * (NTH / PER);
+                const uint4 w = R::load(p + int64_t(r) * step + col, r < rows ? dim - col : 0);
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    if (k == i) v[k] = w;
+            }
         }
     }
+    template <int STRIDE>
     __device__ __forceinline__ void store(uint16_t* tile) const {
+        static_assert(NTH % PER == 0, "rows of whole threads");
+        uint16_t* to = tile + int(threadIdx.x) / PER * STRIDE + int(threadIdx.x) % PER * R::VE;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = int(threadIdx.x) + i * NTH;
-            uint16_t* to = tile + at / PER * KST + at % PER * R::VE;
+        for (int i = 0; i < N; ++i, to += NTH / PER * STRIDE) {
+            if (ALL % NTH != 0 && int(threadIdx.x) + i * NTH >= ALL) continue;
             if constexpr (KT == 1) {
                 *reinterpret_cast<uint4*>(to) = v[i];
             } else {
                 float x[R::VE];
                 R::unpack(v[i], x);
-                uint32_t t[R::VE / 2][KT];
 #pragma unroll
-                for (int k = 0; k < R::VE / 2; ++k) split<KT>(x[2 * k], x[2 * k + 1], t[k]);
-#pragma unroll
-                for (int n = 0; n < KT; ++n) {
-                    if constexpr (R::VE == 8) *reinterpret_cast<uint4*>(to + n * TERM) = make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]);
-                    else *reinterpret_cast<uint2*>(to + n * TERM) = make_uint2(t[0][n], t[1][n]);
-                }
+                for (int h = 0; h < R::VE; h += 4) put4<KT, C * STRIDE>(to + h, f4{x[h], x[h + 1], x[h + 2], x[h + 3]});
             }
         }
     }
+    template <int STRIDE>
+    __device__ __forceinline__ void store_raw(T* tile) const {
+        T* to = tile + int(threadIdx.x) / PER * STRIDE + int(threadIdx.x) % PER * R::VE;
+#pragma unroll
+        for (int i = 0; i < N; ++i, to += NTH / PER * STRIDE) {
+            if (ALL % NTH != 0 && int(threadIdx.x) + i * NTH >= ALL) continue;
+            *reinterpret_cast<uint4*>(to) = v[i];
+        }
+    }
 };
+// 32 rows of column `block16(t)` + c of a raw tile, in the order of two result tiles; and as an operand
+template <typename T, int STRIDE>
+__device__ __forceinline__ void raw_col(const T* at, int t, int lane, f4& lo, f4& hi, u4 (&f)[kTerms<T>]) {
+    if constexpr (sizeof(T) == 2) {
+        const u4 w = load_tokens<STRIDE>(reinterpret_cast<const uint16_t*>(at), block16(t, lane), lane);
+        float x[8];
+        rowvec<T>::unpack(make_uint4(w.x, w.y, w.z, w.w), x);
+        lo = f4{x[0], x[1], x[2], x[3]};
+        hi = f4{x[4], x[5], x[6], x[7]};
+        if constexpr (kTerms<T> == 1) f[0] = w;
+        else pack<kTerms<T>>(lo, hi, f);
+    } else {
+        const T* p = at + 4 * (lane >> 4) * STRIDE + 16 * t + (lane & 15);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            lo[r] = p[r * STRIDE];
+            hi[r] = p[(16 + r) * STRIDE];
+        }
+        pack<kTerms<T>>(lo, hi, f);
+    }
+}
 
 // A chunk's decays and rates.  G: sums of log2 decays from the chunk's start, in 64
 // bits, so that a difference of two keeps its bits however far they run.
@@ -183,6 +262,15 @@ __device__ __forceinline__ void put_gates(Gates<C>& s, float g, float beta, int 
 }
 __device__ __forceinline__ float factor(double Gi, double Gj) { return __builtin_amdgcn_exp2f(float(Gi - Gj)); }
 
+// What dr_prep leaves of a chunk: its gates, and T's lower tiles in fp32, each transposed
+// (element (row, column) of tile n at n * 256 + column * 16 + row).
+template <typename T, int KP> struct Plan {
+    Gates<Dims<T, KP>::C> gates;
+    float tri[Dims<T, KP>::NT * 256];
+};
+template <typename T, int KP>
+__device__ __forceinline__ Plan<T, KP>* plan_at(const DrParams& p, int64_t chunk) { return static_cast<Plan<T, KP>*>(p.plan) + chunk; }
+
 struct Head {
     int64_t bh, b, h, len;                 // len: the row's tokens
     __device__ __forceinline__ Head(const DrParams& p, int64_t bh_) : bh(bh_) {
@@ -193,10 +281,6 @@ struct Head {
     }
     template <typename T> __device__ __forceinline__ const T* rows(const LaRows& r, int64_t t) const {
         return static_cast<const T*>(r.p) + b * r.b + t * r.l + (h / r.rep) * r.h;
-    }
-    __device__ __forceinline__ float g(const DrParams& p, int64_t t) const { return t < len ? p.g[b * p.g_b + t * p.g_l + h * p.g_h] : 0.f; }
-    __device__ __forceinline__ float beta(const DrParams& p, int64_t t) const {
-        return t < len ? p.beta[b * p.be_b + t * p.be_l + h * p.be_h] : 0.f;
     }
 };
 
@@ -209,7 +293,7 @@ struct Head {
 template <typename T, int KP>
 __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams p) {
     using D = Dims<T, KP>;
-    constexpr int C = D::C, NR = D::NR, KT = D::KT, KST = D::KST, TERM = C * KST, NST = C + 4;
+    constexpr int C = D::C, NR = D::NR, KT = D::KT, KST = D::KST, TERM = C * KST, NST = C + 4, NTH = kPrepThreads<T, KP>;
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * TERM];
     __shared__ __attribute__((aligned(16))) float ns[C * NST], ts[NR][16 * 20];
     __shared__ Gates<C> gates;
@@ -218,16 +302,20 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
     if (t0 >= head.len) return;
     const int lane = int(threadIdx.x) & 63, w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), g = lane >> 4, c = lane & 15;
     const int cnt = head.len - t0 < C ? int(head.len - t0) : C;
+    Plan<T, KP>* plan = plan_at<T, KP>(p, head.bh * p.nch + n);
     {
-        Tile<T, KP, C, 64 * NR> k;
+        Tile<T, KP, C, NTH> k;
         k.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
         if (w == 0) {
-            const bool in = lane < C;
-            put_gates(gates, in ? head.g(p, t0 + lane) : 0.f, in ? head.beta(p, t0 + lane) : 0.f, lane);
+            const bool in = lane < cnt;
+            const float gv = in ? p.g[head.b * p.g_b + (t0 + lane) * p.g_l + head.h * p.g_h] : 0.f;
+            put_gates(gates, gv, in ? p.beta[head.b * p.be_b + (t0 + lane) * p.be_l + head.h * p.be_h] : 0.f, lane);
         }
-        k.store(ks);
+        k.template store<KST>(ks);
     }
     __syncthreads();
+    for (int i = int(threadIdx.x); i < int(sizeof(Gates<C>) / 16); i += NTH)
+        reinterpret_cast<uint4*>(&plan->gates)[i] = reinterpret_cast<const uint4*>(&gates)[i];
     // N's row of tiles, transposed: rows j, column i
     const double Gi = gates.G[16 * w + c];
 #pragma unroll
@@ -280,7 +368,6 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
         acc = __builtin_amdgcn_mfma_f32_16x16x4f32(v.z, b[2], acc, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_16x16x4f32(v.w, b[3], acc, 0, 0, 0);
     };
-    float* out = p.tri + (head.bh * p.nch + n) * (D::NT * 256);
 #pragma unroll
     for (int d = 0; d < NR; ++d) {
         const int i = w + d;
@@ -289,42 +376,34 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
             f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m < d; ++m) acc = mm(ns + (16 * i + c) * NST + 16 * (w + m) + 4 * g, t[m], acc);
-            f4 r = mm(&ts[i][c * 20 + 4 * g], acc, f4{0.f, 0.f, 0.f, 0.f});
-            t[d] = -r;
+            t[d] = -mm(&ts[i][c * 20 + 4 * g], acc, f4{0.f, 0.f, 0.f, 0.f});
         }
-        float* to = out + (i * (i + 1) / 2 + w) * 256;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) to[(4 * g + r) * 16 + c] = t[d][r];
+        *reinterpret_cast<f4*>(plan->tri + tile_at(i, w) * 256 + 16 * c + 4 * g) = t[d];
     }
 }
 
 // ----------------------------------------------------------------- walk --
-// A chunk's inverse on its way into LDS, in 3 terms (row-major, zero above the
-// diagonal tiles: the caller clears the tiles (2 p, 2 p + 1) once)
-template <int C, int NTH>
-struct Tri {
-    static constexpr int NR = C / 16, NT = NR * (NR + 1) / 2, N = (NT * 64 + NTH - 1) / NTH, CST = C + 8, TERM = C * CST;
-    float4 v[N];
-    __device__ __forceinline__ void load(const float* p) {
+// A chunk's plan on its way into LDS: the gates as they are, T in 3 terms.
+template <typename T, int KP, int NTH>
+struct PlanIn {
+    using D = Dims<T, KP>;
+    static constexpr int NG = sizeof(Gates<D::C>) / 16, N = (D::NT * 64 + NTH - 1) / NTH;
+    static_assert(NG <= NTH && sizeof(Gates<D::C>) % 16 == 0, "a vector of the gates a thread");
+    uint4 gates;
+    f4 v[N];
+    __device__ __forceinline__ void load(const Plan<T, KP>* p) {
+        const int tid = int(threadIdx.x);
+        if (tid < NG) gates = reinterpret_cast<const uint4*>(&p->gates)[tid];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = int(threadIdx.x) + i * NTH;
-            if (at < NT * 64) v[i] = *reinterpret_cast<const float4*>(p + 4 * at);
-        }
+        for (int i = 0; i < N; ++i)
+            if (D::NT * 64 % NTH == 0 || i + 1 < N || tid + i * NTH < D::NT * 64) v[i] = *reinterpret_cast<const f4*>(p->tri + 4 * (tid + i * NTH));
     }
-    __device__ __forceinline__ void store(uint16_t* tile) const {
+    __device__ __forceinline__ void store(Gates<D::C>& g, uint16_t* tri) const {
+        const int tid = int(threadIdx.x);
+        if (tid < NG) reinterpret_cast<uint4*>(&g)[tid] = gates;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = int(threadIdx.x) + i * NTH;
-            if (at >= NT * 64) continue;
-            const int idx = at >> 6, row = idx < 1 ? 0 : idx < 3 ? 1 : idx < 6 ? 2 : 3, col = idx - row * (row + 1) / 2;
-            uint16_t* to = tile + (16 * row + ((at >> 2) & 15)) * CST + 16 * col + 4 * (at & 3);
-            uint32_t s0[3], s1[3];
-            split<3>(v[i].x, v[i].y, s0);
-            split<3>(v[i].z, v[i].w, s1);
-#pragma unroll
-            for (int n = 0; n < 3; ++n) *reinterpret_cast<uint2*>(to + n * TERM) = make_uint2(s0[n], s1[n]);
-        }
+        for (int i = 0; i < N; ++i)
+            if (D::NT * 64 % NTH == 0 || i + 1 < N || tid + i * NTH < D::NT * 64) put4<3, D::NT * 256>(tri + 4 * (tid + i * NTH), v[i]);
     }
 };
 
@@ -337,121 +416,88 @@ struct Tri {
 template <typename T, int KP, bool REV, bool LOCAL>
 __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
     using D = Dims<T, KP>;
-    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, CST = D::CST;
-    constexpr int KTERM = C * KST, CTERM = C * CST;
+    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NT = D::NT, VST = D::VST;
+    constexpr int KTERM = C * KST, CTERM = NT * 256;
     constexpr int PT = REV ? 3 : D::OT;                   // P's terms
     constexpr bool Q = REV || !LOCAL;                     // whether q is read
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * KTERM], qs[Q ? KT * KTERM : 8], tri[3 * CTERM], prob[Q ? PT * CTERM : 8];
-    __shared__ Gates<C> gates[2];
+    __shared__ __attribute__((aligned(16))) T vs[C * VST];
+    __shared__ __attribute__((aligned(16))) Gates<C> G;
     const int segs = p.segs, seg = int(blockIdx.x % unsigned(segs));
     const Head head(p, blockIdx.x / unsigned(segs));
     const int vt = int(blockIdx.y), vtiles = (p.V + 63) / 64;
     const int tid = int(threadIdx.x), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const bool unit = LOCAL && vt >= vtiles;              // columns of the identity
-    const int col0 = (unit ? vt - vtiles : vt) * 64 + 16 * w, col = col0 + c;
-    const int cols = unit ? p.K : p.V, pitch = unit ? dr_round16(p.K) : p.Vp;
-    const bool live = col0 < cols, mine = !unit && col < p.V;
+    const int v0 = (unit ? vt - vtiles : vt) * 64, col0 = v0 + 16 * w, col = col0 + c;
+    const bool live = col0 < (unit ? p.K : p.V), mine = !unit && col < p.V;
     const int chunks = int((head.len + C - 1) / C);       // of the row
     const int n0 = seg * p.seg_chunks, n1 = n0 + p.seg_chunks < chunks ? n0 + p.seg_chunks : chunks;
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
 
-    // the state: tile t, register r is row state_row(t, g, r), column col
+    // the state: tile t, register r is row state_row(t, g, r), column col; 8 neighbouring rows a pair of tiles
     f4 S[NS];
-    {
-        const float* from = nullptr;
-        int64_t step = 0;
-        if (!LOCAL) {
-            if (segs > 1) from = p.seg_add + (head.bh * segs + seg) * p.K * p.Vp + col, step = p.Vp;
-            else if (p.init) from = p.init + head.bh * p.K * p.V + col, step = p.V;
+#pragma unroll
+    for (int t = 0; t < NS; ++t) S[t] = zero;
+    if (unit) {
+#pragma unroll
+        for (int t = 0; t < NS; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[t][r] = state_row(t, g, r) == col && col < p.K ? 1.f : 0.f;
+    } else if (!LOCAL && segs > 1) {
+        if (live) {
+#pragma unroll
+            for (int t = 0; t < NS; ++t)
+                if (state_row(t, g, 0) < p.Kp)
+                    S[t] = *reinterpret_cast<const f4*>(p.seg_add + ((head.bh * segs + seg) * p.Vp + col) * p.Kp + state_row(t, g, 0));
         }
+    } else if (!LOCAL && p.init) {
 #pragma unroll
         for (int t = 0; t < NS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int key = state_row(t, g, r);
-                S[t][r] = from && mine && key < p.K ? from[key * step] : unit && key == col && key < p.K ? 1.f : 0.f;
+                if (mine && key < p.K) S[t][r] = p.init[(head.bh * p.K + key) * p.V + col];
             }
     }
-    const auto put_state = [&](float* to, int64_t step, bool in) {
+    // kept states: a column's rows side by side (value column, key)
+    const auto keep_state = [&](float* to) {
+        float* at = to + int64_t(col) * p.Kp + 8 * g;
 #pragma unroll
         for (int t = 0; t < NS; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = state_row(t, g, r);
-                if (in && key < p.K) to[key * step] = S[t][r];
-            }
+            if (KP == p.Kp || state_row(t, g, 0) < p.Kp) *reinterpret_cast<f4*>(at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
     };
 
     Tile<T, KP, C, 256> kin, qin;
-    Tri<C, 256> tin;
-    float xin[NR][4], gin = 0.f, bin = 0.f;               // v (back: dout), rows 16 i + 4 g + r of column col
+    Tile<T, 64, C, 256> vin;                              // v (back: dout)
+    PlanIn<T, KP, 256> plan;
     const int step = REV ? -1 : 1, first = REV ? n1 - 1 : n0;
-    const auto count = [&](int n) { return head.len - int64_t(n) * C < C ? int(head.len - int64_t(n) * C) : C; };
-    const auto fetch_gates = [&](int n) {
-        const bool in = n >= n0 && n < n1 && lane < C;
-        gin = in ? head.g(p, int64_t(n) * C + lane) : 0.f;
-        bin = in ? head.beta(p, int64_t(n) * C + lane) : 0.f;
-    };
     const auto fetch = [&](int n) {
         if (n < n0 || n >= n1) return;
         const int64_t t0 = int64_t(n) * C;
-        const int cnt = count(n);
+        const int cnt = head.len - t0 < C ? int(head.len - t0) : C;
+        plan.load(plan_at<T, KP>(p, head.bh * p.nch + n));
         kin.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
         if constexpr (Q) qin.load(head.rows<T>(p.q, t0), p.q.l, cnt, p.K);
-        tin.load(p.tri + (head.bh * p.nch + n) * (D::NT * 256));
         const LaRows& rows = REV ? p.o : p.v;
-        const T* x = head.rows<T>(rows, t0) + col;
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r;
-                xin[i][r] = mine && row < cnt ? io<T>::load(x + row * rows.l) : 0.f;
-            }
+        vin.load(head.rows<T>(rows, t0) + v0, rows.l, unit ? 0 : cnt, p.V - v0);
     };
-    // (tiles above the diagonal that pairs of tiles take in: zero for good)
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        for (int e = tid; e < 16 * 16; e += 256) {
-            const int at = (32 * i + (e >> 4)) * CST + 32 * i + 16 + (e & 15);
-#pragma unroll
-            for (int n = 0; n < 3; ++n) tri[n * CTERM + at] = 0;
-            if constexpr (Q) {
-#pragma unroll
-                for (int n = 0; n < PT; ++n) prob[n * CTERM + at] = 0;
-            }
-        }
-    }
-    if (n0 < n1) {
-        fetch_gates(first);
-        fetch(first);
-        if (w == 0) put_gates(gates[first & 1], gin, bin, lane);
-        fetch_gates(first + step);
-    }
+    fetch(first);
     for (int n = first; n >= n0 && n < n1; n += step) {
         const int64_t at = head.bh * p.nch + n, t0 = int64_t(n) * C;
-        const Gates<C>& G = gates[n & 1];
-        __syncthreads();                                  // (the tiles of the chunk before are done with)
-        kin.store(ks);
-        if constexpr (Q) qin.store(qs);
-        tin.store(tri);
-        f4 x[NR];
-#pragma unroll
-        for (int i = 0; i < NR; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[i][r] = xin[i][r];
-        __syncthreads();
+        lds_barrier();                                    // (the tiles of the chunk before are done with)
+        kin.template store<KST>(ks);
+        if constexpr (Q) qin.template store<KST>(qs);
+        vin.template store_raw<VST>(vs);
+        plan.store(G, tri);
+        lds_barrier();
         fetch(n + step);
-        if (w == 0) {
-            put_gates(gates[(n + 1) & 1], gin, bin, lane);
-            fetch_gates(n + 2 * step);
-        }
         if constexpr (Q) {                                // P, a share of its tiles a wave; formed transposed, rows j, column i
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
 #pragma unroll
                 for (int j = 0; j <= i; ++j) {
-                    if (((i * (i + 1) / 2 + j) & 3) != w) continue;
-                    f4 acc = {0.f, 0.f, 0.f, 0.f};
+                    if ((tile_at(i, j) & 3) != w) continue;
+                    f4 acc = zero;
 #pragma unroll
                     for (int kk = 0; kk < NK; ++kk) {
                         u4 a[KT], b[KT];
@@ -463,14 +509,10 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int row = 16 * j + 4 * g + r;
-                        acc[r] = row <= 16 * i + c ? acc[r] * factor(Gi, G.G[row]) : 0.f;
+                        const float f = factor(Gi, G.G[row]);
+                        acc[r] = j < i || row <= 16 * i + c ? acc[r] * f : 0.f;
                     }
-                    uint32_t s0[PT], s1[PT];
-                    split<PT>(acc[0], acc[1], s0);
-                    split<PT>(acc[2], acc[3], s1);
-#pragma unroll
-                    for (int m = 0; m < PT; ++m)
-                        *reinterpret_cast<uint2*>(prob + m * CTERM + (16 * i + c) * CST + 16 * j + 4 * g) = make_uint2(s0[m], s1[m]);
+                    put4<PT, CTERM>(prob + tile_at(i, j) * 256 + 16 * c + 4 * g, acc);
                 }
             }
         }
@@ -478,10 +520,10 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
             f4 O[NR];                                     // out, transposed: rows value columns, column token i
             u4 uf[NP][D::OT];
             if (live) {
-                if (!LOCAL && p.states) put_state(p.states + at * p.K * p.Vp + col, p.Vp, true);
+                if (!LOCAL && p.states) keep_state(p.states + at * p.Vp * p.Kp);
                 f4 Y[NR];
 #pragma unroll
-                for (int i = 0; i < NR; ++i) Y[i] = O[i] = f4{0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < NR; ++i) Y[i] = O[i] = zero;
 #pragma unroll
                 for (int kk = 0; kk < NK; ++kk) {
                     u4 sf[3];
@@ -499,53 +541,58 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 }
                 u4 yf[NP][3];
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    const f4 gam = *reinterpret_cast<const f4*>(G.gam + 16 * i + 4 * g);
+                for (int q = 0; q < NP; ++q) {
+                    f4 lo, hi;
+                    u4 raw[KT];
+                    raw_col<T, VST>(vs + 32 * q * VST, w, lane, lo, hi, raw);
+                    const f4 glo = *reinterpret_cast<const f4*>(G.gam + 32 * q + 4 * g), ghi = *reinterpret_cast<const f4*>(G.gam + 32 * q + 16 + 4 * g);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) Y[i][r] = __builtin_fmaf(-gam[r], Y[i][r], x[i][r]);
+                    for (int r = 0; r < 4; ++r) {
+                        lo[r] = __builtin_fmaf(-glo[r], Y[2 * q][r], lo[r]);
+                        hi[r] = __builtin_fmaf(-ghi[r], Y[2 * q + 1][r], hi[r]);
+                    }
+                    pack<3>(lo, hi, yf[q]);
                 }
-#pragma unroll
-                for (int q = 0; q < NP; ++q) pack<3>(Y[2 * q], Y[2 * q + 1], yf[q]);
                 f4 U[NR];
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
-                    f4 E = {0.f, 0.f, 0.f, 0.f};
+                    U[i] = zero;
 #pragma unroll
                     for (int q = 0; q <= i / 2; ++q) {
                         u4 a[3];
-                        frag44<3, CTERM>(tri + (16 * i + c) * CST + 32 * q + 4 * g, a);
-                        mac<3, 3, 2>(a, yf[q], E);
+                        frag_tiles<3, CTERM, true>(tri, tile_at(i, 2 * q), tile_at(i, 2 * q + 1), lane, a);
+                        mac<3, 3, 2>(a, yf[q], U[i]);
                     }
-                    if (!LOCAL && p.err) {
-                        float* to = p.err + (at * C + 16 * i + 4 * g) * p.Vp + col;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) to[r * p.Vp] = E[r];
-                    }
-                    U[i] = E * *reinterpret_cast<const f4*>(G.beta + 16 * i + 4 * g);
                 }
+                if (!LOCAL && p.err) {                    // (value column, token)
+                    float* to = p.err + (at * p.Vp + col) * C + 4 * g;
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) *reinterpret_cast<f4*>(to + 16 * i) = U[i];
+                }
+#pragma unroll
+                for (int i = 0; i < NR; ++i) U[i] *= *reinterpret_cast<const f4*>(G.beta + 16 * i + 4 * g);
                 if constexpr (!LOCAL) {
 #pragma unroll
                     for (int q = 0; q < NP; ++q) pack<D::OT>(U[2 * q], U[2 * q + 1], uf[q]);
                 }
-                u4 wf[NP][3];
-#pragma unroll
-                for (int q = 0; q < NP; ++q)
-                    pack<3>(U[2 * q] * *reinterpret_cast<const f4*>(G.end + 32 * q + 4 * g),
-                            U[2 * q + 1] * *reinterpret_cast<const f4*>(G.end + 32 * q + 16 + 4 * g), wf[q]);
                 const float total = G.total;
 #pragma unroll
-                for (int t = 0; t < NS; ++t) {
-                    S[t] *= total;
+                for (int t = 0; t < NS; ++t) S[t] *= total;
 #pragma unroll
-                    for (int q = 0; q < NP; ++q) {
+                for (int q = 0; q < NP; ++q) {
+                    u4 wf[3];
+                    pack<3>(U[2 * q] * *reinterpret_cast<const f4*>(G.end + 32 * q + 4 * g),
+                            U[2 * q + 1] * *reinterpret_cast<const f4*>(G.end + 32 * q + 16 + 4 * g), wf);
+#pragma unroll
+                    for (int t = 0; t < NS; ++t) {
                         u4 a[KT];
                         frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a);
-                        mac<KT, 3, 2>(a, wf[q], S[t]);
+                        mac<KT, 3, 2>(a, wf, S[t]);
                     }
                 }
             }
             if constexpr (!LOCAL) {
-                __syncthreads();                          // P is there
+                lds_barrier();                            // P is there
                 if (live) {
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
@@ -553,7 +600,7 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
 #pragma unroll
                         for (int q = 0; q <= i / 2; ++q) {
                             u4 b[PT];
-                            frag44<PT, CTERM>(prob + (16 * i + c) * CST + 32 * q + 4 * g, b);
+                            frag_tiles<PT, CTERM, false>(prob, tile_at(i, 2 * q), tile_at(i, 2 * q + 1), lane, b);
                             mac<D::OT, PT, D::OT - 1>(uf[q], b, O[i]);
                         }
                         const int64_t t = t0 + 16 * i + c;
@@ -564,12 +611,11 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 }
             }
         } else {
-            if (live && !LOCAL) put_state(p.dstates + at * p.K * p.Vp + col, p.Vp, true);
-            __syncthreads();                              // P is there
+            if (live && !LOCAL) keep_state(p.dstates + at * p.Vp * p.Kp);
+            f4 X[NR];
             if (live) {
-                f4 X[NR];
 #pragma unroll
-                for (int i = 0; i < NR; ++i) X[i] = f4{0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < NR; ++i) X[i] = zero;
 #pragma unroll
                 for (int kk = 0; kk < NK; ++kk) {
                     u4 sf[3];
@@ -581,16 +627,20 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                         mac<KT, 3, 2>(a, sf, X[i]);
                     }
                 }
+            }
+            lds_barrier();                                // P is there
+            if (live) {
+                f4 x[NR];
                 u4 df[NP][KT];
 #pragma unroll
-                for (int q = 0; q < NP; ++q) pack<KT>(x[2 * q], x[2 * q + 1], df[q]);
+                for (int q = 0; q < NP; ++q) raw_col<T, VST>(vs + 32 * q * VST, w, lane, x[2 * q], x[2 * q + 1], df[q]);
 #pragma unroll
                 for (int j = 0; j < NR; ++j) {
-                    f4 acc = {0.f, 0.f, 0.f, 0.f};
+                    f4 acc = zero;
 #pragma unroll
                     for (int q = j / 2; q < NP; ++q) {
                         u4 a[PT];
-                        frag_col<PT, CTERM, CST>(prob + 32 * q * CST, block16(j, lane), lane, a);
+                        frag_tiles<PT, CTERM, true>(prob, tile_at(2 * q, j), tile_at(2 * q + 1, j), lane, a);
                         mac<PT, KT, 2>(a, df[q], acc);
                     }
                     const f4 end = *reinterpret_cast<const f4*>(G.end + 16 * j + 4 * g), beta = *reinterpret_cast<const f4*>(G.beta + 16 * j + 4 * g);
@@ -603,54 +653,60 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 f4 F[NR];
 #pragma unroll
                 for (int j = 0; j < NR; ++j) {
-                    F[j] = f4{0.f, 0.f, 0.f, 0.f};
+                    F[j] = zero;
 #pragma unroll
                     for (int q = j / 2; q < NP; ++q) {
                         u4 a[3];
-                        frag_col<3, CTERM, CST>(tri + 32 * q * CST, block16(j, lane), lane, a);
+                        frag_tiles<3, CTERM, false>(tri, tile_at(2 * q, j), tile_at(2 * q + 1, j), lane, a);
                         mac<3, 3, 2>(a, xf[q], F[j]);
                     }
-                    if (!LOCAL) {
-                        float* to = p.derr + (at * C + 16 * j + 4 * g) * p.Vp + col;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) to[r * p.Vp] = F[j][r];
-                    }
                 }
-                u4 gf[NP][3], ff[NP][3];
+                if (!LOCAL) {                             // (value column, token)
+                    float* to = p.derr + (at * p.Vp + col) * C + 4 * g;
 #pragma unroll
-                for (int q = 0; q < NP; ++q) {
-                    const f4 lo = *reinterpret_cast<const f4*>(G.gam + 32 * q + 4 * g), hi = *reinterpret_cast<const f4*>(G.gam + 32 * q + 16 + 4 * g);
-                    pack<3>(x[2 * q] * (p.scale * lo), x[2 * q + 1] * (p.scale * hi), gf[q]);
-                    pack<3>(-(F[2 * q] * lo), -(F[2 * q + 1] * hi), ff[q]);
+                    for (int j = 0; j < NR; ++j) *reinterpret_cast<f4*>(to + 16 * j) = F[j];
                 }
                 const float total = G.total;
 #pragma unroll
-                for (int t = 0; t < NS; ++t) {
-                    S[t] *= total;
+                for (int t = 0; t < NS; ++t) S[t] *= total;
 #pragma unroll
-                    for (int q = 0; q < NP; ++q) {
+                for (int q = 0; q < NP; ++q) {
+                    const f4 lo = *reinterpret_cast<const f4*>(G.gam + 32 * q + 4 * g), hi = *reinterpret_cast<const f4*>(G.gam + 32 * q + 16 + 4 * g);
+                    u4 gf[3], ff[3];
+                    pack<3>(x[2 * q] * (p.scale * lo), x[2 * q + 1] * (p.scale * hi), gf);
+                    pack<3>(-(F[2 * q] * lo), -(F[2 * q + 1] * hi), ff);
+#pragma unroll
+                    for (int t = 0; t < NS; ++t) {
                         u4 a[KT];
                         frag_col<KT, KTERM, KST>(qs + 32 * q * KST, state_block(t, lane), lane, a);
-                        mac<KT, 3, 2>(a, gf[q], S[t]);
+                        mac<KT, 3, 2>(a, gf, S[t]);
                         frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a);
-                        mac<KT, 3, 2>(a, ff[q], S[t]);
+                        mac<KT, 3, 2>(a, ff, S[t]);
                     }
                 }
             }
         }
     }
     if constexpr (LOCAL) {
-        float* to = unit ? p.seg_mul : p.seg_add;
-        if (live) put_state(to + (head.bh * segs + seg) * p.K * pitch + col, pitch, col < pitch);
+        if (live && unit) keep_state(p.seg_mul + (head.bh * segs + seg) * p.Kp * p.Kp);
+        else if (live) keep_state(p.seg_add + (head.bh * segs + seg) * p.Vp * p.Kp);
     } else {
         // the segment that the walk ends with: forward the one with the row's last token
         const int end = REV || chunks == 0 ? 0 : (chunks - 1) / p.seg_chunks;
-        if (p.last && seg == end) put_state(p.last + head.bh * p.K * p.V + col, p.V, mine);
+        if (p.last && seg == end && mine) {
+#pragma unroll
+            for (int t = 0; t < NS; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int key = state_row(t, g, r);
+                    if (key < p.K) p.last[(head.bh * p.K + key) * p.V + col] = S[t][r];
+                }
+        }
         if (!REV) {                                       // zero out past the row's tokens
             const int64_t from = head.len > int64_t(n0) * C ? head.len : int64_t(n0) * C, all = int64_t(n0 + p.seg_chunks) * C;
             const int64_t to = all < p.L ? all : p.L;
             for (int64_t t = from + w; t < to; t += 4)
-                if (vt * 64 + lane < p.V) io<T>::store(const_cast<T*>(head.rows<T>(p.o, t)) + vt * 64 + lane, 0.f);
+                if (v0 + lane < p.V) io<T>::store(const_cast<T*>(head.rows<T>(p.o, t)) + v0 + lane, 0.f);
         }
     }
 }
@@ -671,20 +727,23 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
 // formula, and dg_t is zero where the decay empties the state.
 //
 // Waves 0 .. NR - 1 take 16 tokens each as readers (columns i of the transposed
-// tiles), waves NR .. 2 NR - 1 as writers (columns j); the writer's share of dk passes
-// to the reader through LDS.
+// tiles), waves NR .. 2 NR - 1 as writers (columns j): a reader has w + 1 tiles of M and R and the
+// writer on its SIMD the other NR - w.  The writer's share of dk passes to the reader
+// through LDS.  Value columns pass 32 at a time, those of the next step on their way meanwhile.
 template <typename T, int KP>
 __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams p) {
     using D = Dims<T, KP>;
-    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, VST = D::VST, NTH = kGradThreads<T, KP>;
-    constexpr int KTERM = C * KST, VTERM = C * VST, XT = D::OT;
-    struct Rows { uint16_t e[3 * VTERM], f[3 * VTERM], d[KT * VTERM]; };
+    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NTH = kGradThreads<T, KP>;
+    constexpr int VW = D::VW, KW = D::KW, SST = KW + 8, EST = C + 8, DST = VW + 8, XT = D::OT;
+    constexpr int KTERM = C * KST, STERM = VW * SST, ETERM = VW * EST, DTERM = C * DST;
+    // S, dS' (rows value columns, columns keys), E, F (columns tokens), dout (rows tokens)
+    struct Stage { uint16_t s[3 * STERM], t[3 * STERM], e[3 * ETERM], f[3 * ETERM], d[KT * DTERM]; };
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * KTERM], qs[KT * KTERM];
-    __shared__ __attribute__((aligned(16))) Rows rows;
-    __shared__ Gates<C> gates;
-    __shared__ float across[NR][C], reads[C], writes[C], inner[NR], dbeta[C];
+    __shared__ __attribute__((aligned(16))) Stage st;
+    __shared__ __attribute__((aligned(16))) Gates<C> gates;
+    __shared__ float across[NR][C], reads[C], writes[C], inner[2 * NR], dbeta[C];
     constexpr int HALF = KP > 128 ? 128 : KP;             // keys of dk that pass through LDS at a time
-    static_assert(sizeof(Rows) >= sizeof(float) * C * (HALF + 4), "dk's share over the rows' tiles");
+    static_assert(sizeof(Stage) >= sizeof(float) * C * (HALF + 4), "dk's share over the tiles");
     const Head head(p, blockIdx.x / unsigned(p.nch));
     const int n = int(blockIdx.x % unsigned(p.nch));
     const int64_t t0 = int64_t(n) * C, at = head.bh * p.nch + n;
@@ -693,136 +752,158 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     const int w = reader ? wave : wave - NR, own = 16 * w + c;
     const int cnt = head.len - t0 < C ? int(head.len > t0 ? head.len - t0 : 0) : C;
     const int toks = p.L - t0 < C ? int(p.L - t0) : C;    // to be written
-    // element (t, h, 0) of a contiguous (B, L, heads, dim) tensor
-    const auto row_of = [&](int64_t t, int64_t heads, int64_t h, int dim) { return ((head.b * p.L + t) * heads + h) * dim; };
     const bool part = p.rep > 1;
-    // 4 neighbouring elements of dq or dk
-    const auto put_keys = [&](void* to, int64_t t, int key, const float (&v)[4]) {
-        if (key >= p.K) return;
-        if (part) store4<float>(static_cast<float*>(to) + row_of(t, p.H, head.h, p.K) + key, v, p.K - key);
-        else store4<T>(static_cast<T*>(to) + row_of(t, p.H, head.h, p.K) + key, v, p.K - key);
+    // rows of contiguous (B, L, heads, dim) tensors
+    const auto row_of = [&](int t, int dim) { return ((head.b * p.L + t0 + t) * p.H + head.h) * dim; };
+    // 8 neighbouring elements of a row of type O, those below dim
+    const auto put8 = [&](auto* row, int from, int dim, const f4& lo, const f4& hi) {
+        using O = std::remove_pointer_t<decltype(row)>;
+        using R = rowvec<O>;
+        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+        for (int h = 0; h < 8; h += R::VE) {
+            float x[R::VE];
+#pragma unroll
+            for (int e = 0; e < R::VE; ++e) x[e] = v[h + e];
+            R::store(row + from + h, x, dim - (from + h));
+        }
     };
+    const auto put_keys = [&](void* to, int t, int key, const f4& lo, const f4& hi) {
+        if (part) put8(static_cast<float*>(to) + row_of(t, p.K), key, p.K, lo, hi);
+        else put8(static_cast<T*>(to) + row_of(t, p.K), key, p.K, lo, hi);
+    };
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
     if (cnt == 0) {                                       // (no token: every gradient is zero)
-        const float none[4] = {0.f, 0.f, 0.f, 0.f};
         for (int t = wave; t < toks; t += NTH / 64) {
-            put_keys(p.dq, t0 + t, 4 * lane, none);
-            put_keys(p.dk, t0 + t, 4 * lane, none);
-            if (4 * lane < p.V) store4<T>(static_cast<T*>(p.dv) + row_of(t0 + t, p.H, head.h, p.V) + 4 * lane, none, p.V - 4 * lane);
-            if (lane == 0) p.dg[row_of(t0 + t, p.H, head.h, 1)] = p.dbeta[row_of(t0 + t, p.H, head.h, 1)] = 0.f;
+            put_keys(p.dq, t, 8 * lane, zero, zero);
+            put_keys(p.dk, t, 8 * lane, zero, zero);
+            put8(static_cast<T*>(p.dv) + row_of(t, p.V), 8 * lane, p.V, zero, zero);
+            if (lane == 0) p.dg[row_of(t, 1)] = p.dbeta[row_of(t, 1)] = 0.f;
         }
         return;
     }
-    {
-        Tile<T, KP, C, NTH> in;
-        in.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
-        if (wave == 0) {
-            const bool on = lane < C;
-            put_gates(gates, on ? head.g(p, t0 + lane) : 0.f, on ? head.beta(p, t0 + lane) : 0.f, lane);
+
+    // a step: VW value columns of E, F and dout (with the first of its states' keys), KW keys of S and dS'
+    constexpr int NSV = VW * KW / 4 / NTH, NEV = VW * C / 4 / NTH;
+    static_assert(VW * KW / 4 % NTH == 0 && VW * C / 4 % NTH == 0, "whole vectors a thread");
+    f4 si[NSV], ti[NSV], ei[NEV], fi[NEV];
+    Tile<T, VW, C, NTH> di;
+    const auto fetch = [&](int v0, int k0) {
+        if (v0 >= p.V) return;
+#pragma unroll
+        for (int i = 0; i < NSV; ++i) {
+            const int x = tid + i * NTH, v = v0 + x / (KW / 4), key = k0 + x % (KW / 4) * 4;
+            const bool in = v < p.Vp && key < p.Kp;
+            const int64_t from = (at * p.Vp + v) * p.Kp + key;
+            si[i] = in ? *reinterpret_cast<const f4*>(p.states + from) : zero;
+            ti[i] = in ? *reinterpret_cast<const f4*>(p.dstates + from) : zero;
         }
-        in.store(ks);
-        in.load(head.rows<T>(p.q, t0), p.q.l, cnt, p.K);
-        in.store(qs);
+        if (k0 > 0) return;
+#pragma unroll
+        for (int i = 0; i < NEV; ++i) {
+            const int x = tid + i * NTH, v = v0 + x / (C / 4);
+            const int64_t from = (at * p.Vp + v) * C + x % (C / 4) * 4;
+            ei[i] = v < p.Vp ? *reinterpret_cast<const f4*>(p.err + from) : zero;
+            fi[i] = v < p.Vp ? *reinterpret_cast<const f4*>(p.derr + from) : zero;
+        }
+        di.load(head.rows<T>(p.o, t0) + v0, p.o.l, cnt, p.V - v0);
+    };
+    fetch(0, 0);
+    {
+        Tile<T, KP, C, NTH> kin, qin;
+        kin.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
+        qin.load(head.rows<T>(p.q, t0), p.q.l, cnt, p.K);
+        if (tid < int(sizeof(Gates<C>) / 16))
+            reinterpret_cast<uint4*>(&gates)[tid] = reinterpret_cast<const uint4*>(&plan_at<T, KP>(p, at)->gates)[tid];
+        kin.template store<KST>(ks);
+        qin.template store<KST>(qs);
     }
-    const f4 zero = {0.f, 0.f, 0.f, 0.f};
     f4 M[NR], R[NR], dq[NS], dk[NS];                      // reader: M, R transposed (rows j); writer: rows i, and no dq
 #pragma unroll
     for (int i = 0; i < NR; ++i) M[i] = R[i] = zero;
 #pragma unroll
     for (int t = 0; t < NS; ++t) dq[t] = dk[t] = zero;
     float z = 0.f;
-    for (int v0 = 0; v0 < p.V; v0 += 64) {
-        __syncthreads();
-        {
-            Tile<T, 64, C, NTH> in;
-            static_assert(Tile<T, 64, C, NTH>::KST == VST, "the same rows");
-            in.load(head.rows<T>(p.o, t0) + v0, p.o.l, cnt, p.V - v0);
-            in.store(rows.d);
-            // E and F: 16 vectors of 4 a row
+    for (int v0 = 0; v0 < p.V; v0 += VW) {
 #pragma unroll
-            for (int i = 0; i < C * 16 / NTH; ++i) {
-                const int e = tid + i * NTH, row = e >> 4, col = 4 * (e & 15);
-                const bool on = v0 + col < p.Vp;
-                const int64_t from = (at * C + row) * p.Vp + v0 + col;
-                const f4 ev = on ? *reinterpret_cast<const f4*>(p.err + from) : zero, fv = on ? *reinterpret_cast<const f4*>(p.derr + from) : zero;
-                uint32_t a[3], b[3], x[3], y[3];
-                split<3>(ev[0], ev[1], a);
-                split<3>(ev[2], ev[3], b);
-                split<3>(fv[0], fv[1], x);
-                split<3>(fv[2], fv[3], y);
+        for (int k0 = 0; k0 < KP; k0 += KW) {
+            lds_barrier();
 #pragma unroll
-                for (int m = 0; m < 3; ++m) {
-                    *reinterpret_cast<uint2*>(rows.e + m * VTERM + row * VST + col) = make_uint2(a[m], b[m]);
-                    *reinterpret_cast<uint2*>(rows.f + m * VTERM + row * VST + col) = make_uint2(x[m], y[m]);
-                }
-                if (row < toks && v0 + col < p.V) {
-                    const bool is = row < cnt && gates.beta[row] != 0.f;
-                    const float o[4] = {is ? fv[0] : 0.f, is ? fv[1] : 0.f, is ? fv[2] : 0.f, is ? fv[3] : 0.f};
-                    store4<T>(static_cast<T*>(p.dv) + row_of(t0 + row, p.H, head.h, p.V) + v0 + col, o, p.V - (v0 + col));
-                }
+            for (int i = 0; i < NSV; ++i) {
+                const int x = tid + i * NTH, to = x / (KW / 4) * SST + x % (KW / 4) * 4;
+                put4<3, STERM>(st.s + to, si[i]);
+                put4<3, STERM>(st.t + to, ti[i]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z = __builtin_fmaf(si[i][r], ti[i][r], z);
             }
-        }
-        __syncthreads();
-        const int vks = p.Vp - v0 > 32 ? 2 : 1;
-        for (int kk = 0; kk < vks; ++kk) {
-            const int vcol = 32 * kk + 8 * g;
-            // operand rows of the state at `s`: row state_row's m = c of tile t, 8 value columns
-            const auto state_at = [&](const float* s, int t, f4& lo, f4& hi) {
-                const int key = 32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3);
-                const bool on = key < p.K && v0 + vcol < p.Vp;
-                const float* from = s + (at * p.K + key) * p.Vp + v0 + vcol;
-                lo = on ? *reinterpret_cast<const f4*>(from) : zero;
-                hi = on ? *reinterpret_cast<const f4*>(from + 4) : zero;
-            };
+            if (k0 == 0) {
+#pragma unroll
+                for (int i = 0; i < NEV; ++i) {
+                    const int x = tid + i * NTH, to = x / (C / 4) * EST + x % (C / 4) * 4;
+                    put4<3, ETERM>(st.e + to, ei[i]);
+                    put4<3, ETERM>(st.f + to, fi[i]);
+                }
+                di.template store<DST>(st.d);
+            }
+            lds_barrier();
+            if (k0 + KW < KP) fetch(v0, k0 + KW);
+            else fetch(v0 + VW, 0);
             if (reader) {
                 u4 df[KT], ff[3];
-                frag8<KT, VTERM>(rows.d + own * VST + vcol, df);
-                frag8<3, VTERM>(rows.f + own * VST + vcol, ff);
+                frag8<KT, DTERM>(st.d + own * DST + 8 * g, df);
+                frag_col8<3, ETERM, EST>(st.f, block16(w, lane), lane, ff);
+                if (k0 == 0) {
 #pragma unroll
-                for (int j = 0; j < NR; ++j) {
-                    if (j > w) continue;
-                    u4 a[3];
-                    frag8<3, VTERM>(rows.e + (16 * j + c) * VST + vcol, a);
-                    mac<3, KT, 2>(a, df, R[j]);
-                    mac<3, 3, 2>(a, ff, M[j]);
+                    for (int j = 0; j < NR; ++j) {
+                        if (j > w) continue;
+                        u4 a[3];
+                        frag_col8<3, ETERM, EST>(st.e, block16(j, lane), lane, a);
+                        mac<3, KT, 2>(a, df, R[j]);
+                        mac<3, 3, 2>(a, ff, M[j]);
+                    }
+                    if (own < toks) {                     // dv: F of the own token
+                        const bool is = own < cnt && gates.beta[own] != 0.f;
+                        f4 x[2];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const auto half = [&](const u4& t) { return e & 1 ? hi_half(t[e >> 1]) : lo_half(t[e >> 1]); };
+                            x[e >> 2][e & 3] = is ? half(ff[0]) + (half(ff[1]) + half(ff[2])) : 0.f;
+                        }
+                        put8(static_cast<T*>(p.dv) + row_of(own, p.V), v0 + 8 * g, p.V, x[0], x[1]);
+                    }
                 }
 #pragma unroll
-                for (int t = 0; t < NS; ++t) {
-                    f4 lo, hi;
+                for (int t = k0 / 16; t < (k0 + KW) / 16; ++t) {
                     u4 a[3];
-                    state_at(p.states, t, lo, hi);
-                    pack<3>(lo, hi, a);
+                    frag_col8<3, STERM, SST>(st.s - k0, state_block(t, lane), lane, a);
                     mac<3, KT, 2>(a, df, dq[t]);
                     mac<3, 3, 2>(a, ff, dk[t]);
                 }
             } else {
                 u4 ef[3];
-                frag8<3, VTERM>(rows.e + own * VST + vcol, ef);
+                frag_col8<3, ETERM, EST>(st.e, block16(w, lane), lane, ef);
+                if (k0 == 0) {
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    if (i < w) continue;
-                    u4 a[3], d[KT];
-                    frag8<3, VTERM>(rows.f + (16 * i + c) * VST + vcol, a);
-                    frag8<KT, VTERM>(rows.d + (16 * i + c) * VST + vcol, d);
-                    mac<3, 3, 2>(a, ef, M[i]);
-                    mac<KT, 3, 2>(d, ef, R[i]);
+                    for (int i = 0; i < NR; ++i) {
+                        if (i < w) continue;
+                        u4 a[3], d[KT];
+                        frag_col8<3, ETERM, EST>(st.f, block16(i, lane), lane, a);
+                        frag8<KT, DTERM>(st.d + (16 * i + c) * DST + 8 * g, d);
+                        mac<3, 3, 2>(a, ef, M[i]);
+                        mac<KT, 3, 2>(d, ef, R[i]);
+                    }
                 }
 #pragma unroll
-                for (int t = 0; t < NS; ++t) {
-                    f4 lo, hi;
+                for (int t = k0 / 16; t < (k0 + KW) / 16; ++t) {
                     u4 a[3];
-                    state_at(p.dstates, t, lo, hi);
-                    pack<3>(lo, hi, a);
+                    frag_col8<3, STERM, SST>(st.t - k0, state_block(t, lane), lane, a);
                     mac<3, 3, 2>(a, ef, dk[t]);
-                    if (t % NR == w) {
-                        f4 slo, shi;
-                        state_at(p.states, t, slo, shi);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) z = __builtin_fmaf(lo[r], slo[r], __builtin_fmaf(hi[r], shi[r], z));
-                    }
                 }
             }
         }
     }
+    z = lanes_sum<64>(z);
+    if (lane == 0) inner[wave] = z;
     // 8 keys 32 a + 8 g .. of the own token, of a row tile
     const auto keys8 = [&](const uint16_t* tile, int a, float (&v)[8]) {
         u4 t[KT];
@@ -840,12 +921,6 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     };
     const double Gown = gates.G[own];
     const float bown = gates.beta[own];
-    u4 qf[NK][KT], kf[NK][KT];                            // the own tokens' rows as operands
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-        frag8<KT, KTERM>(qs + own * KST + 32 * kk + 8 * g, qf[kk]);
-        frag8<KT, KTERM>(ks + own * KST + 32 * kk + 8 * g, kf[kk]);
-    }
     if (reader) {
         const float gam = gates.gam[own];
         float r = 0.f;
@@ -871,10 +946,12 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             f4 kq = zero, kk2 = zero;
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) {
-                u4 a[KT];
+                u4 a[KT], b[KT];
                 frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a);
-                mac<KT, KT, 2>(a, qf[kk], kq);
-                mac<KT, KT, 2>(a, kf[kk], kk2);
+                frag8<KT, KTERM>(qs + own * KST + 32 * kk + 8 * g, b);
+                mac<KT, KT, 2>(a, b, kq);
+                frag8<KT, KTERM>(ks + own * KST + 32 * kk + 8 * g, b);
+                mac<KT, KT, 2>(a, b, kk2);
             }
             const f4 beta = *reinterpret_cast<const f4*>(gates.beta + 16 * j + 4 * g);
             float term[4], sum = 0.f;
@@ -891,7 +968,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             // dg of token t, tile j's rows: the terms of earlier rows, over the columns i >= t
             float lead = __shfl_up(sum, 16, 64);
             lead = g >= 1 ? lead : 0.f;
-            float two = __shfl_up(lead + sum, 32, 64);    // (groups g - 2 and g - 3)
+            const float two = __shfl_up(lead + sum, 32, 64);    // (groups g - 2 and g - 3)
             float pre = before + lead + (g >= 2 ? two : 0.f);
             before += groups_sum(sum);
 #pragma unroll
@@ -932,8 +1009,6 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         }
         r = groups_sum(r);
         if (g == 0) writes[own] = r;
-        z = lanes_sum<64>(z);
-        if (lane == 0) inner[w] = z;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             if (i < w) continue;
@@ -961,26 +1036,25 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             }
         }
     }
-    float* share = reinterpret_cast<float*>(&rows);       // (C, HALF + 4)
+    float* share = reinterpret_cast<float*>(&st);         // (C, HALF + 4)
     const bool on = own < cnt;
 #pragma unroll
     for (int k0 = 0; k0 < KP; k0 += HALF) {
-        __syncthreads();                                  // (the rows' tiles, or the half before, are done with)
+        lds_barrier();                                    // (the tiles, or the half before, are done with)
         if (!reader) {
 #pragma unroll
             for (int t = k0 / 16; t < (k0 + HALF) / 16; ++t)
                 *reinterpret_cast<f4*>(share + own * (HALF + 4) + state_row(t, g, 0) - k0) = dk[t];
         }
-        __syncthreads();
+        lds_barrier();
         if (reader && own < toks) {
 #pragma unroll
-            for (int t = k0 / 16; t < (k0 + HALF) / 16; ++t) {
+            for (int t = k0 / 16; t < (k0 + HALF) / 16; t += 2) {
                 const int key = state_row(t, g, 0);
-                const f4 sum = dk[t] + *reinterpret_cast<const f4*>(share + own * (HALF + 4) + key - k0);
-                const float a[4] = {on ? dq[t][0] : 0.f, on ? dq[t][1] : 0.f, on ? dq[t][2] : 0.f, on ? dq[t][3] : 0.f};
-                const float b[4] = {on ? sum[0] : 0.f, on ? sum[1] : 0.f, on ? sum[2] : 0.f, on ? sum[3] : 0.f};
-                put_keys(p.dq, t0 + own, key, a);
-                put_keys(p.dk, t0 + own, key, b);
+                const float* with = share + own * (HALF + 4) + key - k0;
+                const f4 lo = dk[t] + *reinterpret_cast<const f4*>(with), hi = dk[t + 1] + *reinterpret_cast<const f4*>(with + 4);
+                put_keys(p.dq, own, key, on ? dq[t] : zero, on ? dq[t + 1] : zero);
+                put_keys(p.dk, own, key, on ? lo : zero, on ? hi : zero);
             }
         }
     }
@@ -996,16 +1070,15 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         lead = __shfl_up(lead, 1, 64);
         lead = lane > 0 ? lead : 0.f;
         if (in) {
+            z = 0.f;
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                sum += 16 * i + 15 >= lane ? across[i][lane] : 0.f;
-                z = i == 0 ? inner[0] : z + inner[i];
-            }
+            for (int i = 0; i < NR; ++i) sum += 16 * i + 15 >= lane ? across[i][lane] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * NR; ++i) z += inner[i];
             sum += suffix + lead + gates.total * z;
             if (lane < toks) {
-                const int64_t to = row_of(t0 + lane, p.H, head.h, 1);
-                p.dg[to] = lane < cnt ? sum : 0.f;
-                p.dbeta[to] = lane < cnt ? dbeta[lane] : 0.f;
+                p.dg[row_of(lane, 1)] = lane < cnt ? sum : 0.f;
+                p.dbeta[row_of(lane, 1)] = lane < cnt ? dbeta[lane] : 0.f;
             }
         }
     }
