@@ -248,6 +248,13 @@ DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
     return p;
 }
 
+// (p.o is set by then: out, or the backward's dout)
+void set_whole(DrParams& p, int32_t dtype) {
+    const int size = dtype == SS_F32 ? 4 : 2;
+    p.whole = dr_whole(p.q, p.K, p.L, size) && dr_whole(p.k, p.K, p.L, size) && dr_whole(p.v, p.V, p.L, size) &&
+              dr_whole(p.o, p.V, p.L, size);
+}
+
 float* at(void* base, int64_t bytes) { return reinterpret_cast<float*>(static_cast<char*>(base) + bytes); }
 
 // the walk, of segments side by side after what they start from
@@ -291,6 +298,7 @@ hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream
     const Saved sv = saved_of(plan);
     DrParams p = params_of(*a, plan);
     p.o = {a->out, a->out_batch_stride, a->out_len_stride, a->out_head_stride, 1};
+    set_whole(p, a->dtype);
     p.init = a->initial_state; p.last = a->last_state;
     p.seg_add = at(a->workspace, sp.add);
     if (a->saved) {
@@ -314,6 +322,7 @@ hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t st
     const Saved sv = saved_of(plan);
     DrParams p = params_of(a, plan);
     p.o = {g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1};
+    set_whole(p, a.dtype);
     p.init = g->dlast_state; p.last = g->dinitial_state;
     p.plan = at(a.saved, sv.plan); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = at(a.saved, sv.mul);
     p.dstates = at(a.workspace, sp.dstates); p.derr = at(a.workspace, sp.derr); p.seg_add = at(a.workspace, sp.add);

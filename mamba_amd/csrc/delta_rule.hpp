@@ -16,6 +16,13 @@ constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
 constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 ? 64 : 32; }
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
 
+// Rows of whole 16-byte vectors that do not overlap, a chunk's within 2^31 bytes: read and written through
+// buffer resources, which end with the chunk's last row.  (8 x 2048 tokens x 24 heads of 64 x 64, bf16: the walk
+// took 198 us with rows of any kind read behind branches, after each of which the compiler waits for all loads.)
+inline bool dr_whole(const LaRows& r, int64_t dim, int64_t len, int size) {
+    return dim * size % 16 == 0 && r.l < (int64_t(1) << 22) && (r.l >= dim || len <= 1);
+}
+
 // Per (batch, head) pair and chunk, what the kernels hand on (fp32):
 //   plan    the chunk's gates and triangular inverse (delta_rule_chunk.hpp), dr_plan_bytes()
 //   states  the state before the chunk, (Vp, Kp): a value column's keys side by side
@@ -27,6 +34,7 @@ struct DrParams {
     int64_t B, L, H;
     int K, V, Kp, Vp, rep, nch;               // rep: heads per group; nch: chunks of a row of L tokens
     float scale;
+    int whole;                            // dr_whole of all rows (DrParams' q, k, v, o)
     LaRows q, k, v, o;                    // o: out, or the backward's dout
     const float* g; int64_t g_b, g_l, g_h;
     const float* beta; int64_t be_b, be_l, be_h;

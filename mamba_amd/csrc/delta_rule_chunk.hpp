@@ -155,7 +155,9 @@ __device__ __forceinline__ int block16(int t, int lane) { return 16 * t + 4 * (l
 __device__ __forceinline__ int state_block(int t, int lane) { return 32 * (t >> 1) + 8 * (lane & 3) + 4 * (t & 1); }
 
 // A chunk's rows (C x W of type T) from global memory by NTH threads: into term tiles, or as they are.
-template <typename T, int W, int C, int NTH>
+// WHOLE (dr_whole): rows of whole vectors, read through a buffer resource that ends with the last
+// one: no branch, so nothing waits for the loads before they are stored.
+template <typename T, int W, int C, int NTH, bool WHOLE>
 struct Tile {
     using R = rowvec<T>;
     static constexpr int PER = W / R::VE, ALL = C * PER, N = (ALL + NTH - 1) / NTH, KT = kTerms<T>;
@@ -163,25 +165,18 @@ struct Tile {
     // the first `rows` rows and `dim` columns; zero past them
     __device__ __forceinline__ void load(const T* p, int64_t step, int rows, int dim) {
         const int row = int(threadIdx.x) / PER, col = int(threadIdx.x) % PER * R::VE;
-        if (rows == C && dim > 0 && dim % R::VE == 0 && step < (int64_t(1) << 24)) {
-            // whole vectors: a lane past the row's end reads its first, for nothing
-            const bool in = col < dim;
-            const uint32_t off = (uint32_t(row) * uint32_t(step) + uint32_t(in ? col : 0)) * uint32_t(sizeof(T));
+        if constexpr (WHOLE) {
+            constexpr uint32_t es = sizeof(T), none = 0x80000000u;
+            const rsrc_t r = make_rsrc_n(p, rows > 0 && dim > 0 ? int((uint32_t(rows - 1) * uint32_t(step) + uint32_t(dim)) * es) : 0);
+            const uint32_t off = col < dim ? (uint32_t(row) * uint32_t(step) + uint32_t(col)) * es : none;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                if (ALL % NTH != 0 && int(threadIdx.x) + i * NTH >= ALL) continue;
-                const typename R::words w = *reinterpret_cast<const typename R::words*>(
-                    reinterpret_cast<const char*>(p + int64_t(i * (NTH / PER)) * step) + off);
-                v[i] = in ? make_uint4(w.x, w.y, w.z, w.w) : make_uint4(0u, 0u, 0u, 0u);
-            }
+            for (int i = 0; i < N; ++i)
+                v[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, int(off + uint32_t(i * (NTH / PER)) * uint32_t(step) * es), 0, 0));
         } else {
-#pragma unroll 1
+#pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int r = row + i * (NTH / PER);
-                const uint4 w = R::load(p + int64_t(r) * step + col, r < rows ? dim - col : 0);
-#pragma unroll
-                for (int k = 0; k < N; ++k)
-                    if (k == i) v[k] = w;
+                v[i] = R::load(p + int64_t(r) * step + col, r < rows ? dim - col : 0);
             }
         }
     }
@@ -272,15 +267,18 @@ template <typename T, int KP>
 __device__ __forceinline__ Plan<T, KP>* plan_at(const DrParams& p, int64_t chunk) { return static_cast<Plan<T, KP>*>(p.plan) + chunk; }
 
 struct Head {
-    int64_t bh, b, h, len;                 // len: the row's tokens
-    __device__ __forceinline__ Head(const DrParams& p, int64_t bh_) : bh(bh_) {
-        b = bh / p.H;
-        h = bh % p.H;
+    int64_t bh, b, h, group, len;          // len: the row's tokens
+    __device__ __forceinline__ Head(const DrParams& p, uint32_t bh_) : bh(bh_) {
+        const uint32_t heads = uint32_t(p.H), row = bh_ / heads, head = bh_ - row * heads;
+        b = row;
+        h = head;
+        group = head / uint32_t(p.rep);
         const int64_t n = p.lens ? p.lens[b] : p.L;
         len = n < 0 ? 0 : n < p.L ? n : p.L;
     }
-    template <typename T> __device__ __forceinline__ const T* rows(const LaRows& r, int64_t t) const {
-        return static_cast<const T*>(r.p) + b * r.b + t * r.l + (h / r.rep) * r.h;
+    // the head's (rep above 1: its group's) first row
+    template <typename T> __device__ __forceinline__ const T* rows(const LaRows& r) const {
+        return static_cast<const T*>(r.p) + b * r.b + (r.rep > 1 ? group : h) * r.h;
     }
 };
 
@@ -290,22 +288,22 @@ struct Head {
 // diagonal one, T_ij = -T_ii sum_{j <= m < i} N_im T_mj, on fp32 matrix instructions.
 // Substitution and these products keep the bits of a stable solve, which powers of N
 // would not: for equal keys they reach binomial coefficients.
-template <typename T, int KP>
+template <typename T, int KP, bool WHOLE>
 __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams p) {
     using D = Dims<T, KP>;
     constexpr int C = D::C, NR = D::NR, KT = D::KT, KST = D::KST, TERM = C * KST, NST = C + 4, NTH = kPrepThreads<T, KP>;
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * TERM];
     __shared__ __attribute__((aligned(16))) float ns[C * NST], ts[NR][16 * 20];
     __shared__ Gates<C> gates;
-    const Head head(p, blockIdx.x / unsigned(p.nch));
+    const Head head(p, blockIdx.x / uint32_t(p.nch));
     const int64_t n = blockIdx.x % unsigned(p.nch), t0 = n * C;
     if (t0 >= head.len) return;
     const int lane = int(threadIdx.x) & 63, w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), g = lane >> 4, c = lane & 15;
     const int cnt = head.len - t0 < C ? int(head.len - t0) : C;
     Plan<T, KP>* plan = plan_at<T, KP>(p, head.bh * p.nch + n);
     {
-        Tile<T, KP, C, NTH> k;
-        k.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
+        Tile<T, KP, C, NTH, WHOLE> k;
+        k.load(head.rows<T>(p.k) + t0 * p.k.l, p.k.l, cnt, p.K);
         if (w == 0) {
             const bool in = lane < cnt;
             const float gv = in ? p.g[head.b * p.g_b + (t0 + lane) * p.g_l + head.h * p.g_h] : 0.f;
@@ -393,10 +391,13 @@ struct PlanIn {
     f4 v[N];
     __device__ __forceinline__ void load(const Plan<T, KP>* p) {
         const int tid = int(threadIdx.x);
-        if (tid < NG) gates = reinterpret_cast<const uint4*>(&p->gates)[tid];
+        // (a thread past the last vector reads it too)
+        gates = reinterpret_cast<const uint4*>(&p->gates)[tid < NG ? tid : NG - 1];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (D::NT * 64 % NTH == 0 || i + 1 < N || tid + i * NTH < D::NT * 64) v[i] = *reinterpret_cast<const f4*>(p->tri + 4 * (tid + i * NTH));
+        for (int i = 0; i < N; ++i) {
+            const int at = tid + i * NTH;
+            v[i] = *reinterpret_cast<const f4*>(p->tri + 4 * (at < D::NT * 64 ? at : D::NT * 64 - 1));
+        }
     }
     __device__ __forceinline__ void store(Gates<D::C>& g, uint16_t* tri) const {
         const int tid = int(threadIdx.x);
@@ -413,7 +414,7 @@ struct PlanIn {
 // last state; back, from dout, the states' and errors' gradients and the initial state's.
 // LOCAL: the states only, from zero, and beside them what the segment makes of the
 // columns of the identity (value tiles past the last: no values, the state starts as I).
-template <typename T, int KP, bool REV, bool LOCAL>
+template <typename T, int KP, bool REV, bool LOCAL, bool WHOLE>
 __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
     using D = Dims<T, KP>;
     constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NT = D::NT, VST = D::VST;
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
     __shared__ __attribute__((aligned(16))) T vs[C * VST];
     __shared__ __attribute__((aligned(16))) Gates<C> G;
     const int segs = p.segs, seg = int(blockIdx.x % unsigned(segs));
-    const Head head(p, blockIdx.x / unsigned(segs));
+    const Head head(p, blockIdx.x / uint32_t(segs));
     const int vt = int(blockIdx.y), vtiles = (p.V + 63) / 64;
     const int tid = int(threadIdx.x), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const bool unit = LOCAL && vt >= vtiles;              // columns of the identity
@@ -461,35 +462,52 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
     }
     // kept states: a column's rows side by side (value column, key)
     const auto keep_state = [&](float* to) {
-        float* at = to + int64_t(col) * p.Kp + 8 * g;
+        float* at = to + col * p.Kp + 8 * g;
+        if (KP == p.Kp) {
+#pragma unroll
+            for (int t = 0; t < NS; ++t) *reinterpret_cast<f4*>(at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
+            return;
+        }
 #pragma unroll
         for (int t = 0; t < NS; ++t)
-            if (KP == p.Kp || state_row(t, g, 0) < p.Kp) *reinterpret_cast<f4*>(at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
+            if (state_row(t, g, 0) < p.Kp) *reinterpret_cast<f4*>(at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
     };
 
-    Tile<T, KP, C, 256> kin, qin;
-    Tile<T, 64, C, 256> vin;                              // v (back: dout)
+    Tile<T, KP, C, 256, WHOLE> kin, qin;
+    Tile<T, 64, C, 256, WHOLE> vin;                              // v (back: dout)
     PlanIn<T, KP, 256> plan;
     const int step = REV ? -1 : 1, first = REV ? n1 - 1 : n0;
-    const auto fetch = [&](int n) {
-        if (n < n0 || n >= n1) return;
+    const T* const kp = head.rows<T>(p.k);
+    const T* const qp = head.rows<T>(p.q);
+    const T* const vp = head.rows<T>(REV ? p.o : p.v) + v0;
+    T* const op = const_cast<T*>(head.rows<T>(p.o)) + v0;  // out (back: not written)
+    const int64_t vstep = REV ? p.o.l : p.v.l;
+    const auto count = [&](int n) { return head.len - int64_t(n) * C < C ? int(head.len - int64_t(n) * C) : C; };
+    const auto fetch = [&](int n) {                       // (past the last chunk: that one again)
+        n = n < n0 ? n0 : n < n1 ? n : n1 - 1;
         const int64_t t0 = int64_t(n) * C;
-        const int cnt = head.len - t0 < C ? int(head.len - t0) : C;
+        const int cnt = count(n);
         plan.load(plan_at<T, KP>(p, head.bh * p.nch + n));
-        kin.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
-        if constexpr (Q) qin.load(head.rows<T>(p.q, t0), p.q.l, cnt, p.K);
-        const LaRows& rows = REV ? p.o : p.v;
-        vin.load(head.rows<T>(rows, t0) + v0, rows.l, unit ? 0 : cnt, p.V - v0);
+        kin.load(kp + t0 * p.k.l, p.k.l, cnt, p.K);
+        if constexpr (Q) qin.load(qp + t0 * p.q.l, p.q.l, cnt, p.K);
+        vin.load(vp + t0 * vstep, vstep, unit ? 0 : cnt, p.V - v0);
     };
-    fetch(first);
-    for (int n = first; n >= n0 && n < n1; n += step) {
-        const int64_t at = head.bh * p.nch + n, t0 = int64_t(n) * C;
-        lds_barrier();                                    // (the tiles of the chunk before are done with)
+    const auto stage = [&] {
         kin.template store<KST>(ks);
         if constexpr (Q) qin.template store<KST>(qs);
         vin.template store_raw<VST>(vs);
         plan.store(G, tri);
+    };
+    if (n0 < n1) {
+        fetch(first);
+        stage();
         lds_barrier();
+    }
+    for (int n = first; n >= n0 && n < n1; n += step) {
+        const int64_t at = head.bh * p.nch + n, t0 = int64_t(n) * C;
+        // Stores first and last: the loads of the next chunk then wait for no younger store.
+        if (!LOCAL && live && (REV || p.states)) keep_state((REV ? p.dstates : p.states) + at * p.Vp * p.Kp);
+        f4 kept[NR];                                      // E (back: F), column col
         fetch(n + step);
         if constexpr (Q) {                                // P, a share of its tiles a wave; formed transposed, rows j, column i
 #pragma unroll
@@ -520,7 +538,6 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
             f4 O[NR];                                     // out, transposed: rows value columns, column token i
             u4 uf[NP][D::OT];
             if (live) {
-                if (!LOCAL && p.states) keep_state(p.states + at * p.Vp * p.Kp);
                 f4 Y[NR];
 #pragma unroll
                 for (int i = 0; i < NR; ++i) Y[i] = O[i] = zero;
@@ -564,11 +581,8 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                         mac<3, 3, 2>(a, yf[q], U[i]);
                     }
                 }
-                if (!LOCAL && p.err) {                    // (value column, token)
-                    float* to = p.err + (at * p.Vp + col) * C + 4 * g;
 #pragma unroll
-                    for (int i = 0; i < NR; ++i) *reinterpret_cast<f4*>(to + 16 * i) = U[i];
-                }
+                for (int i = 0; i < NR; ++i) kept[i] = U[i];
 #pragma unroll
                 for (int i = 0; i < NR; ++i) U[i] *= *reinterpret_cast<const f4*>(G.beta + 16 * i + 4 * g);
                 if constexpr (!LOCAL) {
@@ -603,15 +617,31 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                             frag_tiles<PT, CTERM, false>(prob, tile_at(i, 2 * q), tile_at(i, 2 * q + 1), lane, b);
                             mac<D::OT, PT, D::OT - 1>(uf[q], b, O[i]);
                         }
-                        const int64_t t = t0 + 16 * i + c;
-                        const float o[4] = {p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]};
-                        if (t < head.len)
-                            store4<T>(const_cast<T*>(head.rows<T>(p.o, t)) + col0 + 4 * g, o, p.V - (col0 + 4 * g));
+                    }
+                }
+                lds_barrier();                            // (the chunk's tiles are done with)
+                stage();
+                if (live) {
+                    const int cnt = count(n);
+                    T* const out = op + t0 * p.o.l;
+                    const int at_col = 16 * w + 4 * g, cols = p.V - v0 - at_col;
+                    if constexpr (WHOLE) {
+                        const rsrc_t r = make_rsrc_n(out, int((uint32_t(cnt - 1) * uint32_t(p.o.l) + uint32_t(p.V - v0)) * uint32_t(sizeof(T))));
+                        const uint32_t off = cols > 0 ? (uint32_t(c) * uint32_t(p.o.l) + uint32_t(at_col)) * uint32_t(sizeof(T)) : 0x80000000u;
+#pragma unroll
+                        for (int i = 0; i < NR; ++i)
+                            bstore4<T>(r, off + uint32_t(16 * i) * uint32_t(p.o.l) * uint32_t(sizeof(T)),
+                                       make_float4(p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NR; ++i) {
+                            const float o[4] = {p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]};
+                            if (16 * i + c < cnt) store4<T>(out + (16 * i + c) * p.o.l + at_col, o, cols);
+                        }
                     }
                 }
             }
         } else {
-            if (live && !LOCAL) keep_state(p.dstates + at * p.Vp * p.Kp);
             f4 X[NR];
             if (live) {
 #pragma unroll
@@ -661,11 +691,8 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                         mac<3, 3, 2>(a, xf[q], F[j]);
                     }
                 }
-                if (!LOCAL) {                             // (value column, token)
-                    float* to = p.derr + (at * p.Vp + col) * C + 4 * g;
 #pragma unroll
-                    for (int j = 0; j < NR; ++j) *reinterpret_cast<f4*>(to + 16 * j) = F[j];
-                }
+                for (int j = 0; j < NR; ++j) kept[j] = F[j];
                 const float total = G.total;
 #pragma unroll
                 for (int t = 0; t < NS; ++t) S[t] *= total;
@@ -686,6 +713,17 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 }
             }
         }
+        if constexpr (REV || LOCAL) {
+            lds_barrier();                                // (the chunk's tiles are done with)
+            stage();
+        }
+        float* const err = REV ? p.derr : p.err;
+        if (!LOCAL && live && err) {                      // (value column, token)
+            float* to = err + (at * p.Vp + col) * C + 4 * g;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) *reinterpret_cast<f4*>(to + 16 * i) = kept[i];
+        }
+        lds_barrier();
     }
     if constexpr (LOCAL) {
         if (live && unit) keep_state(p.seg_mul + (head.bh * segs + seg) * p.Kp * p.Kp);
@@ -706,7 +744,7 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
             const int64_t from = head.len > int64_t(n0) * C ? head.len : int64_t(n0) * C, all = int64_t(n0 + p.seg_chunks) * C;
             const int64_t to = all < p.L ? all : p.L;
             for (int64_t t = from + w; t < to; t += 4)
-                if (v0 + lane < p.V) io<T>::store(const_cast<T*>(head.rows<T>(p.o, t)) + v0 + lane, 0.f);
+                if (v0 + lane < p.V) io<T>::store(op + t * p.o.l + lane, 0.f);
         }
     }
 }
@@ -730,7 +768,7 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
 // tiles), waves NR .. 2 NR - 1 as writers (columns j): a reader has w + 1 tiles of M and R and the
 // writer on its SIMD the other NR - w.  The writer's share of dk passes to the reader
 // through LDS.  Value columns pass 32 at a time, those of the next step on their way meanwhile.
-template <typename T, int KP>
+template <typename T, int KP, bool WHOLE>
 __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams p) {
     using D = Dims<T, KP>;
     constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NTH = kGradThreads<T, KP>;
@@ -744,7 +782,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     __shared__ float across[NR][C], reads[C], writes[C], inner[2 * NR], dbeta[C];
     constexpr int HALF = KP > 128 ? 128 : KP;             // keys of dk that pass through LDS at a time
     static_assert(sizeof(Stage) >= sizeof(float) * C * (HALF + 4), "dk's share over the tiles");
-    const Head head(p, blockIdx.x / unsigned(p.nch));
+    const Head head(p, blockIdx.x / uint32_t(p.nch));
     const int n = int(blockIdx.x % unsigned(p.nch));
     const int64_t t0 = int64_t(n) * C, at = head.bh * p.nch + n;
     const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
@@ -787,7 +825,8 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     constexpr int NSV = VW * KW / 4 / NTH, NEV = VW * C / 4 / NTH;
     static_assert(VW * KW / 4 % NTH == 0 && VW * C / 4 % NTH == 0, "whole vectors a thread");
     f4 si[NSV], ti[NSV], ei[NEV], fi[NEV];
-    Tile<T, VW, C, NTH> di;
+    Tile<T, VW, C, NTH, WHOLE> di;
+    const T* const dp = head.rows<T>(p.o) + t0 * p.o.l;
     const auto fetch = [&](int v0, int k0) {
         if (v0 >= p.V) return;
 #pragma unroll
@@ -806,13 +845,13 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             ei[i] = v < p.Vp ? *reinterpret_cast<const f4*>(p.err + from) : zero;
             fi[i] = v < p.Vp ? *reinterpret_cast<const f4*>(p.derr + from) : zero;
         }
-        di.load(head.rows<T>(p.o, t0) + v0, p.o.l, cnt, p.V - v0);
+        di.load(dp + v0, p.o.l, cnt, p.V - v0);
     };
     fetch(0, 0);
     {
-        Tile<T, KP, C, NTH> kin, qin;
-        kin.load(head.rows<T>(p.k, t0), p.k.l, cnt, p.K);
-        qin.load(head.rows<T>(p.q, t0), p.q.l, cnt, p.K);
+        Tile<T, KP, C, NTH, WHOLE> kin, qin;
+        kin.load(head.rows<T>(p.k) + t0 * p.k.l, p.k.l, cnt, p.K);
+        qin.load(head.rows<T>(p.q) + t0 * p.q.l, p.q.l, cnt, p.K);
         if (tid < int(sizeof(Gates<C>) / 16))
             reinterpret_cast<uint4*>(&gates)[tid] = reinterpret_cast<const uint4*>(&plan_at<T, KP>(p, at)->gates)[tid];
         kin.template store<KST>(ks);
@@ -1097,7 +1136,9 @@ template <typename T>
 hipError_t dr_prep_launch(const DrParams& p, hipStream_t stream) {
     return dr_by_keys<T>(p.K, [&](auto kp) {
         constexpr int KP = decltype(kp)::value;
-        hipLaunchKernelGGL((dr::dr_prep<T, KP>), dim3(unsigned(p.B * p.H * p.nch)), dim3(dr::kPrepThreads<T, KP>), 0, stream, p);
+        const dim3 grid(unsigned(p.B * p.H * p.nch)), block(dr::kPrepThreads<T, KP>);
+        if (p.whole) hipLaunchKernelGGL((dr::dr_prep<T, KP, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((dr::dr_prep<T, KP, false>), grid, block, 0, stream, p);
         return hipGetLastError();
     });
 }
@@ -1108,10 +1149,15 @@ hipError_t dr_walk_launch(const DrParams& p, bool rev, hipStream_t stream) {
     const dim3 grid(unsigned(p.B * p.H * p.segs), tiles + units);
     return dr_by_keys<T>(p.K, [&](auto kp) {
         constexpr int KP = decltype(kp)::value;
-        if (rev && p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, true, true>), grid, dim3(256), 0, stream, p);
-        else if (rev) hipLaunchKernelGGL((dr::dr_walk<T, KP, true, false>), grid, dim3(256), 0, stream, p);
-        else if (p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, false, true>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((dr::dr_walk<T, KP, false, false>), grid, dim3(256), 0, stream, p);
+        const auto go = [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            if (rev && p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, true, true, WHOLE>), grid, dim3(256), 0, stream, p);
+            else if (rev) hipLaunchKernelGGL((dr::dr_walk<T, KP, true, false, WHOLE>), grid, dim3(256), 0, stream, p);
+            else if (p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, false, true, WHOLE>), grid, dim3(256), 0, stream, p);
+            else hipLaunchKernelGGL((dr::dr_walk<T, KP, false, false, WHOLE>), grid, dim3(256), 0, stream, p);
+        };
+        if (p.whole) go(std::true_type{});
+        else go(std::false_type{});
         return hipGetLastError();
     });
 }
@@ -1120,7 +1166,9 @@ template <typename T>
 hipError_t dr_grads_launch(const DrParams& p, hipStream_t stream) {
     return dr_by_keys<T>(p.K, [&](auto kp) {
         constexpr int KP = decltype(kp)::value;
-        hipLaunchKernelGGL((dr::dr_grads<T, KP>), dim3(unsigned(p.B * p.H * p.nch)), dim3(dr::kGradThreads<T, KP>), 0, stream, p);
+        const dim3 grid(unsigned(p.B * p.H * p.nch)), block(dr::kGradThreads<T, KP>);
+        if (p.whole) hipLaunchKernelGGL((dr::dr_grads<T, KP, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((dr::dr_grads<T, KP, false>), grid, block, 0, stream, p);
         return hipGetLastError();
     });
 }
