@@ -148,6 +148,12 @@ __device__ __forceinline__ void frag_tiles(const uint16_t* at, int lo, int hi, i
         t[n] = u4{a.x, a.y, b.x, b.y};
     }
 }
+// f(integral_constant<0>), f(integral_constant<1>): the pairs of tiles of a chunk
+template <int N, typename F>
+__device__ __forceinline__ void each_pair(F&& f) {
+    f(std::integral_constant<int, 0>{});
+    if constexpr (N > 1) f(std::integral_constant<int, 1>{});
+}
 // place of the lower tile (i, j); none above the diagonal
 constexpr __device__ __forceinline__ int tile_at(int i, int j) { return j <= i ? i * (i + 1) / 2 + j : -1; }
 // first of the 4 columns a lane reads for its group: of 16 neighbouring ones, and of the state's tile t
@@ -492,6 +498,20 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
         if constexpr (Q) qin.load(qp + t0 * p.q.l, p.q.l, cnt, p.K);
         vin.load(vp + t0 * vstep, vstep, unit ? 0 : cnt, p.V - v0);
     };
+    // S += sum over 32 tokens of a tile's rows by the columns f, 4 tiles at a time
+    const auto add_rows = [&](const uint16_t* rows, const u4 (&f)[1][3]) {
+#pragma unroll
+        for (int t = 0; t < NS; t += 4) {
+            u4 a[4][KT];
+            f4* to[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                frag_col<KT, KTERM, KST>(rows, state_block(t + i, lane), lane, a[i]);
+                to[i] = &S[t + i];
+            }
+            mfma_terms<4, 1, 0, KT, 3, 2>(a, f, to);
+        }
+    };
     const auto stage = [&] {
         kin.template store<KST>(ks);
         if constexpr (Q) qin.template store<KST>(qs);
@@ -511,27 +531,25 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
         fetch(n + step);
         if constexpr (Q) {                                // P, a share of its tiles a wave; formed transposed, rows j, column i
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
+            for (int e = 0; e < (NT + 3) / 4; ++e) {
+                // (past the last: that one again, the same values to the same place)
+                const int tile = w + 4 * e < NT ? w + 4 * e : NT - 1, i = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, j = tile - i * (i + 1) / 2;
+                f4 acc = zero;
 #pragma unroll
-                for (int j = 0; j <= i; ++j) {
-                    if ((tile_at(i, j) & 3) != w) continue;
-                    f4 acc = zero;
-#pragma unroll
-                    for (int kk = 0; kk < NK; ++kk) {
-                        u4 a[KT], b[KT];
-                        frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a);
-                        frag8<KT, KTERM>(qs + (16 * i + c) * KST + 32 * kk + 8 * g, b);
-                        mac<KT, KT, 2>(a, b, acc);
-                    }
-                    const double Gi = G.G[16 * i + c];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int row = 16 * j + 4 * g + r;
-                        const float f = factor(Gi, G.G[row]);
-                        acc[r] = j < i || row <= 16 * i + c ? acc[r] * f : 0.f;
-                    }
-                    put4<PT, CTERM>(prob + tile_at(i, j) * 256 + 16 * c + 4 * g, acc);
+                for (int kk = 0; kk < NK; ++kk) {
+                    u4 a[KT], b[KT];
+                    frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a);
+                    frag8<KT, KTERM>(qs + (16 * i + c) * KST + 32 * kk + 8 * g, b);
+                    mac<KT, KT, 2>(a, b, acc);
                 }
+                const double Gi = G.G[16 * i + c];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * j + 4 * g + r;
+                    const float f = factor(Gi, G.G[row]);
+                    acc[r] = row <= 16 * i + c ? acc[r] * f : 0.f;
+                }
+                put4<PT, CTERM>(prob + tile * 256 + 16 * c + 4 * g, acc);
             }
         }
         if constexpr (!REV) {
@@ -543,17 +561,22 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 for (int i = 0; i < NR; ++i) Y[i] = O[i] = zero;
 #pragma unroll
                 for (int kk = 0; kk < NK; ++kk) {
-                    u4 sf[3];
-                    pack<3>(S[2 * kk], S[2 * kk + 1], sf);
+                    u4 sf[1][3], a[NR][KT];
+                    pack<3>(S[2 * kk], S[2 * kk + 1], sf[0]);
+                    f4* to[NR];
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
-                        u4 a[KT];
-                        frag8<KT, KTERM>(ks + (16 * i + c) * KST + 32 * kk + 8 * g, a);
-                        mac<KT, 3, 2>(a, sf, Y[i]);
-                        if constexpr (!LOCAL) {
-                            frag8<KT, KTERM>(qs + (16 * i + c) * KST + 32 * kk + 8 * g, a);
-                            mac<3, KT, D::OT - 1>(sf, a, O[i]);
+                        frag8<KT, KTERM>(ks + (16 * i + c) * KST + 32 * kk + 8 * g, a[i]);
+                        to[i] = &Y[i];
+                    }
+                    mfma_terms<NR, 1, 0, KT, 3, 2>(a, sf, to);
+                    if constexpr (!LOCAL) {
+#pragma unroll
+                        for (int i = 0; i < NR; ++i) {
+                            frag8<KT, KTERM>(qs + (16 * i + c) * KST + 32 * kk + 8 * g, a[i]);
+                            to[i] = &O[i];
                         }
+                        mfma_terms<NR, 0, 1, 3, KT, D::OT - 1>(sf, a, to);
                     }
                 }
                 u4 yf[NP][3];
@@ -572,15 +595,19 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 }
                 f4 U[NR];
 #pragma unroll
-                for (int i = 0; i < NR; ++i) {
-                    U[i] = zero;
+                for (int i = 0; i < NR; ++i) U[i] = zero;
+                // (independent sums in turn: a product need not wait for the one before it)
+                each_pair<NP>([&](auto qc) {
+                    constexpr int q = decltype(qc)::value, I = NR - 2 * q;
+                    u4 a[I][3];
+                    f4* to[I];
 #pragma unroll
-                    for (int q = 0; q <= i / 2; ++q) {
-                        u4 a[3];
-                        frag_tiles<3, CTERM, true>(tri, tile_at(i, 2 * q), tile_at(i, 2 * q + 1), lane, a);
-                        mac<3, 3, 2>(a, yf[q], U[i]);
+                    for (int i = 0; i < I; ++i) {
+                        frag_tiles<3, CTERM, true>(tri, tile_at(2 * q + i, 2 * q), tile_at(2 * q + i, 2 * q + 1), lane, a[i]);
+                        to[i] = &U[2 * q + i];
                     }
-                }
+                    mfma_terms<I, 1, 0, 3, 3, 2>(a, &yf[q], to);
+                });
 #pragma unroll
                 for (int i = 0; i < NR; ++i) kept[i] = U[i];
 #pragma unroll
@@ -594,30 +621,28 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 for (int t = 0; t < NS; ++t) S[t] *= total;
 #pragma unroll
                 for (int q = 0; q < NP; ++q) {
-                    u4 wf[3];
+                    u4 wf[1][3];
                     pack<3>(U[2 * q] * *reinterpret_cast<const f4*>(G.end + 32 * q + 4 * g),
-                            U[2 * q + 1] * *reinterpret_cast<const f4*>(G.end + 32 * q + 16 + 4 * g), wf);
-#pragma unroll
-                    for (int t = 0; t < NS; ++t) {
-                        u4 a[KT];
-                        frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a);
-                        mac<KT, 3, 2>(a, wf, S[t]);
-                    }
+                            U[2 * q + 1] * *reinterpret_cast<const f4*>(G.end + 32 * q + 16 + 4 * g), wf[0]);
+                    add_rows(ks + 32 * q * KST, wf);
                 }
             }
             if constexpr (!LOCAL) {
                 lds_barrier();                            // P is there
                 if (live) {
 #pragma unroll
-                    for (int i = 0; i < NR; ++i) {
-                        O[i] *= G.gam[16 * i + c];
+                    for (int i = 0; i < NR; ++i) O[i] *= G.gam[16 * i + c];
+                    each_pair<NP>([&](auto qc) {
+                        constexpr int q = decltype(qc)::value, I = NR - 2 * q;
+                        u4 b[I][PT];
+                        f4* to[I];
 #pragma unroll
-                        for (int q = 0; q <= i / 2; ++q) {
-                            u4 b[PT];
-                            frag_tiles<PT, CTERM, false>(prob, tile_at(i, 2 * q), tile_at(i, 2 * q + 1), lane, b);
-                            mac<D::OT, PT, D::OT - 1>(uf[q], b, O[i]);
+                        for (int i = 0; i < I; ++i) {
+                            frag_tiles<PT, CTERM, false>(prob, tile_at(2 * q + i, 2 * q), tile_at(2 * q + i, 2 * q + 1), lane, b[i]);
+                            to[i] = &O[2 * q + i];
                         }
-                    }
+                        mfma_terms<I, 0, 1, D::OT, PT, D::OT - 1>(&uf[q], b, to);
+                    });
                 }
                 lds_barrier();                            // (the chunk's tiles are done with)
                 stage();
@@ -648,14 +673,15 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 for (int i = 0; i < NR; ++i) X[i] = zero;
 #pragma unroll
                 for (int kk = 0; kk < NK; ++kk) {
-                    u4 sf[3];
-                    pack<3>(S[2 * kk], S[2 * kk + 1], sf);
+                    u4 sf[1][3], a[NR][KT];
+                    pack<3>(S[2 * kk], S[2 * kk + 1], sf[0]);
+                    f4* to[NR];
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
-                        u4 a[KT];
-                        frag8<KT, KTERM>(ks + (16 * i + c) * KST + 32 * kk + 8 * g, a);
-                        mac<KT, 3, 2>(a, sf, X[i]);
+                        frag8<KT, KTERM>(ks + (16 * i + c) * KST + 32 * kk + 8 * g, a[i]);
+                        to[i] = &X[i];
                     }
+                    mfma_terms<NR, 1, 0, KT, 3, 2>(a, sf, to);
                 }
             }
             lds_barrier();                                // P is there
@@ -664,33 +690,43 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 u4 df[NP][KT];
 #pragma unroll
                 for (int q = 0; q < NP; ++q) raw_col<T, VST>(vs + 32 * q * VST, w, lane, x[2 * q], x[2 * q + 1], df[q]);
+                f4 acc[NR];
+#pragma unroll
+                for (int j = 0; j < NR; ++j) acc[j] = zero;
+                each_pair<NP>([&](auto qc) {
+                    constexpr int q = decltype(qc)::value, I = 2 * q + 2;
+                    u4 a[I][PT];
+                    f4* to[I];
+#pragma unroll
+                    for (int j = 0; j < I; ++j) {
+                        frag_tiles<PT, CTERM, true>(prob, tile_at(2 * q, j), tile_at(2 * q + 1, j), lane, a[j]);
+                        to[j] = &acc[j];
+                    }
+                    mfma_terms<I, 1, 0, PT, KT, 2>(a, &df[q], to);
+                });
 #pragma unroll
                 for (int j = 0; j < NR; ++j) {
-                    f4 acc = zero;
-#pragma unroll
-                    for (int q = j / 2; q < NP; ++q) {
-                        u4 a[PT];
-                        frag_tiles<PT, CTERM, true>(prob, tile_at(2 * q, j), tile_at(2 * q + 1, j), lane, a);
-                        mac<PT, KT, 2>(a, df[q], acc);
-                    }
                     const f4 end = *reinterpret_cast<const f4*>(G.end + 16 * j + 4 * g), beta = *reinterpret_cast<const f4*>(G.beta + 16 * j + 4 * g);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) X[j][r] = beta_or_least(beta[r]) * __builtin_fmaf(end[r], X[j][r], p.scale * acc[r]);
+                    for (int r = 0; r < 4; ++r) X[j][r] = beta_or_least(beta[r]) * __builtin_fmaf(end[r], X[j][r], p.scale * acc[j][r]);
                 }
                 u4 xf[NP][3];
 #pragma unroll
                 for (int q = 0; q < NP; ++q) pack<3>(X[2 * q], X[2 * q + 1], xf[q]);
                 f4 F[NR];
 #pragma unroll
-                for (int j = 0; j < NR; ++j) {
-                    F[j] = zero;
+                for (int j = 0; j < NR; ++j) F[j] = zero;
+                each_pair<NP>([&](auto qc) {
+                    constexpr int q = decltype(qc)::value, I = 2 * q + 2;
+                    u4 a[I][3];
+                    f4* to[I];
 #pragma unroll
-                    for (int q = j / 2; q < NP; ++q) {
-                        u4 a[3];
-                        frag_tiles<3, CTERM, false>(tri, tile_at(2 * q, j), tile_at(2 * q + 1, j), lane, a);
-                        mac<3, 3, 2>(a, xf[q], F[j]);
+                    for (int j = 0; j < I; ++j) {
+                        frag_tiles<3, CTERM, false>(tri, tile_at(2 * q, j), tile_at(2 * q + 1, j), lane, a[j]);
+                        to[j] = &F[j];
                     }
-                }
+                    mfma_terms<I, 1, 0, 3, 3, 2>(a, &xf[q], to);
+                });
 #pragma unroll
                 for (int j = 0; j < NR; ++j) kept[j] = F[j];
                 const float total = G.total;
@@ -699,17 +735,11 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
 #pragma unroll
                 for (int q = 0; q < NP; ++q) {
                     const f4 lo = *reinterpret_cast<const f4*>(G.gam + 32 * q + 4 * g), hi = *reinterpret_cast<const f4*>(G.gam + 32 * q + 16 + 4 * g);
-                    u4 gf[3], ff[3];
-                    pack<3>(x[2 * q] * (p.scale * lo), x[2 * q + 1] * (p.scale * hi), gf);
-                    pack<3>(-(F[2 * q] * lo), -(F[2 * q + 1] * hi), ff);
-#pragma unroll
-                    for (int t = 0; t < NS; ++t) {
-                        u4 a[KT];
-                        frag_col<KT, KTERM, KST>(qs + 32 * q * KST, state_block(t, lane), lane, a);
-                        mac<KT, 3, 2>(a, gf, S[t]);
-                        frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a);
-                        mac<KT, 3, 2>(a, ff, S[t]);
-                    }
+                    u4 gf[1][3], ff[1][3];
+                    pack<3>(x[2 * q] * (p.scale * lo), x[2 * q + 1] * (p.scale * hi), gf[0]);
+                    add_rows(qs + 32 * q * KST, gf);
+                    pack<3>(-(F[2 * q] * lo), -(F[2 * q + 1] * hi), ff[0]);
+                    add_rows(ks + 32 * q * KST, ff);
                 }
             }
         }
