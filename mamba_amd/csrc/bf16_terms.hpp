@@ -48,6 +48,10 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&t)[N]) {
     }
 }
 
+// No instruction moves across: without it the scheduler raises the loads and
+// splits of all steps to the front and runs out of registers.
+__device__ __forceinline__ void stage_end() { __builtin_amdgcn_sched_barrier(0); }
+
 // c[i] += sum of the products of a[i]'s NA and b[i]'s NB terms whose order is at
 // most kMax (left out: with 2 up to 2^-22 of a product, with 1 2^-16), small ones first.  I independent sums
 // at once: a product then need not wait for the one before it.  ai, bi: which operand

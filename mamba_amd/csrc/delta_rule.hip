@@ -50,8 +50,8 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
         const float* mul = p.seg_mul + seg_of(i) * p.Kp * p.Kp;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int x = tid + k * 256, at = c0 + x / (KP / 4), key = x % (KP / 4) * 4;
-            in[k] = at < p.Kp && key < p.Kp ? *reinterpret_cast<const f4*>(mul + int64_t(at) * p.Kp + key) : zero;
+            const int x = tid + k * 256, at = c0 + x / (KP / 4), place = x % (KP / 4) * 4;
+            in[k] = at < p.Kp && place < p.Kp ? *reinterpret_cast<const f4*>(mul + int64_t(at) * p.Kp + place) : zero;
         }
     };
     fetch(0, 0);
@@ -72,10 +72,10 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
             float* add = p.seg_add + (seg_of(i) * p.Vp + col) * p.Kp;
 #pragma unroll
             for (int t = 0; t < NS; ++t) {
-                const int key = state_row(t, g, 0);
-                if (key >= p.Kp) continue;
-                const f4 own = *reinterpret_cast<const f4*>(add + key);
-                *reinterpret_cast<f4*>(add + key) = S[t];
+                const int place = 16 * t + 4 * g;
+                if (32 * (t >> 1) >= p.Kp) continue;
+                const f4 own = *reinterpret_cast<const f4*>(add + place);
+                *reinterpret_cast<f4*>(add + place) = S[t];
                 S[t] = own;
             }
         }
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
                 split<3>(in[k][2], in[k][3], b);
 #pragma unroll
                 for (int n = 0; n < 3; ++n)
-                    *reinterpret_cast<uint2*>(ms + n * TERM + x / (KP / 4) * MST + x % (KP / 4) * 4) = make_uint2(a[n], b[n]);
+                    *reinterpret_cast<uint2*>(ms + n * TERM + x / (KP / 4) * MST + state_key(x % (KP / 4) * 4)) = make_uint2(a[n], b[n]);
             }
             lds_barrier();
             if (c0 + CW < KP) fetch(i, c0 + CW);
@@ -157,8 +157,9 @@ hipError_t for_type(int32_t dtype, F&& f) {
 
 int terms(int32_t dtype) { return dtype == SS_F32 ? 3 : dtype == SS_BF16 ? 1 : 2; }
 
-// Rows are cut into segments where fewer than half the 256 compute units would walk, and a
-// segment keeps at least 8 chunks.
+// Compute units.  Rows are cut into segments where fewer than half of them would walk, into enough
+// for one workgroup each, or for the two that fit where tiles and registers are small; a segment
+// keeps at least 8 chunks.
 constexpr int64_t kUnits = 256, kSegChunksMin = 8;
 
 struct Plan {
@@ -170,13 +171,14 @@ Plan plan_of(const ss_delta_rule_args& a) {
     p.chunk = dr_chunk(a.d_key, terms(a.dtype));
     p.bh = a.batch * a.heads;
     p.nch = (a.seqlen + p.chunk - 1) / p.chunk;
-    const int64_t kp = dr_round16(a.d_key), vp = dr_round16(a.d_value);
+    const int64_t kp = dr_round32(a.d_key), vp = dr_round16(a.d_value);
     p.plan = dr_plan_bytes(p.chunk) / 4;
     p.state = kp * vp;
     p.rows = p.chunk * vp;
     p.mul = kp * kp;
     const int64_t walks = p.bh * ((a.d_value + 63) / 64);
-    int64_t segs = walks > 0 ? kUnits / walks : 1;
+    const bool two = a.d_key <= 64 && a.dtype != SS_F32;
+    int64_t segs = walks > 0 && walks <= kUnits / 2 ? (two ? 2 : 1) * kUnits / walks : 1;
     if (segs > p.nch / kSegChunksMin) segs = p.nch / kSegChunksMin;
     if (segs < 1) segs = 1;
     const int64_t per = p.nch > 0 ? (p.nch + segs - 1) / segs : 1;
@@ -234,8 +236,8 @@ BwdSpace bwd_space(const ss_delta_rule_args& a, const Plan& p) {
 
 DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
     DrParams p{};
-    p.B = a.batch; p.L = a.seqlen; p.H = a.heads;
-    p.K = int(a.d_key); p.V = int(a.d_value); p.Kp = dr_round16(a.d_key); p.Vp = dr_round16(a.d_value);
+    p.B = a.batch; p.L = a.seqlen; p.H = a.heads; p.BH = a.batch * a.heads;
+    p.K = int(a.d_key); p.V = int(a.d_value); p.Kp = dr_round32(a.d_key); p.Vp = dr_round16(a.d_value);
     p.rep = int(a.heads / a.groups); p.nch = int(plan.nch);
     p.scale = a.scale;
     p.q = {a.q, a.q_batch_stride, a.q_len_stride, a.q_head_stride, p.rep};

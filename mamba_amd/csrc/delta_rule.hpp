@@ -15,6 +15,7 @@ namespace ss {
 constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
 constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 ? 64 : 32; }
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
+constexpr int dr_round32(int64_t n) { return int((n + 31) / 32 * 32); }
 
 // Rows of whole 16-byte vectors that do not overlap, a chunk's within 2^31 bytes: read and written through
 // buffer resources, which end with the chunk's last row.  (8 x 2048 tokens x 24 heads of 64 x 64, bf16: the walk
@@ -25,13 +26,19 @@ inline bool dr_whole(const LaRows& r, int64_t dim, int64_t len, int size) {
 
 // Per (batch, head) pair and chunk, what the kernels hand on (fp32):
 //   plan    the chunk's gates and triangular inverse (delta_rule_chunk.hpp), dr_plan_bytes()
-//   states  the state before the chunk, (Vp, Kp): a value column's keys side by side
+//   states  the state before the chunk, (Vp, Kp): a value column's keys side by side, in the order of state_key
 //   err     the tokens' prediction errors, (Vp, chunk)
 //   dstates the gradient of the state after the chunk;  derr: of the errors, as err
-// Kp, Vp: keys and value columns rounded up to 16, zero past the last.
+// Kp: keys rounded up to 32, Vp: value columns rounded up to 16, zero past the last.  Chunk n of pair bh is at n BH + bh: pairs
+// walk side by side, and what they read and write at a time then lies together (a pair's chunks in a row of 16 KB each
+// put all pairs on the same memory channels: @@).
 constexpr int64_t dr_plan_bytes(int64_t chunk) { return chunk * 20 + 16 + chunk / 16 * (chunk / 16 + 1) / 2 * 1024; }
+// Key at a place of a kept state: tile t of the walk's registers holds, in lane group g, keys 32 (t / 2) + 8 g + 4 (t % 2) ..
+// (places 16 t + 4 g ..).
+__host__ __device__ constexpr int state_key(int place) { return (place & ~31) + (place >> 2 & 3) * 8 + (place >> 4 & 1) * 4 + (place & 3); }
+
 struct DrParams {
-    int64_t B, L, H;
+    int64_t B, L, H, BH;
     int K, V, Kp, Vp, rep, nch;               // rep: heads per group; nch: chunks of a row of L tokens
     float scale;
     int whole;                            // dr_whole of all rows (DrParams' q, k, v, o)
@@ -49,7 +56,7 @@ struct DrParams {
     int segs, seg_chunks;
     int local;                            // the segments' own states from zero and what becomes of a state over one
     float* seg_add;                       // (B, H, segs, Vp, Kp): their states; then the states that they start from
-    float* seg_mul;                       // (B, H, segs, Kp, Kp): over a segment S becomes M S + its own; column i of M at i Kp
+    float* seg_mul;                       // (B, H, segs, Kp, Kp): over a segment S becomes M S + its own; column i of M at i Kp, its rows in that order too
     // gradients
     void* dq; void* dk; void* dv;         // contiguous; dq and dk in fp32 per head with rep > 1
     float* dg; float* dbeta;              // (B, L, H)

@@ -73,6 +73,11 @@ struct Dims {
     static constexpr int VW = 32, KW = KP <= 128 ? KP : KT == 3 ? 64 : 128;
 };
 template <typename T, int KP> constexpr int kPrepThreads = 64 * Dims<T, KP>::NR;
+// A walk's workgroup: 4 waves, 64 value columns; of the segments' own states 8, 4 of them the identity's columns.
+// Waves a SIMD that it is compiled for: with 2 its results stay out of the accumulation registers, where
+// vector instructions do not reach them.
+template <bool REV, bool LOCAL> constexpr int kWalkThreads = LOCAL && !REV ? 512 : 256;
+template <int KP> constexpr int kWalkWaves = KP == 64 ? 2 : 1;
 template <typename T, int KP> constexpr int kGradThreads = 128 * Dims<T, KP>::NR;
 
 template <int NA, int NB, int MAX>
@@ -203,6 +208,30 @@ struct Tile {
             }
         }
     }
+    // the first `rows` rows and `dim` columns of a raw tile to global memory
+    template <int STRIDE>
+    static __device__ __forceinline__ void put(T* p, int64_t step, const T* tile, int rows, int dim) {
+        const int row = int(threadIdx.x) / PER, col = int(threadIdx.x) % PER * R::VE;
+        const T* from = tile + row * STRIDE + col;
+        if constexpr (WHOLE) {
+            constexpr uint32_t es = sizeof(T), none = 0x80000000u;
+            const rsrc_t r = make_rsrc_n(p, rows > 0 && dim > 0 ? int((uint32_t(rows - 1) * uint32_t(step) + uint32_t(dim)) * es) : 0);
+            const uint32_t off = col < dim ? (uint32_t(row) * uint32_t(step) + uint32_t(col)) * es : none;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const u4 w = *reinterpret_cast<const u4*>(from + i * (NTH / PER) * STRIDE);
+                __builtin_amdgcn_raw_buffer_store_b128(w, r, int(off + uint32_t(i * (NTH / PER)) * uint32_t(step) * es), 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                float x[R::VE];
+                R::unpack(*reinterpret_cast<const uint4*>(from + i * (NTH / PER) * STRIDE), x);
+                const int r = row + i * (NTH / PER);
+                R::store(p + int64_t(r) * step + col, x, r < rows ? dim - col : 0);
+            }
+        }
+    }
     template <int STRIDE>
     __device__ __forceinline__ void store_raw(T* tile) const {
         T* to = tile + int(threadIdx.x) / PER * STRIDE + int(threadIdx.x) % PER * R::VE;
@@ -306,7 +335,7 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
     if (t0 >= head.len) return;
     const int lane = int(threadIdx.x) & 63, w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), g = lane >> 4, c = lane & 15;
     const int cnt = head.len - t0 < C ? int(head.len - t0) : C;
-    Plan<T, KP>* plan = plan_at<T, KP>(p, head.bh * p.nch + n);
+    Plan<T, KP>* plan = plan_at<T, KP>(p, n * p.BH + head.bh);
     {
         Tile<T, KP, C, NTH, WHOLE> k;
         k.load(head.rows<T>(p.k) + t0 * p.k.l, p.k.l, cnt, p.K);
@@ -418,25 +447,25 @@ struct PlanIn {
 //
 // Forward it writes out, the states and errors that a backward needs (unless null) and the
 // last state; back, from dout, the states' and errors' gradients and the initial state's.
-// LOCAL: the states only, from zero, and beside them what the segment makes of the
-// columns of the identity (value tiles past the last: no values, the state starts as I).
+// LOCAL: the states only, from zero, and (forward) in 4 waves more what the segment makes of
+// the columns of the identity: no values, the state starts as I.
 template <typename T, int KP, bool REV, bool LOCAL, bool WHOLE>
-__global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
+__global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<KP>)) void dr_walk(const DrParams p) {
     using D = Dims<T, KP>;
+    constexpr int NTH = kWalkThreads<REV, LOCAL>;
     constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NT = D::NT, VST = D::VST;
     constexpr int KTERM = C * KST, CTERM = NT * 256;
     constexpr int PT = REV ? 3 : D::OT;                   // P's terms
     constexpr bool Q = REV || !LOCAL;                     // whether q is read
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * KTERM], qs[Q ? KT * KTERM : 8], tri[3 * CTERM], prob[Q ? PT * CTERM : 8];
-    __shared__ __attribute__((aligned(16))) T vs[C * VST];
+    __shared__ __attribute__((aligned(16))) T vs[C * VST], os[!REV && !LOCAL ? C * VST : 4];
     __shared__ __attribute__((aligned(16))) Gates<C> G;
     const int segs = p.segs, seg = int(blockIdx.x % unsigned(segs));
     const Head head(p, blockIdx.x / uint32_t(segs));
-    const int vt = int(blockIdx.y), vtiles = (p.V + 63) / 64;
-    const int tid = int(threadIdx.x), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const bool unit = LOCAL && vt >= vtiles;              // columns of the identity
-    const int v0 = (unit ? vt - vtiles : vt) * 64, col0 = v0 + 16 * w, col = col0 + c;
-    const bool live = col0 < (unit ? p.K : p.V), mine = !unit && col < p.V;
+    const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3, g = lane >> 4, c = lane & 15;
+    const bool unit = wave >= 4;                          // columns of the identity
+    const int v0 = 64 * int(blockIdx.y), col0 = v0 + 16 * w, col = col0 + c;
+    const bool live = col0 < (unit ? p.Kp : p.V), mine = !unit && col < p.V;
     const int chunks = int((head.len + C - 1) / C);       // of the row
     const int n0 = seg * p.seg_chunks, n1 = n0 + p.seg_chunks < chunks ? n0 + p.seg_chunks : chunks;
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -454,8 +483,8 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
         if (live) {
 #pragma unroll
             for (int t = 0; t < NS; ++t)
-                if (state_row(t, g, 0) < p.Kp)
-                    S[t] = *reinterpret_cast<const f4*>(p.seg_add + ((head.bh * segs + seg) * p.Vp + col) * p.Kp + state_row(t, g, 0));
+                if (32 * (t >> 1) < p.Kp)
+                    S[t] = *reinterpret_cast<const f4*>(p.seg_add + ((head.bh * segs + seg) * p.Vp + col) * p.Kp + 16 * t + 4 * g);
         }
     } else if (!LOCAL && p.init) {
 #pragma unroll
@@ -466,37 +495,46 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                 if (mine && key < p.K) S[t][r] = p.init[(head.bh * p.K + key) * p.V + col];
             }
     }
-    // kept states: a column's rows side by side (value column, key)
+    // kept states: a column's rows side by side in the order of the tiles, so that a store covers 64 bytes of each
     const auto keep_state = [&](float* to) {
-        float* at = to + col * p.Kp + 8 * g;
+        float* at = to + col * p.Kp + 4 * g;
         if (KP == p.Kp) {
 #pragma unroll
-            for (int t = 0; t < NS; ++t) *reinterpret_cast<f4*>(at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
+            for (int t = 0; t < NS; ++t) *reinterpret_cast<f4*>(at + 16 * t) = S[t];
             return;
         }
 #pragma unroll
         for (int t = 0; t < NS; ++t)
-            if (state_row(t, g, 0) < p.Kp) *reinterpret_cast<f4*>(at + 32 * (t >> 1) + 4 * (t & 1)) = S[t];
+            if (32 * (t >> 1) < p.Kp) *reinterpret_cast<f4*>(at + 16 * t) = S[t];
     };
 
-    Tile<T, KP, C, 256, WHOLE> kin, qin;
-    Tile<T, 64, C, 256, WHOLE> vin;                              // v (back: dout)
-    PlanIn<T, KP, 256> plan;
+    Tile<T, KP, C, NTH, WHOLE> kin, qin;
+    Tile<T, 64, C, NTH, WHOLE> vin;                       // v (back: dout)
+    PlanIn<T, KP, NTH> plan;
     const int step = REV ? -1 : 1, first = REV ? n1 - 1 : n0;
-    const T* const kp = head.rows<T>(p.k);
-    const T* const qp = head.rows<T>(p.q);
-    const T* const vp = head.rows<T>(REV ? p.o : p.v) + v0;
     T* const op = const_cast<T*>(head.rows<T>(p.o)) + v0;  // out (back: not written)
-    const int64_t vstep = REV ? p.o.l : p.v.l;
     const auto count = [&](int n) { return head.len - int64_t(n) * C < C ? int(head.len - int64_t(n) * C) : C; };
-    const auto fetch = [&](int n) {                       // (past the last chunk: that one again)
-        n = n < n0 ? n0 : n < n1 ? n : n1 - 1;
-        const int64_t t0 = int64_t(n) * C;
-        const int cnt = count(n);
-        plan.load(plan_at<T, KP>(p, head.bh * p.nch + n));
-        kin.load(kp + t0 * p.k.l, p.k.l, cnt, p.K);
-        if constexpr (Q) qin.load(qp + t0 * p.q.l, p.q.l, cnt, p.K);
-        vin.load(vp + t0 * vstep, vstep, unit ? 0 : cnt, p.V - v0);
+    const int64_t vstep = REV ? p.o.l : p.v.l;
+    // the next chunk to fetch, and where its rows and plan are
+    int next = first;
+    const T* kp = head.rows<T>(p.k) + int64_t(first) * C * p.k.l;
+    const T* qp = head.rows<T>(p.q) + int64_t(first) * C * p.q.l;
+    const T* vp = head.rows<T>(REV ? p.o : p.v) + v0 + int64_t(first) * C * vstep;
+    const Plan<T, KP>* pp = plan_at<T, KP>(p, first * p.BH + head.bh);
+    const int64_t kstep = int64_t(step) * C * p.k.l, qstep = int64_t(step) * C * p.q.l, rstep = int64_t(step) * C * vstep;
+    const auto fetch = [&] {
+        const int cnt = count(next);
+        plan.load(pp);
+        kin.load(kp, p.k.l, cnt, p.K);
+        if constexpr (Q) qin.load(qp, p.q.l, cnt, p.K);
+        vin.load(vp, vstep, cnt, p.V - v0);
+        if (next + step >= n0 && next + step < n1) {      // (past the last chunk: that one again)
+            next += step;
+            kp += kstep;
+            qp += qstep;
+            vp += rstep;
+            pp += step * p.BH;
+        }
     };
     // S += sum over 32 tokens of a tile's rows by the columns f, 4 tiles at a time
     const auto add_rows = [&](const uint16_t* rows, const u4 (&f)[1][3]) {
@@ -519,37 +557,59 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
         plan.store(G, tri);
     };
     if (n0 < n1) {
-        fetch(first);
+        fetch();
         stage();
         lds_barrier();
     }
     for (int n = first; n >= n0 && n < n1; n += step) {
-        const int64_t at = head.bh * p.nch + n, t0 = int64_t(n) * C;
+        const int64_t at = n * p.BH + head.bh, t0 = int64_t(n) * C;
         // Stores first and last: the loads of the next chunk then wait for no younger store.
         if (!LOCAL && live && (REV || p.states)) keep_state((REV ? p.dstates : p.states) + at * p.Vp * p.Kp);
         f4 kept[NR];                                      // E (back: F), column col
-        fetch(n + step);
+        fetch();
         if constexpr (Q) {                                // P, a share of its tiles a wave; formed transposed, rows j, column i
+            // As many tiles side by side as their operands have registers for: all is read ahead of
+            // the first product, else each product waits for its own reads.
+            constexpr int TILES = (NT + 3) / 4, SIDE = NK * KT <= 2 ? TILES : 1;
 #pragma unroll
-            for (int e = 0; e < (NT + 3) / 4; ++e) {
-                // (past the last: that one again, the same values to the same place)
-                const int tile = w + 4 * e < NT ? w + 4 * e : NT - 1, i = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, j = tile - i * (i + 1) / 2;
-                f4 acc = zero;
+            for (int e0 = 0; e0 < TILES; e0 += SIDE) {
+                u4 a[SIDE][NK][KT], b[SIDE][NK][KT];
+                double Gi[SIDE], Gj[SIDE][4];
+                int tile[SIDE], row[SIDE], col_[SIDE];
 #pragma unroll
-                for (int kk = 0; kk < NK; ++kk) {
-                    u4 a[KT], b[KT];
-                    frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a);
-                    frag8<KT, KTERM>(qs + (16 * i + c) * KST + 32 * kk + 8 * g, b);
-                    mac<KT, KT, 2>(a, b, acc);
+                for (int e = 0; e < SIDE; ++e) {
+                    // (past the last: that one again, the same values to the same place)
+                    const int at_tile = w + 4 * (e0 + e);
+                    tile[e] = at_tile < NT ? at_tile : NT - 1;
+                    const int i = tile[e] < 1 ? 0 : tile[e] < 3 ? 1 : tile[e] < 6 ? 2 : 3, j = tile[e] - i * (i + 1) / 2;
+                    row[e] = 16 * j + 4 * g;
+                    col_[e] = 16 * i + c;
+#pragma unroll
+                    for (int kk = 0; kk < NK; ++kk) {
+                        frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a[e][kk]);
+                        frag8<KT, KTERM>(qs + col_[e] * KST + 32 * kk + 8 * g, b[e][kk]);
+                    }
+                    Gi[e] = G.G[col_[e]];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) Gj[e][r] = G.G[row[e] + r];
                 }
-                const double Gi = G.G[16 * i + c];
+                if constexpr (SIDE > 1) stage_end();
+                f4 acc[SIDE];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * j + 4 * g + r;
-                    const float f = factor(Gi, G.G[row]);
-                    acc[r] = row <= 16 * i + c ? acc[r] * f : 0.f;
+                for (int e = 0; e < SIDE; ++e) acc[e] = zero;
+#pragma unroll
+                for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+                    for (int e = 0; e < SIDE; ++e) mac<KT, KT, 2>(a[e][kk], b[e][kk], acc[e]);
+#pragma unroll
+                for (int e = 0; e < SIDE; ++e) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float f = factor(Gi[e], Gj[e][r]);
+                        acc[e][r] = row[e] + r <= col_[e] ? acc[e][r] * f : 0.f;
+                    }
+                    put4<PT, CTERM>(prob + tile[e] * 256 + 16 * c + 4 * g, acc[e]);
                 }
-                put4<PT, CTERM>(prob + tile * 256 + 16 * c + 4 * g, acc);
             }
         }
         if constexpr (!REV) {
@@ -585,6 +645,7 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                     f4 lo, hi;
                     u4 raw[KT];
                     raw_col<T, VST>(vs + 32 * q * VST, w, lane, lo, hi, raw);
+                    if (LOCAL && unit) lo = hi = zero;
                     const f4 glo = *reinterpret_cast<const f4*>(G.gam + 32 * q + 4 * g), ghi = *reinterpret_cast<const f4*>(G.gam + 32 * q + 16 + 4 * g);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -644,27 +705,16 @@ __global__ __launch_bounds__(256) void dr_walk(const DrParams p) {
                         mfma_terms<I, 0, 1, D::OT, PT, D::OT - 1>(&uf[q], b, to);
                     });
                 }
-                lds_barrier();                            // (the chunk's tiles are done with)
-                stage();
-                if (live) {
-                    const int cnt = count(n);
-                    T* const out = op + t0 * p.o.l;
-                    const int at_col = 16 * w + 4 * g, cols = p.V - v0 - at_col;
-                    if constexpr (WHOLE) {
-                        const rsrc_t r = make_rsrc_n(out, int((uint32_t(cnt - 1) * uint32_t(p.o.l) + uint32_t(p.V - v0)) * uint32_t(sizeof(T))));
-                        const uint32_t off = cols > 0 ? (uint32_t(c) * uint32_t(p.o.l) + uint32_t(at_col)) * uint32_t(sizeof(T)) : 0x80000000u;
+                if (live) {                               // out's rows meet in LDS, to be stored whole
 #pragma unroll
-                        for (int i = 0; i < NR; ++i)
-                            bstore4<T>(r, off + uint32_t(16 * i) * uint32_t(p.o.l) * uint32_t(sizeof(T)),
-                                       make_float4(p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < NR; ++i) {
-                            const float o[4] = {p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]};
-                            if (16 * i + c < cnt) store4<T>(out + (16 * i + c) * p.o.l + at_col, o, cols);
-                        }
+                    for (int i = 0; i < NR; ++i) {
+                        const float o[4] = {p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]};
+                        store4<T>(os + (16 * i + c) * VST + 16 * w + 4 * g, o, 4);
                     }
                 }
+                lds_barrier();                            // (the chunk's tiles are done with)
+                stage();
+                Tile<T, 64, C, NTH, WHOLE>::template put<VST>(op + t0 * p.o.l, p.o.l, os, count(n), p.V - v0);
             }
         } else {
             f4 X[NR];
@@ -812,9 +862,9 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     __shared__ float across[NR][C], reads[C], writes[C], inner[2 * NR], dbeta[C];
     constexpr int HALF = KP > 128 ? 128 : KP;             // keys of dk that pass through LDS at a time
     static_assert(sizeof(Stage) >= sizeof(float) * C * (HALF + 4), "dk's share over the tiles");
-    const Head head(p, blockIdx.x / uint32_t(p.nch));
-    const int n = int(blockIdx.x % unsigned(p.nch));
-    const int64_t t0 = int64_t(n) * C, at = head.bh * p.nch + n;
+    const Head head(p, blockIdx.x % uint32_t(p.BH));
+    const int n = int(blockIdx.x / uint32_t(p.BH));
+    const int64_t t0 = int64_t(n) * C, at = n * p.BH + head.bh;
     const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const bool reader = wave < NR;
     const int w = reader ? wave : wave - NR, own = 16 * w + c;
@@ -861,9 +911,9 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         if (v0 >= p.V) return;
 #pragma unroll
         for (int i = 0; i < NSV; ++i) {
-            const int x = tid + i * NTH, v = v0 + x / (KW / 4), key = k0 + x % (KW / 4) * 4;
-            const bool in = v < p.Vp && key < p.Kp;
-            const int64_t from = (at * p.Vp + v) * p.Kp + key;
+            const int x = tid + i * NTH, v = v0 + x / (KW / 4), place = k0 + x % (KW / 4) * 4;
+            const bool in = v < p.Vp && place < p.Kp;
+            const int64_t from = (at * p.Vp + v) * p.Kp + place;
             si[i] = in ? *reinterpret_cast<const f4*>(p.states + from) : zero;
             ti[i] = in ? *reinterpret_cast<const f4*>(p.dstates + from) : zero;
         }
@@ -899,7 +949,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             lds_barrier();
 #pragma unroll
             for (int i = 0; i < NSV; ++i) {
-                const int x = tid + i * NTH, to = x / (KW / 4) * SST + x % (KW / 4) * 4;
+                const int x = tid + i * NTH, to = x / (KW / 4) * SST + state_key(x % (KW / 4) * 4);
                 put4<3, STERM>(st.s + to, si[i]);
                 put4<3, STERM>(st.t + to, ti[i]);
 #pragma unroll
@@ -1175,15 +1225,15 @@ hipError_t dr_prep_launch(const DrParams& p, hipStream_t stream) {
 
 template <typename T>
 hipError_t dr_walk_launch(const DrParams& p, bool rev, hipStream_t stream) {
-    const unsigned tiles = unsigned(p.V + 63) / 64, units = p.local && !rev ? unsigned(p.K + 63) / 64 : 0;
-    const dim3 grid(unsigned(p.B * p.H * p.segs), tiles + units);
+    const int64_t widest = p.local && !rev && p.Kp > p.V ? p.Kp : p.V;
+    const dim3 grid(unsigned(p.B * p.H * p.segs), unsigned(widest + 63) / 64);
     return dr_by_keys<T>(p.K, [&](auto kp) {
         constexpr int KP = decltype(kp)::value;
         const auto go = [&](auto whole) {
             constexpr bool WHOLE = decltype(whole)::value;
             if (rev && p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, true, true, WHOLE>), grid, dim3(256), 0, stream, p);
             else if (rev) hipLaunchKernelGGL((dr::dr_walk<T, KP, true, false, WHOLE>), grid, dim3(256), 0, stream, p);
-            else if (p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, false, true, WHOLE>), grid, dim3(256), 0, stream, p);
+            else if (p.local) hipLaunchKernelGGL((dr::dr_walk<T, KP, false, true, WHOLE>), grid, dim3(512), 0, stream, p);
             else hipLaunchKernelGGL((dr::dr_walk<T, KP, false, false, WHOLE>), grid, dim3(256), 0, stream, p);
         };
         if (p.whole) go(std::true_type{});

@@ -70,10 +70,6 @@ constexpr float kDeepest = -300.f;        // log2 decays below it empty the stat
 // LDS of a wave: its accesses run in order; this keeps the compiler's order.
 __device__ __forceinline__ void lds_in_order() { __asm__ volatile("" ::: "memory"); }
 
-// No instruction moves across: without it the scheduler raises the loads and
-// splits of all steps to the front and runs out of registers.
-__device__ __forceinline__ void stage_end() { __builtin_amdgcn_sched_barrier(0); }
-
 // The lane again, unknown to the compiler: what a rarely taken path derives from it
 // is then computed there, and not once ahead of the loop and kept in registers.
 __device__ __forceinline__ int late(int lane) {
