@@ -254,7 +254,7 @@ DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
 void set_whole(DrParams& p, int32_t dtype) {
     const int size = dtype == SS_F32 ? 4 : 2;
     p.whole = dr_whole(p.q, p.K, p.L, size) && dr_whole(p.k, p.K, p.L, size) && dr_whole(p.v, p.V, p.L, size) &&
-              dr_whole(p.o, p.V, p.L, size);
+              dr_whole(p.o, p.V, p.L, size) && p.H * (p.K > p.V ? p.K : p.V) < (int64_t(1) << 22);
 }
 
 float* at(void* base, int64_t bytes) { return reinterpret_cast<float*>(static_cast<char*>(base) + bytes); }

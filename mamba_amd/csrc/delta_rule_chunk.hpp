@@ -78,7 +78,9 @@ template <typename T, int KP> constexpr int kPrepThreads = 64 * Dims<T, KP>::NR;
 // vector instructions do not reach them.
 template <bool REV, bool LOCAL> constexpr int kWalkThreads = LOCAL && !REV ? 512 : 256;
 template <int KP> constexpr int kWalkWaves = KP == 64 ? 2 : 1;
-template <typename T, int KP> constexpr int kGradThreads = 128 * Dims<T, KP>::NR;
+// dr_grads: a wave takes its tokens in both roles where two such workgroups fit a compute unit's LDS
+template <typename T, int KP> constexpr bool kGradBoth = sizeof(T) == 2 && kTerms<T> == 1 && KP == 64;
+template <typename T, int KP> constexpr int kGradThreads = (kGradBoth<T, KP> ? 64 : 128) * Dims<T, KP>::NR;
 
 template <int NA, int NB, int MAX>
 __device__ __forceinline__ void mac(const u4 (&a)[NA], const u4 (&b)[NB], f4& c) {
@@ -844,14 +846,15 @@ __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<KP>)) void 
 // Every term of dg_t has the factor exp(g_t): nothing cancels that does not in the
 // formula, and dg_t is zero where the decay empties the state.
 //
-// Waves 0 .. NR - 1 take 16 tokens each as readers (columns i of the transposed
-// tiles), waves NR .. 2 NR - 1 as writers (columns j): a reader has w + 1 tiles of M and R and the
-// writer on its SIMD the other NR - w.  The writer's share of dk passes to the reader
-// through LDS.  Value columns pass 32 at a time, those of the next step on their way meanwhile.
+// Waves 0 .. NR - 1 take 16 tokens each as readers (columns i of the transposed tiles: w + 1 tiles
+// of M and R) and waves NR .. 2 NR - 1 as writers (columns j: the other NR - w), whose share of dk
+// passes to the reader through LDS; or (kGradBoth) a wave is both for its tokens.  Value columns
+// pass 32 at a time, those of the next step on their way meanwhile.
 template <typename T, int KP, bool WHOLE>
-__global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams p) {
+__global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 || kGradBoth<T, KP> ? 2 : 1)) void dr_grads(const DrParams p) {
     using D = Dims<T, KP>;
-    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NTH = kGradThreads<T, KP>;
+    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NTH = kGradThreads<T, KP>, NW = NTH / 64;
+    constexpr bool BOTH = kGradBoth<T, KP>;
     constexpr int VW = D::VW, KW = D::KW, SST = KW + 8, EST = C + 8, DST = VW + 8, XT = D::OT;
     constexpr int KTERM = C * KST, STERM = VW * SST, ETERM = VW * EST, DTERM = C * DST;
     // S, dS' (rows value columns, columns keys), E, F (columns tokens), dout (rows tokens)
@@ -859,19 +862,19 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * KTERM], qs[KT * KTERM];
     __shared__ __attribute__((aligned(16))) Stage st;
     __shared__ __attribute__((aligned(16))) Gates<C> gates;
-    __shared__ float across[NR][C], reads[C], writes[C], inner[2 * NR], dbeta[C];
+    __shared__ float across[NR][C], reads[C], writes[C], inner[NW];
     constexpr int HALF = KP > 128 ? 128 : KP;             // keys of dk that pass through LDS at a time
     static_assert(sizeof(Stage) >= sizeof(float) * C * (HALF + 4), "dk's share over the tiles");
+    const int tid = int(threadIdx.x);
+    const bool part = p.rep > 1;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const bool reader = BOTH || wave < NR, writer = BOTH || wave >= NR;
+    const int w = wave < NR ? wave : wave - NR, own = 16 * w + c;
     const Head head(p, blockIdx.x % uint32_t(p.BH));
-    const int n = int(blockIdx.x / uint32_t(p.BH));
-    const int64_t t0 = int64_t(n) * C, at = n * p.BH + head.bh;
-    const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const bool reader = wave < NR;
-    const int w = reader ? wave : wave - NR, own = 16 * w + c;
+    const int64_t n = blockIdx.x / uint32_t(p.BH), t0 = n * C, at = blockIdx.x;
     const int cnt = head.len - t0 < C ? int(head.len > t0 ? head.len - t0 : 0) : C;
     const int toks = p.L - t0 < C ? int(p.L - t0) : C;    // to be written
-    const bool part = p.rep > 1;
-    // rows of contiguous (B, L, heads, dim) tensors
+    // token t's row of a contiguous (B, L, heads, dim) tensor
     const auto row_of = [&](int t, int dim) { return ((head.b * p.L + t0 + t) * p.H + head.h) * dim; };
     // 8 neighbouring elements of a row of type O, those below dim
     const auto put8 = [&](auto* row, int from, int dim, const f4& lo, const f4& hi) {
@@ -886,29 +889,13 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             R::store(row + from + h, x, dim - (from + h));
         }
     };
-    const auto put_keys = [&](void* to, int t, int key, const f4& lo, const f4& hi) {
-        if (part) put8(static_cast<float*>(to) + row_of(t, p.K), key, p.K, lo, hi);
-        else put8(static_cast<T*>(to) + row_of(t, p.K), key, p.K, lo, hi);
-    };
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    if (cnt == 0) {                                       // (no token: every gradient is zero)
-        for (int t = wave; t < toks; t += NTH / 64) {
-            put_keys(p.dq, t, 8 * lane, zero, zero);
-            put_keys(p.dk, t, 8 * lane, zero, zero);
-            put8(static_cast<T*>(p.dv) + row_of(t, p.V), 8 * lane, p.V, zero, zero);
-            if (lane == 0) p.dg[row_of(t, 1)] = p.dbeta[row_of(t, 1)] = 0.f;
-        }
-        return;
-    }
-
     // a step: VW value columns of E, F and dout (with the first of its states' keys), KW keys of S and dS'
     constexpr int NSV = VW * KW / 4 / NTH, NEV = VW * C / 4 / NTH;
     static_assert(VW * KW / 4 % NTH == 0 && VW * C / 4 % NTH == 0, "whole vectors a thread");
     f4 si[NSV], ti[NSV], ei[NEV], fi[NEV];
     Tile<T, VW, C, NTH, WHOLE> di;
-    const T* const dp = head.rows<T>(p.o) + t0 * p.o.l;
     const auto fetch = [&](int v0, int k0) {
-        if (v0 >= p.V) return;
 #pragma unroll
         for (int i = 0; i < NSV; ++i) {
             const int x = tid + i * NTH, v = v0 + x / (KW / 4), place = k0 + x % (KW / 4) * 4;
@@ -925,8 +912,28 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             ei[i] = v < p.Vp ? *reinterpret_cast<const f4*>(p.err + from) : zero;
             fi[i] = v < p.Vp ? *reinterpret_cast<const f4*>(p.derr + from) : zero;
         }
-        di.load(dp + v0, p.o.l, cnt, p.V - v0);
+        di.load(head.rows<T>(p.o) + t0 * p.o.l + v0, p.o.l, cnt, p.V - v0);
     };
+    T* const dq_rows = static_cast<T*>(p.dq) + row_of(0, p.K);
+    T* const dk_rows = static_cast<T*>(p.dk) + row_of(0, p.K);
+    T* const dv_rows = static_cast<T*>(p.dv) + row_of(0, p.V);
+    if (cnt == 0) {                                       // (no token: every gradient is zero)
+        for (int t = wave; t < toks; t += NTH / 64) {
+            if (8 * lane < p.K) {
+                if (part) {
+                    put8(static_cast<float*>(p.dq) + row_of(t, p.K), 8 * lane, p.K, zero, zero);
+                    put8(static_cast<float*>(p.dk) + row_of(t, p.K), 8 * lane, p.K, zero, zero);
+                } else {
+                    put8(static_cast<T*>(p.dq) + row_of(t, p.K), 8 * lane, p.K, zero, zero);
+                    put8(static_cast<T*>(p.dk) + row_of(t, p.K), 8 * lane, p.K, zero, zero);
+                }
+            }
+            if (8 * lane < p.V) put8(static_cast<T*>(p.dv) + row_of(t, p.V), 8 * lane, p.V, zero, zero);
+            if (lane == 0) p.dg[row_of(t, 1)] = p.dbeta[row_of(t, 1)] = 0.f;
+        }
+        return;
+    }
+    // its q, k, gates and first step
     fetch(0, 0);
     {
         Tile<T, KP, C, NTH, WHOLE> kin, qin;
@@ -937,11 +944,15 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         kin.template store<KST>(ks);
         qin.template store<KST>(qs);
     }
-    f4 M[NR], R[NR], dq[NS], dk[NS];                      // reader: M, R transposed (rows j); writer: rows i, and no dq
+    // reader: M, R transposed (rows j); writer: rows i, and no dq
+    f4 Ms[1 + BOTH][NR], Rs[1 + BOTH][NR], dq[NS], dks[1 + BOTH][NS];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) M[i] = R[i] = zero;
+    for (int b = 0; b <= BOTH; ++b) {
 #pragma unroll
-    for (int t = 0; t < NS; ++t) dq[t] = dk[t] = zero;
+        for (int i = 0; i < NR; ++i) Ms[b][i] = Rs[b][i] = zero;
+#pragma unroll
+        for (int t = 0; t < NS; ++t) dq[t] = dks[b][t] = zero;
+    }
     float z = 0.f;
     for (int v0 = 0; v0 < p.V; v0 += VW) {
 #pragma unroll
@@ -966,21 +977,25 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             }
             lds_barrier();
             if (k0 + KW < KP) fetch(v0, k0 + KW);
-            else fetch(v0 + VW, 0);
+            else if (v0 + VW < p.V) fetch(v0 + VW, 0);
             if (reader) {
+                f4 (&M)[NR] = Ms[0], (&R)[NR] = Rs[0], (&dk)[NS] = dks[0];
                 u4 df[KT], ff[3];
                 frag8<KT, DTERM>(st.d + own * DST + 8 * g, df);
                 frag_col8<3, ETERM, EST>(st.f, block16(w, lane), lane, ff);
                 if (k0 == 0) {
 #pragma unroll
-                    for (int j = 0; j < NR; ++j) {
+                    for (int j = 0; j < NR; j += 2) {     // (two tiles side by side: the one past w is masked below)
                         if (j > w) continue;
-                        u4 a[3];
-                        frag_col8<3, ETERM, EST>(st.e, block16(j, lane), lane, a);
-                        mac<3, KT, 2>(a, df, R[j]);
-                        mac<3, 3, 2>(a, ff, M[j]);
+                        u4 a[2][3];
+                        f4* const r2[2] = {&R[j], &R[j + 1]};
+                        f4* const m2[2] = {&M[j], &M[j + 1]};
+                        frag_col8<3, ETERM, EST>(st.e, block16(j, lane), lane, a[0]);
+                        frag_col8<3, ETERM, EST>(st.e, block16(j + 1, lane), lane, a[1]);
+                        mfma_terms<2, 1, 0, 3, KT, 2>(a, &df, r2);
+                        mfma_terms<2, 1, 0, 3, 3, 2>(a, &ff, m2);
                     }
-                    if (own < toks) {                     // dv: F of the own token
+                    if (own < toks && v0 + 8 * g < p.V) { // dv: F of the own token
                         const bool is = own < cnt && gates.beta[own] != 0.f;
                         f4 x[2];
 #pragma unroll
@@ -988,35 +1003,47 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
                             const auto half = [&](const u4& t) { return e & 1 ? hi_half(t[e >> 1]) : lo_half(t[e >> 1]); };
                             x[e >> 2][e & 3] = is ? half(ff[0]) + (half(ff[1]) + half(ff[2])) : 0.f;
                         }
-                        put8(static_cast<T*>(p.dv) + row_of(own, p.V), v0 + 8 * g, p.V, x[0], x[1]);
+                        put8(dv_rows + int64_t(own) * p.H * p.V, v0 + 8 * g, p.V, x[0], x[1]);
                     }
                 }
 #pragma unroll
-                for (int t = k0 / 16; t < (k0 + KW) / 16; ++t) {
-                    u4 a[3];
-                    frag_col8<3, STERM, SST>(st.s - k0, state_block(t, lane), lane, a);
-                    mac<3, KT, 2>(a, df, dq[t]);
-                    mac<3, 3, 2>(a, ff, dk[t]);
+                for (int t = k0 / 16; t < (k0 + KW) / 16; t += 2) {
+                    u4 a[2][3];
+                    f4* const q2[2] = {&dq[t], &dq[t + 1]};
+                    f4* const k2[2] = {&dk[t], &dk[t + 1]};
+                    frag_col8<3, STERM, SST>(st.s - k0, state_block(t, lane), lane, a[0]);
+                    frag_col8<3, STERM, SST>(st.s - k0, state_block(t + 1, lane), lane, a[1]);
+                    mfma_terms<2, 1, 0, 3, KT, 2>(a, &df, q2);
+                    mfma_terms<2, 1, 0, 3, 3, 2>(a, &ff, k2);
                 }
-            } else {
+            }
+            if (writer) {
+                f4 (&M)[NR] = Ms[BOTH], (&R)[NR] = Rs[BOTH], (&dk)[NS] = dks[BOTH];
                 u4 ef[3];
                 frag_col8<3, ETERM, EST>(st.e, block16(w, lane), lane, ef);
                 if (k0 == 0) {
 #pragma unroll
-                    for (int i = 0; i < NR; ++i) {
-                        if (i < w) continue;
-                        u4 a[3], d[KT];
-                        frag_col8<3, ETERM, EST>(st.f, block16(i, lane), lane, a);
-                        frag8<KT, DTERM>(st.d + (16 * i + c) * DST + 8 * g, d);
-                        mac<3, 3, 2>(a, ef, M[i]);
-                        mac<KT, 3, 2>(d, ef, R[i]);
+                    for (int i = 0; i < NR; i += 2) {
+                        if (i + 1 < w) continue;
+                        u4 a[2][3], d[2][KT];
+                        f4* const r2[2] = {&R[i], &R[i + 1]};
+                        f4* const m2[2] = {&M[i], &M[i + 1]};
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            frag_col8<3, ETERM, EST>(st.f, block16(i + e, lane), lane, a[e]);
+                            frag8<KT, DTERM>(st.d + (16 * (i + e) + c) * DST + 8 * g, d[e]);
+                        }
+                        mfma_terms<2, 1, 0, 3, 3, 2>(a, &ef, m2);
+                        mfma_terms<2, 1, 0, KT, 3, 2>(d, &ef, r2);
                     }
                 }
 #pragma unroll
-                for (int t = k0 / 16; t < (k0 + KW) / 16; ++t) {
-                    u4 a[3];
-                    frag_col8<3, STERM, SST>(st.t - k0, state_block(t, lane), lane, a);
-                    mac<3, 3, 2>(a, ef, dk[t]);
+                for (int t = k0 / 16; t < (k0 + KW) / 16; t += 2) {
+                    u4 a[2][3];
+                    f4* const k2[2] = {&dk[t], &dk[t + 1]};
+                    frag_col8<3, STERM, SST>(st.t - k0, state_block(t, lane), lane, a[0]);
+                    frag_col8<3, STERM, SST>(st.t - k0, state_block(t + 1, lane), lane, a[1]);
+                    mfma_terms<2, 1, 0, 3, 3, 2>(a, &ef, k2);
                 }
             }
         }
@@ -1041,6 +1068,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
     const double Gown = gates.G[own];
     const float bown = gates.beta[own];
     if (reader) {
+        f4 (&M)[NR] = Ms[0], (&R)[NR] = Rs[0], (&dk)[NS] = dks[0];
         const float gam = gates.gam[own];
         float r = 0.f;
 #pragma unroll
@@ -1061,7 +1089,10 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         float before = 0.f;                               // sum of the column's terms in earlier tiles
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
-            if (j > w) continue;
+            if (j > w) {
+                R[j] = M[j] = zero;
+                continue;
+            }
             f4 kq = zero, kk2 = zero;
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) {
@@ -1078,7 +1109,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             for (int q = 0; q < 4; ++q) {
                 const int row = 16 * j + 4 * g + q;
                 const float f = row <= own ? factor(Gown, gates.G[row]) : 0.f;
-                if (row == own) dbeta[own] = M[j][q] / beta_or_least(bown);
+                if (row == own && own < toks) p.dbeta[row_of(own, 1)] = own < cnt ? M[j][q] / beta_or_least(bown) : 0.f;
                 R[j][q] = row <= own ? f * (p.scale * beta[q]) * R[j][q] : 0.f;
                 M[j][q] = row < own ? -f * beta[q] * M[j][q] : 0.f;
                 term[q] = __builtin_fmaf(R[j][q], kq[q], M[j][q] * kk2[q]);
@@ -1106,13 +1137,17 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
             pack<XT>(M[2 * q], M[2 * q + 1], mf);
 #pragma unroll
             for (int t = 0; t < NS; ++t) {
-                u4 a[KT];
-                frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a);
-                mac<KT, XT, XT - 1>(a, rf, dq[t]);
-                mac<KT, XT, XT - 1>(a, mf, dk[t]);
+                u4 a[1][KT], b[2][XT];
+                f4* const to[2] = {&dq[t], &dk[t]};
+                frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a[0]);
+#pragma unroll
+                for (int n = 0; n < XT; ++n) b[0][n] = rf[n], b[1][n] = mf[n];
+                mfma_terms<2, 0, 1, KT, XT, XT - 1>(a, b, to);
             }
         }
-    } else {
+    }
+    if (writer) {
+        f4 (&M)[NR] = Ms[BOTH], (&R)[NR] = Rs[BOTH], (&dk)[NS] = dks[BOTH];
         const float by = gates.end[own] * bown;
         float r = 0.f;
 #pragma unroll
@@ -1130,7 +1165,10 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         if (g == 0) writes[own] = r;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            if (i < w) continue;
+            if (i < w) {
+                R[i] = M[i] = zero;
+                continue;
+            }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int row = 16 * i + 4 * g + q;
@@ -1156,26 +1194,48 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
         }
     }
     float* share = reinterpret_cast<float*>(&st);         // (C, HALF + 4)
+    T* const q_out = reinterpret_cast<T*>(qs);            // dq and dk in the rows' type, over q and k
+    T* const k_out = reinterpret_cast<T*>(ks);
     const bool on = own < cnt;
 #pragma unroll
     for (int k0 = 0; k0 < KP; k0 += HALF) {
         lds_barrier();                                    // (the tiles, or the half before, are done with)
-        if (!reader) {
+        if constexpr (!BOTH) {
+            if (writer) {
 #pragma unroll
-            for (int t = k0 / 16; t < (k0 + HALF) / 16; ++t)
-                *reinterpret_cast<f4*>(share + own * (HALF + 4) + state_row(t, g, 0) - k0) = dk[t];
+                for (int t = k0 / 16; t < (k0 + HALF) / 16; ++t)
+                    *reinterpret_cast<f4*>(share + own * (HALF + 4) + state_row(t, g, 0) - k0) = dks[0][t];
+            }
+            lds_barrier();
         }
-        lds_barrier();
-        if (reader && own < toks) {
+        if (reader) {
 #pragma unroll
             for (int t = k0 / 16; t < (k0 + HALF) / 16; t += 2) {
                 const int key = state_row(t, g, 0);
-                const float* with = share + own * (HALF + 4) + key - k0;
-                const f4 lo = dk[t] + *reinterpret_cast<const f4*>(with), hi = dk[t + 1] + *reinterpret_cast<const f4*>(with + 4);
-                put_keys(p.dq, own, key, on ? dq[t] : zero, on ? dq[t + 1] : zero);
-                put_keys(p.dk, own, key, on ? lo : zero, on ? hi : zero);
+                f4 lo = dks[0][t], hi = dks[0][t + 1];
+                if constexpr (BOTH) {
+                    lo += dks[BOTH][t];
+                    hi += dks[BOTH][t + 1];
+                } else {
+                    const float* with = share + own * (HALF + 4) + key - k0;
+                    lo += *reinterpret_cast<const f4*>(with);
+                    hi += *reinterpret_cast<const f4*>(with + 4);
+                }
+                if (!on) lo = hi = dq[t] = dq[t + 1] = zero;
+                if (!part) {
+                    put8(q_out + own * KST, key, KP, dq[t], dq[t + 1]);
+                    put8(k_out + own * KST, key, KP, lo, hi);
+                } else if (own < toks && key < p.K) {
+                    put8(static_cast<float*>(p.dq) + row_of(own, p.K), key, p.K, dq[t], dq[t + 1]);
+                    put8(static_cast<float*>(p.dk) + row_of(own, p.K), key, p.K, lo, hi);
+                }
             }
         }
+    }
+    if (!part) {
+        lds_barrier();
+        Tile<T, KP, C, NTH, WHOLE>::template put<KST>(dq_rows, p.H * p.K, q_out, toks, p.K);
+        Tile<T, KP, C, NTH, WHOLE>::template put<KST>(dk_rows, p.H * p.K, k_out, toks, p.K);
     }
     if (wave == 0) {                                      // (after the barriers above)
         const bool in = lane < C;
@@ -1193,12 +1253,9 @@ __global__ __launch_bounds__((kGradThreads<T, KP>)) void dr_grads(const DrParams
 #pragma unroll
             for (int i = 0; i < NR; ++i) sum += 16 * i + 15 >= lane ? across[i][lane] : 0.f;
 #pragma unroll
-            for (int i = 0; i < 2 * NR; ++i) z += inner[i];
+            for (int i = 0; i < NW; ++i) z += inner[i];
             sum += suffix + lead + gates.total * z;
-            if (lane < toks) {
-                p.dg[row_of(lane, 1)] = lane < cnt ? sum : 0.f;
-                p.dbeta[row_of(lane, 1)] = lane < cnt ? dbeta[lane] : 0.f;
-            }
+            if (lane < toks) p.dg[row_of(lane, 1)] = lane < cnt ? sum : 0.f;
         }
     }
 }
@@ -1246,7 +1303,9 @@ template <typename T>
 hipError_t dr_grads_launch(const DrParams& p, hipStream_t stream) {
     return dr_by_keys<T>(p.K, [&](auto kp) {
         constexpr int KP = decltype(kp)::value;
-        const dim3 grid(unsigned(p.B * p.H * p.nch)), block(dr::kGradThreads<T, KP>);
+        // (a workgroup a compute unit, which its tiles fill: it goes from chunk to chunk)
+        const int64_t all = p.BH * p.nch;
+        const dim3 grid(unsigned(all), 1), block(dr::kGradThreads<T, KP>);
         if (p.whole) hipLaunchKernelGGL((dr::dr_grads<T, KP, true>), grid, block, 0, stream, p);
         else hipLaunchKernelGGL((dr::dr_grads<T, KP, false>), grid, block, 0, stream, p);
         return hipGetLastError();
