@@ -328,16 +328,19 @@ struct Head {
 template <typename T, int KP, bool WHOLE>
 __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams p) {
     using D = Dims<T, KP>;
-    constexpr int C = D::C, NR = D::NR, KT = D::KT, KST = D::KST, TERM = C * KST, NST = C + 4, NTH = kPrepThreads<T, KP>;
-    __shared__ __attribute__((aligned(16))) uint16_t ks[KT * TERM];
-    __shared__ __attribute__((aligned(16))) float ns[C * NST], ts[NR][16 * 20];
-    __shared__ Gates<C> gates;
-    const Head head(p, blockIdx.x / uint32_t(p.nch));
-    const int64_t n = blockIdx.x % unsigned(p.nch), t0 = n * C;
+    constexpr int C = D::C, NR = D::NR, KT = D::KT, KST = D::KST, TERM = C * KST, NST = 20, NTH = kPrepThreads<T, KP>;
+    // k, and over it N's lower tiles (rows of 16 + 4), the diagonal ones then their inverses
+    union Lds { uint16_t k[KT * TERM]; float n[D::NT * 16 * NST]; };
+    __shared__ __attribute__((aligned(16))) Lds lds;
+    __shared__ __attribute__((aligned(16))) Gates<C> gates;
+    uint16_t* const ks = lds.k;
+    const auto tile = [&](int i, int j) { return lds.n + tile_at(i, j) * (16 * NST); };
+    const Head head(p, blockIdx.x % uint32_t(p.BH));
+    const int64_t n = blockIdx.x / uint32_t(p.BH), t0 = n * C;
     if (t0 >= head.len) return;
     const int lane = int(threadIdx.x) & 63, w = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6), g = lane >> 4, c = lane & 15;
     const int cnt = head.len - t0 < C ? int(head.len - t0) : C;
-    Plan<T, KP>* plan = plan_at<T, KP>(p, n * p.BH + head.bh);
+    Plan<T, KP>* plan = plan_at<T, KP>(p, blockIdx.x);
     {
         Tile<T, KP, C, NTH, WHOLE> k;
         k.load(head.rows<T>(p.k) + t0 * p.k.l, p.k.l, cnt, p.K);
@@ -353,6 +356,7 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
         reinterpret_cast<uint4*>(&plan->gates)[i] = reinterpret_cast<const uint4*>(&gates)[i];
     // N's row of tiles, transposed: rows j, column i
     const double Gi = gates.G[16 * w + c];
+    f4 x[NR];
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
         if (j > w) continue;
@@ -364,36 +368,39 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
             frag8<KT, TERM>(ks + (16 * w + c) * KST + 32 * kk + 8 * g, b);
             mac<KT, KT, 2>(a, b, acc);
         }
-        float x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * j + 4 * g + r;
-            x[r] = row < 16 * w + c ? acc[r] * factor(Gi, gates.G[row]) * beta_or_least(gates.beta[row]) : 0.f;
+            x[j][r] = row < 16 * w + c ? acc[r] * factor(Gi, gates.G[row]) * beta_or_least(gates.beta[row]) : 0.f;
         }
-        *reinterpret_cast<float4*>(ns + (16 * w + c) * NST + 16 * j + 4 * g) = make_float4(x[0], x[1], x[2], x[3]);
     }
     __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NR; ++j)
+        if (j <= w) *reinterpret_cast<f4*>(tile(w, j) + c * NST + 4 * g) = x[j];
+    __syncthreads();
     // the diagonal tile's inverse: column c, the rows of it
-    float x[16];
+    float y[16];
+    float* const own = tile(w, w);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         float row[16];
 #pragma unroll
         for (int j = 0; j < r; j += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(ns + (16 * w + r) * NST + 16 * w + j);
+            const float4 v = *reinterpret_cast<const float4*>(own + r * NST + j);
             row[j] = v.x; row[j + 1] = v.y; row[j + 2] = v.z; row[j + 3] = v.w;
         }
         float s0 = r == c ? 1.f : 0.f, s1 = 0.f;
 #pragma unroll
-        for (int j = 0; j < r; ++j) (j & 1 ? s1 : s0) = __builtin_fmaf(-row[j], x[j], j & 1 ? s1 : s0);
-        x[r] = s0 + s1;
+        for (int j = 0; j < r; ++j) (j & 1 ? s1 : s0) = __builtin_fmaf(-row[j], y[j], j & 1 ? s1 : s0);
+        y[r] = s0 + s1;
     }
     f4 t[NR];                                  // column w's tiles, from the diagonal one on
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const float lo = g & 1 ? x[4 + r] : x[r], hi = g & 1 ? x[12 + r] : x[8 + r];
+        const float lo = g & 1 ? y[4 + r] : y[r], hi = g & 1 ? y[12 + r] : y[8 + r];
         t[0][r] = g & 2 ? hi : lo;
-        ts[w][(4 * g + r) * 20 + c] = t[0][r];
+        own[(4 * g + r) * NST + c] = t[0][r];     // (of this wave's tile, which it has read)
     }
     __syncthreads();
     const auto mm = [&](const float* a, const f4& b, f4 acc) {       // a: 16 rows of this lane's, 4 summands from 4 g on
@@ -410,8 +417,8 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
         if (d > 0) {
             f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int m = 0; m < d; ++m) acc = mm(ns + (16 * i + c) * NST + 16 * (w + m) + 4 * g, t[m], acc);
-            t[d] = -mm(&ts[i][c * 20 + 4 * g], acc, f4{0.f, 0.f, 0.f, 0.f});
+            for (int m = 0; m < d; ++m) acc = mm(tile(i, w + m) + c * NST + 4 * g, t[m], acc);
+            t[d] = -mm(tile(i, i) + c * NST + 4 * g, acc, f4{0.f, 0.f, 0.f, 0.f});
         }
         *reinterpret_cast<f4*>(plan->tri + tile_at(i, w) * 256 + 16 * c + 4 * g) = t[d];
     }
