@@ -26,17 +26,19 @@ using namespace la;
 
 // The states that the segments start from, in place of their own: S <- M S + N along the
 // row (REV: M^T, from the last segment on).  A wave 16 value columns, which do not meet; M comes
-// through LDS in 3 terms (in halves of its columns past 128 keys), the next one on its way meanwhile.
+// through LDS in 3 terms, CW columns at a time, two such slices and the next N on their way meanwhile.
 template <int KP, bool REV>
 __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
     constexpr int NS = KP / 16, NK = KP / 32, CW = KP < 128 ? KP : KP == 128 ? 64 : 32, MST = KP + 8, TERM = CW * MST, N = CW * KP / 4 / 256;
+    constexpr int SL = KP / CW, STEPS = SL == 1 ? 2 : 1;                 // slices of an M, segments that the loop takes at a time
     __shared__ __attribute__((aligned(16))) uint16_t ms[3 * TERM];       // CW columns of M, a row each
     const int tid = int(threadIdx.x), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int64_t bh = blockIdx.x;
-    const int col = int(blockIdx.y) * 64 + 16 * (tid >> 6) + c;
+    const int col = int(blockIdx.y) * 64 + 16 * __builtin_amdgcn_readfirstlane(tid >> 6) + c, steps = p.segs - 1;
     const bool live = col - c < p.V;
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 S[NS], in[N];
+    f4 S[NS], own[NS], in[2][N];
+    u4 sf[NK][3];                                         // S before the step
 #pragma unroll
     for (int t = 0; t < NS; ++t)
 #pragma unroll
@@ -45,92 +47,111 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
             S[t][r] = p.init && key < p.K && col < p.V ? p.init[(bh * p.K + key) * p.V + col] : 0.f;
         }
     const auto seg_of = [&](int i) { return bh * p.segs + (REV ? p.segs - 1 - i : i); };
-    const auto fetch = [&](int i, int c0) {
-        if (i >= p.segs) return;
-        const float* mul = p.seg_mul + seg_of(i) * p.Kp * p.Kp;
+    // (what is past the tensors reads as zero and is not stored: no branch waits for the loads)
+    constexpr int none = int(0x80000000u);
+    const int row = c * p.Kp * 4;
+    const auto add_of = [&](int i) {
+        return make_rsrc_n(p.seg_add + (seg_of(i) * p.Vp + (live ? col - c : 0)) * p.Kp, live ? 16 * p.Kp * 4 : 0);
+    };
+    const auto fetch = [&](int slice, f4 (&to)[N]) {
+        const int i = slice / SL, c0 = slice % SL * CW;
+        const rsrc_t from = make_rsrc_n(p.seg_mul + seg_of(i < steps ? i : 0) * p.Kp * p.Kp, i < steps ? p.Kp * p.Kp * 4 : 0);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int x = tid + k * 256, at = c0 + x / (KP / 4), place = x % (KP / 4) * 4;
-            in[k] = at < p.Kp && place < p.Kp ? *reinterpret_cast<const f4*>(mul + int64_t(at) * p.Kp + place) : zero;
+            to[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(from, place < p.Kp ? (at * p.Kp + place) * 4 : none, 0, 0));
         }
     };
-    fetch(0, 0);
-    for (int i = 0; i < p.segs; ++i) {
-        u4 sf[NK][3];
+    const auto fetch_own = [&](int i) {
+        const rsrc_t from = add_of(i < steps ? i : 0);
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
+        for (int t = 0; t < NS; ++t)
+            own[t] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(from, 32 * (t >> 1) < p.Kp ? row + (16 * t + 4 * g) * 4 : none, 0, 0));
+    };
+    const auto keep = [&](int i) {
+        const rsrc_t to = add_of(i);
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const f4& x = S[2 * k + (h >> 1)];
-                uint32_t t[3];
-                split<3>(x[2 * (h & 1)], x[2 * (h & 1) + 1], t);
+        for (int t = 0; t < NS; ++t)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, S[t]), to, 32 * (t >> 1) < p.Kp ? row + (16 * t + 4 * g) * 4 : none, 0, 0);
+    };
+    fetch_own(0);
+    fetch(0, in[0]);
+    fetch(1, in[1]);
+    for (int i0 = 0; i0 < steps; i0 += STEPS) {
 #pragma unroll
-                for (int n = 0; n < 3; ++n) sf[k][n][h] = t[n];
+        for (int x = 0; x < SL * STEPS; ++x) {
+            const int i = i0 + x / SL, c0 = x % SL * CW;
+            if (i >= steps) break;
+            if (x % SL == 0) {
+                keep(i);
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const f4& from = S[2 * k + (h >> 1)];
+                        uint32_t t[3];
+                        split<3>(from[2 * (h & 1)], from[2 * (h & 1) + 1], t);
+#pragma unroll
+                        for (int n = 0; n < 3; ++n) sf[k][n][h] = t[n];
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NS; ++t) S[t] = own[t];
+                fetch_own(i + 1);
             }
-        }
-        if (live) {
-            float* add = p.seg_add + (seg_of(i) * p.Vp + col) * p.Kp;
-#pragma unroll
-            for (int t = 0; t < NS; ++t) {
-                const int place = 16 * t + 4 * g;
-                if (32 * (t >> 1) >= p.Kp) continue;
-                const f4 own = *reinterpret_cast<const f4*>(add + place);
-                *reinterpret_cast<f4*>(add + place) = S[t];
-                S[t] = own;
-            }
-        }
-#pragma unroll
-        for (int c0 = 0; c0 < KP; c0 += CW) {
             lds_barrier();
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const int x = tid + k * 256;
+                const int at = tid + k * 256;
                 uint32_t a[3], b[3];
-                split<3>(in[k][0], in[k][1], a);
-                split<3>(in[k][2], in[k][3], b);
+                split<3>(in[x & 1][k][0], in[x & 1][k][1], a);
+                split<3>(in[x & 1][k][2], in[x & 1][k][3], b);
 #pragma unroll
                 for (int n = 0; n < 3; ++n)
-                    *reinterpret_cast<uint2*>(ms + n * TERM + x / (KP / 4) * MST + state_key(x % (KP / 4) * 4)) = make_uint2(a[n], b[n]);
+                    *reinterpret_cast<uint2*>(ms + n * TERM + at / (KP / 4) * MST + state_key(at % (KP / 4) * 4)) = make_uint2(a[n], b[n]);
             }
             lds_barrier();
-            if (c0 + CW < KP) fetch(i, c0 + CW);
-            else fetch(i + 1, 0);
-            if (!live) continue;
-            f4* to[1];
+            fetch(i0 * SL + x + 2, in[x & 1]);
             if constexpr (REV) {                          // rows of M^T: these columns, all keys
 #pragma unroll
-                for (int t = c0 / 16; t < (c0 + CW) / 16; ++t) {
-                    const uint16_t* row = ms + (32 * (t >> 1) + 8 * (c >> 2) + 4 * (t & 1) + (c & 3) - c0) * MST + 8 * g;
-                    to[0] = &S[t];
+                for (int t = c0 / 16; t < (c0 + CW) / 16; t += 2) {
+                    f4* const to[2] = {&S[t], &S[t + 1]};
 #pragma unroll
                     for (int k = 0; k < NK; ++k) {
-                        u4 a[3];
+                        u4 a[2][3];
 #pragma unroll
-                        for (int n = 0; n < 3; ++n) a[n] = *reinterpret_cast<const u4*>(row + n * TERM + 32 * k);
-                        mfma_terms<1, 0, 0, 3, 3, 2>(&a, &sf[k], to);
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int n = 0; n < 3; ++n)
+                                a[e][n] = *reinterpret_cast<const u4*>(ms + n * TERM + (16 * t + 8 * (c >> 2) + 4 * e + (c & 3) - c0) * MST + 8 * g + 32 * k);
+                        mfma_terms<2, 1, 0, 3, 3, 2>(a, &sf[k], to);
                     }
                 }
             } else {                                      // all rows of M, these columns
                 typedef __attribute__((address_space(3))) s4 lds_s4;
 #pragma unroll
-                for (int t = 0; t < NS; ++t) {
-                    to[0] = &S[t];
+                for (int t = 0; t < NS; t += 2) {
+                    f4* const to[2] = {&S[t], &S[t + 1]};
 #pragma unroll
                     for (int k = c0 / 32; k < (c0 + CW) / 32; ++k) {
-                        const uint16_t* at = ms + (32 * k - c0 + 8 * g + (c >> 2)) * MST + 32 * (t >> 1) + 8 * (c & 3) + 4 * (t & 1);
-                        u4 a[3];
+                        u4 a[2][3];
 #pragma unroll
-                        for (int n = 0; n < 3; ++n) {
-                            const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM)));
-                            const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM + 4 * MST)));
-                            a[n] = u4{lo.x, lo.y, hi.x, hi.y};
+                        for (int e = 0; e < 2; ++e) {
+                            const uint16_t* at = ms + (32 * k - c0 + 8 * g + (c >> 2)) * MST + 16 * t + 8 * (c & 3) + 4 * e;
+#pragma unroll
+                            for (int n = 0; n < 3; ++n) {
+                                const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM)));
+                                const u2 hi = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM + 4 * MST)));
+                                a[e][n] = u4{lo.x, lo.y, hi.x, hi.y};
+                            }
                         }
-                        mfma_terms<1, 0, 0, 3, 3, 2>(&a, &sf[k], to);
+                        mfma_terms<2, 1, 0, 3, 3, 2>(a, &sf[k], to);
                     }
                 }
             }
         }
     }
+    keep(steps);
 }
 
 // The heads of a group share q and k: out[r, j, :] = sum over i of part[r, j * rep + i, :]
@@ -157,10 +178,9 @@ hipError_t for_type(int32_t dtype, F&& f) {
 
 int terms(int32_t dtype) { return dtype == SS_F32 ? 3 : dtype == SS_BF16 ? 1 : 2; }
 
-// Compute units.  Rows are cut into segments where fewer than half of them would walk, into enough
-// for one workgroup each, or for the two that fit where tiles and registers are small; a segment
-// keeps at least 8 chunks.
-constexpr int64_t kUnits = 256, kSegChunksMin = 8;
+// Compute units.  Rows are cut into segments, enough for one workgroup each, or for the two that fit
+// where tiles and registers are small; a segment keeps at least 4 chunks.
+constexpr int64_t kUnits = 256, kSegChunksMin = 4, kSegsMin = 3;
 
 struct Plan {
     int64_t bh, nch, plan, state, rows, mul;     // (batch, head) pairs, chunks; floats of a chunk's plan, a state, a chunk's rows, an M
@@ -178,9 +198,9 @@ Plan plan_of(const ss_delta_rule_args& a) {
     p.mul = kp * kp;
     const int64_t walks = p.bh * ((a.d_value + 63) / 64);
     const bool two = a.d_key <= 64 && a.dtype != SS_F32;
-    int64_t segs = walks > 0 && walks <= kUnits / 2 ? (two ? 2 : 1) * kUnits / walks : 1;
+    int64_t segs = walks > 0 ? (two ? 2 : 1) * kUnits / walks : 1;
     if (segs > p.nch / kSegChunksMin) segs = p.nch / kSegChunksMin;
-    if (segs < 1) segs = 1;
+    if (segs < kSegsMin) segs = 1;
     const int64_t per = p.nch > 0 ? (p.nch + segs - 1) / segs : 1;
     p.segs = p.nch > 0 ? int((p.nch + per - 1) / per) : 1;
     p.seg_chunks = int(per);

@@ -470,6 +470,8 @@ __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<KP>)) void 
     __shared__ __attribute__((aligned(16))) T vs[C * VST], os[!REV && !LOCAL ? C * VST : 4];
     __shared__ __attribute__((aligned(16))) Gates<C> G;
     const int segs = p.segs, seg = int(blockIdx.x % unsigned(segs));
+    // (nothing starts from the last segment's own state; a backward takes its M)
+    if (LOCAL && seg == (REV ? 0 : segs - 1) && (REV || !p.states)) return;
     const Head head(p, blockIdx.x / uint32_t(segs));
     const int tid = int(threadIdx.x), lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3, g = lane >> 4, c = lane & 15;
     const bool unit = wave >= 4;                          // columns of the identity
