@@ -293,6 +293,15 @@ __device__ __forceinline__ void put_gates(Gates<C>& s, float g, float beta, int 
     if (lane == 0) s.total = __builtin_amdgcn_exp2f(float(all));
 }
 __device__ __forceinline__ float factor(double Gi, double Gj) { return __builtin_amdgcn_exp2f(float(Gi - Gj)); }
+// factors of one token with 4 neighbouring ones: of it over them, or with OVER false of them over it
+// (read before any of them is chosen: no branch per element)
+template <bool OVER>
+__device__ __forceinline__ f4 factors(double own, const double* four) {
+    typedef double d2 __attribute__((ext_vector_type(2)));
+    const d2 a = reinterpret_cast<const d2*>(four)[0], b = reinterpret_cast<const d2*>(four)[1];
+    return OVER ? f4{factor(own, a[0]), factor(own, a[1]), factor(own, b[0]), factor(own, b[1])}
+                : f4{factor(a[0], own), factor(a[1], own), factor(b[0], own), factor(b[1], own)};
+}
 
 // What dr_prep leaves of a chunk: its gates, and T's lower tiles in fp32, each transposed
 // (element (row, column) of tile n at n * 256 + column * 16 + row).
@@ -368,10 +377,11 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
             frag8<KT, TERM>(ks + (16 * w + c) * KST + 32 * kk + 8 * g, b);
             mac<KT, KT, 2>(a, b, acc);
         }
+        const f4 f = factors<true>(Gi, gates.G + 16 * j + 4 * g), beta = *reinterpret_cast<const f4*>(gates.beta + 16 * j + 4 * g);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * j + 4 * g + r;
-            x[j][r] = row < 16 * w + c ? acc[r] * factor(Gi, gates.G[row]) * beta_or_least(gates.beta[row]) : 0.f;
+            const float v = acc[r] * f[r] * beta_or_least(beta[r]);
+            x[j][r] = 16 * j + 4 * g + r < 16 * w + c ? v : 0.f;
         }
     }
     __syncthreads();
@@ -398,7 +408,8 @@ __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams 
     f4 t[NR];                                  // column w's tiles, from the diagonal one on
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const float lo = g & 1 ? y[4 + r] : y[r], hi = g & 1 ? y[12 + r] : y[8 + r];
+        const float y0 = y[r], y1 = y[4 + r], y2 = y[8 + r], y3 = y[12 + r];
+        const float lo = g & 1 ? y1 : y0, hi = g & 1 ? y3 : y2;
         t[0][r] = g & 2 ? hi : lo;
         own[(4 * g + r) * NST + c] = t[0][r];     // (of this wave's tile, which it has read)
     }
@@ -871,7 +882,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * KTERM], qs[KT * KTERM];
     __shared__ __attribute__((aligned(16))) Stage st;
     __shared__ __attribute__((aligned(16))) Gates<C> gates;
-    __shared__ float across[NR][C], reads[C], writes[C], inner[NW];
+    __shared__ __attribute__((aligned(16))) float across[NR][C], reads[C], writes[C], inner[NW];
     constexpr int HALF = KP > 128 ? 128 : KP;             // keys of dk that pass through LDS at a time
     static_assert(sizeof(Stage) >= sizeof(float) * C * (HALF + 4), "dk's share over the tiles");
     const int tid = int(threadIdx.x);
@@ -895,7 +906,8 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
             float x[R::VE];
 #pragma unroll
             for (int e = 0; e < R::VE; ++e) x[e] = v[h + e];
-            R::store(row + from + h, x, dim - (from + h));
+            if (!WHOLE) R::store(row + from + h, x, dim - (from + h));
+            else if (from + h < dim) R::store(row + from + h, x, R::VE);
         }
     };
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -1005,12 +1017,12 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
                         mfma_terms<2, 1, 0, 3, 3, 2>(a, &ff, m2);
                     }
                     if (own < toks && v0 + 8 * g < p.V) { // dv: F of the own token
-                        const bool is = own < cnt && gates.beta[own] != 0.f;
+                        const uint32_t is = own < cnt && gates.beta[own] != 0.f ? ~0u : 0u;
                         f4 x[2];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const auto half = [&](const u4& t) { return e & 1 ? hi_half(t[e >> 1]) : lo_half(t[e >> 1]); };
-                            x[e >> 2][e & 3] = is ? half(ff[0]) + (half(ff[1]) + half(ff[2])) : 0.f;
+                            x[e >> 2][e & 3] = __builtin_bit_cast(float, is & __builtin_bit_cast(uint32_t, half(ff[0]) + (half(ff[1]) + half(ff[2]))));
                         }
                         put8(dv_rows + int64_t(own) * p.H * p.V, v0 + 8 * g, p.V, x[0], x[1]);
                     }
@@ -1095,7 +1107,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
         }
         r = groups_sum(r);
         if (g == 0) reads[own] = r;
-        float before = 0.f;                               // sum of the column's terms in earlier tiles
+        float before = 0.f, diag = 0.f;                   // sum of the column's terms in earlier tiles; M_ii
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
             if (j > w) {
@@ -1105,22 +1117,23 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
             f4 kq = zero, kk2 = zero;
 #pragma unroll
             for (int kk = 0; kk < NK; ++kk) {
-                u4 a[KT], b[KT];
-                frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a);
-                frag8<KT, KTERM>(qs + own * KST + 32 * kk + 8 * g, b);
-                mac<KT, KT, 2>(a, b, kq);
-                frag8<KT, KTERM>(ks + own * KST + 32 * kk + 8 * g, b);
-                mac<KT, KT, 2>(a, b, kk2);
+                u4 a[1][KT], b[2][KT];
+                f4* const to[2] = {&kq, &kk2};
+                frag8<KT, KTERM>(ks + (16 * j + c) * KST + 32 * kk + 8 * g, a[0]);
+                frag8<KT, KTERM>(qs + own * KST + 32 * kk + 8 * g, b[0]);
+                frag8<KT, KTERM>(ks + own * KST + 32 * kk + 8 * g, b[1]);
+                mfma_terms<2, 0, 1, KT, KT, 2>(a, b, to);
             }
             const f4 beta = *reinterpret_cast<const f4*>(gates.beta + 16 * j + 4 * g);
+            const f4 fs = factors<true>(Gown, gates.G + 16 * j + 4 * g);
             float term[4], sum = 0.f;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int row = 16 * j + 4 * g + q;
-                const float f = row <= own ? factor(Gown, gates.G[row]) : 0.f;
-                if (row == own && own < toks) p.dbeta[row_of(own, 1)] = own < cnt ? M[j][q] / beta_or_least(bown) : 0.f;
-                R[j][q] = row <= own ? f * (p.scale * beta[q]) * R[j][q] : 0.f;
-                M[j][q] = row < own ? -f * beta[q] * M[j][q] : 0.f;
+                diag = row == own ? M[j][q] : diag;
+                const float rv = fs[q] * (p.scale * beta[q]) * R[j][q], mv = -fs[q] * beta[q] * M[j][q];
+                R[j][q] = row <= own ? rv : 0.f;
+                M[j][q] = row < own ? mv : 0.f;
                 term[q] = __builtin_fmaf(R[j][q], kq[q], M[j][q] * kk2[q]);
                 sum += term[q];
             }
@@ -1130,14 +1143,15 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
             const float two = __shfl_up(lead + sum, 32, 64);    // (groups g - 2 and g - 3)
             float pre = before + lead + (g >= 2 ? two : 0.f);
             before += groups_sum(sum);
+            f4 all;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int row = 16 * j + 4 * g + q;
-                const float all = lanes_sum<16>(row <= own ? pre : 0.f);
-                if (c == 0) across[w][row] = all;
+                all[q] = lanes_sum<16>(16 * j + 4 * g + q <= own ? pre : 0.f);
                 pre += term[q];
             }
+            if (c == 0) *reinterpret_cast<f4*>(&across[w][16 * j + 4 * g]) = all;
         }
+        if (c >> 2 == g && own < toks) p.dbeta[row_of(own, 1)] = own < cnt ? diag / beta_or_least(bown) : 0.f;
 #pragma unroll
         for (int q = 0; q < NP; ++q) {
             if (2 * q > w) continue;
@@ -1178,12 +1192,13 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
                 R[i] = M[i] = zero;
                 continue;
             }
+            const f4 fs = factors<false>(Gown, gates.G + 16 * i + 4 * g);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int row = 16 * i + 4 * g + q;
-                const float f = row >= own ? factor(gates.G[row], Gown) : 0.f;
-                R[i][q] = row >= own ? f * (p.scale * bown) * R[i][q] : 0.f;
-                M[i][q] = row > own ? -f * bown * M[i][q] : 0.f;
+                const float rv = fs[q] * (p.scale * bown) * R[i][q], mv = -fs[q] * bown * M[i][q];
+                R[i][q] = row >= own ? rv : 0.f;
+                M[i][q] = row > own ? mv : 0.f;
             }
         }
 #pragma unroll
@@ -1193,12 +1208,16 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
             pack<XT>(R[2 * q], R[2 * q + 1], rf);
             pack<XT>(M[2 * q], M[2 * q + 1], mf);
 #pragma unroll
-            for (int t = 0; t < NS; ++t) {
-                u4 a[KT];
-                frag_col<KT, KTERM, KST>(qs + 32 * q * KST, state_block(t, lane), lane, a);
-                mac<KT, XT, XT - 1>(a, rf, dk[t]);
-                frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t, lane), lane, a);
-                mac<KT, XT, XT - 1>(a, mf, dk[t]);
+            for (int t = 0; t < NS; t += 2) {
+                u4 a[2][KT], b[2][KT];
+                f4* const to[2] = {&dk[t], &dk[t + 1]};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    frag_col<KT, KTERM, KST>(qs + 32 * q * KST, state_block(t + e, lane), lane, a[e]);
+                    frag_col<KT, KTERM, KST>(ks + 32 * q * KST, state_block(t + e, lane), lane, b[e]);
+                }
+                mfma_terms<2, 1, 0, KT, XT, XT - 1>(a, &rf, to);
+                mfma_terms<2, 1, 0, KT, XT, XT - 1>(b, &mf, to);
             }
         }
     }
