@@ -64,6 +64,45 @@ def test_forward_and_backward(shape, dtype):
     compare(x, run(x))
 
 
+WHOLE = [
+    # rows of whole 16-byte vectors, narrower than the tiles
+    (1, 70, 2, 2, 8, 8), (2, 65, 3, 1, 24, 16), (1, 100, 2, 1, 72, 40), (1, 129, 2, 2, 136, 24), (1, 97, 1, 1, 200, 136),
+    # many segments, at every tile of keys
+    (1, 4000, 1, 1, 64, 64), (1, 1700, 2, 1, 128, 128), (1, 1500, 1, 1, 256, 48),
+]
+
+
+@TYPES
+@pytest.mark.parametrize("shape", WHOLE, ids=lambda s: "x".join(map(str, s)))
+def test_whole_rows_and_segments(shape, dtype):
+    x = make(*shape, dtype, seed=50 + sum(shape), initial=True)
+    compare(x, run(x))
+
+
+@TYPES
+def test_lengths_within_segments(dtype):
+    """Rows that end in the first, a middle and the last segment, and one without tokens."""
+    lengths = [0, 100, 1000, 1699, 1700]
+    x = make(5, 1700, 1, 1, 96, 64, dtype, seed=51, initial=True, lengths=lengths)
+    got = run(x)
+    compare(x, got)
+    for b, n in enumerate(lengths):
+        for name in ("out", "dq", "dk", "dv", "dg", "dbeta"):
+            assert not got[name][b, n:].any(), (name, n)
+
+
+def test_backward_twice():
+    """What a forward keeps is left as it is by a backward."""
+    for L in (200, 2000):
+        x = make(1, L, 2, 1, 64, 64, BF16, seed=52, initial=True)
+        leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v", "g", "beta", "initial")]
+        o, last = delta_rule_fn(*leaves[:5], initial_state=leaves[5], return_last_state=True)
+        first = torch.autograd.grad([o, last], leaves, [x["dout"], x["dlast"]], retain_graph=True)
+        torch.autograd.grad([o], leaves, [x["dout"] * 2], retain_graph=True)
+        for a, b in zip(first, torch.autograd.grad([o, last], leaves, [x["dout"], x["dlast"]])):
+            assert torch.equal(a, b)
+
+
 @TYPES
 @pytest.mark.parametrize("shape", [(2, 1100, 4, 4, 64, 64), (1, 700, 2, 2, 128, 128)], ids=lambda s: "x".join(map(str, s)))
 def test_precision(shape, dtype):
