@@ -91,6 +91,16 @@ def test_lengths_within_segments(dtype):
             assert not got[name][b, n:].any(), (name, n)
 
 
+def test_lengths_of_64_bits():
+    """Whole numbers of either width, past 32 bits too."""
+    x = make(4, 100, 2, 2, 32, 32, F32, seed=53, initial=True, lengths=[0, 37, 100, 100])
+    want = run(x)
+    x["lengths"] = torch.tensor([-(1 << 40), 37, 1 << 32, (1 << 40) + 5], device=DEV)
+    got = run(x)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
 def test_backward_twice():
     """What a forward keeps is left as it is by a backward."""
     for L in (200, 2000):
