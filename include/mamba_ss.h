@@ -632,7 +632,7 @@ typedef struct ss_delta_rule_bwd_args {
 } ss_delta_rule_bwd_args;
 
 /* Bytes of `saved` and of workspace that the calls need (0: none), or -1 (with
-   ss_last_error set) on failing checks.  The forward's workspace is smaller with saved given.
+   ss_last_error set) on failing checks.  The forward's workspace goes by whether saved is given.
    No device work. */
 int64_t ss_delta_rule_saved_bytes(const ss_delta_rule_args* a);
 int64_t ss_delta_rule_fwd_workspace_bytes(const ss_delta_rule_args* a);

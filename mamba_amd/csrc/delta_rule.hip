@@ -182,6 +182,8 @@ int terms(int32_t dtype) { return dtype == SS_F32 ? 3 : dtype == SS_BF16 ? 1 : 2
 
 // Compute units.  Rows are cut into segments, enough for one workgroup each, or for the two that fit
 // where tiles and registers are small (1 x 32768 tokens x 24 heads of 64 x 64: walk 223 us with 10 segments, 170 with 21).
+// With wider keys or fp32 rows only the walk back gains from the second one (bf16, 1 x 32768 tokens x 16 heads of 128 x 128:
+// forward and backward 2,422 us to 2,246, forward alone 710 to 729, as its join takes twice the steps), so a prompt has one.
 // The segments' own states cost about what their walk does, so two are not worth it: 5 x 1021 tokens
 // x 24 heads, fp32, 109 us in two and 64 in one.  A segment keeps at least 4 chunks (2 x 515 tokens x 6 heads of 96 x 80, fp32:
 // 104 us in two of 9 chunks, 76 in four).
@@ -191,7 +193,8 @@ struct Plan {
     int64_t bh, nch, plan, state, rows, mul;     // (batch, head) pairs, chunks; floats of a chunk's plan, a state, a chunk's rows, an M
     int segs, seg_chunks, chunk;
 };
-Plan plan_of(const ss_delta_rule_args& a) {
+// train: of a forward whose states are kept, and of its backward
+Plan plan_of(const ss_delta_rule_args& a, bool train) {
     Plan p{};
     p.chunk = dr_chunk(a.d_key, terms(a.dtype));
     p.bh = a.batch * a.heads;
@@ -202,7 +205,7 @@ Plan plan_of(const ss_delta_rule_args& a) {
     p.rows = p.chunk * vp;
     p.mul = kp * kp;
     const int64_t walks = p.bh * ((a.d_value + 63) / 64);
-    const bool two = a.d_key <= 64 && a.dtype != SS_F32;
+    const bool two = train ? dr_two(a.d_key, terms(a.dtype)) : a.d_key <= 64 && a.dtype != SS_F32;
     int64_t segs = walks > 0 ? (two ? 2 : 1) * kUnits / walks : 1;
     if (segs > p.nch / kSegChunksMin) segs = p.nch / kSegChunksMin;
     if (segs < kSegsMin) segs = 1;
@@ -312,15 +315,15 @@ hipError_t walk(int32_t dtype, DrParams p, bool rev, hipStream_t stream) {
 }  // namespace
 
 int64_t delta_rule_chunks(const ss_delta_rule_args* a) {
-    const Plan p = plan_of(*a);
+    const Plan p = plan_of(*a, false);
     return p.bh * p.nch;
 }
-int64_t delta_rule_saved_bytes(const ss_delta_rule_args* a) { return saved_of(plan_of(*a)).bytes; }
-int64_t delta_rule_fwd_space(const ss_delta_rule_args* a) { return fwd_space(*a, plan_of(*a)).bytes; }
-int64_t delta_rule_bwd_space(const ss_delta_rule_bwd_args* g) { return bwd_space(g->f, plan_of(g->f)).bytes; }
+int64_t delta_rule_saved_bytes(const ss_delta_rule_args* a) { return saved_of(plan_of(*a, true)).bytes; }
+int64_t delta_rule_fwd_space(const ss_delta_rule_args* a) { return fwd_space(*a, plan_of(*a, a->saved)).bytes; }
+int64_t delta_rule_bwd_space(const ss_delta_rule_bwd_args* g) { return bwd_space(g->f, plan_of(g->f, true)).bytes; }
 
 hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream) {
-    const Plan plan = plan_of(*a);
+    const Plan plan = plan_of(*a, a->saved);
     const FwdSpace sp = fwd_space(*a, plan);
     const Saved sv = saved_of(plan);
     DrParams p = params_of(*a, plan);
@@ -344,7 +347,7 @@ hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream
 
 hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t stream) {
     const ss_delta_rule_args& a = g->f;
-    const Plan plan = plan_of(a);
+    const Plan plan = plan_of(a, true);
     const BwdSpace sp = bwd_space(a, plan);
     const Saved sv = saved_of(plan);
     DrParams p = params_of(a, plan);

@@ -14,6 +14,8 @@ namespace ss {
 // fit the 160 KB of LDS, else 32.  terms: bf16 terms of a row's element (bf16 1, fp16 2, fp32 3).
 constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
 constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 ? 64 : 32; }
+// Where two workgroups of a walk share a compute unit: tiles of at most 80 KB.
+constexpr bool dr_two(int64_t k, int terms) { return dr_keys(k) * terms <= 128 || (dr_keys(k) == 128 && terms == 3); }
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
 constexpr int dr_round32(int64_t n) { return int((n + 31) / 32 * 32); }
 

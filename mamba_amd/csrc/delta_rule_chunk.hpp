@@ -76,9 +76,9 @@ template <typename T, int KP> constexpr int kPrepThreads = 64 * Dims<T, KP>::NR;
 // A walk's workgroup: 4 waves, 64 value columns; of the segments' own states 8, 4 of them the identity's columns.
 // Waves a SIMD that it is compiled for: with 2 its results stay out of the accumulation registers, where
 // vector instructions do not reach them, and of 64 keys two workgroups share a compute unit (1 x 32768 tokens x 24
-// heads: 223 us to 170).  Wider states take one wave's registers.
+// heads: 223 us to 170).  Wider tiles leave room for one.
 template <bool REV, bool LOCAL> constexpr int kWalkThreads = LOCAL && !REV ? 512 : 256;
-template <int KP> constexpr int kWalkWaves = KP == 64 ? 2 : 1;
+template <typename T, int KP> constexpr int kWalkWaves = dr_two(KP, kTerms<T>) ? 2 : 1;
 // dr_grads: a wave takes its tokens in both roles where two such workgroups fit a compute unit's LDS (80 KB each:
 // one is at its products while the other waits for its loads; 317 us to 218 with what came along)
 template <typename T, int KP> constexpr bool kGradBoth = sizeof(T) == 2 && kTerms<T> == 1 && KP == 64;
@@ -481,7 +481,7 @@ struct PlanIn {
 // a column tile (half the rows each, joined through LDS) took 187 us for 172 then, fp16 of 128 keys 216 for 157, fp32 51
 // for 62; one design was kept.
 template <typename T, int KP, bool REV, bool LOCAL, bool WHOLE>
-__global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<KP>)) void dr_walk(const DrParams p) {
+__global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<T, KP>)) void dr_walk(const DrParams p) {
     using D = Dims<T, KP>;
     constexpr int NTH = kWalkThreads<REV, LOCAL>;
     constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NT = D::NT, VST = D::VST;
