@@ -25,33 +25,39 @@ namespace {
 using namespace la;
 
 // The states that the segments start from, in place of their own: S <- M S + N along the
-// row (REV: M^T, from the last segment on).  A wave 16 value columns, which do not meet; M comes
-// through LDS in 3 terms, CW columns at a time, two such slices and the next N on their way meanwhile.
-// Serial along the row, a latency a segment: 24 rows of 20 steps at 64 keys 36 us, 32 rows of 3 steps at 128 23 us (56 and 34
-// with loads behind branches, one step ahead).
+// row (REV: M^T, from the last segment on).  Value columns do not meet: a wave has 16, up to 128 keys with another
+// one (every second pair of tiles each; S's terms through LDS).  M comes through LDS in 3 terms, CW columns
+// at a time, two such slices and the next N on their way meanwhile.
+// Serial along the row, a latency a segment: 24 rows of 20 steps at 64 keys 33 us, 32 rows of 3 steps at 128 21 us (56 and 34
+// with loads behind branches, one step ahead, and one wave a column tile).
+template <int KP> constexpr int kJoinThreads = KP <= 128 ? 512 : 256;
 template <int KP, bool REV>
-__global__ __launch_bounds__(256) void dr_join(const DrParams p) {
-    constexpr int NS = KP / 16, NK = KP / 32, CW = KP < 128 ? KP : KP == 128 ? 64 : 32, MST = KP + 8, TERM = CW * MST, N = CW * KP / 4 / 256;
+__global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
+    constexpr int NTH = kJoinThreads<KP>, WAVES = NTH / 256;             // of a column tile
+    constexpr int NK = KP / 32, NP = NK / WAVES, CW = KP < 128 ? KP : KP == 128 ? 64 : 32, MST = KP + 8, TERM = CW * MST, N = CW * KP / 4 / NTH;
     constexpr int SL = KP / CW, STEPS = SL == 1 ? 2 : 1;                 // slices of an M, segments that the loop takes at a time
     __shared__ __attribute__((aligned(16))) uint16_t ms[3 * TERM];       // CW columns of M, a row each
+    __shared__ __attribute__((aligned(16))) u4 parts[WAVES > 1 ? 4 : 1][NK][3][64];
     const int tid = int(threadIdx.x), lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), ct = wave & 3, own_pair = wave >> 2;    // pairs own_pair, + WAVES ...
     const int64_t bh = blockIdx.x;
-    const int col = int(blockIdx.y) * 64 + 16 * __builtin_amdgcn_readfirstlane(tid >> 6) + c, steps = p.segs - 1;
+    const int col = int(blockIdx.y) * 64 + 16 * ct + c, steps = p.segs - 1;
     const bool live = col - c < p.V;
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 S[NS], own[NS], in[2][N];
-    u4 sf[NK][3];                                         // S before the step
+    f4 S[2 * NP], own[2 * NP], in[2][N];                  // tiles 2 (own_pair + WAVES j) + e at 2 j + e
+    u4 sf[NK][3];                                         // S before the step, all keys
+    const auto tile = [&](int t) { return 2 * ((t >> 1) * WAVES + own_pair) + (t & 1); };
 #pragma unroll
-    for (int t = 0; t < NS; ++t)
+    for (int t = 0; t < 2 * NP; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int key = state_row(t, g, r);
+            const int key = state_row(tile(t), g, r);
             S[t][r] = p.init && key < p.K && col < p.V ? p.init[(bh * p.K + key) * p.V + col] : 0.f;
         }
     const auto seg_of = [&](int i) { return bh * p.segs + (REV ? p.segs - 1 - i : i); };
     // (what is past the tensors reads as zero and is not stored: no branch waits for the loads)
     constexpr int none = int(0x80000000u);
-    const int row = c * p.Kp * 4;
+    const auto place = [&](int t) { return 32 * (tile(t) >> 1) < p.Kp ? (c * p.Kp + 16 * tile(t) + 4 * g) * 4 : none; };
     const auto add_of = [&](int i) {
         return make_rsrc_n(p.seg_add + (seg_of(i) * p.Vp + (live ? col - c : 0)) * p.Kp, live ? 16 * p.Kp * 4 : 0);
     };
@@ -60,21 +66,20 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
         const rsrc_t from = make_rsrc_n(p.seg_mul + seg_of(i < steps ? i : 0) * p.Kp * p.Kp, i < steps ? p.Kp * p.Kp * 4 : 0);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int x = tid + k * 256, at = c0 + x / (KP / 4), place = x % (KP / 4) * 4;
+            const int x = tid + k * NTH, at = c0 + x / (KP / 4), place = x % (KP / 4) * 4;
             to[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(from, place < p.Kp ? (at * p.Kp + place) * 4 : none, 0, 0));
         }
     };
     const auto fetch_own = [&](int i) {
         const rsrc_t from = add_of(i < steps ? i : 0);
 #pragma unroll
-        for (int t = 0; t < NS; ++t)
-            own[t] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(from, 32 * (t >> 1) < p.Kp ? row + (16 * t + 4 * g) * 4 : none, 0, 0));
+        for (int t = 0; t < 2 * NP; ++t)
+            own[t] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(from, place(t), 0, 0));
     };
     const auto keep = [&](int i) {
         const rsrc_t to = add_of(i);
 #pragma unroll
-        for (int t = 0; t < NS; ++t)
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, S[t]), to, 32 * (t >> 1) < p.Kp ? row + (16 * t + 4 * g) * 4 : none, 0, 0);
+        for (int t = 0; t < 2 * NP; ++t) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, S[t]), to, place(t), 0, 0);
     };
     fetch_own(0);
     fetch(0, in[0]);
@@ -87,7 +92,7 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
             if (x % SL == 0) {
                 keep(i);
 #pragma unroll
-                for (int k = 0; k < NK; ++k) {
+                for (int k = 0; k < NP; ++k) {
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         const f4& from = S[2 * k + (h >> 1)];
@@ -98,13 +103,19 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
                     }
                 }
 #pragma unroll
-                for (int t = 0; t < NS; ++t) S[t] = own[t];
+                for (int t = 0; t < 2 * NP; ++t) S[t] = own[t];
                 fetch_own(i + 1);
             }
             lds_barrier();
+            if (WAVES > 1 && x % SL == 0) {
+#pragma unroll
+                for (int k = 0; k < NP; ++k)
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) parts[ct][k * WAVES + own_pair][n][lane] = sf[k][n];
+            }
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const int at = tid + k * 256;
+                const int at = tid + k * NTH;
                 uint32_t a[3], b[3];
                 split<3>(in[x & 1][k][0], in[x & 1][k][1], a);
                 split<3>(in[x & 1][k][2], in[x & 1][k][3], b);
@@ -114,10 +125,16 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
             }
             lds_barrier();
             fetch(i0 * SL + x + 2, in[x & 1]);
+            if (WAVES > 1 && x % SL == 0) {
+#pragma unroll
+                for (int k = 0; k < NK; ++k)
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) sf[k][n] = parts[ct][k][n][lane];
+            }
             if constexpr (REV) {                          // rows of M^T: these columns, all keys
 #pragma unroll
-                for (int t = c0 / 16; t < (c0 + CW) / 16; t += 2) {
-                    f4* const to[2] = {&S[t], &S[t + 1]};
+                for (int j = c0 / 32 / WAVES; j < (c0 + CW) / 32 / WAVES; ++j) {
+                    f4* const to[2] = {&S[2 * j], &S[2 * j + 1]};
 #pragma unroll
                     for (int k = 0; k < NK; ++k) {
                         u4 a[2][3];
@@ -125,21 +142,21 @@ __global__ __launch_bounds__(256) void dr_join(const DrParams p) {
                         for (int e = 0; e < 2; ++e)
 #pragma unroll
                             for (int n = 0; n < 3; ++n)
-                                a[e][n] = *reinterpret_cast<const u4*>(ms + n * TERM + (16 * t + 8 * (c >> 2) + 4 * e + (c & 3) - c0) * MST + 8 * g + 32 * k);
+                                a[e][n] = *reinterpret_cast<const u4*>(ms + n * TERM + (16 * tile(2 * j) + 8 * (c >> 2) + 4 * e + (c & 3) - c0) * MST + 8 * g + 32 * k);
                         mfma_terms<2, 1, 0, 3, 3, 2>(a, &sf[k], to);
                     }
                 }
             } else {                                      // all rows of M, these columns
                 typedef __attribute__((address_space(3))) s4 lds_s4;
 #pragma unroll
-                for (int t = 0; t < NS; t += 2) {
-                    f4* const to[2] = {&S[t], &S[t + 1]};
+                for (int j = 0; j < NP; ++j) {
+                    f4* const to[2] = {&S[2 * j], &S[2 * j + 1]};
 #pragma unroll
                     for (int k = c0 / 32; k < (c0 + CW) / 32; ++k) {
                         u4 a[2][3];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const uint16_t* at = ms + (32 * k - c0 + 8 * g + (c >> 2)) * MST + 16 * t + 8 * (c & 3) + 4 * e;
+                            const uint16_t* at = ms + (32 * k - c0 + 8 * g + (c >> 2)) * MST + 16 * tile(2 * j) + 8 * (c & 3) + 4 * e;
 #pragma unroll
                             for (int n = 0; n < 3; ++n) {
                                 const u2 lo = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + n * TERM)));
@@ -300,8 +317,8 @@ hipError_t walk(int32_t dtype, DrParams p, bool rev, hipStream_t stream) {
         const dim3 grid(unsigned(p.B * p.H), unsigned(p.V + 63) / 64);
         const auto join = [&](auto kp) {
             constexpr int KP = decltype(kp)::value;
-            if (rev) hipLaunchKernelGGL((dr_join<KP, true>), grid, dim3(256), 0, stream, p);
-            else hipLaunchKernelGGL((dr_join<KP, false>), grid, dim3(256), 0, stream, p);
+            if (rev) hipLaunchKernelGGL((dr_join<KP, true>), grid, dim3(kJoinThreads<KP>), 0, stream, p);
+            else hipLaunchKernelGGL((dr_join<KP, false>), grid, dim3(kJoinThreads<KP>), 0, stream, p);
             return hipGetLastError();
         };
         const int64_t kp = dr_keys(p.K);
