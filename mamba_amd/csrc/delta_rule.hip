@@ -173,16 +173,29 @@ __global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
     keep(steps);
 }
 
-// The heads of a group share q and k: out[r, j, :] = sum over i of part[r, j * rep + i, :]
-template <typename T>
-__global__ __launch_bounds__(256) void dr_group_sum(const float* dq, T* outq, const float* dk, T* outk, int64_t n, int rep, int dim) {
+// The heads of a group share q and k: out[r, j, :] = sum over i of part[r, j * rep + i, :], heads in order.
+// W neighbouring elements a thread (4 where dim is a multiple of 4).  16384 rows of 4 groups of 6 heads of 64 keys, bf16: 36 us
+// for both, 218 MB (64 with one element a thread and 64-bit divisions).
+template <typename T, int W>
+__global__ __launch_bounds__(256) void dr_group_sum(const float* dq, T* outq, const float* dk, T* outk, int64_t rows, int rep, int dim) {
     const float* part = blockIdx.y ? dk : dq;
     T* out = blockIdx.y ? outk : outq;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-        const int64_t g = i / dim, c = i % dim;
-        float s = 0.f;
-        for (int r = 0; r < rep; ++r) s += part[(g * rep + r) * dim + c];
-        io<T>::store(out + i, s);
+    const uint32_t per = uint32_t(dim / W);
+    const int64_t step = int64_t(gridDim.x) * 256, n = rows * per;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
+        const int64_t row = n <= 0xffffffffll ? int64_t(uint32_t(i) / per) : i / per;
+        const int c = int(i - row * per) * W;
+        const float* from = part + row * rep * dim + c;
+        if constexpr (W == 4) {
+            f4 s = *reinterpret_cast<const f4*>(from);
+            for (int r = 1; r < rep; ++r) s += *reinterpret_cast<const f4*>(from + int64_t(r) * dim);
+            const float v[4] = {s[0], s[1], s[2], s[3]};
+            store4<T>(out + row * dim + c, v, 4);
+        } else {
+            float s = from[0];
+            for (int r = 1; r < rep; ++r) s += from[int64_t(r) * dim];
+            io<T>::store(out + row * dim + c, s);
+        }
     }
 }
 
@@ -382,10 +395,16 @@ hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t st
     if (e != hipSuccess || !part) return e;
     return for_type(a.dtype, [&](auto t) {
         using T = decltype(t);
-        const int64_t n = a.batch * a.seqlen * a.groups * a.d_key, want = (n + 255) / 256;
-        hipLaunchKernelGGL((dr_group_sum<T>), dim3(unsigned(want < 65536 ? want : 65536), 2), dim3(256), 0, stream,
-                           static_cast<const float*>(p.dq), static_cast<T*>(g->dq), static_cast<const float*>(p.dk),
-                           static_cast<T*>(g->dk), n, p.rep, p.K);
+        const int64_t rows = a.batch * a.seqlen * a.groups;
+        const auto go = [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            const int64_t want = (rows * (p.K / W) + 255) / 256;
+            hipLaunchKernelGGL((dr_group_sum<T, W>), dim3(unsigned(want < 65536 ? want : 65536), 2), dim3(256), 0, stream,
+                               static_cast<const float*>(p.dq), static_cast<T*>(g->dq), static_cast<const float*>(p.dk),
+                               static_cast<T*>(g->dk), rows, p.rep, p.K);
+        };
+        if (p.K % 4 == 0) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 1>{});
         return hipGetLastError();
     });
 }
