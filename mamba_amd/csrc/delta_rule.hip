@@ -25,27 +25,28 @@ namespace {
 using namespace la;
 
 // The states that the segments start from, in place of their own: S <- M S + N along the
-// row (REV: M^T, from the last segment on).  Value columns do not meet: a wave has 16, up to 128 keys with another
-// one (every second pair of tiles each; S's terms through LDS).  M comes through LDS in 3 terms, CW columns
-// at a time, two such slices and the next N on their way meanwhile.
-// Serial along the row, a latency a segment: 24 rows of 20 steps at 64 keys 33 us, 32 rows of 3 steps at 128 21 us (56 and 34
-// with loads behind branches, one step ahead, and one wave a column tile).
-template <int KP> constexpr int kJoinThreads = KP <= 128 ? 512 : 256;
+// row (REV: M^T, from the last segment on).  Value columns do not meet: two waves have 16 (every second pair
+// of tiles each; S's terms through LDS).  M comes through LDS in 3 terms, as the walk left it, CW columns at a time,
+// the next slices and the next N on their way meanwhile.
+// Serial along the row, a latency a segment: 24 rows of 20 steps at 64 keys 30 us, 32 rows of 3 steps at 128 20 (56 and 34 with
+// loads behind branches, one step ahead, and one wave a column tile), 4 rows of 15 steps at 256 187 (319 with one wave).
+template <int KP> constexpr int kJoinTiles = KP <= 128 ? 4 : 2;           // column tiles of a workgroup, two waves each
 template <int KP, bool REV>
-__global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
-    constexpr int NTH = kJoinThreads<KP>, WAVES = NTH / 256;             // of a column tile
-    constexpr int NK = KP / 32, NP = NK / WAVES, CW = KP < 128 ? KP : KP == 128 ? 64 : 32, MST = KP + 8, TERM = CW * MST, N = CW * KP / 4 / NTH;
-    constexpr int SL = KP / CW, STEPS = SL == 1 ? 2 : 1;                 // slices of an M, segments that the loop takes at a time
+__global__ __launch_bounds__(128 * kJoinTiles<KP>) void dr_join(const DrParams p) {
+    constexpr int CT = kJoinTiles<KP>, WAVES = 2, NTH = 64 * CT * WAVES;
+    constexpr int NK = KP / 32, NP = NK / WAVES, CW = 64, MST = KP + 8, TERM = CW * MST, PER = KP / 8, N = 3 * CW * PER / NTH;
+    constexpr int SL = KP / CW, AHEAD = KP <= 128 ? 2 : 1, STEPS = SL < AHEAD ? 2 : 1;    // slices of an M, those on their way, segments the loop takes at a time
     __shared__ __attribute__((aligned(16))) uint16_t ms[3 * TERM];       // CW columns of M, a row each
-    __shared__ __attribute__((aligned(16))) u4 parts[WAVES > 1 ? 4 : 1][NK][3][64];
+    __shared__ __attribute__((aligned(16))) u4 parts[CT][NK][3][64];
     const int tid = int(threadIdx.x), lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), ct = wave & 3, own_pair = wave >> 2;    // pairs own_pair, + WAVES ...
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), ct = wave % CT, own_pair = wave / CT;    // pairs own_pair, + WAVES ...
     const int64_t bh = blockIdx.x;
-    const int col = int(blockIdx.y) * 64 + 16 * ct + c, steps = p.segs - 1;
+    const int col = int(blockIdx.y) * 16 * CT + 16 * ct + c, steps = p.segs - 1;
     const bool live = col - c < p.V;
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 S[2 * NP], own[2 * NP], in[2][N];                  // tiles 2 (own_pair + WAVES j) + e at 2 j + e
+    f4 S[2 * NP], own[2 * NP];                            // tiles 2 (own_pair + WAVES j) + e at 2 j + e
     u4 sf[NK][3];                                         // S before the step, all keys
+    u4 in[AHEAD][N];
     const auto tile = [&](int t) { return 2 * ((t >> 1) * WAVES + own_pair) + (t & 1); };
 #pragma unroll
     for (int t = 0; t < 2 * NP; ++t)
@@ -61,13 +62,14 @@ __global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
     const auto add_of = [&](int i) {
         return make_rsrc_n(p.seg_add + (seg_of(i) * p.Vp + (live ? col - c : 0)) * p.Kp, live ? 16 * p.Kp * 4 : 0);
     };
-    const auto fetch = [&](int slice, f4 (&to)[N]) {
+    const auto fetch = [&](int slice, u4 (&to)[N]) {
         const int i = slice / SL, c0 = slice % SL * CW;
-        const rsrc_t from = make_rsrc_n(p.seg_mul + seg_of(i < steps ? i : 0) * p.Kp * p.Kp, i < steps ? p.Kp * p.Kp * 4 : 0);
+        const rsrc_t from = make_rsrc_n(p.seg_mul + seg_of(i < steps ? i : 0) * 3 * p.Kp * p.Kp, i < steps ? p.Kp * p.Kp * 6 : 0);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int x = tid + k * NTH, at = c0 + x / (KP / 4), place = x % (KP / 4) * 4;
-            to[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(from, place < p.Kp ? (at * p.Kp + place) * 4 : none, 0, 0));
+            const int x = tid + k * NTH, at = c0 + x / PER % CW, key = x % PER * 8;
+            const int off = ((x / (CW * PER) * p.Kp + at) * p.Kp + key) * 2;
+            to[k] = __builtin_amdgcn_raw_buffer_load_b128(from, at < p.Kp && key < p.Kp ? off : none, 0, 0);
         }
     };
     const auto fetch_own = [&](int i) {
@@ -82,8 +84,8 @@ __global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
         for (int t = 0; t < 2 * NP; ++t) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, S[t]), to, place(t), 0, 0);
     };
     fetch_own(0);
-    fetch(0, in[0]);
-    fetch(1, in[1]);
+#pragma unroll
+    for (int x = 0; x < AHEAD; ++x) fetch(x, in[x]);
     for (int i0 = 0; i0 < steps; i0 += STEPS) {
 #pragma unroll
         for (int x = 0; x < SL * STEPS; ++x) {
@@ -107,7 +109,7 @@ __global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
                 fetch_own(i + 1);
             }
             lds_barrier();
-            if (WAVES > 1 && x % SL == 0) {
+            if (x % SL == 0) {
 #pragma unroll
                 for (int k = 0; k < NP; ++k)
 #pragma unroll
@@ -116,16 +118,12 @@ __global__ __launch_bounds__(kJoinThreads<KP>) void dr_join(const DrParams p) {
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 const int at = tid + k * NTH;
-                uint32_t a[3], b[3];
-                split<3>(in[x & 1][k][0], in[x & 1][k][1], a);
-                split<3>(in[x & 1][k][2], in[x & 1][k][3], b);
-#pragma unroll
-                for (int n = 0; n < 3; ++n)
-                    *reinterpret_cast<uint2*>(ms + n * TERM + at / (KP / 4) * MST + state_key(at % (KP / 4) * 4)) = make_uint2(a[n], b[n]);
+                *reinterpret_cast<u4*>(ms + at / (CW * PER) * TERM + at / PER % CW * MST + at % PER * 8) = in[x % AHEAD][k];
             }
             lds_barrier();
-            fetch(i0 * SL + x + 2, in[x & 1]);
-            if (WAVES > 1 && x % SL == 0) {
+            fetch(i0 * SL + x + AHEAD, in[x % AHEAD]);
+            stage_end();                                  // (the compiler would issue them after the products)
+            if (x % SL == 0) {
 #pragma unroll
                 for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -233,7 +231,7 @@ Plan plan_of(const ss_delta_rule_args& a, bool train) {
     p.plan = dr_plan_bytes(p.chunk) / 4;
     p.state = kp * vp;
     p.rows = p.chunk * vp;
-    p.mul = kp * kp;
+    p.mul = kp * kp * 3 / 2;
     const int64_t walks = p.bh * ((a.d_value + 63) / 64);
     const bool two = train ? dr_two(a.d_key, terms(a.dtype)) : a.d_key <= 64 && a.dtype != SS_F32;
     int64_t segs = walks > 0 ? (two ? 2 : 1) * kUnits / walks : 1;
@@ -327,11 +325,11 @@ hipError_t walk(int32_t dtype, DrParams p, bool rev, hipStream_t stream) {
         own.local = 1;
         hipError_t e = launch(own);
         if (e != hipSuccess) return e;
-        const dim3 grid(unsigned(p.B * p.H), unsigned(p.V + 63) / 64);
         const auto join = [&](auto kp) {
-            constexpr int KP = decltype(kp)::value;
-            if (rev) hipLaunchKernelGGL((dr_join<KP, true>), grid, dim3(kJoinThreads<KP>), 0, stream, p);
-            else hipLaunchKernelGGL((dr_join<KP, false>), grid, dim3(kJoinThreads<KP>), 0, stream, p);
+            constexpr int KP = decltype(kp)::value, CT = kJoinTiles<KP>;
+            const dim3 grid(unsigned(p.B * p.H), unsigned(p.V + 16 * CT - 1) / (16 * CT)), block(128 * CT);
+            if (rev) hipLaunchKernelGGL((dr_join<KP, true>), grid, block, 0, stream, p);
+            else hipLaunchKernelGGL((dr_join<KP, false>), grid, block, 0, stream, p);
             return hipGetLastError();
         };
         const int64_t kp = dr_keys(p.K);
@@ -363,10 +361,10 @@ hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream
     p.seg_add = at(a->workspace, sp.add);
     if (a->saved) {
         p.plan = at(a->saved, sv.plan); p.states = at(a->saved, sv.states); p.err = at(a->saved, sv.err);
-        p.seg_mul = at(a->saved, sv.mul);
+        p.seg_mul = reinterpret_cast<uint16_t*>(at(a->saved, sv.mul));
     } else {
         p.plan = at(a->workspace, sp.plan);
-        p.seg_mul = at(a->workspace, sp.mul);
+        p.seg_mul = reinterpret_cast<uint16_t*>(at(a->workspace, sp.mul));
     }
     if (plan.nch > 0) {
         const hipError_t e = for_type(a->dtype, [&](auto t) { return dr_prep_launch<decltype(t)>(p, stream); });
@@ -384,7 +382,7 @@ hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t st
     p.o = {g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1};
     set_whole(p, a.dtype);
     p.init = g->dlast_state; p.last = g->dinitial_state;
-    p.plan = at(a.saved, sv.plan); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = at(a.saved, sv.mul);
+    p.plan = at(a.saved, sv.plan); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = reinterpret_cast<uint16_t*>(at(a.saved, sv.mul));
     p.dstates = at(a.workspace, sp.dstates); p.derr = at(a.workspace, sp.derr); p.seg_add = at(a.workspace, sp.add);
     hipError_t e = walk(a.dtype, p, true, stream);
     if (e != hipSuccess || plan.nch == 0) return e;

@@ -59,7 +59,7 @@ struct DrParams {
     int segs, seg_chunks;
     int local;                            // the segments' own states from zero and what becomes of a state over one
     float* seg_add;                       // (B, H, segs, Vp, Kp): their states; then the states that they start from
-    float* seg_mul;                       // (B, H, segs, Kp, Kp): over a segment S becomes M S + its own; column i of M at i Kp, its rows in that order too
+    uint16_t* seg_mul;                    // (B, H, segs, 3, Kp, Kp): over a segment S becomes M S + its own; M in 3 bf16 terms, columns side by side
     // gradients
     void* dq; void* dk; void* dv;         // contiguous; dq and dk in fp32 per head with rep > 1
     float* dg; float* dbeta;              // (B, L, H)

@@ -839,8 +839,17 @@ __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<T, KP>)) vo
         lds_barrier();
     }
     if constexpr (LOCAL) {
-        if (live && unit) keep_state(p.seg_mul + (head.bh * segs + seg) * p.Kp * p.Kp);
-        else if (live) keep_state(p.seg_add + (head.bh * segs + seg) * p.Vp * p.Kp);
+        if (live && unit) {                               // in the terms and the order that dr_join takes it in
+            uint16_t* to = p.seg_mul + ((head.bh * segs + seg) * 3 * p.Kp + col) * p.Kp + 8 * g;
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                if (32 * k >= p.Kp) continue;
+                u4 t[3];
+                pack<3>(S[2 * k], S[2 * k + 1], t);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) *reinterpret_cast<u4*>(to + int64_t(i) * p.Kp * p.Kp + 32 * k) = t[i];
+            }
+        } else if (live) keep_state(p.seg_add + (head.bh * segs + seg) * p.Vp * p.Kp);
     } else {
         // the segment that the walk ends with: forward the one with the row's last token
         const int end = REV || chunks == 0 ? 0 : (chunks - 1) / p.seg_chunks;
