@@ -586,7 +586,7 @@ int ss_linear_attn_update(const ss_linear_attn_update_args* a, void* stream);
  * Shapes, strides, lengths and states as for the linear attention above; g and
  * beta: fp32 (batch, seqlen, heads), any strides (0 too).  d_key and d_value: 1
  * to 256; batch * heads up to 2^20; seqlen up to 2^24; batch * heads * seqlen
- * below 2^28 (fp32 keys above 64, fp16 above 128) or 2^29.
+ * below 2^28 (fp32, and fp16 keys above 128) or 2^29.
  * saved: what the backward takes from the forward (ss_delta_rule_saved_bytes() bytes,
  * 16-byte aligned), or NULL.
  * ------------------------------------------------------------------------ */

@@ -210,10 +210,10 @@ int terms(int32_t dtype) { return dtype == SS_F32 ? 3 : dtype == SS_BF16 ? 1 : 2
 
 // Compute units.  Rows are cut into segments, enough for one workgroup each, or for the two that fit
 // where tiles and registers are small (1 x 32768 tokens x 24 heads of 64 x 64: walk 223 us with 10 segments, 170 with 21).
-// With wider keys or fp32 rows only the walk back gains from the second one (bf16, 1 x 32768 tokens x 16 heads of 128 x 128:
+// With wider keys only the walk back gains from the second one (bf16, 1 x 32768 tokens x 16 heads of 128 x 128:
 // forward and backward 2,422 us to 2,246, forward alone 710 to 729, as its join takes twice the steps), so a prompt has one.
-// The segments' own states cost about what their walk does, so two are not worth it: 5 x 1021 tokens
-// x 24 heads, fp32, 109 us in two and 64 in one.  A segment keeps at least 4 chunks (2 x 515 tokens x 6 heads of 96 x 80, fp32:
+// The segments' own states cost about what their walk does, so two are not worth it: 8 x 2048 tokens
+// x 24 heads of 64 x 64, bf16, 88 us for the states and 113 for the walk, 157 in one.  A segment keeps at least 4 chunks (2 x 515 tokens x 6 heads of 96 x 80, fp32:
 // 104 us in two of 9 chunks, 76 in four).
 constexpr int64_t kUnits = 256, kSegChunksMin = 4, kSegsMin = 3;
 
@@ -233,7 +233,7 @@ Plan plan_of(const ss_delta_rule_args& a, bool train) {
     p.rows = p.chunk * vp;
     p.mul = kp * kp * 3 / 2;
     const int64_t walks = p.bh * ((a.d_value + 63) / 64);
-    const bool two = train ? dr_two(a.d_key, terms(a.dtype)) : a.d_key <= 64 && a.dtype != SS_F32;
+    const bool two = train ? dr_two(a.d_key, terms(a.dtype)) : a.d_key <= 64;
     int64_t segs = walks > 0 ? (two ? 2 : 1) * kUnits / walks : 1;
     if (segs > p.nch / kSegChunksMin) segs = p.nch / kSegChunksMin;
     if (segs < kSegsMin) segs = 1;

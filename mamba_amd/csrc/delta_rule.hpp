@@ -9,13 +9,15 @@
 
 namespace ss {
 
-// Key columns of the kernels' tiles, and tokens a chunk: 64 where the gradients' tiles of
-// a chunk (q, k, and of 32 value columns dout, the states, errors and their gradients in 3 terms)
-// fit the 160 KB of LDS, else 32.  terms: bf16 terms of a row's element (bf16 1, fp16 2, fp32 3).
+// Key columns of the kernels' tiles, and tokens a chunk.  terms: bf16 terms of a row's element (bf16 1, fp16 2, fp32 3).
+// 64 tokens keep and read half the states of 32.  The tiles of fp16 keys above 128 do not fit the LDS at
+// 64; fp32 rows are better off with two workgroups a compute unit at 32, at every size (us forward / with
+// backward: 8 x 2048 tokens x 12 heads of 64 x 64 142 / 469 for 230 / 667, 1 x 16384 x 12 190 / 544 for 205 / 637, 2 x 500 x 6 41 / 100
+// for 59 / 139); others are not: fp16 of 128 keys 258 / 883 for 263 / 805 (2 x 4096 x 16), bf16 of 256 316 / 1,162 for 300 / 1,108 (2 x 4096 x 8).
 constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
-constexpr int dr_chunk(int64_t k, int terms) { return dr_keys(k) * terms <= 256 ? 64 : 32; }
+constexpr int dr_chunk(int64_t k, int terms) { return terms < 3 && dr_keys(k) * terms <= 256 ? 64 : 32; }
 // Where two workgroups of a walk share a compute unit: tiles of at most 80 KB.
-constexpr bool dr_two(int64_t k, int terms) { return dr_keys(k) * terms <= 128 || (dr_keys(k) == 128 && terms == 3); }
+constexpr bool dr_two(int64_t k, int terms) { return dr_keys(k) * terms <= 128 || (dr_keys(k) <= 128 && terms == 3); }
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
 constexpr int dr_round32(int64_t n) { return int((n + 31) / 32 * 32); }
 
