@@ -296,9 +296,9 @@ DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
     p.K = int(a.d_key); p.V = int(a.d_value); p.Kp = dr_round32(a.d_key); p.Vp = dr_round16(a.d_value);
     p.rep = int(a.heads / a.groups); p.nch = int(plan.nch);
     p.scale = a.scale;
-    p.q = {a.q, a.q_batch_stride, a.q_len_stride, a.q_head_stride, p.rep};
-    p.k = {a.k, a.k_batch_stride, a.k_len_stride, a.k_head_stride, p.rep};
-    p.v = {a.v, a.v_batch_stride, a.v_len_stride, a.v_head_stride, 1};
+    p.q = dr_rows(a.q, a.q_batch_stride, a.q_len_stride, a.q_head_stride, p.rep, p.K, p.L);
+    p.k = dr_rows(a.k, a.k_batch_stride, a.k_len_stride, a.k_head_stride, p.rep, p.K, p.L);
+    p.v = dr_rows(a.v, a.v_batch_stride, a.v_len_stride, a.v_head_stride, 1, p.V, p.L);
     p.g = a.g; p.g_b = a.g_batch_stride; p.g_l = a.g_len_stride; p.g_h = a.g_head_stride;
     p.beta = a.beta; p.be_b = a.beta_batch_stride; p.be_l = a.beta_len_stride; p.be_h = a.beta_head_stride;
     p.lens = a.lengths;
@@ -309,8 +309,8 @@ DrParams params_of(const ss_delta_rule_args& a, const Plan& plan) {
 // (p.o is set by then: out, or the backward's dout)
 void set_whole(DrParams& p, int32_t dtype) {
     const int size = dtype == SS_F32 ? 4 : 2;
-    p.whole = dr_whole(p.q, p.K, p.L, size) && dr_whole(p.k, p.K, p.L, size) && dr_whole(p.v, p.V, p.L, size) &&
-              dr_whole(p.o, p.V, p.L, size) && p.H * (p.K > p.V ? p.K : p.V) < (int64_t(1) << 22);
+    p.whole = dr_whole(p.q, p.K, size) && dr_whole(p.k, p.K, size) && dr_whole(p.v, p.V, size) && dr_whole(p.o, p.V, size) &&
+              p.H * (p.K > p.V ? p.K : p.V) < (int64_t(1) << 22);
 }
 
 float* at(void* base, int64_t bytes) { return reinterpret_cast<float*>(static_cast<char*>(base) + bytes); }
@@ -355,7 +355,7 @@ hipError_t delta_rule_fwd_launch(const ss_delta_rule_args* a, hipStream_t stream
     const FwdSpace sp = fwd_space(*a, plan);
     const Saved sv = saved_of(plan);
     DrParams p = params_of(*a, plan);
-    p.o = {a->out, a->out_batch_stride, a->out_len_stride, a->out_head_stride, 1};
+    p.o = dr_rows(a->out, a->out_batch_stride, a->out_len_stride, a->out_head_stride, 1, p.V, p.L);
     set_whole(p, a->dtype);
     p.init = a->initial_state; p.last = a->last_state;
     p.seg_add = at(a->workspace, sp.add);
@@ -379,7 +379,7 @@ hipError_t delta_rule_bwd_launch(const ss_delta_rule_bwd_args* g, hipStream_t st
     const BwdSpace sp = bwd_space(a, plan);
     const Saved sv = saved_of(plan);
     DrParams p = params_of(a, plan);
-    p.o = {g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1};
+    p.o = dr_rows(g->dout, g->dout_batch_stride, g->dout_len_stride, g->dout_head_stride, 1, p.V, p.L);
     set_whole(p, a.dtype);
     p.init = g->dlast_state; p.last = g->dinitial_state;
     p.plan = at(a.saved, sv.plan); p.states = at(a.saved, sv.states); p.err = at(a.saved, sv.err); p.seg_mul = reinterpret_cast<uint16_t*>(at(a.saved, sv.mul));

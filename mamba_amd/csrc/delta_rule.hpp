@@ -25,8 +25,13 @@ constexpr int dr_round32(int64_t n) { return int((n + 31) / 32 * 32); }
 // buffer resources, which end with the chunk's last row.  (8 x 2048 tokens x 24 heads of 64 x 64, bf16: a walk
 // of 198 us with rows of any kind read behind branches, after each of which the compiler waits for all loads, was
 // 170 without them; 157 by now.)
-inline bool dr_whole(const LaRows& r, int64_t dim, int64_t len, int size) {
-    return dim * size % 16 == 0 && r.l < (int64_t(1) << 22) && (r.l >= dim || len <= 1);
+inline bool dr_whole(const LaRows& r, int64_t dim, int size) {
+    return dim * size % 16 == 0 && r.l < (int64_t(1) << 22) && r.l >= dim;
+}
+// The rows of a tensor.  The token stride of a single token may be anything (0 or 1 of a permuted tensor, say): nothing
+// is read or written by it, and the places past the row's only one lie past its end with a stride of the row's own width.
+inline LaRows dr_rows(const void* p, int64_t b, int64_t l, int64_t h, int rep, int64_t dim, int64_t len) {
+    return {p, b, len > 1 ? l : dim, h, rep};
 }
 
 // Per (batch, head) pair and chunk, what the kernels hand on (fp32):
