@@ -57,10 +57,11 @@ using namespace la;
 // a chunk's tokens 30 bits below the point
 constexpr double kEmpty = -1e5;
 // Where beta is zero (or smaller) the inverse takes this in its place, and so do F and M
-// of the backward: then dbeta, the sum F . E over beta, keeps its value, and what else they
-// enter changes by 2^-60 of E.
+// of the backward: then dbeta, the sum F . E over beta, keeps its value.  The token's own dv and
+// dk, which have the factor beta, are scaled back (least_to_beta); what else F and M enter changes by 2^-60 of E.
 constexpr float kLeastBeta = 8.673617379884035e-19f;      // 2^-60
 __device__ __forceinline__ float beta_or_least(float b) { return fabsf(b) < kLeastBeta ? kLeastBeta : b; }
+__device__ __forceinline__ float least_to_beta(float b) { return fabsf(b) < kLeastBeta ? b * (1.f / kLeastBeta) : 1.f; }
 
 template <typename T, int KP>
 struct Dims {
@@ -1042,11 +1043,12 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
                     }
                     if (own < toks && v0 + 8 * g < p.V) { // dv: F of the own token
                         const uint32_t is = own < cnt && gates.beta[own] != 0.f ? ~0u : 0u;
+                        const float to_beta = least_to_beta(gates.beta[own]);
                         f4 x[2];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const auto half = [&](const u4& t) { return e & 1 ? hi_half(t[e >> 1]) : lo_half(t[e >> 1]); };
-                            x[e >> 2][e & 3] = __builtin_bit_cast(float, is & __builtin_bit_cast(uint32_t, half(ff[0]) + (half(ff[1]) + half(ff[2]))));
+                            x[e >> 2][e & 3] = __builtin_bit_cast(float, is & __builtin_bit_cast(uint32_t, to_beta * (half(ff[0]) + (half(ff[1]) + half(ff[2])))));
                         }
                         put8(dv_rows + int64_t(own) * p.H * p.V, v0 + 8 * g, p.V, x[0], x[1]);
                     }
@@ -1114,7 +1116,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
     const float bown = gates.beta[own];
     if (reader) {
         f4 (&M)[NR] = Ms[0], (&R)[NR] = Rs[0], (&dk)[NS] = dks[0];
-        const float gam = gates.gam[own];
+        const float gam = gates.gam[own], to_beta = least_to_beta(bown);
         float r = 0.f;
 #pragma unroll
         for (int a = 0; a < NK; ++a) {
@@ -1123,7 +1125,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
             keys8(ks, a, kv);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float x = dq[2 * a + (e >> 2)][e & 3] * (p.scale * gam), y = dk[2 * a + (e >> 2)][e & 3] * -gam;
+                const float x = dq[2 * a + (e >> 2)][e & 3] * (p.scale * gam), y = dk[2 * a + (e >> 2)][e & 3] * (-gam * to_beta);
                 dq[2 * a + (e >> 2)][e & 3] = x;
                 dk[2 * a + (e >> 2)][e & 3] = y;
                 r = __builtin_fmaf(qv[e], x, __builtin_fmaf(kv[e], y, r));
@@ -1155,7 +1157,7 @@ __global__ __launch_bounds__((kGradThreads<T, KP>), (kGradThreads<T, KP> > 256 |
             for (int q = 0; q < 4; ++q) {
                 const int row = 16 * j + 4 * g + q;
                 diag = row == own ? M[j][q] : diag;
-                const float rv = fs[q] * (p.scale * beta[q]) * R[j][q], mv = -fs[q] * beta[q] * M[j][q];
+                const float rv = fs[q] * (p.scale * beta[q]) * R[j][q], mv = -fs[q] * (to_beta * beta[q]) * M[j][q];
                 R[j][q] = row <= own ? rv : 0.f;
                 M[j][q] = row < own ? mv : 0.f;
                 term[q] = __builtin_fmaf(R[j][q], kq[q], M[j][q] * kk2[q]);

@@ -107,3 +107,35 @@ def test_one_token_through_c(stride, dtype):
     rc = nat.load().ss_delta_rule_fwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
     assert rc == 0, nat.load().ss_last_error()
     assert torch.equal(out[1:-1], want) and bool((out[0] == 7).all()) and bool((out[-1] == 7).all())
+
+
+TINY = (0.0, 1e-20, -1e-22, 2.0 ** -60, 1e-30, -0.0, 1e-42)
+
+
+@TYPES
+@pytest.mark.parametrize("shape", [(1, 200, 2, 2, 64, 64), (1, 700, 2, 1, 128, 96)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_tiny_rates(shape, dtype):
+    """dv and dk of a token have the factor beta: zero where it is, and as small as it is where it is tiny.
+
+    Relative to beta their errors are those of other tokens', but for the type's smallest values.  A matrix instruction
+    takes an operand's term below 2^-126 for zero: dk sums, over the 64 tokens of a chunk, two products of a factor beta R
+    or beta M, in up to 3 terms, with an element of q or k, and so loses up to 64 * 2 * 3 * 2^-126 of the largest element.
+    """
+    x = make(*shape, dtype, seed=63)
+    for i, b in enumerate(TINY):
+        x["beta"][0, 3 + i::29] = b
+    want, room = want_of(x)
+    got = run(x)
+    for n, t in got.items():
+        check(t, want[n], room[n], n)
+    for n, group in (("dv", 1), ("dk", shape[2] // shape[3])):
+        smallest = 2.0 ** -24 if dtype == F16 else 2.0 ** -133 if dtype == BF16 else 2.0 ** -149
+        if n == "dk":
+            smallest += 64 * 2 * 3 * 2.0 ** -126 * max(float(x[m].abs().max()) for m in "qk")
+        for i, b in enumerate(TINY):
+            t, w, r = (y[0, 3 + i::29].double().cpu() for y in (got[n], want[n], room[n]))
+            if b == 0.0:
+                assert not t.any(), (n, b)
+            else:
+                step = torch.finfo(dtype).eps
+                assert bool(((t - w).abs() <= r * abs(b) * (1 + step) + step * w.abs() + group * smallest).all()), (n, b)
