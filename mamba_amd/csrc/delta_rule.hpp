@@ -16,7 +16,8 @@ namespace ss {
 // for 59 / 139); others are not: fp16 of 128 keys 258 / 883 for 263 / 805 (2 x 4096 x 16), bf16 of 256 316 / 1,162 for 300 / 1,108 (2 x 4096 x 8).
 constexpr int dr_keys(int64_t k) { return k <= 64 ? 64 : k <= 128 ? 128 : 256; }
 constexpr int dr_chunk(int64_t k, int terms) { return terms < 3 && dr_keys(k) * terms <= 256 ? 64 : 32; }
-// Where two workgroups of a walk share a compute unit: tiles of at most 80 KB.
+// Where two workgroups of a walk share a compute unit, each with half of its LDS.
+constexpr int64_t kTwoTiles = 80 * 1024;
 constexpr bool dr_two(int64_t k, int terms) { return dr_keys(k) * terms <= 128 || (dr_keys(k) <= 128 && terms == 3); }
 constexpr int dr_round16(int64_t n) { return int((n + 15) / 16 * 16); }
 constexpr int dr_round32(int64_t n) { return int((n + 31) / 32 * 32); }

@@ -69,6 +69,9 @@ struct Dims {
     static constexpr int NT = NR * (NR + 1) / 2;             // lower tiles of a chunk's square
     static constexpr int KST = KP + 8;                       // row stride of q and k in LDS, elements
     static constexpr int VST = sizeof(T) == 4 ? 68 : 72;     // of 64 value columns as they are
+    // of out's rows on their way to memory (fp16: with 72, 272 bytes too many for two walks of 64 keys on a compute unit;
+    // prompts of 24 heads of 64 x 64, 1 x 32768 tokens 543 us with one, 497 with two, 16 x 2048 390 and 304)
+    static constexpr int OST = KT == 2 && KP == 64 ? 68 : VST;
     static constexpr int OT = sizeof(T) == 4 ? 3 : 2;        // terms of what only a result of type T is formed from
     // dr_grads: value columns and keys of the states that it takes at a time (tiles of q, k and these fill the LDS)
     static constexpr int VW = 32, KW = KP <= 128 ? KP : KT == 3 ? 64 : 128;
@@ -76,8 +79,8 @@ struct Dims {
 template <typename T, int KP> constexpr int kPrepThreads = 64 * Dims<T, KP>::NR;
 // A walk's workgroup: 4 waves, 64 value columns; of the segments' own states 8, 4 of them the identity's columns.
 // Waves a SIMD that it is compiled for: with 2 its results stay out of the accumulation registers, where
-// vector instructions do not reach them, and of 64 keys two workgroups share a compute unit (1 x 32768 tokens x 24
-// heads: 223 us to 170).  Wider tiles leave room for one.
+// vector instructions do not reach them, and two workgroups share a compute unit (dr_two: up to 64 keys, bf16 and fp32 up to 128;
+// 1 x 32768 tokens x 24 heads of 64 x 64, bf16: 223 us to 170).  Wider tiles leave room for one.
 template <bool REV, bool LOCAL> constexpr int kWalkThreads = LOCAL && !REV ? 512 : 256;
 template <typename T, int KP> constexpr int kWalkWaves = dr_two(KP, kTerms<T>) ? 2 : 1;
 // dr_grads: a wave takes its tokens in both roles where two such workgroups fit a compute unit's LDS (80 KB each:
@@ -213,6 +216,13 @@ struct Tile {
             }
         }
     }
+    // a vector of a raw tile whose rows are STRIDE elements, whole vectors or halves of them
+    template <int STRIDE>
+    static __device__ __forceinline__ u4 read16(const T* at) {
+        if constexpr (STRIDE * sizeof(T) % 16 == 0) return *reinterpret_cast<const u4*>(at);
+        const u2 lo = reinterpret_cast<const u2*>(at)[0], hi = reinterpret_cast<const u2*>(at)[1];
+        return u4{lo.x, lo.y, hi.x, hi.y};
+    }
     // the first `rows` rows and `dim` columns of a raw tile to global memory
     template <int STRIDE>
     static __device__ __forceinline__ void put(T* p, int64_t step, const T* tile, int rows, int dim) {
@@ -224,14 +234,14 @@ struct Tile {
             const uint32_t off = col < dim ? (uint32_t(row) * uint32_t(step) + uint32_t(col)) * es : none;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const u4 w = *reinterpret_cast<const u4*>(from + i * (NTH / PER) * STRIDE);
+                const u4 w = read16<STRIDE>(from + i * (NTH / PER) * STRIDE);
                 __builtin_amdgcn_raw_buffer_store_b128(w, r, int(off + uint32_t(i * (NTH / PER)) * uint32_t(step) * es), 0, 0);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 float x[R::VE];
-                R::unpack(*reinterpret_cast<const uint4*>(from + i * (NTH / PER) * STRIDE), x);
+                R::unpack(__builtin_bit_cast(uint4, read16<STRIDE>(from + i * (NTH / PER) * STRIDE)), x);
                 const int r = row + i * (NTH / PER);
                 R::store(p + int64_t(r) * step + col, x, r < rows ? dim - col : 0);
             }
@@ -485,13 +495,15 @@ template <typename T, int KP, bool REV, bool LOCAL, bool WHOLE>
 __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<T, KP>)) void dr_walk(const DrParams p) {
     using D = Dims<T, KP>;
     constexpr int NTH = kWalkThreads<REV, LOCAL>;
-    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NT = D::NT, VST = D::VST;
+    constexpr int C = D::C, NR = D::NR, NP = D::NP, NK = D::NK, NS = D::NS, KT = D::KT, KST = D::KST, NT = D::NT, VST = D::VST, OST = D::OST;
     constexpr int KTERM = C * KST, CTERM = NT * 256;
     constexpr int PT = REV ? 3 : D::OT;                   // P's terms
     constexpr bool Q = REV || !LOCAL;                     // whether q is read
     __shared__ __attribute__((aligned(16))) uint16_t ks[KT * KTERM], qs[Q ? KT * KTERM : 8], tri[3 * CTERM], prob[Q ? PT * CTERM : 8];
-    __shared__ __attribute__((aligned(16))) T vs[C * VST], os[!REV && !LOCAL ? C * VST : 4];
+    __shared__ __attribute__((aligned(16))) T vs[C * VST], os[!REV && !LOCAL ? C * OST : 4];
     __shared__ __attribute__((aligned(16))) Gates<C> G;
+    static_assert(!dr_two(KP, KT) || sizeof(ks) + sizeof(qs) + sizeof(tri) + sizeof(prob) + sizeof(vs) + sizeof(os) + sizeof(G) <= kTwoTiles,
+                  "two workgroups' tiles in a compute unit's LDS");
     const int segs = p.segs, seg = int(blockIdx.x % unsigned(segs));
     // (nothing starts from the last segment's own state; a backward takes its M)
     if (LOCAL && seg == (REV ? 0 : segs - 1) && (REV || !p.states)) return;
@@ -743,12 +755,12 @@ __global__ __launch_bounds__((kWalkThreads<REV, LOCAL>), (kWalkWaves<T, KP>)) vo
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
                         const float o[4] = {p.scale * O[i][0], p.scale * O[i][1], p.scale * O[i][2], p.scale * O[i][3]};
-                        store4<T>(os + (16 * i + c) * VST + 16 * w + 4 * g, o, 4);
+                        store4<T>(os + (16 * i + c) * OST + 16 * w + 4 * g, o, 4);
                     }
                 }
                 lds_barrier();                            // (the chunk's tiles are done with)
                 stage();
-                Tile<T, 64, C, NTH, WHOLE>::template put<VST>(op + t0 * p.o.l, p.o.l, os, count(n), p.V - v0);
+                Tile<T, 64, C, NTH, WHOLE>::template put<OST>(op + t0 * p.o.l, p.o.l, os, count(n), p.V - v0);
             }
         } else {
             f4 X[NR];
