@@ -13,7 +13,6 @@ without gradients.
 All on the HIP library: tensors on a ROCm device.
 """
 import torch
-import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops.block_norm import gated_rms_norm_fn
@@ -23,12 +22,8 @@ from .linear_attn import LinearAttn
 
 
 class DeltaRule(LinearAttn):
-    def __init__(self, model_dim, head_dim=64, key_dim=None, n_groups=None, expansion_factor=2, delta_min=0.001,
-                 delta_max=0.1, eps=1e-6, device=None, dtype=None):
-        super().__init__(model_dim, head_dim, key_dim, n_groups, expansion_factor, delta_min, delta_max, eps, device, dtype)
-        qk = self.n_groups * self.key_dim
-        self.sizes = [2 * qk, self.inner_dim, self.inner_dim, self.n_heads, self.n_heads]
-        self.input_proj = nn.Linear(model_dim, sum(self.sizes), bias=False, device=device, dtype=dtype)
+    def _sizes(self, qk):
+        return [2 * qk, self.inner_dim, self.inner_dim, self.n_heads, self.n_heads]
 
     def _split(self, hidden_states):
         qk, v, z, dt, b = self.input_proj(hidden_states).split(self.sizes, -1)

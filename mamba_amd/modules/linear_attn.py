@@ -31,14 +31,17 @@ class LinearAttn(nn.Module):
         self.n_heads, self.head_dim = self.inner_dim // head_dim, head_dim
         self.key_dim, self.n_groups = key_dim or head_dim, n_groups or self.n_heads
         self.eps = eps
-        qk = self.n_groups * self.key_dim
-        self.sizes = [qk, qk, self.inner_dim, self.inner_dim, self.n_heads]
+        self.sizes = self._sizes(self.n_groups * self.key_dim)
         self.input_proj = nn.Linear(model_dim, sum(self.sizes), bias=False, **fk)
         self.norm = nn.Parameter(torch.zeros(self.inner_dim, **fk))
         self.output_proj = nn.Linear(self.inner_dim, model_dim, bias=False, **fk)
         delta = torch.exp(torch.rand(self.n_heads, device=device) * math.log(delta_max / delta_min) + math.log(delta_min))
         self.dt_bias = nn.Parameter(delta + torch.log(-torch.expm1(-delta)))            # softplus of it is delta
         self.log_A = nn.Parameter(torch.log(1 + 15 * torch.rand(self.n_heads, device=device)))
+
+    def _sizes(self, qk):
+        """Widths of the input projection's parts; qk: of all groups' queries (or keys)."""
+        return [qk, qk, self.inner_dim, self.inner_dim, self.n_heads]
 
     def _split(self, hidden_states):
         q, k, v, z, dt = self.input_proj(hidden_states).split(self.sizes, -1)
