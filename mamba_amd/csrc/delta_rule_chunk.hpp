@@ -1369,7 +1369,6 @@ template <typename T>
 hipError_t dr_grads_launch(const DrParams& p, hipStream_t stream) {
     return dr_by_keys<T>(p.K, [&](auto kp) {
         constexpr int KP = decltype(kp)::value;
-        // (a workgroup a compute unit, which its tiles fill: it goes from chunk to chunk)
         const int64_t all = p.BH * p.nch;
         const dim3 grid(unsigned(all), 1), block(dr::kGradThreads<T, KP>);
         if (p.whole) hipLaunchKernelGGL((dr::dr_grads<T, KP, true>), grid, block, 0, stream, p);

@@ -28,7 +28,7 @@ their sums have a fixed order, so the same bits on every run, and every term of
 dg has the factor exp(g): it is zero where the decay empties the state.  With
 gradients, a state for each 32 or 64 tokens is kept until the backward.
 Tokens are computed in chunks of up to 64: a token's infinities or NaN reach the outputs
-of its chunk and of later ones.
+of its whole chunk, earlier tokens among them, and of later ones.
 Forward-mode and second derivatives are refused.
 
 ``delta_rule_update(state, q, k, v, g, beta, scale=None, out=None)`` advances
